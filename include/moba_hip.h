@@ -58,7 +58,7 @@ extern "C" {
 
 enum { MOBA_DTYPE_BF16 = 0, MOBA_DTYPE_F16 = 1 };
 
-#define MOBA_ABI_VERSION 120 /* the signatures below; moba_version() returns the number the library was built with */
+#define MOBA_ABI_VERSION 121 /* the signatures below; moba_version() returns the number the library was built with */
 int moba_version(void);
 const char* moba_strerror(int code);
 
@@ -370,6 +370,30 @@ int moba_decode_splits(int B, int Hkv, int Skv);
 int moba_decode(const void* q, const void* k, const void* v, void* out, float* part_o, float* part_lse, int B, int H,
                 int Hkv, int Skv, int D, int64_t q_stride_b, int64_t q_stride_h, int64_t kv_stride_b,
                 int64_t kv_stride_h, float scale, int dtype, void* stream);
+
+/* Norm and rotation of the query and key heads, what precedes the operator in a decoder layer (the reference's models do
+ * it with torch ops of transformers):
+ *   y = R(x * w / sqrt(mean(x^2) + eps))  for every (token, head) row x of q and of k,
+ * R turning pair i of the first `rotary` elements by positions[token] * inv_freq[i]: pairs (i, i + rotary / 2), or
+ * (2i, 2i + 1) with interleaved != 0.  A side whose weight is NULL is turned only.
+ *   q [S,H,D], k [S,Hkv,D] elem, D contiguous elements; strides {q token, q head, k token, k head} in elements, multiples of 4;
+ *   yq [S,H,D], yk [S,Hkv,D] elem, packed (they must not overlap q, k); all 8-byte aligned
+ *   q_weight, k_weight [D] elem, or fp32 with weight_f32 != 0; positions [S] int32 or int64 (position_bits 32 or 64);
+ *   inv_freq [rotary / 2] fp32.  D at most 128; D and rotary multiples of 8.  S at most 2^25.
+ * 32-bit arithmetic (the angles 64-bit), one rounding.
+ * Backward: dq, dk [S,H,D], [S,Hkv,D] packed from packed dyq, dyk and the forward's inputs; dq_weight, dk_weight [D] of the
+ * weights' type or NULL: sums over tokens and heads in a fixed order; workspace (only for these)
+ * moba_qk_norm_rope_bwd_workspace_bytes(S, D) bytes, 4-byte aligned. */
+int moba_qk_norm_rope(const void* q, const void* k, void* yq, void* yk, const void* q_weight, const void* k_weight,
+                      const void* positions, const float* inv_freq, int64_t S, int H, int Hkv, int D, int rotary,
+                      const int64_t* strides, int position_bits, int interleaved, int weight_f32, float eps, int dtype,
+                      void* stream);
+size_t moba_qk_norm_rope_bwd_workspace_bytes(int64_t S, int D);
+int moba_qk_norm_rope_bwd(const void* dyq, const void* dyk, const void* q, const void* k, void* dq, void* dk,
+                          const void* q_weight, const void* k_weight, void* dq_weight, void* dk_weight, void* workspace,
+                          const void* positions, const float* inv_freq, int64_t S, int H, int Hkv, int D, int rotary,
+                          const int64_t* strides, int position_bits, int interleaved, int weight_f32, float eps, int dtype,
+                          void* stream);
 
 /* Measurement aid, no counterpart in the reference: what the matrix pipes sustain when they do nothing else.
  * Launches `workgroups` workgroups (0: one per compute unit) of eight waves, two per SIMD as in the forward kernel;

@@ -5,9 +5,10 @@ from functools import partial
 
 from .config import MoBAConfig
 from .moba_efficient import moba_attn_varlen, moba_attn_varlen_gqa
+from .norm_rope import qk_norm_rope
 from .wrapper import moba_layer
 
-__all__ = ["MoBAConfig", "register_moba", "moba_attn_varlen", "moba_attn_varlen_gqa", "moba_layer"]
+__all__ = ["MoBAConfig", "register_moba", "moba_attn_varlen", "moba_attn_varlen_gqa", "moba_layer", "qk_norm_rope"]
 
 
 def register_moba(cfg: MoBAConfig):

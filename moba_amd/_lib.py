@@ -59,6 +59,10 @@ _SIGNATURES = {
     "moba_bwd_dq_key_split": (c_int, [c_int64, c_int, c_int, c_int, c_int64, c_int64]),
     "moba_bwd": (c_int, [c_void_p] * 23 + [c_int, c_int64] + [c_void_p] * 5 + [c_int64, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int64, c_int64,
                                           c_int64, c_int, c_strides, c_void_p, c_void_p, c_int64, c_int, c_int, c_float, c_int, c_void_p]),
+    "moba_qk_norm_rope": (c_int, [c_void_p] * 8 + [c_int64] + [c_int] * 4 + [c_strides] + [c_int] * 3 + [c_float, c_int, c_void_p]),
+    "moba_qk_norm_rope_bwd_workspace_bytes": (c_size_t, [c_int64, c_int]),
+    "moba_qk_norm_rope_bwd": (c_int, [c_void_p] * 13 + [c_int64] + [c_int] * 4 + [c_strides] + [c_int] * 3
+                                     + [c_float, c_int, c_void_p]),
     "moba_mfma_probe": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p]),
     "moba_tail_splits": (c_int, [c_int] * 5),
     "moba_tail": (c_int, [c_void_p] * 6 + [c_int] * 6 + [c_strides, c_float, c_int, c_void_p]),
@@ -88,7 +92,7 @@ class SizesStruct(ctypes.Structure):
     _fields_ = [(n, c_int64) for n in ("kbar_elems", "chunk_mean_workspace_bytes", "sel_ints", "cnt_ints", "seg_off_ints",
                                        "seg_dest_ints", "fwd_hist_bound", "bwd_hist_bound", "part_rows", "redo_ints",
                                        "lse_floats", "delta_floats")]
-ABI_VERSION = 120  # MOBA_ABI_VERSION of include/moba_hip.h, the signatures above
+ABI_VERSION = 121  # MOBA_ABI_VERSION of include/moba_hip.h, the signatures above
 DTYPE_BF16, DTYPE_F16 = 0, 1
 
 
