@@ -395,6 +395,28 @@ int moba_qk_norm_rope_bwd(const void* dyq, const void* dyk, const void* q, const
                           const int64_t* strides, int position_bits, int interleaved, int weight_f32, float eps, int dtype,
                           void* stream);
 
+/* The paged key/value cache (no counterpart in the reference, whose decode branch reads transformers' contiguous cache,
+ * moba/wrapper.py:76-82).
+ *   k_pages, v_pages [num_pages, Hkv, page_size, D]: elem, or e4m3 bytes with cache8 != 0; page_size 16, 32, 64, 128 or 256;
+ *   D 64 or 128; Hkv at most 256
+ *   k_scales, v_scales [num_pages, Hkv] fp32 (cache8 only): an element stands for its value times its page's and head's scale
+ *   page_table [B, max_pages] int32 (row stride: an entry of `strides`), lengths [B] int32 (tokens of a sequence, the new ones
+ *   included), cu_new [B+1] int32 (its new tokens are rows cu_new[b] .. cu_new[b+1]-1 of the T packed rows; the last of them
+ *   has position lengths[b] - 1).  Read on the device; whatever they hold, no access leaves the tensors.
+ *
+ * moba_paged_append: the new tokens' k and v [T,Hkv,D] go to their pages, k, and q [T,H,D] -> yq [T,H,D] (packed; both
+ * NULL: none), turned by their positions as in moba_qk_norm_rope (rotary = 0: not turned).  Rows of yq that belong to no
+ * sequence are zeros.  A token without a valid page is not written.  A page that receives tokens must be named by one sequence
+ * only.  cache8: scales are powers of two, 2^k with the smallest k >= -100 for which the page's largest magnitude is at most
+ * 448 * 2^k, and not less than that of the tokens the page already holds, which are rounded again where it grows.
+ *   strides {q token, q head, k token, k head, v token, v head, page_table row} in elements, multiples of 4 (the last: any);
+ *   q, k, v and the pages 8-byte aligned; T < 2^30 */
+int moba_paged_append(const void* k, const void* v, const void* q, void* yq, void* k_pages, void* v_pages, float* k_scales,
+                      float* v_scales, const int32_t* page_table, const int32_t* lengths, const int32_t* cu_new,
+                      const float* inv_freq, int64_t T, int B, int H, int Hkv, int D, int rotary, int page_size,
+                      int64_t num_pages, int64_t max_pages, const int64_t* strides, int cache8, int interleaved, int dtype,
+                      void* stream);
+
 /* Measurement aid, no counterpart in the reference: what the matrix pipes sustain when they do nothing else.
  * Launches `workgroups` workgroups (0: one per compute unit) of eight waves, two per SIMD as in the forward kernel;
  * every wave issues iters * 16 v_mfma_f32_32x32x16_bf16 on sixteen operand registers it loads once from

@@ -1,0 +1,168 @@
+"""A paged key/value cache on MI355X, with 16-bit elements or 8-bit ones and a scale for every page and head, and the operators on
+it: ``paged_append`` writes the keys and values of new tokens, rotated by position on the way.  Sequences of any lengths are
+served together.  (The reference keeps transformers' contiguous cache, one length for the whole batch, moba/wrapper.py:76-82.)"""
+
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from . import _lib
+from . import moba_efficient as E
+from .norm_rope import _check_inv_freq, _readable, _strides_of
+
+E4M3 = torch.float8_e4m3fn
+PAGE_SIZES = (16, 32, 64, 128, 256)
+HEAD_DIMS = (64, 128)
+MAX_KV_HEADS = 256
+MAX_TOKENS = (1 << 30) - 1   # packed rows of a call
+
+
+@dataclass
+class PagedKVCache:
+    """The pages of one layer.
+
+    k_pages, v_pages: [num_pages, kv_heads, page_size, head_dim], bf16, fp16 or e4m3 (``torch.float8_e4m3fn``); page_size
+        16, 32, 64, 128 or 256, head_dim 64 or 128
+    k_scales, v_scales: [num_pages, kv_heads] float32, for e4m3 only: an element stands for its value times the scale of its
+        page and head.  ``paged_append`` keeps them powers of two.
+
+    Which pages belong to which sequence is the caller's affair (the ``page_table`` of the calls).  Pages may be shared by
+    sequences that only read them; a page that receives tokens in a call must be named by one sequence only.
+    """
+
+    k_pages: torch.Tensor
+    v_pages: torch.Tensor
+    k_scales: Optional[torch.Tensor] = None
+    v_scales: Optional[torch.Tensor] = None
+
+    def __post_init__(self):
+        k = self.k_pages
+        if k.dtype not in (torch.bfloat16, torch.float16, E4M3) or self.v_pages.dtype != k.dtype:
+            raise TypeError("the pages must be bfloat16, float16 or float8_e4m3fn, keys and values alike")
+        if k.dim() != 4 or self.v_pages.shape != k.shape:
+            raise ValueError("k_pages and v_pages must be [num_pages, kv_heads, page_size, head_dim]")
+        if k.shape[2] not in PAGE_SIZES or k.shape[3] not in HEAD_DIMS:
+            raise ValueError(f"page_size must be one of {PAGE_SIZES} and head_dim one of {HEAD_DIMS}")
+        if not (0 < k.shape[0] < 1 << 31 and 0 < k.shape[1] <= MAX_KV_HEADS):
+            raise ValueError(f"there must be pages, and 1 to {MAX_KV_HEADS} key/value heads")
+        scales = [s for s in (self.k_scales, self.v_scales) if s is not None]
+        if len(scales) != (2 if k.dtype == E4M3 else 0):
+            raise ValueError("e4m3 pages need k_scales and v_scales, others take none")
+        if any(s.dtype != torch.float32 for s in scales):
+            raise TypeError("the scales must be float32")
+        if any(s.shape != k.shape[:2] for s in scales):
+            raise ValueError("the scales must be [num_pages, kv_heads]")
+        held = [k, self.v_pages, *scales]
+        if any(t.device != k.device for t in held):
+            raise ValueError("all tensors of a cache must be on one device")
+        if any(not t.is_contiguous() or t.data_ptr() % 16 for t in held):
+            raise ValueError("the tensors of a cache must be contiguous and 16-byte aligned")
+
+    @classmethod
+    def empty(cls, num_pages: int, kv_heads: int, head_dim: int = 128, page_size: int = 64, dtype: torch.dtype = E4M3,
+              device="cuda") -> "PagedKVCache":
+        """A cache of zeros."""
+        shape = (num_pages, kv_heads, page_size, head_dim)
+        pages = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(2)]
+        if dtype != E4M3:
+            return cls(*pages)
+        return cls(*pages, *(torch.ones(shape[:2], dtype=torch.float32, device=device) for _ in range(2)))
+
+    @property
+    def quantized(self) -> bool:
+        return self.k_scales is not None
+
+
+def _check_table(cache, page_table, lengths, cu_new, device):
+    for name, t, dims in (("page_table", page_table, 2), ("lengths", lengths, 1), ("cu_new", cu_new, 1)):
+        if t.dtype != torch.int32:
+            raise TypeError(f"{name} must be int32")
+        if t.dim() != dims:
+            raise ValueError("page_table must be [sequences, pages], lengths [sequences], cu_new [sequences + 1]")
+        if t.device != device:
+            raise ValueError("all tensors must be on one device")
+    b = page_table.shape[0]
+    if lengths.shape[0] != b or cu_new.shape[0] != b + 1 or (b and not page_table.shape[1]):
+        raise ValueError("page_table must be [sequences, pages], lengths [sequences], cu_new [sequences + 1]")
+    if cache.k_pages.device != device:
+        raise ValueError("all tensors must be on one device")
+
+
+def _table(page_table):
+    """The page table with contiguous rows."""
+    return page_table if page_table.stride(1) == 1 or page_table.shape[1] <= 1 else page_table.contiguous()
+
+
+def _check_rows(cache, name, x, heads=None):
+    if x.dtype not in (torch.bfloat16, torch.float16) or not (cache.quantized or x.dtype == cache.k_pages.dtype):
+        raise TypeError(f"{name} must be bfloat16 or float16, and of the pages' dtype unless that is float8_e4m3fn")
+    if x.dim() != 3 or x.shape[2] != cache.k_pages.shape[3] or (heads is not None and x.shape[1] != heads):
+        raise ValueError(f"{name} must be [tokens, heads, head_dim] with the cache's head_dim (and, keys and values, its heads)")
+    if x.shape[0] > MAX_TOKENS:
+        raise ValueError(f"at most {MAX_TOKENS} tokens")
+
+
+def paged_append(cache: PagedKVCache, key: torch.Tensor, value: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
+                 cu_new: torch.Tensor, inv_freq: Optional[torch.Tensor] = None, query: Optional[torch.Tensor] = None,
+                 interleaved: bool = False) -> Optional[torch.Tensor]:
+    """The keys and values of new tokens go into the cache; keys, and queries if given, are rotated by their positions first.
+
+    Args:
+        key, value: [tokens, kv_heads, head_dim] bf16 or fp16, the new tokens of all sequences one after the other
+        page_table: [sequences, pages] int32, the pages of every sequence in the order of their tokens (entries behind its
+            last page are not read)
+        lengths: [sequences] int32, tokens of every sequence, the new ones included: the last new token of sequence b has
+            position ``lengths[b] - 1``
+        cu_new: [sequences + 1] int32, 0 and the running sum of the numbers of new tokens; a sequence may have none.  Rows of
+            key and value behind ``cu_new[-1]`` are not read.
+        inv_freq, interleaved: the rotation, as for ``qk_norm_rope``; without inv_freq nothing is rotated
+        query: [tokens, heads, head_dim] of key's dtype, or None
+    Returns:
+        the rotated queries (rows that belong to no sequence: zeros), or None without ``query``.
+
+    The three index tensors stay on the device, and a captured call follows their contents.  A token whose position has no
+    page (beyond the table's row, or an entry that is no page) is not written.  Elements of 8-bit pages are rounded from
+    the rotated 32-bit values; the scale of a page and head is the smallest power of two that takes its largest
+    magnitude into e4m3's range, and where new tokens raise the scale of a page, what it holds is rounded again.  An
+    infinite value is held as the largest number the page has.
+    """
+    hkv, d = cache.k_pages.shape[1], cache.k_pages.shape[3]
+    for name, x in (("key", key), ("value", value)):
+        _check_rows(cache, name, x, hkv)
+    if value.shape != key.shape or value.dtype != key.dtype:
+        raise ValueError("key and value must have one shape and dtype")
+    if query is not None:
+        _check_rows(cache, "query", query)
+        if query.dtype != key.dtype or query.shape[0] != key.shape[0] or not 0 < query.shape[1] <= 65536:
+            raise ValueError("query must have key's dtype and tokens")
+    _check_table(cache, page_table, lengths, cu_new, key.device)
+    if inv_freq is not None:
+        _check_inv_freq(inv_freq, d)
+    if any(t is not None and t.device != key.device for t in (value, query, inv_freq)):
+        raise ValueError("all tensors must be on one device")
+    if not key.is_cuda:
+        raise RuntimeError("paged_append needs tensors on an AMD GPU (there is no CPU path)")
+    tokens, b = key.shape[0], page_table.shape[0]
+    out = None if query is None else torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    if not tokens:
+        return out
+    if not b:
+        return out if out is None else out.zero_()
+    key, value, query = _readable(key), _readable(value), None if query is None else _readable(query)
+    page_table, lengths, cu_new = _table(page_table), lengths.contiguous(), cu_new.contiguous()
+    inv_freq = None if inv_freq is None else inv_freq.contiguous()
+    strides = (ctypes.c_int64 * 7)(*(_strides_of(query) if query is not None else (0, 0)), *_strides_of(key), *_strides_of(value),
+                                   page_table.stride(0))
+    with torch.cuda.device(key.device):
+        _lib.check(_lib.load().moba_paged_append(
+            E._ptr(key), E._ptr(value), E._ptr(query), E._ptr(out), E._ptr(cache.k_pages), E._ptr(cache.v_pages),
+            E._ptr(cache.k_scales), E._ptr(cache.v_scales), E._ptr(page_table), E._ptr(lengths), E._ptr(cu_new),
+            E._ptr(inv_freq), tokens, b, 0 if query is None else query.shape[1], hkv, d,
+            0 if inv_freq is None else 2 * inv_freq.numel(), cache.k_pages.shape[2], cache.k_pages.shape[0],
+            page_table.shape[1], strides, int(cache.quantized), int(interleaved), E._dtype_code(key),
+            E._stream(key.device)), "moba_paged_append")
+    return out

@@ -189,6 +189,22 @@ def test_odd_inputs():
     assert dk.isfinite().all() and not dw.any()
 
 
+def test_elements_that_are_not_turned_stay_alone():
+    """An infinity or a NaN among them reaches no other element, forward or backward."""
+    from moba_amd import qk_norm_rope
+    q, k, dq, dk, positions, _ = make(6, 2, 1, 96, BF16)
+    inv_freq = frequencies(24, "cuda")
+    q[:, 0, 60], q[:, 1, 90], dq[:, 0, 70], dk[:, 0, 64] = float("inf"), float("nan"), float("-inf"), float("nan")
+    leaf, leaf_k = q.clone().requires_grad_(), k.clone().requires_grad_()
+    for interleaved in (False, True):
+        y = qk_norm_rope(leaf, leaf_k, positions, inv_freq, interleaved=interleaved)
+        g = torch.autograd.grad(y, (leaf, leaf_k), (dq, dk))
+        for got, given in ((y[0], q), (y[1], k), (g[0], dq), (g[1], dk)):
+            assert torch.equal(got[..., 48:].isfinite(), given[..., 48:].isfinite()) and got[..., :48].isfinite().all()
+            fine = given[..., 48:].isfinite()
+            assert torch.equal(got[..., 48:][fine], given[..., 48:][fine])
+
+
 def test_same_bits_every_time_on_every_stream_and_in_a_graph():
     from moba_amd import qk_norm_rope
     q, k, dq, dk, positions, weights = make(3000, 8, 2, 128, BF16, seed=7)

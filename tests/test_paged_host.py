@@ -1,0 +1,90 @@
+"""What the paged cache's operators and entry points refuse, before anything is launched (no GPU)."""
+
+import ctypes
+
+import pytest
+import torch
+
+from rotary_reference import frequencies
+
+E4M3, BF16 = torch.float8_e4m3fn, torch.bfloat16
+
+
+def make(dtype=E4M3, pages=3, heads=2, page=16, d=64):
+    from moba_amd import PagedKVCache
+    return PagedKVCache.empty(pages, heads, head_dim=d, page_size=page, dtype=dtype, device="cpu")
+
+
+def test_the_cache_refuses():
+    from moba_amd import PagedKVCache
+    k = torch.zeros((3, 2, 16, 64), dtype=E4M3)
+    s, k16 = torch.ones((3, 2)), torch.zeros((3, 2, 16, 64), dtype=BF16)
+    assert make().quantized and not make(BF16).quantized and make(torch.float16).k_pages.shape == (3, 2, 16, 64)
+    wrong = [
+        (TypeError, (k.float(), k.float())), (TypeError, (k, k16, s, s)), (TypeError, (k, k, s.double(), s)),
+        (TypeError, (k.to(torch.float8_e5m2), k.to(torch.float8_e5m2), s, s)),
+        (ValueError, (k, k)), (ValueError, (k, k, s)), (ValueError, (k16, k16, s, s)), (ValueError, (k, k, s[:2], s)),
+        (ValueError, (k[0], k[0], s, s)), (ValueError, (k, k[:2], s, s)), (ValueError, (k[:, :, :8], k[:, :, :8], s, s)),
+        (ValueError, (k[:0], k[:0], s[:0], s[:0])), (ValueError, (k[:, :0], k[:, :0], s[:, :0], s[:, :0])),
+        (ValueError, (k[..., :32], k[..., :32], s, s)), (ValueError, (k.transpose(0, 1), k.transpose(0, 1), s.T, s.T)),
+        (ValueError, (k, k, s, s.T.contiguous().T)),
+        (ValueError, (torch.zeros(3 * 2 * 16 * 64 + 1, dtype=BF16)[1:].view(3, 2, 16, 64), k16)),
+    ]
+    for error, args in wrong:
+        with pytest.raises(error):
+            PagedKVCache(*args)
+    with pytest.raises(ValueError):
+        make(heads=257)
+
+
+def append_args(**changes):
+    args = dict(cache=make(), key=torch.zeros((5, 2, 64), dtype=BF16), value=torch.zeros((5, 2, 64), dtype=BF16),
+                page_table=torch.zeros((2, 1), dtype=torch.int32), lengths=torch.ones(2, dtype=torch.int32),
+                cu_new=torch.zeros(3, dtype=torch.int32), inv_freq=frequencies(32), query=torch.zeros((5, 4, 64), dtype=BF16))
+    args.update(changes)
+    return args
+
+
+def test_append_refuses():
+    from moba_amd import paged_append
+    with pytest.raises(RuntimeError, match="AMD GPU"):
+        paged_append(**append_args())
+    x, t = torch.zeros((5, 2, 64)), torch.zeros((2, 1), dtype=torch.int32)
+    wrong = [
+        (TypeError, dict(key=x)), (TypeError, dict(value=x)), (TypeError, dict(query=x)), (TypeError, dict(cache=make(torch.float16))),
+        (TypeError, dict(page_table=t.long())), (TypeError, dict(lengths=torch.ones(2))), (TypeError, dict(cu_new=torch.zeros(3).long())),
+        (TypeError, dict(inv_freq=frequencies(32).double())),
+        (ValueError, dict(key=x.to(BF16)[:4])), (ValueError, dict(value=x.half())), (ValueError, dict(query=x.half())),
+        (ValueError, dict(query=x.to(BF16)[:4])), (ValueError, dict(query=x.to(BF16)[:, :0])), (ValueError, dict(key=x.to(BF16)[0])),
+        (ValueError, dict(key=x.to(BF16)[..., :32], value=x.to(BF16)[..., :32])), (ValueError, dict(query=x.to(BF16)[..., :32])),
+        (ValueError, dict(cache=make(heads=3))), (ValueError, dict(cache=make(d=128))),
+        (ValueError, dict(page_table=t[0])), (ValueError, dict(page_table=t[:1])), (ValueError, dict(page_table=t[:, :0])),
+        (ValueError, dict(lengths=t)), (ValueError, dict(lengths=t[:1, 0])), (ValueError, dict(cu_new=torch.zeros(2, dtype=torch.int32))),
+        (ValueError, dict(inv_freq=frequencies(36))), (ValueError, dict(inv_freq=frequencies(30))),
+    ]
+    for error, changes in wrong:
+        with pytest.raises(error):
+            paged_append(**append_args(**changes))
+
+
+def test_append_entry_point_refuses():
+    from moba_amd import _lib
+    lib = _lib.load()
+    some = 256   # (never read)
+
+    def call(k=some, v=some, q=some, yq=some, kp=some, vp=some, ks=some, vs=some, table=some, lengths=some, cu=some, f=some, T=5,
+             B=2, H=4, Hkv=2, D=64, rotary=64, page=16, pool=3, wide=1, strides=(256, 64, 128, 64, 128, 64, 1), cache8=1, dtype=0):
+        s = None if strides is None else (ctypes.c_int64 * 7)(*strides)
+        return lib.moba_paged_append(k, v, q, yq, kp, vp, ks, vs, table, lengths, cu, f, T, B, H, Hkv, D, rotary, page, pool, wide,
+                                     s, cache8, 0, dtype, None)
+
+    for wrong in (dict(k=None), dict(v=None), dict(yq=None), dict(kp=None), dict(vp=None), dict(ks=None), dict(vs=None), dict(table=None),
+                  dict(lengths=None), dict(cu=None), dict(f=None), dict(strides=None), dict(T=0), dict(B=0), dict(H=0), dict(Hkv=0),
+                  dict(rotary=12), dict(rotary=72), dict(rotary=-8), dict(pool=0), dict(wide=0), dict(k=some + 4), dict(q=some + 2),
+                  dict(kp=some + 4), dict(strides=(256, 64, 128, 62, 128, 64, 1))):
+        assert call(**wrong) == -1, wrong
+    for wrong in (dict(D=96), dict(page=48), dict(page=8), dict(page=512), dict(dtype=2)):
+        assert call(**wrong) == -2, wrong
+    for wrong in (dict(T=1 << 30), dict(pool=1 << 31), dict(wide=1 << 31), dict(Hkv=257), dict(H=(1 << 16) + 1), dict(B=1 << 22),
+                  dict(T=(1 << 30) - 1)):
+        assert call(**wrong) == -4, wrong
