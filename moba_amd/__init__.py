@@ -6,11 +6,11 @@ from functools import partial
 from .config import MoBAConfig
 from .moba_efficient import moba_attn_varlen, moba_attn_varlen_gqa
 from .norm_rope import qk_norm_rope
-from .paged import PagedKVCache, paged_append
+from .paged import PagedKVCache, paged_append, paged_attention
 from .wrapper import moba_layer
 
 __all__ = ["MoBAConfig", "register_moba", "moba_attn_varlen", "moba_attn_varlen_gqa", "moba_layer", "qk_norm_rope", "PagedKVCache",
-           "paged_append"]
+           "paged_append", "paged_attention"]
 
 
 def register_moba(cfg: MoBAConfig):

@@ -1,6 +1,6 @@
 """A paged key/value cache on MI355X, with 16-bit elements or 8-bit ones and a scale for every page and head, and the operators on
-it: ``paged_append`` writes the keys and values of new tokens, rotated by position on the way.  Sequences of any lengths are
-served together.  (The reference keeps transformers' contiguous cache, one length for the whole batch, moba/wrapper.py:76-82.)"""
+it: ``paged_append`` writes the keys and values of new tokens, rotated by position on the way, and ``paged_attention`` attends
+them.  Sequences of any lengths and any numbers of new tokens are served together.  (The reference keeps transformers' contiguous cache, one length for the whole batch, moba/wrapper.py:76-82.)"""
 
 from __future__ import annotations
 
@@ -166,3 +166,55 @@ def paged_append(cache: PagedKVCache, key: torch.Tensor, value: torch.Tensor, pa
             page_table.shape[1], strides, int(cache.quantized), int(interleaved), E._dtype_code(key),
             E._stream(key.device)), "moba_paged_append")
     return out
+
+
+def paged_attention(query: torch.Tensor, cache: PagedKVCache, page_table: torch.Tensor, lengths: torch.Tensor, cu_new: torch.Tensor,
+                    scaling: Optional[float] = None, max_new: Optional[int] = None) -> torch.Tensor:
+    """Attention of new tokens over the cache that holds them: full causal attention, as in ``decode_attention``.
+
+    Args:
+        query: [tokens, heads, head_dim] bf16 or fp16, the new tokens of all sequences one after the other; heads a multiple
+            of the cache's.  With 8-bit pages it may be either type.
+        page_table, lengths, cu_new: as for ``paged_append``: row ``cu_new[b + 1] - 1`` of query is token ``lengths[b] - 1`` of
+            sequence b, and every row sees its sequence's tokens up to itself
+        scaling: softmax scale, ``head_dim ** -0.5`` by default
+        max_new: the most new tokens that a sequence has, if that is known: a hint that spares the search for sequences
+            with many (results do not depend on it)
+    Returns:
+        [tokens, heads, head_dim] in query's dtype.  Rows that see no token (those of no sequence, of a sequence without
+        pages) are zeros; a page that the table names wrongly (no page of the pool) holds no tokens.
+    """
+    _check_rows(cache, "query", query)
+    hkv, d = cache.k_pages.shape[1], cache.k_pages.shape[3]
+    tokens, heads = query.shape[:2]
+    if not heads or heads % hkv:
+        raise ValueError("the number of query heads must be a multiple of the number of key/value heads")
+    if max_new is not None and max_new < 0:
+        raise ValueError("max_new must not be negative")
+    _check_table(cache, page_table, lengths, cu_new, query.device)
+    if not query.is_cuda:
+        raise RuntimeError("paged_attention needs tensors on an AMD GPU (there is no CPU path)")
+    b = page_table.shape[0]
+    out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    if not tokens or not b:
+        return out.zero_()
+    lib = _lib.load()
+    if not _addressable(query):
+        query = E._aligned(query)
+    page_table, lengths, cu_new = _table(page_table), lengths.contiguous(), cu_new.contiguous()
+    strides = (ctypes.c_int64 * 3)(*E._row_strides(query), page_table.stride(0))
+    with torch.cuda.device(query.device):
+        space = torch.empty(lib.moba_paged_attention_workspace_bytes(tokens, b, heads, hkv, d, int(cache.quantized)),
+                            dtype=torch.uint8, device=query.device)
+        _lib.check(lib.moba_paged_attention(
+            E._ptr(query), E._ptr(out), E._ptr(cache.k_pages), E._ptr(cache.v_pages), E._ptr(cache.k_scales),
+            E._ptr(cache.v_scales), E._ptr(page_table), E._ptr(lengths), E._ptr(cu_new), E._ptr(space), tokens, b, heads, hkv,
+            d, cache.k_pages.shape[2], cache.k_pages.shape[0], page_table.shape[1], strides, int(cache.quantized),
+            float(scaling) if scaling is not None else d ** -0.5, E._dtype_code(query), E._stream(query.device)),
+            "moba_paged_attention")
+    return out
+
+
+def _addressable(query):
+    ts, hs = E._row_strides(query)
+    return query.stride(2) == 1 and ts % 8 == 0 and hs % 8 == 0 and query.data_ptr() % 16 == 0

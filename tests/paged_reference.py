@@ -158,19 +158,21 @@ def check_query(batch, got, query, inv_freq, interleaved):
 
 def attended(batch, query, scaling=None):
     """[rows, heads, d] in 64 bits: every new token against its sequence's tokens up to itself; rows that see nothing: zeros.
-    Returns also the largest magnitude among the values a row sees, [rows, heads]."""
+    Returns also how far a result in 32 bits may be off, [rows, heads, 1]: with e the error of a score, a probability is off by
+    2e of itself (its own and the sum's), and by 2^-15 for the exponential, the two elements it is split into and the sums; all of
+    it times the largest finite value that the row sees.  e: D roundings of a sum of products, and 2^-22 of the score in the base-2 domain."""
     d, hkv = query.shape[2], batch.pages[0].shape[1]
     rep = query.shape[1] // hkv
     scale = d ** -0.5 if scaling is None else scaling
-    out, size, row = torch.zeros(query.shape, dtype=torch.float64), torch.zeros(query.shape[:2], dtype=torch.float64), 0
+    out, slack, row = torch.zeros(query.shape, dtype=torch.float64), torch.zeros((*query.shape[:2], 1), dtype=torch.float64), 0
     for b, (o, c) in enumerate(zip(batch.old, batch.new)):
         if not c:
             continue
-        length = o + c
-        table = batch.table[b]
+        length, table = o + c, batch.table[b]
         pages = [int(table[i]) if i < table.shape[0] else -1 for i in range(-(-length // batch.page))]
-        there = torch.tensor([0 <= p < batch.pages[0].shape[0] for p in pages]).repeat_interleave(batch.page)[:length]
-        ids = torch.tensor([p if 0 <= p < batch.pages[0].shape[0] else 0 for p in pages])
+        good = [0 <= p < batch.pages[0].shape[0] for p in pages]
+        there = torch.tensor(good).repeat_interleave(batch.page)[:length]
+        ids = torch.tensor([p if g else 0 for p, g in zip(pages, good)])
         kv = []
         for half in range(2):
             x = batch.pages[half][ids].double()
@@ -181,9 +183,25 @@ def attended(batch, query, scaling=None):
             seen = there & (torch.arange(length) <= o + j)
             if not seen.any():
                 continue
-            k, v = (x[seen].repeat_interleave(rep, 1) for x in kv)
-            p = torch.softmax(torch.einsum("hd,khd->hk", query[row + j].double(), k) * scale, -1)
-            out[row + j] = torch.einsum("hk,khd->hd", p, v)
-            size[row + j] = v.abs().amax((0, 2))
+            k, v = (x[seen].transpose(0, 1).repeat_interleave(rep, 0) for x in kv)      # [heads, keys, d]
+            q = query[row + j].double()
+            p = torch.softmax(torch.bmm(k, q[:, :, None])[..., 0] * scale, -1)
+            out[row + j] = torch.bmm(p[:, None], v)[:, 0]
+            size = abs(scale) * q.norm(dim=-1) * k.norm(dim=-1).amax(-1)
+            slack[row + j] = ((2 * (d + 12) * 2.0 ** -24 * size + 2.0 ** -15) * v.where(v.isfinite(), 0).abs().amax((1, 2)))[:, None]
         row += c
-    return out, size
+    return out, slack
+
+
+def check_attention(batch, got, query, scaling=None, extra=0.0):
+    """`extra`: more roundings, relative to the largest value a row sees."""
+    want, slack = attended(batch, query, scaling)
+    got = got.cpu()
+    assert got.dtype == query.dtype and got.shape == query.shape
+    assert torch.equal(got.isnan(), want.isnan()), (got.isnan().sum(), want.isnan().sum())
+    fine = want.isfinite()
+    assert torch.equal(got[~fine & ~want.isnan()].double(), want[~fine & ~want.isnan()])
+    bound = torch.finfo(query.dtype).eps / 2 * 1.001 * want.abs() + slack * (1 + extra / 2.0 ** -15) + 2.0 ** -25
+    off = (got.double() - want).abs()
+    bad = fine & ~(off <= bound)
+    assert not bad.any(), (bad.nonzero()[:5].tolist(), (off / bound)[fine].max().item())

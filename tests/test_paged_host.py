@@ -88,3 +88,52 @@ def test_append_entry_point_refuses():
     for wrong in (dict(T=1 << 30), dict(pool=1 << 31), dict(wide=1 << 31), dict(Hkv=257), dict(H=(1 << 16) + 1), dict(B=1 << 22),
                   dict(T=(1 << 30) - 1)):
         assert call(**wrong) == -4, wrong
+
+
+def test_attention_refuses():
+    from moba_amd import paged_attention
+
+    def call(**changes):
+        args = {k: v for k, v in append_args().items() if k in ("query", "cache", "page_table", "lengths", "cu_new")}
+        args.update(changes)
+        return paged_attention(**args)
+
+    with pytest.raises(RuntimeError, match="AMD GPU"):
+        call()
+    q, t = torch.zeros((5, 4, 64), dtype=BF16), torch.zeros((2, 1), dtype=torch.int32)
+    for error, changes in [
+            (TypeError, dict(query=q.float())), (TypeError, dict(cache=make(torch.float16))), (TypeError, dict(lengths=torch.ones(2))),
+            (TypeError, dict(page_table=t.long())), (ValueError, dict(query=q[:, :3])), (ValueError, dict(query=q[:, :0])),
+            (ValueError, dict(query=q[0])), (ValueError, dict(query=q[..., :32])), (ValueError, dict(page_table=t[0])),
+            (ValueError, dict(page_table=t[:, :0])), (ValueError, dict(cu_new=t[:, 0])), (ValueError, dict(max_new=-1))]:
+        with pytest.raises(error):
+            call(**changes)
+
+
+def test_attention_entry_point_refuses():
+    from moba_amd import _lib
+    lib = _lib.load()
+    some = 256   # (never read)
+
+    def call(q=some, out=some, kp=some, vp=some, ks=some, vs=some, table=some, lengths=some, cu=some, space=some, T=5, B=2, H=4,
+             Hkv=2, D=64, page=16, pool=3, wide=1, strides=(256, 64, 1), cache8=1, dtype=0):
+        s = None if strides is None else (ctypes.c_int64 * 3)(*strides)
+        return lib.moba_paged_attention(q, out, kp, vp, ks, vs, table, lengths, cu, space, T, B, H, Hkv, D, page, pool, wide, s,
+                                        cache8, 0.125, dtype, None)
+
+    for wrong in (dict(q=None), dict(out=None), dict(kp=None), dict(vp=None), dict(ks=None), dict(vs=None), dict(table=None),
+                  dict(lengths=None), dict(cu=None), dict(space=None), dict(strides=None), dict(T=0), dict(B=0), dict(H=0), dict(Hkv=0),
+                  dict(H=5), dict(pool=0), dict(wide=0), dict(q=some + 8), dict(kp=some + 8), dict(space=some + 4), dict(out=some + 4),
+                  dict(strides=(256, 60, 1))):
+        assert call(**wrong) == -1, wrong
+    for wrong in (dict(D=96), dict(page=48), dict(page=512), dict(dtype=2)):
+        assert call(**wrong) == -2, wrong
+    for wrong in (dict(T=1 << 30), dict(T=1 << 29), dict(pool=1 << 31), dict(wide=1 << 31), dict(B=1 << 25, T=1 << 25)):
+        assert call(**wrong) == -4, wrong
+    sizes = lib.moba_paged_attention_workspace_bytes
+    assert sizes(0, 2, 4, 2, 64, 1) == 0 and sizes(5, 2, 5, 2, 64, 1) == 0 and sizes(5, 2, 4, 2, 96, 1) == 0
+    # every unit that several runs can make has rows of 32 (a head's output and its log-sum-exp), and no more than a few rounds
+    # of workgroups do
+    for args in ((1, 1, 32, 8, 128, 1), (64, 64, 32, 8, 128, 0), (1 << 20, 3, 8, 8, 64, 1), (1 << 20, 1 << 20, 8, 1, 64, 1)):
+        need = sizes(*args)
+        assert need % (32 * (args[4] + 1) * 4) == 0 and 0 < need < 400 << 20, args
