@@ -422,13 +422,16 @@ int moba_paged_append(const void* k, const void* v, const void* q, void* yq, voi
  *   q [T,H,D] elem, H a multiple of Hkv; strides {q token, q head, page_table row} in elements, the first two multiples of 8;
  *   out [T,H,D] elem, packed; rows that see no token are zeros.  q, the pages and the workspace 16-byte aligned, out 8-byte.
  *   16-bit pages are of q's type; e4m3 pages (cache8) go with either.
- *   workspace: moba_paged_attention_workspace_bytes(T, B, H, Hkv, D, cache8) bytes
- *   T * H < 2^31 */
-size_t moba_paged_attention_workspace_bytes(int64_t T, int B, int H, int Hkv, int D, int cache8);
+ *   workspace: moba_paged_attention_workspace_bytes(T, B, H, Hkv, D, cache8, max_new) bytes; calls that may run at
+ *   the same time need their own
+ *   max_new: the most new tokens that a sequence has, or -1: a hint that spares a launch for sequences of many
+ *   T < 2^24, T * H < 2^31 */
+size_t moba_paged_attention_workspace_bytes(int64_t T, int B, int H, int Hkv, int D, int cache8, int max_new);
 int moba_paged_attention(const void* q, void* out, const void* k_pages, const void* v_pages, const float* k_scales,
                          const float* v_scales, const int32_t* page_table, const int32_t* lengths, const int32_t* cu_new,
                          void* workspace, int64_t T, int B, int H, int Hkv, int D, int page_size, int64_t num_pages,
-                         int64_t max_pages, const int64_t* strides, int cache8, float scale, int dtype, void* stream);
+                         int64_t max_pages, int max_new, const int64_t* strides, int cache8, float scale, int dtype,
+                         void* stream);
 
 /* Measurement aid, no counterpart in the reference: what the matrix pipes sustain when they do nothing else.
  * Launches `workgroups` workgroups (0: one per compute unit) of eight waves, two per SIMD as in the forward kernel;

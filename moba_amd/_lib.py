@@ -64,8 +64,8 @@ _SIGNATURES = {
     "moba_qk_norm_rope_bwd": (c_int, [c_void_p] * 13 + [c_int64] + [c_int] * 4 + [c_strides] + [c_int] * 3
                                      + [c_float, c_int, c_void_p]),
     "moba_paged_append": (c_int, [c_void_p] * 12 + [c_int64] + [c_int] * 6 + [c_int64] * 2 + [c_strides] + [c_int] * 3 + [c_void_p]),
-    "moba_paged_attention_workspace_bytes": (c_size_t, [c_int64] + [c_int] * 5),
-    "moba_paged_attention": (c_int, [c_void_p] * 10 + [c_int64] + [c_int] * 5 + [c_int64] * 2 + [c_strides, c_int, c_float, c_int,
+    "moba_paged_attention_workspace_bytes": (c_size_t, [c_int64] + [c_int] * 6),
+    "moba_paged_attention": (c_int, [c_void_p] * 10 + [c_int64] + [c_int] * 5 + [c_int64] * 2 + [c_int, c_strides, c_int, c_float, c_int,
                                                                                                c_void_p]),
     "moba_mfma_probe": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p]),
     "moba_tail_splits": (c_int, [c_int] * 5),

@@ -19,7 +19,8 @@
 // one by one, every row with the keys that it sees.  (Rows of a page behind the sequence's end are cleared on the way: they
 // hold whatever was there.)
 //
-//   paged_few_kernel    one run of keys: out itself; several: part_o, part_lse (normalised, log2 domain) of every run
+//   paged_few_kernel    one run of keys: out itself; several: the run's rows (normalised) and their log-sum-exps (base 2)
+//   paged_many_kernel   the same for sequences of more than 32 rows
 //   paged_merge_kernel  the runs of a row together; zeros where there is nothing to see
 #include "attn_common.h"
 #include "paged_cut.h"
@@ -39,13 +40,13 @@ template <class E>
 struct PagedParams {
   typedef typename E::elem elem;
   Shape shape;
-  Cut few;
+  Cut few, many;
   const elem* q;
   elem* out;              // [T, H, D]
   const char* pages[2];
   const float* scales[2];
-  float* part_o;          // [parts * Hkv, group_rows, D]
-  float* part_lse;
+  float *few_o, *few_lse, *many_o, *many_lse;  // [parts * Hkv, group_rows, D] and [.., group_rows]
+  Runs* runs;             // [B]
   int64_t q_tok_stride, q_head_stride;
   float scale_log2;
 };
@@ -77,6 +78,83 @@ template <class V> struct ProbShift { static constexpr float value = 0.f; };
 template <> struct ProbShift<F16> { static constexpr float value = 7.f; };
 constexpr float kMaxLag = 8.f;
 constexpr float kNoMax = -3e38f;  // before the first visible key (finite: exp2(m - m_new) stays defined)
+
+// A wave's keys again, one after the other, in 32 bits and relative to the exact maximum, every row with the keys that it
+// sees only: blocks of 32 keys from key_lo on, `step` apart, up to key_hi.  kSplit: the operands' order of elements is that of
+// 16 bytes of e4m3 to two operands.  Leaves the sum of exponentials in the lower half of the wave.
+template <class E, class V, int D, bool k8, bool kSplit>
+__device__ __forceinline__ void one_by_one(const PagedParams<E>& p, int b, int hkv, int key_lo, int step, int key_hi, int limit,
+                                        const typename E::elem8 (&bq)[D / 16], f32x16 (&oacc)[D / 32], float& m_run, float& l_run) {
+  typedef typename E::elem8 elem8;
+  typedef typename E::elem4 elem4;
+  constexpr int kRowBytes = D * (k8 ? 1 : 2);
+  const int hh = (threadIdx.x & 63) >> 5;
+  const Shape& shape = p.shape;
+  const PageTable& table = shape.table;
+  const int64_t page_bytes = ((int64_t)shape.Hkv << table.page_log2) * kRowBytes;
+  const int64_t head_bytes = ((int64_t)hkv << table.page_log2) * kRowBytes;
+  const int page_mask = (1 << table.page_log2) - 1;
+  auto each_key = [&](auto use) __attribute__((always_inline)) {
+    for (int key0 = key_lo; key0 < key_hi; key0 += step) {
+      for (int key = key0; key < min(key0 + 32, key_hi); ++key) {
+        const int id = __builtin_amdgcn_readfirstlane(page_id(table, b, key >> table.page_log2));
+        if (id < 0) continue;
+        const int64_t at = head_bytes + id * page_bytes + (key & page_mask) * kRowBytes;
+        float d = 0.f, ks = 1.f, vs = 1.f;
+        if constexpr (k8) {
+          ks = p.scales[0][(int64_t)id * shape.Hkv + hkv];
+          vs = p.scales[1][(int64_t)id * shape.Hkv + hkv];
+        }
+#pragma unroll
+        for (int s8 = 0; s8 < D / 16; ++s8) {
+          elem8 x;
+          if constexpr (k8) {
+            const u32x2 w = *reinterpret_cast<const u32x2*>(p.pages[0] + at +
+                                                            (kSplit ? 32 * (s8 >> 1) + 16 * hh + 8 * (s8 & 1) : 16 * s8 + 8 * hh));
+            x = widened(w[0], w[1], E{});
+          } else {
+            x = *reinterpret_cast<const elem8*>(p.pages[0] + at + (16 * s8 + 8 * hh) * 2);
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) d += (float)bq[s8][e] * (float)x[e];
+        }
+        const float sc = sum_xhalf(d) * (p.scale_log2 * ks);
+        if (key <= limit) use(at, sc, vs);
+      }
+    }
+  };
+  m_run = kNoMax;
+  each_key([&](int64_t, float sc, float) __attribute__((always_inline)) { m_run = fmaxf(m_run, sc); });
+  const float ref = m_run - ProbShift<V>::value;
+  float l = 0.f;
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) oacc[db][e] = 0.f;
+  each_key([&](int64_t at, float sc, float vs) __attribute__((always_inline)) {
+    float pe = fast_exp2(sc - ref);
+    l += pe;
+    pe *= vs;
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) {   // (elements 8i + 4hh .. + 3)
+      float x[4];
+      if constexpr (k8) {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(p.pages[1] + at + 8 * i + 4 * hh);
+        x[0] = __builtin_amdgcn_cvt_f32_fp8(w, 0);
+        x[1] = __builtin_amdgcn_cvt_f32_fp8(w, 1);
+        x[2] = __builtin_amdgcn_cvt_f32_fp8(w, 2);
+        x[3] = __builtin_amdgcn_cvt_f32_fp8(w, 3);
+      } else {
+        const elem4 w = *reinterpret_cast<const elem4*>(p.pages[1] + at + (8 * i + 4 * hh) * 2);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = (float)w[e];
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) oacc[i >> 2][4 * (i & 3) + e] += pe * x[e];
+    }
+  });
+  l_run = hh == 0 ? l : 0.f;
+}
 
 template <int D, bool k8>
 constexpr int few_stage_bytes() { return 2 * kFewKeys * D * (k8 ? 1 : 2); }  // K and V of a step
@@ -112,9 +190,10 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void paged_few_kernel(const Page
   if (run == 0) return;   // (no work at all)
   const Unit unit = unit_at(shape, p.few, u, run, lane, first);
   if (unit.b < 0 || (unit.runs > 1 && u >= p.few.parts)) return;   // (the latter: row ranges that are none)
-  const int b = __builtin_amdgcn_readfirstlane(unit.b);
-  const Sequence seq = sequence_of(table, b);
+  const int b = unit.b;
+  const Sequence seq = unit.seq;
   const int keys = keys_of(shape, seq);
+  if (u == unit.first && hkv == 0 && tid == 0) p.runs[b] = {unit.first, unit.runs, unit.groups};
   const int count = seq.hi - seq.lo, rows = count * shape.rep, row0 = unit.group * kFewRows;
   const int per = (unit.tiles + unit.runs - 1) / unit.runs;   // tiles of a run
   const int key_lo = __builtin_amdgcn_readfirstlane((int)min((int64_t)unit.run * per * kFewTile, (int64_t)keys));
@@ -328,68 +407,8 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void paged_few_kernel(const Page
       issue(it + 2);
     }
   }
-  if (__builtin_expect(__any(any_not_finite(oacc)), 0)) {  // (never for values of ordinary size)
-    auto each_key = [&](auto use) __attribute__((always_inline)) {
-      for (int it = 0; it < mine; ++it) {
-        const int key0 = own_lo + it * kFewTile, key1 = min(key0 + kFewKeys, key_hi);
-        for (int key = key0; key < key1; ++key) {
-          const int id = __builtin_amdgcn_readfirstlane(page_id(table, b, key >> table.page_log2));
-          if (id < 0) continue;
-          const int64_t at = head_bytes + id * page_bytes + (key & page_mask) * kRowBytes;
-          float d = 0.f, ks = 1.f, vscale = 1.f;
-          if constexpr (k8) {
-            ks = p.scales[0][(int64_t)id * shape.Hkv + hkv];
-            vscale = p.scales[1][(int64_t)id * shape.Hkv + hkv];
-          }
-#pragma unroll
-          for (int s8 = 0; s8 < kSteps; ++s8) {
-            elem8 x;
-            if constexpr (k8) {
-              const u32x2 w = *reinterpret_cast<const u32x2*>(p.pages[0] + at + 32 * (s8 >> 1) + 16 * hh + 8 * (s8 & 1));
-              x = widened(w[0], w[1], E{});
-            } else {
-              x = *reinterpret_cast<const elem8*>(p.pages[0] + at + (16 * s8 + 8 * hh) * 2);
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) d += (float)bq[s8][e] * (float)x[e];
-          }
-          const float sc = sum_xhalf(d) * (p.scale_log2 * ks);
-          if (key <= limit) use(at, sc, vscale);
-        }
-      }
-    };
-    m_run = kNoMax;
-    each_key([&](int64_t, float sc, float) __attribute__((always_inline)) { m_run = fmaxf(m_run, sc); });
-    const float ref = m_run - ProbShift<V>::value;
-    float l = 0.f;
-#pragma unroll
-    for (int db = 0; db < kDb; ++db)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) oacc[db][e] = 0.f;
-    each_key([&](int64_t at, float sc, float vscale) __attribute__((always_inline)) {
-      float pe = fast_exp2(sc - ref);
-      l += pe;
-      pe *= vscale;
-#pragma unroll
-      for (int i = 0; i < 4 * kDb; ++i) {   // (elements 8i + 4hh .. + 3)
-        float x[4];
-        if constexpr (k8) {
-          const uint32_t w = *reinterpret_cast<const uint32_t*>(p.pages[1] + at + 8 * i + 4 * hh);
-          x[0] = __builtin_amdgcn_cvt_f32_fp8(w, 0);
-          x[1] = __builtin_amdgcn_cvt_f32_fp8(w, 1);
-          x[2] = __builtin_amdgcn_cvt_f32_fp8(w, 2);
-          x[3] = __builtin_amdgcn_cvt_f32_fp8(w, 3);
-        } else {
-          const elem4 w = *reinterpret_cast<const elem4*>(p.pages[1] + at + (8 * i + 4 * hh) * 2);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = (float)w[e];
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) oacc[i >> 2][4 * (i & 3) + e] += pe * x[e];
-      }
-    });
-    l_run = hh == 0 ? l : 0.f;
-  }
+  if (__builtin_expect(__any(any_not_finite(oacc)), 0))  // (never for values of ordinary size)
+    one_by_one<E, V, D, k8, k8>(p, b, hkv, own_lo, kFewTile, key_hi, limit, bq, oacc, m_run, l_run);
   l_run = sum_xhalf(l_run);
 
   // ---- the waves meet in LDS.  Element e of lane (n, hh) is O[row n][32*db + 8*(e/4) + 4*hh + e%4].
@@ -433,60 +452,363 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void paged_few_kernel(const Page
       *reinterpret_cast<u32x2*>(p.out + orow * D + d) = u32x2{pack2<E>(oo[0] * inv, oo[1] * inv), pack2<E>(oo[2] * inv, oo[3] * inv)};
     } else {
       const int64_t prow = (int64_t)blockIdx.x * kFewRows + rr;
-      *reinterpret_cast<f32x4*>(p.part_o + prow * D + d) = f32x4{oo[0] * inv, oo[1] * inv, oo[2] * inv, oo[3] * inv};
-      if (d == 0) p.part_lse[prow] = ll == 0.f ? -INFINITY : mm - ProbShift<V>::value + fast_log2(ll);
+      *reinterpret_cast<f32x4*>(p.few_o + prow * D + d) = f32x4{oo[0] * inv, oo[1] * inv, oo[2] * inv, oo[3] * inv};
+      if (d == 0) p.few_lse[prow] = ll == 0.f ? -INFINITY : mm - ProbShift<V>::value + fast_log2(ll);
     }
   }
 }
 
-// One workgroup per row at a time: four waves take a quarter of the runs each, a lane owns D / 64 elements; the four sums meet
-// in LDS.
+// ---- many rows: bound by the products.  A workgroup of four waves takes 128 rows, 32 to a wave; a tile of 64 keys is brought into
+// LDS once for all of them, two stages, one barrier a tile.  8-bit tiles come through registers, where they become 16-bit
+// elements once for the four waves; 16-bit tiles are copied global -> LDS.  Two workgroups fit a compute unit.
+constexpr int kManyWaves = 4;
+constexpr int kManyRows = 32 * kManyWaves;
+constexpr int kManyKeys = 64;
+
+template <int D>
+constexpr int many_lds_bytes() { return 2 * 2 * kManyKeys * D * 2; }
+
+__device__ __forceinline__ float lane_value(float x, int lane) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane((int)float_bits(x), lane));
+}
+
+// Elements of a probability: one, rounded, of the queries' own precision; where queries are fp16 and the products bf16, two.
+template <class E, class V> struct ProbParts { static constexpr int value = 2; };
+template <class E> struct ProbParts<E, E> { static constexpr int value = 1; };
+
+template <class E, int D, bool k8>
+__global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(const PagedParams<E> p) {
+  MOBA_ELEM_TYPES(E)
+  using V = std::conditional_t<k8, Bf16, E>;
+  typedef typename V::elem velem;
+  typedef typename V::elem4 velem4;
+  typedef typename V::elem8 velem8;
+  constexpr int kParts = ProbParts<E, V>::value;
+  constexpr int kRowBytes = D * 2, kCols = kRowBytes / 16;           // in LDS
+  constexpr int kTileBytes = kManyKeys * kRowBytes, kStage = 2 * kTileBytes;
+  constexpr int kFromRow = D * (k8 ? 1 : 2), kFromCols = kFromRow / 16;   // in the pages
+  constexpr int kPieces = kManyKeys * kFromCols / (64 * kManyWaves);      // 16-byte pieces of a tile of K (or V) of a thread
+  constexpr int kSteps = D / 16, kDb = D / 32;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = lane & 31, hh = lane >> 5;
+  const Shape& shape = p.shape;
+  const PageTable& table = shape.table;
+  const int u = (int)blockIdx.x / shape.Hkv, hkv = (int)blockIdx.x - u * shape.Hkv;
+
+  const Share first = share_at(shape, p.many, lane);
+  const int run = run_tiles(shape, p.many, lane, first);
+  if (run == 0) return;
+  const Unit unit = unit_at(shape, p.many, u, run, lane, first);
+  if (unit.b < 0 || (unit.runs > 1 && u >= p.many.parts)) return;
+  const int b = unit.b;
+  const Sequence seq = unit.seq;
+  const int keys = keys_of(shape, seq);
+  if (u == unit.first && hkv == 0 && tid == 0) p.runs[b] = {unit.first, unit.runs, unit.groups};
+  // (the group with the most keys first)
+  const int count = seq.hi - seq.lo, rows = count * shape.rep, row0 = (unit.groups - 1 - unit.group) * kManyRows;
+  const int per = (unit.tiles + unit.runs - 1) / unit.runs;
+  const int before = (int)seq.length - count;
+  const int last_row = min(row0 + kManyRows, rows) - 1;
+  const int seen = min(keys, max(before + last_row / shape.rep + 1, 0));      // keys that the group's last row sees
+  const int key_lo = (int)min((int64_t)unit.run * per * kManyKeys, (int64_t)seen);
+  const int key_hi = (int)min((int64_t)(unit.run + 1) * per * kManyKeys, (int64_t)seen);
+  const int wave_row = row0 + 32 * wave;
+  const int row = min(wave_row + n, rows - 1);
+  const int j = row / shape.rep, g = row - j * shape.rep;
+  const int limit = min(before + j, key_hi - 1);
+  const int first_masked = min(before + min(wave_row, rows - 1) / shape.rep, key_hi - 1);
+  const int tiles = (key_hi - key_lo + kManyKeys - 1) / kManyKeys;
+  const bool works = wave_row < rows;
+
+  // ---- copies.  Thread i's piece c of a tile is 16 bytes of key (c * 256 + i) / kFromCols
+  const int64_t page_bytes = ((int64_t)shape.Hkv << table.page_log2) * kFromRow;
+  const int64_t head_bytes = ((int64_t)hkv << table.page_log2) * kFromRow;
+  const int page_mask = (1 << table.page_log2) - 1;
+  const uint32_t lds = lds_addr(smem);
+  int ids[kPieces];            // of the tile to be fetched next
+  float scales[2][4] = {};     // 8-bit: K's (times the softmax scale) and V's of the tile's four slots of 16 keys
+  uint32_t there = 0;          // the tile's slots that have a page
+  // lane i: slot i % 4's page and scales of the next tile, page of the one behind it
+  int slot_id = -1, slot_id2 = -1;
+  float slot_scale[2] = {};
+  auto key_of = [&](int c) { return (c * 64 * kManyWaves + tid) / kFromCols; };
+  auto fetch_ids = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+    for (int c = 0; c < kPieces; ++c) {
+      const int64_t key = key_lo + (int64_t)t * kManyKeys + key_of(c);
+      ids[c] = key < key_hi ? page_id(table, b, key >> table.page_log2) : -1;
+    }
+  };
+  auto fetch_slots = [&](int t) __attribute__((always_inline)) {
+    const int64_t key = key_lo + (int64_t)t * kManyKeys + (lane & 3) * kSlot;
+    slot_id2 = key < key_hi ? page_id(table, b, key >> table.page_log2) : -1;
+  };
+  auto fetch_scales = [&]() __attribute__((always_inline)) {
+    slot_id = slot_id2;
+    if constexpr (k8) {
+      const int64_t at = (int64_t)max(slot_id, 0) * shape.Hkv + hkv;
+      slot_scale[0] = p.scales[0][at];
+      slot_scale[1] = p.scales[1][at];
+    }
+  };
+  auto source = [&](int half, int t, int c) __attribute__((always_inline)) {
+    const int in_page = (key_lo + t * kManyKeys + key_of(c)) & page_mask;
+    return p.pages[half] + head_bytes + (ids[c] < 0 ? 0 : ids[c] * page_bytes + in_page * kFromRow);
+  };
+  u32x4 raw[2][k8 ? kPieces : 1];
+  auto fetch = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+      for (int c = 0; c < kPieces; ++c) {
+        if constexpr (k8) {
+          raw[half][c] = *reinterpret_cast<const u32x4*>(source(half, t, c) + (tid % kFromCols) * 16);
+        } else {
+          const int col = swizzled<kRowBytes>(key_of(c), tid % kCols);
+          async_copy16(source(half, t, c) + col * 16, lds + (t & 1) * kStage + half * kTileBytes + (c * kManyWaves + wave) * 1024);
+        }
+      }
+  };
+  auto store = [&](int t) __attribute__((always_inline)) {   // 8-bit: 16 elements to two places of 8
+    if constexpr (k8) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int c = 0; c < kPieces; ++c) {
+          const int key = key_of(c), col = 2 * (tid % kFromCols);
+          const uint32_t to = lds + (t & 1) * kStage + half * kTileBytes + key * kRowBytes;
+          const u32x4 w = raw[half][c];
+          if (half == 0) {
+            *lds_ptr<elem8>(to + (swizzled<kRowBytes>(key, col) << 4)) = widened(w[0], w[1], E{});
+            *lds_ptr<elem8>(to + (swizzled<kRowBytes>(key, col + 1) << 4)) = widened(w[2], w[3], E{});
+          } else {
+            *lds_ptr<velem8>(to + (swizzled<kRowBytes>(key, col) << 4)) = widened(w[0], w[1], V{});
+            *lds_ptr<velem8>(to + (swizzled<kRowBytes>(key, col + 1) << 4)) = widened(w[2], w[3], V{});
+          }
+        }
+    }
+  };
+
+  elem8 bq[kSteps];
+  {
+    const elem* src = p.q + (int64_t)(seq.lo + j) * p.q_tok_stride + (int64_t)(hkv * shape.rep + g) * p.q_head_stride + 8 * hh;
+#pragma unroll
+    for (int s8 = 0; s8 < kSteps; ++s8) bq[s8] = *reinterpret_cast<const elem8*>(src + 16 * s8);
+  }
+  // fragment addresses inside stage 0
+  uint32_t koff[kSteps], voff[2][kDb];
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) koff[i] = lds + n * kRowBytes + (swizzled<kRowBytes>(n, 2 * i + hh) << 4);
+  {
+    const int g16 = lane >> 4, l16 = lane & 15, i0 = l16 >> 2, i1 = l16 & 3, sub = (i1 & 1) * 8;
+#pragma unroll
+    for (int db = 0; db < kDb; ++db)
+#pragma unroll
+      for (int eight = 0; eight < 2; ++eight) {
+        const int key = 4 * hh + i0 + 8 * eight, c16 = 4 * db + 2 * (g16 & 1) + (i1 >> 1);
+        voff[eight][db] = lds + kTileBytes + key * kRowBytes + (swizzled<kRowBytes>(key, c16) << 4) + sub;
+      }
+  }
+  f32x16 oacc[kDb];
+#pragma unroll
+  for (int db = 0; db < kDb; ++db)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) oacc[db][e] = 0.f;
+  float m_run = kNoMax, l_run = 0.f;
+
+  auto score = [&](uint32_t st, int blk, f32x16& s) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[e] = 0.f;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) s = mfma32(*lds_ptr<const elem8>(koff[i] + st + blk * 32 * kRowBytes), bq[i], s);
+  };
+  auto block = [&](uint32_t st, int key0, int blk, f32x16& s) __attribute__((always_inline)) {
+    velem8 va[2][kDb];
+#pragma unroll
+    for (int j2 = 0; j2 < 2; ++j2)
+#pragma unroll
+      for (int db = 0; db < kDb; ++db) {
+        const uint32_t at = st + (32 * blk + kSlot * j2) * kRowBytes;
+        const velem4 x = lds_read_tr<velem4>(voff[0][db] + at), y = lds_read_tr<velem4>(voff[1][db] + at);
+        va[j2][db] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+      }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[e] *= k8 ? scales[0][2 * blk + (e >> 3)] : p.scale_log2;
+    const uint32_t has = (there >> (2 * blk)) & 3;
+    const bool edge = key0 + 31 > first_masked || has != 3;
+    if (edge) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (key0 + 8 * (e >> 2) + 4 * hh + (e & 3) > limit || !(has & (1 << (e >> 3)))) s[e] = -INFINITY;
+    }
+    float mx = s[0];
+#pragma unroll
+    for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[e]);
+    mx = max_xhalf(mx);
+    if (__any(mx > m_run + kMaxLag)) {
+      const float m_new = mx > m_run + kMaxLag ? mx : m_run;
+      const float alpha = fast_exp2(m_run - m_new);
+      m_run = m_new;
+      l_run *= alpha;
+#pragma unroll
+      for (int db = 0; db < kDb; ++db)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) oacc[db][e] *= alpha;
+    }
+    const float ref = m_run - ProbShift<V>::value;
+    velem8 hi[2], lo[2];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      float pe = fast_exp2(s[e] - ref);
+      l_run += pe;
+      if constexpr (k8) pe *= scales[1][2 * blk + (e >> 3)];
+      const velem h = (velem)pe;
+      hi[e >> 3][e & 7] = h;
+      if constexpr (kParts == 2) lo[e >> 3][e & 7] = (velem)(pe - (float)h);
+    }
+    if (edge) {
+#pragma unroll
+      for (int j2 = 0; j2 < 2; ++j2)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (key0 + kSlot * j2 + 8 * (i >> 2) + 4 * hh + (i & 3) >= key_hi || !(has & (1 << j2))) {
+#pragma unroll
+            for (int db = 0; db < kDb; ++db) va[j2][db][i] = (velem)0.f;
+          }
+    }
+#pragma unroll
+    for (int j2 = 0; j2 < 2; ++j2)
+#pragma unroll
+      for (int db = 0; db < kDb; ++db) oacc[db] = mfma32(va[j2][db], hi[j2], oacc[db]);
+    if constexpr (kParts == 2) {
+#pragma unroll
+      for (int j2 = 0; j2 < 2; ++j2)
+#pragma unroll
+        for (int db = 0; db < kDb; ++db) oacc[db] = mfma32(va[j2][db], lo[j2], oacc[db]);
+    }
+  };
+
+  if (tiles > 0) {
+    fetch_ids(0);
+    fetch_slots(0);
+    fetch(0);
+    fetch_scales();
+    fetch_ids(1);
+    fetch_slots(1);
+    store(0);
+    if constexpr (!k8) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  }
+  for (int t = 0; t < tiles; ++t) {
+    __syncthreads();   // tile t is complete, and nobody reads tile t - 1 any more
+    const uint32_t st = (t & 1) * kStage;
+    there = (uint32_t)__ballot(slot_id >= 0) & 15;
+    if constexpr (k8) {
+#pragma unroll
+      for (int slot = 0; slot < 4; ++slot) {
+        scales[0][slot] = lane_value(slot_scale[0], slot) * p.scale_log2;
+        scales[1][slot] = lane_value(slot_scale[1], slot);
+      }
+    }
+    if (t + 1 < tiles) {
+      fetch(t + 1);
+      fetch_scales();
+      fetch_ids(t + 2);
+      fetch_slots(t + 2);
+    }
+    const int key0 = key_lo + t * kManyKeys;
+    if (works) {
+      f32x16 s0, s1;
+      score(st, 0, s0);
+      score(st, 1, s1);
+      block(st, key0, 0, s0);
+      block(st, key0 + 32, 1, s1);
+    }
+    if (t + 1 < tiles) {
+      store(t + 1);
+      if constexpr (!k8) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+  }
+  if (!works) return;   // (no barrier follows)
+  if (__builtin_expect(__any(any_not_finite(oacc)), 0))
+    one_by_one<E, V, D, k8, false>(p, b, hkv, key_lo, 32, key_hi, limit, bq, oacc, m_run, l_run);
+  l_run = sum_xhalf(l_run);
+  if (wave_row + n >= rows) return;
+  const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+  if (unit.runs == 1) {
+    elem* to = p.out + ((int64_t)(seq.lo + j) * shape.H + hkv * shape.rep + g) * D + 4 * hh;
+#pragma unroll
+    for (int i = 0; i < 4 * kDb; ++i) {
+      const f32x16& o = oacc[i >> 2];
+      const int e = 4 * (i & 3);
+      *reinterpret_cast<u32x2*>(to + 8 * i) = u32x2{pack2<E>(o[e] * inv, o[e + 1] * inv), pack2<E>(o[e + 2] * inv, o[e + 3] * inv)};
+    }
+  } else {
+    const int64_t prow = (int64_t)blockIdx.x * kManyRows + 32 * wave + n;
+#pragma unroll
+    for (int i = 0; i < 4 * kDb; ++i) {
+      const f32x16& o = oacc[i >> 2];
+      const int e = 4 * (i & 3);
+      *reinterpret_cast<f32x4*>(p.many_o + prow * D + 8 * i + 4 * hh) = f32x4{o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv};
+    }
+    if (hh == 0) p.many_lse[prow] = l_run == 0.f ? -INFINITY : m_run - ProbShift<V>::value + fast_log2(l_run);
+  }
+}
+
+// A workgroup takes `heads` heads of a token, one after the other: four waves take a quarter of the runs each, a lane owns
+// D / 64 elements; the four sums meet in LDS.  Rows of one run are there already.
 template <class E, int D>
-__global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams<E> p) {
+__global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams<E> p, int heads) {
   typedef typename E::elem elem;
   constexpr int kPer = D / 64;
+  typedef float fvec __attribute__((ext_vector_type(kPer)));
   __shared__ float red[4][D];
   __shared__ float red_l[4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Shape& shape = p.shape;
   const PageTable& table = shape.table;
-  const Share first = share_at(shape, p.few, lane);
-  const int run = run_tiles(shape, p.few, lane, first);
-  for (int64_t row = blockIdx.x; row < (int64_t)table.T * shape.H; row += gridDim.x) {
-    const int t = (int)(row / shape.H), h = (int)(row - (int64_t)t * shape.H);
-    const int hkv = h / shape.rep, g = h - hkv * shape.rep;
-    const int b = count_up_to(table.B, t, lane, [&](int i) { return (int64_t)table.cu_new[i + 1]; });
-    int runs = 0, group = 0, groups = 0;
-    int64_t unit0 = 0;
-    int rr = 0;
-    if (b < table.B) {
-      const Sequence seq = sequence_of(table, b);
-      const Share s = share_of(shape, p.few, seq);
-      if (s.groups && t >= seq.lo && t < seq.hi) {
-        runs = runs_of(s.tiles, run);
-        groups = s.groups;
-        const int r = (t - seq.lo) * shape.rep + g;
-        group = r / kFewRows;
-        rr = r - group * kFewRows;
-        unit0 = first_unit(shape, p.few, b, run, lane, first);
-      }
+  const int per_token = shape.H / heads;
+  const int t = (int)blockIdx.x / per_token, h0 = ((int)blockIdx.x - t * per_token) * heads;
+  const int b = count_up_to(table.B, t, lane, [&](int i) { return (int64_t)table.cu_new[i + 1]; });
+  Runs r = {0, 0, 0};
+  bool is_many = false;
+  int row_in_seq = 0;
+  if (b < table.B) {
+    const Sequence seq = sequence_of(table, b);
+    if (keys_of(shape, seq) > 0 && t >= seq.lo && t < seq.hi) {   // (its units have left their numbers)
+      r = p.runs[b];
+      if (r.runs == 1) return;
+      is_many = (seq.hi - seq.lo) * shape.rep > p.many.rows_over && p.many.most > 0;
+      row_in_seq = (t - seq.lo) * shape.rep;
     }
-    if (runs == 1) continue;   // (written by its one run; the same in the whole workgroup)
-    if (unit0 + (int64_t)runs * groups > p.few.parts) runs = 0;   // (row ranges that are none)
-    auto part = [&](int i) { return ((unit0 + (int64_t)i * groups + group) * shape.Hkv + hkv) * kFewRows + rr; };
+  }
+  const Cut& cut = is_many ? p.many : p.few;
+  const float* const part_o = is_many ? p.many_o : p.few_o;
+  const float* const part_lse = is_many ? p.many_lse : p.few_lse;
+  // (numbers that no unit has left, where the row ranges are none)
+  if (r.first < 0 || r.runs < 0 || r.groups < 1 || r.first + (int64_t)r.runs * r.groups > cut.parts) r.runs = 0;
+  for (int h = h0; h < h0 + heads; ++h) {
+    const int hkv = h / shape.rep, row = row_in_seq + h - hkv * shape.rep;
+    int group = row / cut.group_rows;
+    const int rr = row - group * cut.group_rows;
+    if (is_many) group = r.groups - 1 - group;
+    if (group < 0 || group >= r.groups) r.runs = 0;
+    auto part = [&](int i) { return ((r.first + (int64_t)i * r.groups + group) * shape.Hkv + hkv) * cut.group_rows + rr; };
     float mm = -INFINITY;
-    for (int i = lane; i < runs; i += 64) mm = fmaxf(mm, p.part_lse[part(i)]);
+    for (int i = lane; i < r.runs; i += 64) mm = fmaxf(mm, part_lse[part(i)]);
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) mm = fmaxf(mm, __shfl_xor(mm, o, 64));
     const float top = mm == -INFINITY ? 0.f : mm;
     float ll = 0.f, o[kPer] = {};
 #pragma unroll 4
-    for (int i = wave; i < runs; i += 4) {
+    for (int i = wave; i < r.runs; i += 4) {
       const int64_t at = part(i);
-      const float w = fast_exp2(p.part_lse[at] - top);
+      const float w = fast_exp2(part_lse[at] - top);
+      const fvec x = *reinterpret_cast<const fvec*>(part_o + at * D + kPer * lane);
       ll += w;
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) o[e] += w * p.part_o[at * D + kPer * lane + e];
+      for (int e = 0; e < kPer; ++e) o[e] += w * x[e];
     }
 #pragma unroll
     for (int e = 0; e < kPer; ++e) red[wave][kPer * lane + e] = o[e];
@@ -495,7 +817,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams<E> p
     if (threadIdx.x < D) {
       const int d = threadIdx.x;
       const float l4 = red_l[0] + red_l[1] + red_l[2] + red_l[3];
-      p.out[row * D + d] = (elem)(l4 == 0.f ? 0.f : (red[0][d] + red[1][d] + red[2][d] + red[3][d]) / l4);
+      p.out[((int64_t)t * shape.H + h) * D + d] = (elem)(l4 == 0.f ? 0.f : (red[0][d] + red[1][d] + red[2][d] + red[3][d]) / l4);
     }
     __syncthreads();
   }
@@ -508,7 +830,10 @@ using namespace moba;
 // Bounds of a cut's units, for any division of T tokens among B sequences of any lengths: n groups (of every sequence
 // with rows, ceil(rows / group_rows)) in runs of work / left tiles are at most left + n units (run_tiles()).
 static Cut bounded_cut(Cut c, int64_t T, int B, int rep) {
-  const int64_t groups = (T < B ? T : B) + T * rep / c.group_rows;
+  // (of a cut with rows_over, at most T * rep / (rows_over + 1) sequences)
+  const int64_t with_rows = c.rows_over ? T * rep / (c.rows_over + 1) : T, sequences = with_rows < B ? with_rows : B;
+  // (one group each where no sequence has more rows than a group)
+  const int64_t groups = sequences + (c.rows_up_to > c.group_rows ? T * rep / c.group_rows : 0);
   const int64_t several = groups < (int64_t)kWholeAt * c.target ? groups : (int64_t)kWholeAt * c.target;
   const int64_t parts = c.target / 2 + 1 + several > c.target ? c.target / 2 + 1 + several : c.target;
   const int64_t most = groups > parts ? groups : parts;
@@ -517,49 +842,73 @@ static Cut bounded_cut(Cut c, int64_t T, int B, int rep) {
   return c;
 }
 
-// The cut of the few-row kernel: one round of workgroups, two to a compute unit with 8-bit pages and with narrow heads.
-static Cut few_cut(int64_t T, int B, int rep, int Hkv, int D, bool cache8) {
+// One round of workgroups, two to a compute unit (one where a wave's blocks are large).  Sequences of more than 32 rows per
+// key/value head go to the many-row kernel, if it is launched: if there may be any.
+struct Cuts {
+  Cut few, many;
+};
+static Cuts paged_cuts(int64_t T, int B, int rep, int Hkv, int D, bool cache8, int max_new) {
   const int cus = compute_units() > 0 ? compute_units() : 256;
-  const int slots = cus * (D == 128 && !cache8 ? 1 : 2);
-  return bounded_cut({kFewRows, kFewTile, 0, 0x7fffffff, slots / Hkv > 0 ? slots / Hkv : 1, 0, 0}, T, B, rep);
+  auto target = [&](int per_cu) { return per_cu * cus / Hkv > 0 ? per_cu * cus / Hkv : 1; };
+  const int64_t most_new = max_new >= 0 && max_new < T ? max_new : T;
+  Cuts c;
+  const bool many = most_new * rep > kFewRows;
+  c.few = bounded_cut({kFewRows, kFewTile, 0, many ? kFewRows : 0x7fffffff, target(D == 128 && !cache8 ? 1 : 2), 0, 0}, T, B, rep);
+  c.many = {};
+  if (many) c.many = bounded_cut({kManyRows, kManyKeys, kFewRows, 0x7fffffff, target(2), 0, 0}, T, B, rep);
+  return c;
 }
 
 static bool paged_sizes_ok(int64_t T, int B, int H, int Hkv) {
   return T > 0 && B > 0 && H > 0 && Hkv > 0 && H % Hkv == 0;
 }
 static int64_t part_rows(const Cut& c, int Hkv) { return (int64_t)c.parts * Hkv * c.group_rows; }
+static int64_t runs_bytes(int B) { return ((int64_t)B * sizeof(Runs) + 15) / 16 * 16; }
 
-extern "C" size_t moba_paged_attention_workspace_bytes(int64_t T, int B, int H, int Hkv, int D, int cache8) {
+extern "C" size_t moba_paged_attention_workspace_bytes(int64_t T, int B, int H, int Hkv, int D, int cache8, int max_new) {
   if (!paged_sizes_ok(T, B, H, Hkv) || (D != 64 && D != 128)) return 0;
-  return (size_t)part_rows(few_cut(T, B, H / Hkv, Hkv, D, cache8 != 0), Hkv) * (D + 1) * sizeof(float);
+  const Cuts c = paged_cuts(T, B, H / Hkv, Hkv, D, cache8 != 0, max_new);
+  return (size_t)runs_bytes(B) + (size_t)(part_rows(c.few, Hkv) + part_rows(c.many, Hkv)) * (D + 1) * sizeof(float);
 }
 
 template <class E, int D, bool k8>
 static int launch_paged(const PagedParams<E>& p, hipStream_t st) {
   LaunchCheck launch_check;
-  static bool allowed[kMaxDevices];
-  const auto kernel = paged_few_kernel<E, D, k8>;
-  if (!allow_dynamic_lds((const void*)kernel, few_lds_bytes<D, k8>(), allowed)) return MOBA_ERR_LAUNCH;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)p.few.most * p.shape.Hkv), dim3(64 * kFewWaves), (few_lds_bytes<D, k8>()), st, p);
+  static bool allowed[2][kMaxDevices];
+  const auto few = paged_few_kernel<E, D, k8>;
+  if (!allow_dynamic_lds((const void*)few, few_lds_bytes<D, k8>(), allowed[0])) return MOBA_ERR_LAUNCH;
+  hipLaunchKernelGGL(few, dim3((unsigned)p.few.most * p.shape.Hkv), dim3(64 * kFewWaves), (few_lds_bytes<D, k8>()), st, p);
+  if (p.many.most > 0) {
+    const auto many = paged_many_kernel<E, D, k8>;
+    if (!allow_dynamic_lds((const void*)many, many_lds_bytes<D>(), allowed[1])) return MOBA_ERR_LAUNCH;
+    hipLaunchKernelGGL(many, dim3((unsigned)p.many.most * p.shape.Hkv), dim3(64 * kManyWaves), many_lds_bytes<D>(), st, p);
+  }
   const int64_t rows = (int64_t)p.shape.table.T * p.shape.H;
-  hipLaunchKernelGGL((paged_merge_kernel<E, D>), dim3((unsigned)(rows < 8192 ? rows : 8192)), dim3(256), 0, st, p);
+  const int heads = rows <= 8192 ? 1 : p.shape.H;
+  hipLaunchKernelGGL((paged_merge_kernel<E, D>), dim3((unsigned)(rows / heads)), dim3(256), 0, st, p, heads);
   return launch_check.result();
 }
 
 template <class E>
 static int paged_attention(const void* q, void* out, const void* k_pages, const void* v_pages, const float* k_scales,
-                           const float* v_scales, const PageTable& table, float* workspace, int H, int Hkv, int D,
+                           const float* v_scales, const PageTable& table, char* workspace, int H, int Hkv, int D, int max_new,
                            const int64_t* strides, int cache8, float scale, hipStream_t st) {
   typedef typename E::elem elem;
   PagedParams<E> p = {};
   p.shape = {table, H, Hkv, H / Hkv};
-  p.few = few_cut(table.T, table.B, p.shape.rep, Hkv, D, cache8 != 0);
-  if ((int64_t)p.few.most * Hkv >= 1LL << 24) return MOBA_ERR_LIMIT;   // (threads of a launch: 32 bits)
+  const Cuts cuts = paged_cuts(table.T, table.B, p.shape.rep, Hkv, D, cache8 != 0, max_new);
+  p.few = cuts.few;
+  p.many = cuts.many;
+  const int64_t most = p.few.most > p.many.most ? p.few.most : p.many.most;
+  if (most * Hkv >= 1LL << 24 || table.T >= 1 << 24) return MOBA_ERR_LIMIT;   // (threads of a launch: 32 bits)
   p.q = (const elem*)q; p.out = (elem*)out;
   p.pages[0] = (const char*)k_pages; p.pages[1] = (const char*)v_pages;
   p.scales[0] = k_scales; p.scales[1] = v_scales;
-  p.part_o = workspace;
-  p.part_lse = workspace + part_rows(p.few, Hkv) * D;
+  p.runs = (Runs*)workspace;
+  p.few_o = (float*)(workspace + runs_bytes(table.B));
+  p.few_lse = p.few_o + part_rows(p.few, Hkv) * D;
+  p.many_o = p.few_lse + part_rows(p.few, Hkv);
+  p.many_lse = p.many_o + part_rows(p.many, Hkv) * D;
   p.q_tok_stride = strides[0]; p.q_head_stride = strides[1];
   p.scale_log2 = scale * 1.4426950408889634f;
   if (D == 128) return cache8 ? launch_paged<E, 128, true>(p, st) : launch_paged<E, 128, false>(p, st);
@@ -570,8 +919,8 @@ static int paged_attention(const void* q, void* out, const void* k_pages, const 
 extern "C" int moba_paged_attention(const void* q, void* out, const void* k_pages, const void* v_pages, const float* k_scales,
                                     const float* v_scales, const int32_t* page_table, const int32_t* lengths,
                                     const int32_t* cu_new, void* workspace, int64_t T, int B, int H, int Hkv, int D, int page_size,
-                                    int64_t num_pages, int64_t max_pages, const int64_t* strides, int cache8, float scale,
-                                    int dtype, void* stream) {
+                                    int64_t num_pages, int64_t max_pages, int max_new, const int64_t* strides, int cache8,
+                                    float scale, int dtype, void* stream) {
   if (!q || !out || !k_pages || !v_pages || !page_table || !lengths || !cu_new || !workspace || !strides) return MOBA_ERR_ARG;
   if (!paged_sizes_ok(T, B, H, Hkv) || num_pages <= 0 || max_pages <= 0 || (cache8 && (!k_scales || !v_scales))) return MOBA_ERR_ARG;
   const int page_log2 = page_log2_of(page_size);
@@ -586,8 +935,8 @@ extern "C" int moba_paged_attention(const void* q, void* out, const void* k_page
                            (int)(max_pages < reachable ? max_pages : reachable), page_log2};
   hipStream_t st = (hipStream_t)stream;
   return dtype == MOBA_DTYPE_F16
-             ? paged_attention<F16>(q, out, k_pages, v_pages, k_scales, v_scales, table, (float*)workspace, H, Hkv, D, strides,
-                                    cache8, scale, st)
-             : paged_attention<Bf16>(q, out, k_pages, v_pages, k_scales, v_scales, table, (float*)workspace, H, Hkv, D, strides,
-                                     cache8, scale, st);
+             ? paged_attention<F16>(q, out, k_pages, v_pages, k_scales, v_scales, table, (char*)workspace, H, Hkv, D, max_new,
+                                    strides, cache8, scale, st)
+             : paged_attention<Bf16>(q, out, k_pages, v_pages, k_scales, v_scales, table, (char*)workspace, H, Hkv, D, max_new,
+                                     strides, cache8, scale, st);
 }

@@ -4,7 +4,7 @@
 // neither the sequences' lengths nor how their new tokens are divided (both may change between replays of a captured
 // call), so every workgroup finds its own unit: the runs are as long as fills the chip once with the whole batch's work,
 // and the units of the sequences are counted through.  A long sequence among short ones gets the units that its keys ask for.
-// One wave looks at 64 sequences at a time: up to 64 of them the whole cut is a load and a few dozen instructions.
+// One wave looks at 64 sequences at a time: up to 64 of them the whole cut is one load and some hundred cycles.
 #pragma once
 #include "paged.h"
 
@@ -20,35 +20,46 @@ struct Cut {
   int parts;       // no more than this of them where there is a sequence of several runs
 };
 constexpr int kWholeRun = 0x3fffffff;  // tiles
-constexpr int kWholeAt = 4;  // with this many times `target` groups and more, a sequence's keys are one run
+constexpr int kWholeAt = 4;            // with this many times `target` groups and more, a sequence's keys are one run
 
 struct Shape {
   PageTable table;
   int H, Hkv, rep;
 };
 
+// A sequence's part in a cut: groups of rows (0: none of its units are of this cut), tiles of keys
 struct Share {
-  int groups, tiles;  // of one sequence: groups of rows, tiles of keys (groups 0: not of this cut)
+  Sequence seq;
+  int groups, tiles;
 };
 __device__ __forceinline__ int keys_of(const Shape& p, const Sequence& s) { return (int)min(s.length, room(p.table)); }
 __device__ __forceinline__ Share share_of(const Shape& p, const Cut& c, const Sequence& s) {
-  const int rows = (s.hi - s.lo) * p.rep;
+  const int rows = (s.hi - s.lo) * p.rep, keys = keys_of(p, s);
   Share r;
-  r.tiles = (keys_of(p, s) - 1) / c.tile_keys + 1;
-  if (s.length == 0) r.tiles = 0;
-  r.groups = rows > c.rows_over && rows <= c.rows_up_to && r.tiles > 0 ? (rows - 1) / c.group_rows + 1 : 0;
+  r.seq = s;
+  r.tiles = keys > 0 ? (keys - 1) / c.tile_keys + 1 : 0;
+  r.groups = rows > c.rows_over && rows <= c.rows_up_to && keys > 0 ? (rows - 1) / c.group_rows + 1 : 0;
   return r;
 }
+// of sequence b, each lane its own
 __device__ __forceinline__ Share share_at(const Shape& p, const Cut& c, int b) {
-  if (b >= p.table.B) return {0, 0};
+  if (b >= p.table.B) return {{0, 0, 0}, 0, 0};
   return share_of(p, c, sequence_of(p.table, b));
 }
 
-__device__ __forceinline__ int64_t wave_sum(int64_t x) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor(x, o, 64);
+// sum of x over the lanes up to this one (wrapping)
+__device__ __forceinline__ uint32_t upto_sum(uint32_t x) {
+#define MOBA_DPP_ADD(ctrl, rows) x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, ctrl, rows, 0xf, false)
+  MOBA_DPP_ADD(0x111, 0xf);  // from 1, 2, 4, 8 lanes below in the row of 16
+  MOBA_DPP_ADD(0x112, 0xf);
+  MOBA_DPP_ADD(0x114, 0xf);
+  MOBA_DPP_ADD(0x118, 0xf);
+  MOBA_DPP_ADD(0x142, 0xa);  // a row's last lane to the row above
+  MOBA_DPP_ADD(0x143, 0xc);  // lane 31 to the upper half
+#undef MOBA_DPP_ADD
   return x;
 }
+__device__ __forceinline__ uint32_t wave_sum(uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)upto_sum(x), 63); }
 
 // Tiles of a run.  With work = sum of groups * tiles and n = sum of groups, runs of work / (target - n) tiles come to
 // at most `target` units (each group's last run may be short); where the groups alone are more than half the target,
@@ -57,19 +68,21 @@ __device__ __forceinline__ int run_tiles(const Shape& p, const Cut& c, int lane,
   int64_t work = 0, groups = 0;
   for (int b0 = 0; b0 < p.table.B; b0 += 64) {
     const Share s = b0 ? share_at(p, c, b0 + lane) : first;
-    work += (int64_t)s.groups * s.tiles;
-    groups += s.groups;
+    const int64_t w = (int64_t)s.groups * s.tiles;   // (below 2^56: in pieces of 24 bits a wave's sum fits 32)
+    work += wave_sum((uint32_t)w & 0xffffff) + ((int64_t)wave_sum((uint32_t)(w >> 24) & 0xffffff) << 24) +
+            ((int64_t)wave_sum((uint32_t)(w >> 48)) << 48);
+    groups += wave_sum(s.groups);
   }
-  work = wave_sum(work);
-  groups = wave_sum(groups);
   if (groups >= (int64_t)kWholeAt * c.target) return kWholeRun;
   const int64_t left = max(max((int64_t)c.target - groups, (int64_t)c.target / 2), (int64_t)1);
+  if (work < 1LL << 31) return (int)(((uint32_t)work + (uint32_t)left - 1) / (uint32_t)left);   // (64-bit division is slow)
   return (int)min((work + left - 1) / left, (int64_t)kWholeRun);
 }
 __device__ __forceinline__ int runs_of(int tiles, int run) { return (tiles - 1) / run + 1; }
 
 struct Unit {
-  int b, group, run, runs, tiles;  // tiles: of the sequence
+  Sequence seq;
+  int b, group, run, runs, groups, tiles, first;  // tiles: of the sequence; first: number of the sequence's first unit
 };
 // unit number u: all groups of a sequence's first run, then of its second, ...  b = -1 past the last
 __device__ __forceinline__ Unit unit_at(const Shape& p, const Cut& c, int u, int run, int lane, const Share& first) {
@@ -77,38 +90,36 @@ __device__ __forceinline__ Unit unit_at(const Shape& p, const Cut& c, int u, int
   for (int b0 = 0; b0 < p.table.B; b0 += 64) {
     const Share s = b0 ? share_at(p, c, b0 + lane) : first;
     const int runs = s.groups ? runs_of(s.tiles, run) : 0;
-    const int64_t mine = (int64_t)s.groups * runs;
-    int64_t upto = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int64_t below = __shfl_up(upto, o, 64);
-      if (lane >= o) upto += below;
-    }
-    const uint64_t m = __ballot(base + upto > u);
+    const uint32_t mine = (uint32_t)s.groups * runs, upto = upto_sum(mine);
+    const uint64_t m = __ballot(base + upto > u && mine > 0);
     if (m) {
       const int at = __ffsll((unsigned long long)m) - 1;
+      auto of = [&](int x) { return __builtin_amdgcn_readlane(x, at); };
       Unit r;
       r.b = b0 + at;
-      r.runs = __shfl(runs, at, 64);
-      r.tiles = __shfl(s.tiles, at, 64);
-      const int groups = __shfl(s.groups, at, 64);
-      const int rest = (int)(u - (base + __shfl(upto - mine, at, 64)));
-      r.run = rest / groups;
-      r.group = rest - r.run * groups;
+      r.seq.lo = of(s.seq.lo);
+      r.seq.hi = of(s.seq.hi);
+      r.seq.length = of((int)s.seq.length);
+      r.runs = of(runs);
+      r.groups = of(s.groups);
+      r.tiles = of(s.tiles);
+      r.first = (int)(base + (uint32_t)of((int)(upto - mine)));
+      const int rest = u - r.first;
+      r.run = rest / r.groups;
+      r.group = rest - r.run * r.groups;
+      if (rest < 0 || r.run >= r.runs) r.b = -1;   // (row ranges that are none: more units than 32 bits number)
       return r;
     }
-    base += __shfl(upto, 63, 64);
+    base += (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
   }
-  return {-1, 0, 0, 0, 0};
+  Unit none = {};
+  none.b = -1;
+  return none;
 }
-// number of the first unit of sequence b
-__device__ __forceinline__ int64_t first_unit(const Shape& p, const Cut& c, int b, int run, int lane, const Share& first) {
-  int64_t n = 0;
-  for (int b0 = 0; b0 < b; b0 += 64) {
-    const Share s = b0 ? share_at(p, c, b0 + lane) : first;
-    if (b0 + lane < b && s.groups) n += (int64_t)s.groups * runs_of(s.tiles, run);
-  }
-  return wave_sum(n);
-}
+
+// What the merge has to know of a sequence, left for it by the sequence's first unit
+struct Runs {
+  int first, runs, groups;
+};
 
 }  // namespace moba

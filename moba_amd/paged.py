@@ -187,6 +187,8 @@ def paged_attention(query: torch.Tensor, cache: PagedKVCache, page_table: torch.
     _check_rows(cache, "query", query)
     hkv, d = cache.k_pages.shape[1], cache.k_pages.shape[3]
     tokens, heads = query.shape[:2]
+    if tokens >= 1 << 24 or tokens * heads >= 1 << 31:
+        raise ValueError("at most 2^24 - 1 tokens, and fewer than 2^31 rows")
     if not heads or heads % hkv:
         raise ValueError("the number of query heads must be a multiple of the number of key/value heads")
     if max_new is not None and max_new < 0:
@@ -203,13 +205,14 @@ def paged_attention(query: torch.Tensor, cache: PagedKVCache, page_table: torch.
         query = E._aligned(query)
     page_table, lengths, cu_new = _table(page_table), lengths.contiguous(), cu_new.contiguous()
     strides = (ctypes.c_int64 * 3)(*E._row_strides(query), page_table.stride(0))
+    hint = -1 if max_new is None else min(max_new, tokens)
     with torch.cuda.device(query.device):
-        space = torch.empty(lib.moba_paged_attention_workspace_bytes(tokens, b, heads, hkv, d, int(cache.quantized)),
+        space = torch.empty(lib.moba_paged_attention_workspace_bytes(tokens, b, heads, hkv, d, int(cache.quantized), hint),
                             dtype=torch.uint8, device=query.device)
         _lib.check(lib.moba_paged_attention(
             E._ptr(query), E._ptr(out), E._ptr(cache.k_pages), E._ptr(cache.v_pages), E._ptr(cache.k_scales),
             E._ptr(cache.v_scales), E._ptr(page_table), E._ptr(lengths), E._ptr(cu_new), E._ptr(space), tokens, b, heads, hkv,
-            d, cache.k_pages.shape[2], cache.k_pages.shape[0], page_table.shape[1], strides, int(cache.quantized),
+            d, cache.k_pages.shape[2], cache.k_pages.shape[0], page_table.shape[1], hint, strides, int(cache.quantized),
             float(scaling) if scaling is not None else d ** -0.5, E._dtype_code(query), E._stream(query.device)),
             "moba_paged_attention")
     return out

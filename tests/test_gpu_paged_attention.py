@@ -26,6 +26,13 @@ CASES = [  # old, new, page, heads, kv heads, head_dim, dtype, quantized, rows b
     ([70000, 100], [1, 1], 64, 8, 2, 128, BF16, True, 0),                   # runs of more keys than pages are looked up at a time
     ([70000], [2], 16, 4, 4, 64, FP16, False, 0),
     ([0], [130], 32, 4, 2, 128, BF16, False, 0),
+    ([100, 3, 0, 500], [200, 1, 129, 9], 64, 8, 2, 128, BF16, True, 1),     # many rows and few in one batch
+    ([100, 3, 0, 500], [200, 1, 129, 9], 16, 8, 2, 64, FP16, True, 0),
+    ([100, 3, 0, 500], [200, 1, 129, 9], 256, 6, 2, 128, FP16, False, 0),
+    ([100, 3, 0, 500], [200, 1, 129, 9], 32, 9, 3, 64, BF16, False, 0),
+    ([3000], [40], 16, 4, 1, 128, FP16, True, 0),                           # many rows, few groups: several runs each
+    ([3001, 2222], [33, 70], 128, 5, 5, 128, BF16, False, 0),
+    ([63], [65], 16, 1, 1, 128, BF16, True, 0),
 ]
 
 

@@ -116,10 +116,10 @@ def test_attention_entry_point_refuses():
     some = 256   # (never read)
 
     def call(q=some, out=some, kp=some, vp=some, ks=some, vs=some, table=some, lengths=some, cu=some, space=some, T=5, B=2, H=4,
-             Hkv=2, D=64, page=16, pool=3, wide=1, strides=(256, 64, 1), cache8=1, dtype=0):
+             Hkv=2, D=64, page=16, pool=3, wide=1, hint=-1, strides=(256, 64, 1), cache8=1, dtype=0):
         s = None if strides is None else (ctypes.c_int64 * 3)(*strides)
-        return lib.moba_paged_attention(q, out, kp, vp, ks, vs, table, lengths, cu, space, T, B, H, Hkv, D, page, pool, wide, s,
-                                        cache8, 0.125, dtype, None)
+        return lib.moba_paged_attention(q, out, kp, vp, ks, vs, table, lengths, cu, space, T, B, H, Hkv, D, page, pool, wide, hint,
+                                        s, cache8, 0.125, dtype, None)
 
     for wrong in (dict(q=None), dict(out=None), dict(kp=None), dict(vp=None), dict(ks=None), dict(vs=None), dict(table=None),
                   dict(lengths=None), dict(cu=None), dict(space=None), dict(strides=None), dict(T=0), dict(B=0), dict(H=0), dict(Hkv=0),
@@ -128,12 +128,13 @@ def test_attention_entry_point_refuses():
         assert call(**wrong) == -1, wrong
     for wrong in (dict(D=96), dict(page=48), dict(page=512), dict(dtype=2)):
         assert call(**wrong) == -2, wrong
-    for wrong in (dict(T=1 << 30), dict(T=1 << 29), dict(pool=1 << 31), dict(wide=1 << 31), dict(B=1 << 25, T=1 << 25)):
+    for wrong in (dict(T=1 << 30), dict(T=1 << 29), dict(T=1 << 24), dict(pool=1 << 31), dict(wide=1 << 31), dict(B=1 << 25, T=1 << 25)):
         assert call(**wrong) == -4, wrong
     sizes = lib.moba_paged_attention_workspace_bytes
-    assert sizes(0, 2, 4, 2, 64, 1) == 0 and sizes(5, 2, 5, 2, 64, 1) == 0 and sizes(5, 2, 4, 2, 96, 1) == 0
-    # every unit that several runs can make has rows of 32 (a head's output and its log-sum-exp), and no more than a few rounds
-    # of workgroups do
+    assert sizes(0, 2, 4, 2, 64, 1, -1) == 0 and sizes(5, 2, 5, 2, 64, 1, -1) == 0 and sizes(5, 2, 4, 2, 96, 1, -1) == 0
+    # rows (a head's output and its log-sum-exp) for every unit that several runs can make, and these are no more than a few
+    # rounds of workgroups; a hint that there are few new tokens leaves out those of the other kernel
     for args in ((1, 1, 32, 8, 128, 1), (64, 64, 32, 8, 128, 0), (1 << 20, 3, 8, 8, 64, 1), (1 << 20, 1 << 20, 8, 1, 64, 1)):
-        need = sizes(*args)
-        assert need % (32 * (args[4] + 1) * 4) == 0 and 0 < need < 400 << 20, args
+        need, less = sizes(*args, -1), sizes(*args, 1)
+        runs = (args[1] * 12 + 15) // 16 * 16
+        assert (need - runs) % (32 * (args[4] + 1) * 4) == 0 and 0 < less <= need < 2 << 30, args
