@@ -146,6 +146,7 @@ def host():
             raise RuntimeError(f"{module.__file__} was built for PyTorch {built_for}, this is {torch.__version__}: rebuild it with "
                                "`python -m moba_amd.build`")
         bind(module, lib.moba_tail)
+        bind_layer(module)
         _host = module
     return _host
 
@@ -154,6 +155,14 @@ def bind(module, tail):
     """Give the extension module the library's entry points, with `tail` for moba_tail."""
     lib = load()
     module.bind(*(ctypes.cast(f, c_void_p).value for f in (lib.moba_version, lib.moba_tail_splits, tail, lib.moba_strerror)))
+
+
+def bind_layer(module, **instead):
+    """Give the extension module the entry points of the operators around the attention, `instead` in the place of some."""
+    lib = load()
+    names = ("moba_qk_norm_rope", "moba_qk_norm_rope_bwd", "moba_qk_norm_rope_bwd_workspace_bytes", "moba_paged_append",
+             "moba_paged_attention", "moba_paged_attention_workspace_bytes", "moba_strerror")
+    module.bind_layer(*(ctypes.cast(instead.get(n, getattr(lib, n)), c_void_p).value for n in names))
 
 
 def exported_symbols():

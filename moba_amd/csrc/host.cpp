@@ -18,6 +18,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../include/moba_hip.h"
+#include "host_layer.h"
 
 namespace {
 
@@ -154,6 +155,10 @@ PyMethodDef methods[] = {
     {"supported", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_supported)), METH_FASTCALL, nullptr},
     {"tail", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_tail)), METH_FASTCALL, nullptr},
     {"in_place", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_in_place)), METH_FASTCALL, nullptr},
+    {"norm_rope", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_norm_rope)), METH_FASTCALL, nullptr},
+    {"paged_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_paged_append)), METH_FASTCALL, nullptr},
+    {"paged_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_paged_attention)), METH_FASTCALL, nullptr},
+    {"bind_layer", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_bind_layer)), METH_FASTCALL, nullptr},
     {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_bind)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -138,6 +138,10 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_
         the new q and k, packed.  Differentiable once in q, k and the weights; the weights' gradients are summed in a fixed
         order (the same bits on every run).
     """
+    y = _lib.host().norm_rope(q, k, positions, inv_freq, q_weight, k_weight, eps, interleaved)
+    if y is not NotImplemented:
+        return y
+    # tensors that have to be copied first, none at all, or wrong ones
     _check(q, k, positions, inv_freq, q_weight, k_weight, eps)
     positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
     tensors = (q, k, q_weight, k_weight)

@@ -21,7 +21,7 @@ MAX_KV_HEADS = 256
 MAX_TOKENS = (1 << 30) - 1   # packed rows of a call
 
 
-@dataclass
+@dataclass(frozen=True)
 class PagedKVCache:
     """The pages of one layer.
 
@@ -130,6 +130,11 @@ def paged_append(cache: PagedKVCache, key: torch.Tensor, value: torch.Tensor, pa
     magnitude into e4m3's range, and where new tokens raise the scale of a page, what it holds is rounded again.  An
     infinite value is held as the largest number the page has.
     """
+    out = _lib.host().paged_append(cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales, key, value, page_table, lengths,
+                                   cu_new, inv_freq, query, interleaved)
+    if out is not NotImplemented:
+        return out
+    # tensors that have to be copied first, none at all, or wrong ones
     hkv, d = cache.k_pages.shape[1], cache.k_pages.shape[3]
     for name, x in (("key", key), ("value", value)):
         _check_rows(cache, name, x, hkv)
@@ -184,6 +189,11 @@ def paged_attention(query: torch.Tensor, cache: PagedKVCache, page_table: torch.
         [tokens, heads, head_dim] in query's dtype.  Rows that see no token (those of no sequence, of a sequence without
         pages) are zeros; a page that the table names wrongly (no page of the pool) holds no tokens.
     """
+    out = _lib.host().paged_attention(cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales, query, page_table, lengths,
+                                      cu_new, scaling, max_new)
+    if out is not NotImplemented:
+        return out
+    # tensors that have to be copied first, none at all, or wrong ones
     _check_rows(cache, "query", query)
     hkv, d = cache.k_pages.shape[1], cache.k_pages.shape[3]
     tokens, heads = query.shape[:2]

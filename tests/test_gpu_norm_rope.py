@@ -69,6 +69,7 @@ CASES = [  # tokens, heads, kv heads, head_dim, rotated pairs, interleaved, dtyp
     (33, 1, 1, 24, 8, True, FP16, FP16, 0),
     (1000, 8, 2, 128, 64, False, BF16, "", 0),
     (301, 17, 1, 72, 36, False, FP16, "q", 0),
+    (40, 3, 2, 64, 32, False, BF16, "k", 0),
     (5003, 8, 2, 128, 64, False, BF16, BF16, 0),
     (9000, 4, 4, 64, 32, True, FP16, FP32, 1 << 17),
 ]
@@ -79,6 +80,8 @@ def weights_of(weights, dtype, kind):
         return [None, None]
     if kind == "q":
         return [weights[0].to(dtype), None]
+    if kind == "k":
+        return [None, weights[1].to(dtype)]
     return [w.to(kind) for w in weights]
 
 
@@ -278,3 +281,43 @@ def test_refusals_on_the_gpu():
     g, = torch.autograd.grad(y, leaf, torch.ones_like(y).requires_grad_(), create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(g.float().sum(), leaf)
+
+
+def test_the_general_path_gives_the_same(monkeypatch):
+    """The native call takes contiguous tensors and views alike; what it leaves to the Python path is computed the same."""
+    from moba_amd import _lib, qk_norm_rope
+    q, k, dq, dk, positions, weights = make(70, 6, 2, 128, FP16, seed=2)
+    inv_freq, native = frequencies(32, "cuda"), _lib.host().norm_rope
+    taken = []
+
+    def both():
+        leaves = [x.detach().requires_grad_() for x in (q, k, *weights)]
+        y = qk_norm_rope(*leaves[:2], positions, inv_freq, *leaves[2:], interleaved=True)
+        taken.append(type(y[0].grad_fn).__name__)
+        return [*(v.detach() for v in y), *torch.autograd.grad(y, leaves, (dq, dk)), *qk_norm_rope(q, k, positions, inv_freq)]
+
+    want = both()
+    monkeypatch.setattr(_lib.host(), "norm_rope", lambda *a: NotImplemented)
+    got = both()
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and taken[0] != taken[1]
+    monkeypatch.setattr(_lib.host(), "norm_rope", native)
+    for args in ((q[:0], k[:0], positions[:0], inv_freq), (q, k.cpu(), positions, inv_freq), (q.float(), k, positions, inv_freq),
+                 (q, k, positions[:5], inv_freq), (q, k, positions, inv_freq[:3]), (q, k, positions.view(1, -1), inv_freq)):
+        assert native(*args, None, None, 1e-6, False) is NotImplemented
+    with pytest.raises(TypeError):
+        native(q, k)
+
+
+def test_the_native_call_lets_other_threads_run():
+    """In the entry point's place stands CPython's own PyGILState_Check, whose answer -- 1 with the lock -- would be an error code."""
+    import ctypes
+    from moba_amd import _lib, qk_norm_rope
+    q, k, _, _, positions, _ = make(4, 2, 1, 64, BF16)
+    try:
+        _lib.bind_layer(_lib.host(), moba_qk_norm_rope=ctypes.pythonapi.PyGILState_Check)
+        assert qk_norm_rope(q, k, positions, frequencies(32, "cuda"))[0].shape == q.shape
+        _lib.bind_layer(_lib.host(), moba_qk_norm_rope=ctypes.pythonapi.Py_IsInitialized)     # (1: an error)
+        with pytest.raises(RuntimeError, match="moba_qk_norm_rope failed with code 1"):
+            qk_norm_rope(q, k, positions, frequencies(32, "cuda"))
+    finally:
+        _lib.bind_layer(_lib.host())

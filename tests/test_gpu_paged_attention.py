@@ -229,3 +229,47 @@ def test_serving(quantized):
             packed = moba_attn_varlen_gqa(q, k, v, batch.cu.cuda(), 150, 1024, 3)
             assert (packed.float() - out.float()).abs().max() < 2e-2
         batch.old = [o + n for o, n in zip(batch.old, batch.new)]
+
+
+def test_the_general_path_gives_the_same(monkeypatch):
+    """What the native calls leave to the Python path -- tensors to be copied first -- is computed the same."""
+    from moba_amd import _lib, paged_append, paged_attention
+    host = _lib.host()
+    native = {name: getattr(host, name) for name in ("paged_append", "paged_attention")}
+    for quantized, d in ((True, 128), (False, 64)):
+        batch = Batch([100, 3, 70], [1, 50, 4], 32, 2, d, BF16, quantized, seed=3)
+        q, k, v = (x.cuda() for x in batch.tensors(6, 2, 2))
+        index, inv_freq, got = batch.index(), frequencies(16, "cuda"), []
+        for general in (False, True):
+            for name, f in native.items():
+                monkeypatch.setattr(host, name, (lambda *a: NotImplemented) if general else f)
+            cache = batch.cache()
+            turned = paged_append(cache, k, v, *index, inv_freq=inv_freq, query=q, interleaved=True)
+            got.append([turned, cache.k_pages.view(torch.uint8), cache.v_pages.view(torch.uint8), paged_attention(turned, cache, *index),
+                        paged_attention(turned, cache, *index, scaling=0.2, max_new=50)])
+        assert all(torch.equal(a, b) for a, b in zip(*got))
+        fields = (cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales)
+        append = lambda k=k, v=v, i=index, f=inv_freq, q=q: native["paged_append"](*fields, k, v, *i, f, q, False)  # noqa: E731
+        attend = lambda q=q, i=index, hint=None: native["paged_attention"](*fields, q, *i, None, hint)  # noqa: E731
+        short, flat = (index[0], index[1][:2], index[2]), (index[0][0], *index[1:])
+        for args in (dict(k=k[:5]), dict(k=k.cpu()), dict(v=v.float()), dict(q=q[:, :0]), dict(q=q[:4]), dict(f=inv_freq[:3]),
+                     dict(i=short), dict(i=flat), dict(k=k[..., ::2]), dict(k=k[:0], v=v[:0], q=q[:0])):
+            assert append(**args) is NotImplemented, args.keys()
+        for args in (dict(q=q[:0]), dict(q=q[:, :5]), dict(q=q.cpu()), dict(q=q[..., ::2]), dict(i=short), dict(i=flat), dict(hint=-1)):
+            assert attend(**args) is NotImplemented, args.keys()
+
+
+def test_the_native_calls_let_other_threads_run():
+    """In the entry points' places stands CPython's own PyGILState_Check, whose answer -- 1 with the lock -- would be an error code."""
+    import ctypes
+    from moba_amd import _lib, paged_append, paged_attention
+    batch = Batch([10], [1], 16, 2, 64, BF16, True)
+    q, k = (x.cuda() for x in batch.tensors(4, 2))
+    check = ctypes.pythonapi.PyGILState_Check
+    try:
+        _lib.bind_layer(_lib.host(), moba_paged_append=check, moba_paged_attention=check)
+        assert paged_append(batch.cache(), k, k, *batch.index(), query=q).shape == q.shape
+        assert paged_attention(q, batch.cache(), *batch.index()).shape == q.shape
+    finally:
+        _lib.bind_layer(_lib.host())
+    check_attention(batch, paged_attention(q, batch.cache(), *batch.index()), q.cpu())
