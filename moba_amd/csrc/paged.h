@@ -60,6 +60,27 @@ __device__ __forceinline__ int count_up_to(int n, int64_t x, int lane, Value val
   return count;
 }
 
+// The last sequence b with start(b, cu_new[b]) <= x, for ascending starts, its row range and length, found by the lanes of a
+// wave together with one round of loads for every 64 sequences; b = -1 if there is none.
+template <class Start>
+__device__ __forceinline__ int last_up_to(const PageTable& t, int64_t x, int lane, Sequence& seq, Start start) {
+  int found = -1;
+  for (int b0 = 0; b0 < t.B; b0 += 64) {
+    const int b = min(b0 + lane, t.B - 1);
+    const Sequence s = sequence_of(t, b);
+    const uint64_t m = __ballot(b0 + lane < t.B && start(b, s.lo) <= x);
+    if (m) {
+      const int at = 63 - __builtin_clzll(m);
+      found = b0 + at;
+      seq.lo = __builtin_amdgcn_readlane(s.lo, at);
+      seq.hi = __builtin_amdgcn_readlane(s.hi, at);
+      seq.length = __builtin_amdgcn_readlane((int)s.length, at);
+    }
+    if (~m) break;
+  }
+  return found;
+}
+
 inline int page_log2_of(int page_size) {
   for (int l = kLeastPageLog2; l <= kMostPageLog2; ++l)
     if (page_size == 1 << l) return l;

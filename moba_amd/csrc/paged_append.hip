@@ -8,7 +8,7 @@
 // that fall below e4m3's normal numbers (2^-15 of the page's range), and the division exact always.
 //
 // Bound by memory for prompts (each element is read once from memory; the second reading, after the page's maximum is known,
-// comes from L2), by latency for single tokens: the angles of the page's tokens are made once for all heads, by all
+// comes from L2; held in registers instead, two heads to a workgroup, a 131072-token prompt took 863 us instead of 640), by latency for single tokens: the angles of the page's tokens are made once for all heads, by all
 // waves, and wait in LDS.
 #include "paged.h"
 #include "rotary.h"
@@ -17,8 +17,9 @@ namespace moba {
 
 constexpr int kAppendWaves = 8;
 constexpr int kAngleTokens = 64;   // tokens whose angles lie in LDS at a time
-constexpr int kQueryTokens = 16;   // tokens of a workgroup that rotates queries
+constexpr int kQueryTokens = 16;   // tokens of a workgroup that rotates queries, at most
 constexpr int kMostHeads = 256;    // key/value heads
+constexpr int kKeep = 1;           // rows of a lane that stay in registers between the two passes: those of single tokens
 
 template <class E>
 struct AppendParams {
@@ -31,7 +32,8 @@ struct AppendParams {
   float* scales[2];      // 8-bit pages
   const float* inv_freq;
   int64_t tok_stride[2], head_stride[2], q_tok_stride, q_head_stride;
-  int H, Hkv, rotary, interleaved, items;
+  int H, Hkv, rotary, interleaved;
+  int items, query_tokens;  // pages; tokens of a workgroup that rotates queries
 };
 
 // the smallest power of two s with a <= 448 s
@@ -58,6 +60,18 @@ __device__ __forceinline__ uint32_t rescaled(uint32_t w, float by) {
                    __builtin_amdgcn_cvt_f32_fp8(w, 2) * by, __builtin_amdgcn_cvt_f32_fp8(w, 3) * by);
 }
 
+// the largest of a value over the G lanes of a row, in every one of them
+template <int G>
+__device__ __forceinline__ float row_max(float x) {
+#define MOBA_DPP_MAX(ctrl) x = fmaxf(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, (int)float_bits(x), ctrl, 0xf, 0xf, false)))
+  MOBA_DPP_MAX(0xB1);
+  MOBA_DPP_MAX(0x4E);
+  MOBA_DPP_MAX(0x141);
+  if constexpr (G == 16) MOBA_DPP_MAX(0x140);
+#undef MOBA_DPP_MAX
+  return x;
+}
+
 struct Angles {
   float2 cs[kAngleTokens][64];
 };
@@ -73,8 +87,21 @@ __device__ __forceinline__ Turn turn_from(const Angles& a, int token, int u, boo
   return t;
 }
 
+// a lane's two groups of a row, as they are in memory
+template <class E>
+__device__ __forceinline__ u32x4 load_raw(const typename E::elem* row, const RowPlace& p) {
+  const u32x2 a = *reinterpret_cast<const u32x2*>(row + p.a), b = *reinterpret_cast<const u32x2*>(row + p.b);
+  return u32x4{a[0], a[1], b[0], b[1]};
+}
+template <class E>
+__device__ __forceinline__ void unpack(const u32x4& w, float (&x)[8]) {
+  const typename E::elem8 v = __builtin_bit_cast(typename E::elem8, w);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = (float)v[i];
+}
+
 template <class E, int D, bool k8>
-__global__ __launch_bounds__(64 * kAppendWaves) void paged_append_kernel(const AppendParams<E> p) {
+__global__ __launch_bounds__(64 * kAppendWaves, 6) void paged_append_kernel(const AppendParams<E> p) {
   constexpr int G = D / 8, kRows = 64 / G;       // lanes of a row, rows of a wave
   constexpr int kStep = kAppendWaves * kRows;    // rows of the workgroup
   __shared__ Angles angles;
@@ -94,11 +121,12 @@ __global__ __launch_bounds__(64 * kAppendWaves) void paged_append_kernel(const A
     }
   };
 
-  if ((int)blockIdx.x >= p.items) {  // ---- queries: kQueryTokens tokens, all heads
-    const int t0 = ((int)blockIdx.x - p.items) * kQueryTokens, count = min(kQueryTokens, table.T - t0);
+  if ((int)blockIdx.x >= p.items) {  // ---- queries: all heads of some tokens
+    const int t0 = ((int)blockIdx.x - p.items) * p.query_tokens, count = min(p.query_tokens, table.T - t0);
     for (int i = wave; i < count; i += kAppendWaves) {
-      const int b = count_up_to(table.B, t0 + i, lane, [&](int j) { return (int64_t)table.cu_new[j + 1]; });
-      if (lane == 0) place[i] = b < table.B ? (int64_t)table.lengths[b] - table.cu_new[b + 1] + t0 + i : INT64_MIN;
+      Sequence seq;
+      const int b = last_up_to(table, t0 + i, lane, seq, [](int, int lo) { return (int64_t)lo; });
+      if (lane == 0) place[i] = b >= 0 && t0 + i < seq.hi ? seq.length - seq.hi + t0 + i : INT64_MIN;
     }
     __syncthreads();
     make_angles(count, [&](int i) { return place[i]; });
@@ -116,70 +144,103 @@ __global__ __launch_bounds__(64 * kAppendWaves) void paged_append_kernel(const A
   }
 
   // ---- a page: which sequence's, and which of the pages that its new tokens touch.  Sequence b's take the items from
-  // (cu_new[b] >> page_log2) + 2b on, at least as many as its tokens can touch
-  const int item = blockIdx.x;
-  auto first_item = [&](int b) { return (int64_t)(min(max(table.cu_new[b], 0), table.T) >> table.page_log2) + 2 * b; };
-  const int b = count_up_to(table.B, item, lane, first_item) - 1;
-  if (b < 0) return;
-  const Sequence seq = sequence_of(table, b);
+  // (first row >> page_log2) + 2b on, at least as many as its tokens can touch
+  const int item = blockIdx.x, heads = p.Hkv;
+  auto first_item = [&](int b, int lo) { return (int64_t)(lo >> table.page_log2) + 2 * b; };
+  Sequence seq = {0, 0, 0};
+  const int b = last_up_to(table, item, lane, seq, first_item);
+  if (b < 0 || seq.hi == seq.lo) return;
   const int64_t begin = seq.length - (seq.hi - seq.lo);   // position of row seq.lo
-  const int64_t page = (max(begin, (int64_t)0) >> table.page_log2) + (item - first_item(b));
+  const int64_t page = (max(begin, (int64_t)0) >> table.page_log2) + (item - first_item(b, seq.lo));
   const int64_t first = page << table.page_log2;
   const int from = (int)(max(begin, first) - first);      // the page's new tokens: from .. to - 1
   const int to = (int)min(seq.length - first, (int64_t)1 << table.page_log2);
-  if (seq.hi == seq.lo || to <= from) return;
+  if (to <= from) return;
+  const int count = to - from, piece0 = min(kAngleTokens, count);
+  const int64_t row_of_first = seq.lo - begin + first;    // row of the page's token 0, were it new
+  const typename E::elem* const source[2] = {p.x[0] + (row_of_first + from) * p.tok_stride[0],
+                                             p.x[1] + (row_of_first + from) * p.tok_stride[1]};
+  auto raw = [&](int half, int i, int h) __attribute__((always_inline)) {   // token `from` + i, head h
+    return load_raw<E>(source[half] + i * p.tok_stride[half] + h * p.head_stride[half], at);
+  };
+  // the lane's first row is on their way while the page is looked up and the angles are made
+  u32x4 kept[kKeep][2];
+#pragma unroll
+  for (int s = 0; s < kKeep; ++s) {
+    const int r = row0 + s * kStep, i = r / heads;
+    if (r < piece0 * heads) {
+      kept[s][0] = raw(0, i, r - i * heads);
+      kept[s][1] = raw(1, i, r - i * heads);
+    }
+  }
   const int id = page_id(table, b, page);
   if (id < 0) return;
-  const int64_t row_of_first = seq.lo - begin + first;    // row of the page's token 0, were it new
-  const int count = to - from;
   constexpr int kBytes = k8 ? 1 : 2;
   const int64_t page_bytes = ((int64_t)p.Hkv << table.page_log2) * D * kBytes;
+  char* const target[2] = {p.pages[0] + id * page_bytes, p.pages[1] + id * page_bytes};
+  auto row_at = [&](int half, int token, int h) { return target[half] + ((h << table.page_log2) + token) * (D * kBytes); };
 
-  for (int i = tid; i < 2 * p.Hkv; i += 64 * kAppendWaves) most[i >= p.Hkv][i >= p.Hkv ? i - p.Hkv : i] = 0;
+  float former = 0.f;   // thread i: the scale of half i / heads, head i % heads, if the page holds tokens
+  float* scale = nullptr;
+  if constexpr (k8) {
+    if (tid < 2 * heads) {
+      const int half = tid >= heads, h = half ? tid - heads : tid;
+      scale = p.scales[half] + (int64_t)id * heads + h;
+      if (from > 0) former = *scale;
+      most[half][h] = 0;
+    }
+  }
   const bool in_pieces = count > kAngleTokens;
   for (int pass = k8 ? 0 : 1; pass < 2; ++pass) {
     for (int c0 = 0; c0 < count; c0 += kAngleTokens) {
       const int piece = min(kAngleTokens, count - c0);
       if (pass == (k8 ? 0 : 1) || in_pieces) {
-        __syncthreads();   // (the angles before have been read)
-        make_angles(piece, [&](int i) { return first + from + c0 + i; });
+        __syncthreads();   // (the angles before have been read; the maxima are cleared)
+        if (p.rotary) make_angles(piece, [&](int i) { return first + from + c0 + i; });
         __syncthreads();
       }
-      for (int r = row0; r < piece * p.Hkv; r += kStep) {
-        const int i = r / p.Hkv, h = r - i * p.Hkv;
-        const int token = from + c0 + i;
-        const int64_t row = row_of_first + token;
+      auto row = [&](const u32x4 (&w)[2], int i, int h) __attribute__((always_inline)) {
         float x[2][8];
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-          load_row<E>(p.x[half] + row * p.tok_stride[half] + h * p.head_stride[half], at, x[half]);
-        turn_row(x[0], turn_from(angles, i, u, at.turned), p.interleaved);
+        unpack<E>(w[0], x[0]);
+        unpack<E>(w[1], x[1]);
+        if (at.turned) turn_row(x[0], turn_from(angles, i, u, true), p.interleaved);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          if (pass == 0) {
+          if (k8 && pass == 0) {
             float m = 0.f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               const float a = fabsf(x[half][e]);
               m = fmaxf(m, a < INFINITY ? a : 0.f);
             }
-#pragma unroll
-            for (int o = 1; o < G; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+            m = row_max<G>(m);
             if (u == 0) atomicMax(&most[half][h], float_bits(m));
+          } else if constexpr (k8) {
+            store_row8(row_at(half, from + c0 + i, h), at, x[half], over[half][h]);
           } else {
-            char* to_row = p.pages[half] + id * page_bytes + (((int64_t)h << table.page_log2) + token) * (D * kBytes);
-            if constexpr (k8) store_row8(to_row, at, x[half], over[half][h]);
-            else store_row<E>((typename E::elem*)to_row, at, x[half]);
+            store_row<E>((typename E::elem*)row_at(half, from + c0 + i, h), at, x[half]);
           }
         }
+      };
+      int done = 0;
+      if (c0 == 0) {
+#pragma unroll
+        for (int s = 0; s < kKeep; ++s) {
+          const int r = row0 + s * kStep, i = r / heads;
+          if (r < piece * heads) row(kept[s], i, r - i * heads);
+        }
+        done = kKeep * kStep;
+      }
+      for (int r = row0 + done; r < piece * heads; r += kStep) {
+        const int i = r / heads, h = r - i * heads;
+        const u32x4 w[2] = {raw(0, c0 + i, h), raw(1, c0 + i, h)};
+        row(w, i, h);
       }
     }
     if (pass == 1) break;
     __syncthreads();   // the maxima are complete
-    for (int i = tid; i < 2 * p.Hkv; i += 64 * kAppendWaves) {
-      const int half = i >= p.Hkv, h = half ? i - p.Hkv : i;
-      float* scale = p.scales[half] + (int64_t)id * p.Hkv + h;
-      const float former = from > 0 ? *scale : 0.f;
+    if (scale) {
+      const int half = tid >= heads, h = half ? tid - heads : tid;
       const float s = fmaxf(page_scale(__builtin_bit_cast(float, most[half][h])), former);
       over[half][h] = 1.f / s;
       again[half][h] = former > 0.f && s > former ? former / s : 0.f;
@@ -187,13 +248,13 @@ __global__ __launch_bounds__(64 * kAppendWaves) void paged_append_kernel(const A
     }
     __syncthreads();
     // tokens that the page holds, where a scale grew
-    for (int r = row0; r < from * p.Hkv; r += kStep) {
-      const int i = r / p.Hkv, h = r - i * p.Hkv;
+    for (int r = row0; r < from * heads; r += kStep) {
+      const int i = r / heads, h = r - i * heads;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const float by = again[half][h];
         if (by == 0.f) continue;
-        u32x2* w = reinterpret_cast<u32x2*>(p.pages[half] + id * page_bytes + (((int64_t)h << table.page_log2) + i) * D + 8 * u);
+        u32x2* w = reinterpret_cast<u32x2*>(row_at(half, i, h) + 8 * u);
         u32x2 v = *w;
         v[0] = rescaled(v[0], by);
         v[1] = rescaled(v[1], by);
@@ -228,7 +289,12 @@ static int append(const void* k, const void* v, const void* q, void* yq, void* k
   p.tok_stride[0] = strides[2]; p.head_stride[0] = strides[3];
   p.tok_stride[1] = strides[4]; p.head_stride[1] = strides[5];
   const int64_t items = (table.T >> table.page_log2) + 2LL * table.B;
-  const int64_t workgroups = items + (q ? (table.T + kQueryTokens - 1) / kQueryTokens : 0);
+  const int step = kAppendWaves * 512 / D;   // rows
+  // queries: a step of the workgroup at least, sixteen tokens where there are many
+  const int64_t least = H > 0 ? (step + H - 1) / H : 1, many = H > 0 ? (int64_t)table.T * H / (step * 2048) : 1;
+  const int64_t tokens = many > least ? many : least;
+  p.query_tokens = (int)(tokens < kQueryTokens ? tokens : kQueryTokens);
+  const int64_t workgroups = items + (q ? (table.T + p.query_tokens - 1) / p.query_tokens : 0);
   if (workgroups >= 1LL << 23) return MOBA_ERR_LIMIT;   // (threads of a launch: 32 bits)
   p.items = (int)items;
   if (D == 128) return cache8 ? launch_append<E, 128, true>(p, workgroups, st) : launch_append<E, 128, false>(p, workgroups, st);

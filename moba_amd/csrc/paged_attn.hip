@@ -60,10 +60,11 @@ __device__ __forceinline__ int swizzled(int row, int c) {
   else return c ^ ((row >> 2) & 3);
 }
 
-// eight e4m3 numbers as elements of a 16-bit type (exact)
-__device__ __forceinline__ bf16x8 widened(uint32_t a, uint32_t b, Bf16) {
-  const bf16x2 p = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.f, false), q = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.f, true);
-  const bf16x2 r = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.f, false), s = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.f, true);
+// eight e4m3 numbers as elements of a 16-bit type (exact), for bf16 also times the power of two in `by` (its exponent; the
+// instruction leaves out the rest of it)
+__device__ __forceinline__ bf16x8 widened(uint32_t a, uint32_t b, Bf16, float by = 1.f) {
+  const bf16x2 p = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, by, false), q = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, by, true);
+  const bf16x2 r = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, by, false), s = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, by, true);
   return bf16x8{p[0], p[1], q[0], q[1], r[0], r[1], s[0], s[1]};
 }
 __device__ __forceinline__ f16x8 widened(uint32_t a, uint32_t b, F16) {
@@ -84,7 +85,8 @@ constexpr float kNoMax = -3e38f;  // before the first visible key (finite: exp2(
 // 16 bytes of e4m3 to two operands.  Leaves the sum of exponentials in the lower half of the wave.
 template <class E, class V, int D, bool k8, bool kSplit>
 __device__ __forceinline__ void one_by_one(const PagedParams<E>& p, int b, int hkv, int key_lo, int step, int key_hi, int limit,
-                                        const typename E::elem8 (&bq)[D / 16], f32x16 (&oacc)[D / 32], float& m_run, float& l_run) {
+                                        float scale, const typename E::elem8 (&bq)[D / 16], f32x16 (&oacc)[D / 32], float& m_run,
+                                           float& l_run) {
   typedef typename E::elem8 elem8;
   typedef typename E::elem4 elem4;
   constexpr int kRowBytes = D * (k8 ? 1 : 2);
@@ -118,7 +120,7 @@ __device__ __forceinline__ void one_by_one(const PagedParams<E>& p, int b, int h
 #pragma unroll
           for (int e = 0; e < 8; ++e) d += (float)bq[s8][e] * (float)x[e];
         }
-        const float sc = sum_xhalf(d) * (p.scale_log2 * ks);
+        const float sc = sum_xhalf(d) * (scale * ks);
         if (key <= limit) use(at, sc, vs);
       }
     }
@@ -408,7 +410,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void paged_few_kernel(const Page
     }
   }
   if (__builtin_expect(__any(any_not_finite(oacc)), 0))  // (never for values of ordinary size)
-    one_by_one<E, V, D, k8, k8>(p, b, hkv, own_lo, kFewTile, key_hi, limit, bq, oacc, m_run, l_run);
+    one_by_one<E, V, D, k8, k8>(p, b, hkv, own_lo, kFewTile, key_hi, limit, p.scale_log2, bq, oacc, m_run, l_run);
   l_run = sum_xhalf(l_run);
 
   // ---- the waves meet in LDS.  Element e of lane (n, hh) is O[row n][32*db + 8*(e/4) + 4*hh + e%4].
@@ -522,72 +524,100 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(const Pa
   const int tiles = (key_hi - key_lo + kManyKeys - 1) / kManyKeys;
   const bool works = wave_row < rows;
 
-  // ---- copies.  Thread i's piece c of a tile is 16 bytes of key (c * 256 + i) / kFromCols
-  const int64_t page_bytes = ((int64_t)shape.Hkv << table.page_log2) * kFromRow;
+  // ---- copies.  Thread i's piece c of a tile is 16 bytes of key (c * 256 + i) / kFromCols.  A run begins at a multiple of 64 keys,
+  // so where in its page a piece lies is a constant of the thread and, in pages of more than 64 tokens, the tile's place.  Keys
+  // behind the run's last are masked, and read its page again; where the table names no page, page 0 is read
+  const uint32_t page_bytes = (uint32_t)shape.Hkv * kFromRow << table.page_log2;
   const int64_t head_bytes = ((int64_t)hkv << table.page_log2) * kFromRow;
   const int page_mask = (1 << table.page_log2) - 1;
+  const int32_t* const page_row = table.pages + b * table.stride;
   const uint32_t lds = lds_addr(smem);
-  int ids[kPieces];            // of the tile to be fetched next
-  float scales[2][4] = {};     // 8-bit: K's (times the softmax scale) and V's of the tile's four slots of 16 keys
-  uint32_t there = 0;          // the tile's slots that have a page
-  // lane i: slot i % 4's page and scales of the next tile, page of the one behind it
-  int slot_id = -1, slot_id2 = -1;
-  float slot_scale[2] = {};
   auto key_of = [&](int c) { return (c * 64 * kManyWaves + tid) / kFromCols; };
+  uint32_t in_page[kPieces];
+#pragma unroll
+  for (int c = 0; c < kPieces; ++c) {
+    const int col = k8 ? tid % kFromCols : swizzled<kRowBytes>(key_of(c), tid % kCols);
+    in_page[c] = (key_of(c) & page_mask) * kFromRow + col * 16;
+  }
+  auto look_up = [&](int key) __attribute__((always_inline)) {   // the page of a key of the run, -1 where there is none
+    const int id = page_row[(uint32_t)min(key, key_hi - 1) >> table.page_log2];
+    return (uint32_t)id < (uint32_t)table.num_pages ? id : -1;
+  };
+  int ids[kPieces];            // of the tile to be fetched next
+  float k_scale[4] = {};       // 8-bit: K's scales of the tile's four slots of 16 keys, times the softmax scale
+  uint32_t there = 0;          // the tile's slots that have a page
+  // lane i: slot i % 4's page and K scale: of the tile that is brought to LDS, of the one that fetch has asked for (8-bit:
+  // a tile later), and the page of the one behind that
+  int taken_id = -1, slot_id = -1, slot_id2 = -1;
+  float taken_scale = 0.f, slot_scale = 0.f;
   auto fetch_ids = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
-    for (int c = 0; c < kPieces; ++c) {
-      const int64_t key = key_lo + (int64_t)t * kManyKeys + key_of(c);
-      ids[c] = key < key_hi ? page_id(table, b, key >> table.page_log2) : -1;
-    }
-  };
-  auto fetch_slots = [&](int t) __attribute__((always_inline)) {
-    const int64_t key = key_lo + (int64_t)t * kManyKeys + (lane & 3) * kSlot;
-    slot_id2 = key < key_hi ? page_id(table, b, key >> table.page_log2) : -1;
-  };
-  auto fetch_scales = [&]() __attribute__((always_inline)) {
-    slot_id = slot_id2;
-    if constexpr (k8) {
-      const int64_t at = (int64_t)max(slot_id, 0) * shape.Hkv + hkv;
-      slot_scale[0] = p.scales[0][at];
-      slot_scale[1] = p.scales[1][at];
-    }
-  };
-  auto source = [&](int half, int t, int c) __attribute__((always_inline)) {
-    const int in_page = (key_lo + t * kManyKeys + key_of(c)) & page_mask;
-    return p.pages[half] + head_bytes + (ids[c] < 0 ? 0 : ids[c] * page_bytes + in_page * kFromRow);
+    for (int c = 0; c < kPieces; ++c) ids[c] = max(look_up(key_lo + t * kManyKeys + key_of(c)), 0);
+    const int key = key_lo + t * kManyKeys + (lane & 3) * kSlot, id = look_up(key);
+    slot_id2 = key < key_hi ? id : -1;
   };
   u32x4 raw[2][k8 ? kPieces : 1];
+  float raw_scale[kPieces];    // V's of the pieces
   auto fetch = [&](int t) __attribute__((always_inline)) {
+    const int64_t at = head_bytes + (int64_t)((key_lo + t * kManyKeys) & page_mask & -kManyKeys) * kFromRow;
+    const char *const k_from = p.pages[0] + at, *const v_from = p.pages[1] + at;
 #pragma unroll
-    for (int half = 0; half < 2; ++half)
+    for (int c = 0; c < kPieces; ++c) {
+      const uint64_t off = (uint64_t)(uint32_t)ids[c] * page_bytes + in_page[c];
+      if constexpr (k8) {
+        raw[0][c] = *reinterpret_cast<const u32x4*>(k_from + off);
+        raw[1][c] = *reinterpret_cast<const u32x4*>(v_from + off);
+        raw_scale[c] = p.scales[1][(uint32_t)ids[c] * (uint64_t)(uint32_t)shape.Hkv + hkv];
+      } else {
+        const uint32_t to = lds + (t & 1) * kStage + (c * kManyWaves + wave) * 1024;
+        async_copy16(k_from + off, to);
+        async_copy16(v_from + off, to + kTileBytes);
+      }
+    }
+    slot_id = slot_id2;
+    if constexpr (k8) {
+      const uint64_t place = (uint32_t)max(slot_id, 0) * (uint64_t)(uint32_t)shape.Hkv + hkv;
+      slot_scale = p.scales[0][place];
+    }
+  };
+  // V's rows of keys that nobody sees hold whatever lies there, and become zeros: whether there are such among the tile's
+  auto unseen = [&](int t) { return key_lo + (t + 1) * kManyKeys > key_hi || (uint32_t)(__ballot(taken_id >= 0) & 15) != 15; };
+  auto piece_unseen = [&](int t, int c) {
+    const int key = key_lo + t * kManyKeys + key_of(c);
+    return key >= key_hi || !((__ballot(taken_id >= 0) >> (key_of(c) >> 4)) & 1);
+  };
+  // 8-bit: what fetch has brought goes to the tile's stage, 16 elements to two places of 8
+  auto store = [&](int t, auto st) __attribute__((always_inline)) {
+    if constexpr (k8) {
+      if (__builtin_expect(unseen(t), 0)) {
+        asm volatile("");
+#pragma unroll
+        for (int c = 0; c < kPieces; ++c)
+          if (piece_unseen(t, c)) raw[1][c] = u32x4{0, 0, 0, 0};
+      }
 #pragma unroll
       for (int c = 0; c < kPieces; ++c) {
-        if constexpr (k8) {
-          raw[half][c] = *reinterpret_cast<const u32x4*>(source(half, t, c) + (tid % kFromCols) * 16);
-        } else {
-          const int col = swizzled<kRowBytes>(key_of(c), tid % kCols);
-          async_copy16(source(half, t, c) + col * 16, lds + (t & 1) * kStage + half * kTileBytes + (c * kManyWaves + wave) * 1024);
-        }
+        const int key = key_of(c), col = 2 * (tid % kFromCols);
+        const uint32_t to0 = lds + key * kRowBytes + (swizzled<kRowBytes>(key, col) << 4);
+        const uint32_t to1 = lds + key * kRowBytes + (swizzled<kRowBytes>(key, col + 1) << 4);
+        const u32x4 kw = raw[0][c], vw = raw[1][c];
+        *lds_ptr<elem8>(to0 + st * kStage) = widened(kw[0], kw[1], E{});
+        *lds_ptr<elem8>(to1 + st * kStage) = widened(kw[2], kw[3], E{});
+        *lds_ptr<bf16x8>(to0 + (st * kStage + kTileBytes)) = widened(vw[0], vw[1], Bf16{}, raw_scale[c]);
+        *lds_ptr<bf16x8>(to1 + (st * kStage + kTileBytes)) = widened(vw[2], vw[3], Bf16{}, raw_scale[c]);
       }
+    }
   };
-  auto store = [&](int t) __attribute__((always_inline)) {   // 8-bit: 16 elements to two places of 8
-    if constexpr (k8) {
+  // 16-bit: the thread's own copies have landed
+  auto landed = [&](int t, auto st) __attribute__((always_inline)) {
+    if constexpr (!k8) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if (__builtin_expect(unseen(t), 0)) {
+        asm volatile("");
 #pragma unroll
-      for (int half = 0; half < 2; ++half)
-#pragma unroll
-        for (int c = 0; c < kPieces; ++c) {
-          const int key = key_of(c), col = 2 * (tid % kFromCols);
-          const uint32_t to = lds + (t & 1) * kStage + half * kTileBytes + key * kRowBytes;
-          const u32x4 w = raw[half][c];
-          if (half == 0) {
-            *lds_ptr<elem8>(to + (swizzled<kRowBytes>(key, col) << 4)) = widened(w[0], w[1], E{});
-            *lds_ptr<elem8>(to + (swizzled<kRowBytes>(key, col + 1) << 4)) = widened(w[2], w[3], E{});
-          } else {
-            *lds_ptr<velem8>(to + (swizzled<kRowBytes>(key, col) << 4)) = widened(w[0], w[1], V{});
-            *lds_ptr<velem8>(to + (swizzled<kRowBytes>(key, col + 1) << 4)) = widened(w[2], w[3], V{});
-          }
-        }
+        for (int c = 0; c < kPieces; ++c)
+          if (piece_unseen(t, c)) *lds_ptr<u32x4>(lds + (st * kStage + kTileBytes + c * 64 * kManyWaves * 16) + tid * 16) = u32x4{0, 0, 0, 0};
+      }
     }
   };
 
@@ -596,7 +626,13 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(const Pa
     const elem* src = p.q + (int64_t)(seq.lo + j) * p.q_tok_stride + (int64_t)(hkv * shape.rep + g) * p.q_head_stride + 8 * hh;
 #pragma unroll
     for (int s8 = 0; s8 < kSteps; ++s8) bq[s8] = *reinterpret_cast<const elem8*>(src + 16 * s8);
+    // a negative softmax scale: the queries' signs turn, so that the largest product has the largest score
+    if (p.scale_log2 < 0.f) {
+#pragma unroll
+      for (int s8 = 0; s8 < kSteps; ++s8) bq[s8] = -bq[s8];
+    }
   }
+  const float scale = fabsf(p.scale_log2);
   // fragment addresses inside stage 0
   uint32_t koff[kSteps], voff[2][kDb];
 #pragma unroll
@@ -618,37 +654,52 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(const Pa
     for (int e = 0; e < 16; ++e) oacc[db][e] = 0.f;
   float m_run = kNoMax, l_run = 0.f;
 
-  auto score = [&](uint32_t st, int blk, f32x16& s) __attribute__((always_inline)) {
-#pragma unroll
-    for (int e = 0; e < 16; ++e) s[e] = 0.f;
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i) s = mfma32(*lds_ptr<const elem8>(koff[i] + st + blk * 32 * kRowBytes), bq[i], s);
-  };
-  auto block = [&](uint32_t st, int key0, int blk, f32x16& s) __attribute__((always_inline)) {
-    velem8 va[2][kDb];
+  // ---- a block of 32 keys: scores, then the largest of each row (masked where keys are not seen), then probabilities times V.
+  // The scores of a block are computed between the exponentials of the one before it: two chains for the matrix and the
+  // vector pipe where a wave alone would wait for one, then for the other.
+  constexpr std::integral_constant<int, 0> k0;
+  constexpr std::integral_constant<int, 1> k1;
+  velem8 va[2][kDb];           // V^T of the block whose probabilities are next
+  auto read_v = [&](auto st, auto blk) __attribute__((always_inline)) {
 #pragma unroll
     for (int j2 = 0; j2 < 2; ++j2)
 #pragma unroll
       for (int db = 0; db < kDb; ++db) {
-        const uint32_t at = st + (32 * blk + kSlot * j2) * kRowBytes;
+        const uint32_t at = st * kStage + (32 * blk + kSlot * j2) * kRowBytes;
         const velem4 x = lds_read_tr<velem4>(voff[0][db] + at), y = lds_read_tr<velem4>(voff[1][db] + at);
         va[j2][db] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
       }
+  };
+  auto score = [&](auto st, auto blk, f32x16& s) __attribute__((always_inline)) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) s[e] *= k8 ? scales[0][2 * blk + (e >> 3)] : p.scale_log2;
+    for (int e = 0; e < 16; ++e) s[e] = 0.f;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) s = mfma32(*lds_ptr<const elem8>(koff[i] + (st * kStage + blk * 32 * kRowBytes)), bq[i], s);
+  };
+  // f: the factors of the scores' halves (of 16 keys; not negative: see bq)
+  auto mask_and_max = [&](int key0, auto blk, f32x16& s, float (&f)[2]) __attribute__((always_inline)) {
+    f[0] = k8 ? k_scale[2 * blk] : scale;
+    f[1] = k8 ? k_scale[2 * blk + 1] : scale;
     const uint32_t has = (there >> (2 * blk)) & 3;
-    const bool edge = key0 + 31 > first_masked || has != 3;
-    if (edge) {
+    if (__builtin_expect(key0 + 31 > first_masked || has != 3, 0)) {
+      asm volatile("");   // (a branch, not sixteen comparisons in every block)
 #pragma unroll
-      for (int e = 0; e < 16; ++e)
+      for (int e = 0; e < 16; ++e) {
+        s[e] *= f[e >> 3];
         if (key0 + 8 * (e >> 2) + 4 * hh + (e & 3) > limit || !(has & (1 << (e >> 3)))) s[e] = -INFINITY;
+      }
+      f[0] = f[1] = 1.f;
     }
-    float mx = s[0];
+    float mx[2];
 #pragma unroll
-    for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[e]);
-    mx = max_xhalf(mx);
-    if (__any(mx > m_run + kMaxLag)) {
-      const float m_new = mx > m_run + kMaxLag ? mx : m_run;
+    for (int half = 0; half < 2; ++half) {
+      mx[half] = s[8 * half];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) mx[half] = fmaxf(mx[half], s[8 * half + e]);
+    }
+    const float m = max_xhalf(fmaxf(mx[0] * f[0], mx[1] * f[1]));
+    if (__any(m > m_run + kMaxLag)) {
+      const float m_new = m > m_run + kMaxLag ? m : m_run;
       const float alpha = fast_exp2(m_run - m_new);
       m_run = m_new;
       l_run *= alpha;
@@ -657,27 +708,23 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(const Pa
 #pragma unroll
         for (int e = 0; e < 16; ++e) oacc[db][e] *= alpha;
     }
+  };
+  velem8 hi[2], lo[2];
+  auto probabilities = [&](f32x16& s, const float (&f)[2]) __attribute__((always_inline)) {
     const float ref = m_run - ProbShift<V>::value;
-    velem8 hi[2], lo[2];
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      float pe = fast_exp2(s[e] - ref);
-      l_run += pe;
-      if constexpr (k8) pe *= scales[1][2 * blk + (e >> 3)];
-      const velem h = (velem)pe;
+      s[e] = fast_exp2(fmaf(s[e], f[e >> 3], -ref));
+      l_run += s[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const velem h = (velem)s[e];
       hi[e >> 3][e & 7] = h;
-      if constexpr (kParts == 2) lo[e >> 3][e & 7] = (velem)(pe - (float)h);
+      if constexpr (kParts == 2) lo[e >> 3][e & 7] = (velem)(s[e] - (float)h);
     }
-    if (edge) {
-#pragma unroll
-      for (int j2 = 0; j2 < 2; ++j2)
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (key0 + kSlot * j2 + 8 * (i >> 2) + 4 * hh + (i & 3) >= key_hi || !(has & (1 << j2))) {
-#pragma unroll
-            for (int db = 0; db < kDb; ++db) va[j2][db][i] = (velem)0.f;
-          }
-    }
+  };
+  auto add_values = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int j2 = 0; j2 < 2; ++j2)
 #pragma unroll
@@ -689,50 +736,92 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(const Pa
         for (int db = 0; db < kDb; ++db) oacc[db] = mfma32(va[j2][db], lo[j2], oacc[db]);
     }
   };
-
-  if (tiles > 0) {
-    fetch_ids(0);
-    fetch_slots(0);
-    fetch(0);
-    fetch_scales();
-    fetch_ids(1);
-    fetch_slots(1);
-    store(0);
-    if constexpr (!k8) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  }
-  for (int t = 0; t < tiles; ++t) {
-    __syncthreads();   // tile t is complete, and nobody reads tile t - 1 any more
-    const uint32_t st = (t & 1) * kStage;
-    there = (uint32_t)__ballot(slot_id >= 0) & 15;
+  auto interleave = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);            // a matrix instruction,
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);            // LDS reads,
+      __builtin_amdgcn_sched_group_barrier(0x002, 64 / kSteps, 0);  // vector instructions
+    }
+  };
+  // the slots of the tile that has been brought to LDS are those of the tile at hand
+  auto take_slots = [&]() __attribute__((always_inline)) {
+    there = (uint32_t)__ballot(taken_id >= 0) & 15;
     if constexpr (k8) {
 #pragma unroll
-      for (int slot = 0; slot < 4; ++slot) {
-        scales[0][slot] = lane_value(slot_scale[0], slot) * p.scale_log2;
-        scales[1][slot] = lane_value(slot_scale[1], slot);
-      }
+      for (int slot = 0; slot < 4; ++slot) k_scale[slot] = lane_value(taken_scale, slot) * scale;
     }
-    if (t + 1 < tiles) {
-      fetch(t + 1);
-      fetch_scales();
-      fetch_ids(t + 2);
-      fetch_slots(t + 2);
+  };
+  f32x16 s0, s1;
+  float f0[2], f1[2];
+  // Tile t + 1 goes to LDS at the beginning of tile t's work, and is complete long before the barrier at its end: 8-bit tiles
+  // from registers, which fetch fills again with the tile behind it; 16-bit ones from memory.  (Stored just before the barrier, 8-bit tiles
+  // took 1.39 ms for 2048 tokens against 34816 keys.)
+  auto bring = [&](int t, auto st) __attribute__((always_inline)) {
+    if constexpr (!k8) fetch(t);
+    taken_id = slot_id;
+    taken_scale = slot_scale;
+    store(t, st);
+    if constexpr (k8) fetch(t + 1);
+    fetch_ids(t + (k8 ? 2 : 1));
+  };
+  auto barrier = [&]() __attribute__((always_inline)) {
+    // (the wave's LDS instructions are done; loads to registers may be on their way)
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  };
+  if (tiles > 0) {
+    fetch_ids(0);
+    if constexpr (k8) {
+      fetch(0);
+      fetch_ids(1);
     }
+    bring(0, k0);
+    landed(0, k0);
+    barrier();
+  }
+  // (the stage is a constant of each copy of the body, and part of its LDS instructions)
+  auto tile = [&](int t, auto st, auto more) __attribute__((always_inline)) {
+    constexpr std::integral_constant<int, 1 - st> other;
     const int key0 = key_lo + t * kManyKeys;
-    if (works) {
-      f32x16 s0, s1;
-      score(st, 0, s0);
-      score(st, 1, s1);
-      block(st, key0, 0, s0);
-      block(st, key0 + 32, 1, s1);
+    take_slots();
+    if constexpr (more) bring(t + 1, other);
+    __builtin_amdgcn_s_setprio(1);
+    score(st, k0, s0);
+    __builtin_amdgcn_s_setprio(0);
+    mask_and_max(key0, k0, s0, f0);
+    read_v(st, k0);
+    probabilities(s0, f0);
+    __builtin_amdgcn_s_setprio(1);
+    add_values();
+    score(st, k1, s1);
+    __builtin_amdgcn_s_setprio(0);
+    mask_and_max(key0 + 32, k1, s1, f1);
+    read_v(st, k1);
+    probabilities(s1, f1);
+    __builtin_amdgcn_s_setprio(1);
+    add_values();
+    __builtin_amdgcn_s_setprio(0);
+    if constexpr (more) {
+      landed(t + 1, other);
+      barrier();        // tile t + 1 is complete, and nobody reads tile t any more
     }
-    if (t + 1 < tiles) {
-      store(t + 1);
-      if constexpr (!k8) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    }
+  };
+  constexpr std::integral_constant<bool, true> more;
+  constexpr std::integral_constant<bool, false> last;
+  int t = 0;
+  for (; t + 2 < tiles; t += 2) {
+    tile(t, k0, more);
+    tile(t + 1, k1, more);
+  }
+  if (t + 1 < tiles) {
+    tile(t, k0, more);
+    tile(t + 1, k1, last);
+  } else if (t < tiles) {
+    tile(t, k0, last);
   }
   if (!works) return;   // (no barrier follows)
   if (__builtin_expect(__any(any_not_finite(oacc)), 0))
-    one_by_one<E, V, D, k8, false>(p, b, hkv, key_lo, 32, key_hi, limit, bq, oacc, m_run, l_run);
+    one_by_one<E, V, D, k8, false>(p, b, hkv, key_lo, 32, key_hi, limit, scale, bq, oacc, m_run, l_run);
   l_run = sum_xhalf(l_run);
   if (wave_row + n >= rows) return;
   const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
