@@ -158,6 +158,19 @@ __device__ __forceinline__ void one_by_one(const PagedParams<E>& p, int b, int h
   l_run = hh == 0 ? l : 0.f;
 }
 
+__device__ __forceinline__ float lane_value(float x, int lane) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane((int)float_bits(x), lane));
+}
+
+// two numbers, each as the sum of two elements: rounded, and the rounded rest
+template <class V>
+__device__ __forceinline__ void in_two(float a, float b, uint32_t& hi, uint32_t& lo) {
+  hi = pack2<V>(a, b);
+  asm("" : "+v"(hi));  // (not rounded once more, one by one, for the rests)
+  const typename V::elem2 h = __builtin_bit_cast(typename V::elem2, hi);
+  lo = pack2<V>(a - (float)h[0], b - (float)h[1]);
+}
+
 template <int D, bool k8>
 constexpr int few_stage_bytes() { return 2 * kFewKeys * D * (k8 ? 1 : 2); }  // K and V of a step
 template <int D, bool k8>
@@ -257,7 +270,13 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void paged_few_kernel(const Page
 #pragma unroll
     for (int s8 = 0; s8 < kSteps; ++s8)
       bq[s8] = *reinterpret_cast<const elem8*>(src + (k8 ? 32 * (s8 >> 1) + 16 * hh + 8 * (s8 & 1) : 16 * s8 + 8 * hh));
+    // a negative softmax scale: the queries' signs turn, so that the largest product has the largest score
+    if (p.scale_log2 < 0.f) {
+#pragma unroll
+      for (int s8 = 0; s8 < kSteps; ++s8) bq[s8] = -bq[s8];
+    }
   }
+  const float scale = fabsf(p.scale_log2);
   if (mine > 0) issue(0);
   if (mine > 1) issue(1);
 
@@ -292,8 +311,8 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void paged_few_kernel(const Page
   float m_run = kNoMax, l_run = 0.f;
   uint64_t there = 0;   // the slots of the batch that have a page
 
-  for (int it = 0; it < mine; ++it) {
-    const uint32_t st = (it & 1) * kStage;
+  auto step = [&](int it, auto stage) __attribute__((always_inline)) {
+    constexpr uint32_t st = stage * kStage;
     // (the ids at hand are this batch's: the next batch's are fetched behind its last step but one)
     if (it % kBatch == 0) there = __ballot(ids >= 0);
     // this block's copies have landed (the next block's may still be in flight)
@@ -328,39 +347,56 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void paged_few_kernel(const Page
         if constexpr (k8) {
           typedef __attribute__((ext_vector_type(2))) int i32x2;
           vraw[j2][db] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                                                       lds_ptr<i32x2>(voff[0][db] + st + kSlot * j2 * kRowBytes)));
+                                                       lds_ptr<i32x2>(voff[0][db] + (st + kSlot * j2 * kRowBytes))));
         } else {
-          const velem4 x = lds_read_tr<velem4>(voff[0][db] + st + kSlot * j2 * kRowBytes);
-          const velem4 y = lds_read_tr<velem4>(voff[1][db] + st + kSlot * j2 * kRowBytes);
+          const velem4 x = lds_read_tr<velem4>(voff[0][db] + (st + kSlot * j2 * kRowBytes));
+          const velem4 y = lds_read_tr<velem4>(voff[1][db] + (st + kSlot * j2 * kRowBytes));
           va[j2][db] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
         }
       }
     const int key0 = own_lo + it * kFewTile;
-    float vs[2] = {1.f, 1.f};
+    // factors of the two slots' scores (not negative: see bq) and probabilities
+    float f[2] = {scale, scale}, vs[2] = {1.f, 1.f};
     if constexpr (k8) {
       const uint32_t at = scale_base + ((it / kBatch) & 1) * (kScaleBytes / 2) + (it % kBatch) * 8;
       const f32x2 k2 = *lds_ptr<const f32x2>(at), v2 = *lds_ptr<const f32x2>(at + 256);
+      f[0] *= k2[0];
+      f[1] *= k2[1];
       vs[0] = v2[0];
       vs[1] = v2[1];
-#pragma unroll
-      for (int e = 0; e < 16; ++e) s[e] *= p.scale_log2 * k2[e >> 3];
-    } else {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) s[e] *= p.scale_log2;
     }
     const uint32_t has = (uint32_t)(there >> (2 * (it % kBatch))) & 3;
-    const bool edge = key0 + kFewKeys - 1 > first_masked || has != 3;
-    if (edge) {
+    if (__builtin_expect(key0 + kFewKeys - 1 > first_masked || has != 3, 0)) {
+      asm volatile("");   // (a branch, not sixteen comparisons in every block)
 #pragma unroll
-      for (int e = 0; e < 16; ++e)
+      for (int e = 0; e < 16; ++e) {
+        s[e] *= f[e >> 3];
         if (key0 + 8 * (e >> 2) + 4 * hh + (e & 3) > limit || !(has & (1 << (e >> 3)))) s[e] = -INFINITY;
-    }
-    float mx = s[0];
+      }
+      f[0] = f[1] = 1.f;
+      // values of keys that nobody sees: whatever lies there
 #pragma unroll
-    for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[e]);
-    mx = max_xhalf(mx);
-    if (__any(mx > m_run + kMaxLag)) {  // rare once the maximum has settled
-      const float m_new = mx > m_run + kMaxLag ? mx : m_run;
+      for (int j2 = 0; j2 < 2; ++j2)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (key0 + kSlot * j2 + 8 * (i >> 2) + 4 * hh + (i & 3) >= key_hi || !(has & (1 << j2))) {
+#pragma unroll
+            for (int db = 0; db < kDb; ++db) {
+              if constexpr (k8) vraw[j2][db][i >> 2] &= ~(0xffu << (8 * (i & 3)));
+              else va[j2][db][i] = (velem)0.f;
+            }
+          }
+    }
+    float mx[2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      mx[half] = s[8 * half];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) mx[half] = fmaxf(mx[half], s[8 * half + e]);
+    }
+    mx[0] = max_xhalf(fmaxf(mx[0] * f[0], mx[1] * f[1]));
+    if (__any(mx[0] > m_run + kMaxLag)) {  // rare once the maximum has settled
+      const float m_new = mx[0] > m_run + kMaxLag ? mx[0] : m_run;
       const float alpha = fast_exp2(m_run - m_new);
       m_run = m_new;
       l_run *= alpha;
@@ -370,15 +406,20 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void paged_few_kernel(const Page
         for (int e = 0; e < 16; ++e) oacc[db][e] *= alpha;
     }
     const float ref = m_run - ProbShift<V>::value;
-    velem8 hi[2], lo[2];
+    u32x4 hi[2], lo[2];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      float pe = fast_exp2(s[e] - ref);
-      l_run += pe;
-      if constexpr (k8) pe *= vs[e >> 3];
-      const velem h = (velem)pe;
-      hi[e >> 3][e & 7] = h;
-      lo[e >> 3][e & 7] = (velem)(pe - (float)h);
+    for (int e = 0; e < 16; e += 2) {
+      float p0 = fast_exp2(fmaf(s[e], f[e >> 3], -ref)), p1 = fast_exp2(fmaf(s[e + 1], f[e >> 3], -ref));
+      l_run += p0;
+      l_run += p1;
+      if constexpr (k8) {
+        p0 *= vs[e >> 3];
+        p1 *= vs[e >> 3];
+      }
+      uint32_t h, l;
+      in_two<V>(p0, p1, h, l);
+      hi[e >> 3][(e & 7) >> 1] = h;
+      lo[e >> 3][(e & 7) >> 1] = l;
     }
     if constexpr (k8) {
 #pragma unroll
@@ -386,31 +427,26 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void paged_few_kernel(const Page
 #pragma unroll
         for (int db = 0; db < kDb; ++db) va[j2][db] = widened(vraw[j2][db][0], vraw[j2][db][1], Bf16{});
     }
-    if (edge) {   // keys that nobody sees: whatever lies there
-#pragma unroll
-      for (int j2 = 0; j2 < 2; ++j2)
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (key0 + kSlot * j2 + 8 * (i >> 2) + 4 * hh + (i & 3) >= key_hi || !(has & (1 << j2))) {
-#pragma unroll
-            for (int db = 0; db < kDb; ++db) va[j2][db][i] = (velem)0.f;
-          }
-    }
 #pragma unroll
     for (int j2 = 0; j2 < 2; ++j2)
 #pragma unroll
-      for (int db = 0; db < kDb; ++db) oacc[db] = mfma32(va[j2][db], hi[j2], oacc[db]);
+      for (int db = 0; db < kDb; ++db) oacc[db] = mfma32(va[j2][db], __builtin_bit_cast(velem8, hi[j2]), oacc[db]);
 #pragma unroll
     for (int j2 = 0; j2 < 2; ++j2)
 #pragma unroll
-      for (int db = 0; db < kDb; ++db) oacc[db] = mfma32(va[j2][db], lo[j2], oacc[db]);
+      for (int db = 0; db < kDb; ++db) oacc[db] = mfma32(va[j2][db], __builtin_bit_cast(velem8, lo[j2]), oacc[db]);
     if (it + 2 < mine) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // every fragment of this stage is in registers
       issue(it + 2);
     }
+  };
+  // (the stage is a constant of each copy of the body, and part of its LDS instructions)
+  for (int it = 0; it < mine; it += 2) {
+    step(it, std::integral_constant<int, 0>{});
+    if (it + 1 < mine) step(it + 1, std::integral_constant<int, 1>{});
   }
   if (__builtin_expect(__any(any_not_finite(oacc)), 0))  // (never for values of ordinary size)
-    one_by_one<E, V, D, k8, k8>(p, b, hkv, own_lo, kFewTile, key_hi, limit, p.scale_log2, bq, oacc, m_run, l_run);
+    one_by_one<E, V, D, k8, k8>(p, b, hkv, own_lo, kFewTile, key_hi, limit, scale, bq, oacc, m_run, l_run);
   l_run = sum_xhalf(l_run);
 
   // ---- the waves meet in LDS.  Element e of lane (n, hh) is O[row n][32*db + 8*(e/4) + 4*hh + e%4].
@@ -469,10 +505,6 @@ constexpr int kManyKeys = 64;
 
 template <int D>
 constexpr int many_lds_bytes() { return 2 * 2 * kManyKeys * D * 2; }
-
-__device__ __forceinline__ float lane_value(float x, int lane) {
-  return __builtin_bit_cast(float, __builtin_amdgcn_readlane((int)float_bits(x), lane));
-}
 
 // Elements of a probability: one, rounded, of the queries' own precision; where queries are fp16 and the products bf16, two.
 template <class E, class V> struct ProbParts { static constexpr int value = 2; };
@@ -859,18 +891,16 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams<E> p
   const PageTable& table = shape.table;
   const int per_token = shape.H / heads;
   const int t = (int)blockIdx.x / per_token, h0 = ((int)blockIdx.x - t * per_token) * heads;
-  const int b = count_up_to(table.B, t, lane, [&](int i) { return (int64_t)table.cu_new[i + 1]; });
+  Sequence seq = {0, 0, 0};
+  const int b = last_up_to(table, t, lane, seq, [](int, int lo) { return (int64_t)lo; });
   Runs r = {0, 0, 0};
   bool is_many = false;
   int row_in_seq = 0;
-  if (b < table.B) {
-    const Sequence seq = sequence_of(table, b);
-    if (keys_of(shape, seq) > 0 && t >= seq.lo && t < seq.hi) {   // (its units have left their numbers)
-      r = p.runs[b];
-      if (r.runs == 1) return;
-      is_many = (seq.hi - seq.lo) * shape.rep > p.many.rows_over && p.many.most > 0;
-      row_in_seq = (t - seq.lo) * shape.rep;
-    }
+  if (b >= 0 && t < seq.hi && keys_of(shape, seq) > 0) {   // (its units have left their numbers)
+    r = p.runs[b];
+    if (r.runs == 1) return;
+    is_many = (seq.hi - seq.lo) * shape.rep > p.many.rows_over && p.many.most > 0;
+    row_in_seq = (t - seq.lo) * shape.rep;
   }
   const Cut& cut = is_many ? p.many : p.few;
   const float* const part_o = is_many ? p.many_o : p.few_o;
@@ -884,21 +914,35 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams<E> p
     if (is_many) group = r.groups - 1 - group;
     if (group < 0 || group >= r.groups) r.runs = 0;
     auto part = [&](int i) { return ((r.first + (int64_t)i * r.groups + group) * shape.Hkv + hkv) * cut.group_rows + rr; };
-    float mm = -INFINITY;
-    for (int i = lane; i < r.runs; i += 64) mm = fmaxf(mm, part_lse[part(i)]);
+    // Rows and log-sum-exps of up to 64 runs are asked for together, a wave's quarter of the rows and, lane by lane, all of
+    // the others; more runs come 64 at a time, with a running maximum.
+    float top = kNoMax, ll = 0.f, o[kPer] = {};
+    auto some = [&](int i0, auto count) __attribute__((always_inline)) {   // runs i0 .., 4 * count of them
+      fvec x[count];
 #pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) mm = fmaxf(mm, __shfl_xor(mm, o, 64));
-    const float top = mm == -INFINITY ? 0.f : mm;
-    float ll = 0.f, o[kPer] = {};
-#pragma unroll 4
-    for (int i = wave; i < r.runs; i += 4) {
-      const int64_t at = part(i);
-      const float w = fast_exp2(part_lse[at] - top);
-      const fvec x = *reinterpret_cast<const fvec*>(part_o + at * D + kPer * lane);
-      ll += w;
+      for (int k = 0; k < count; ++k)
+        x[k] = *reinterpret_cast<const fvec*>(part_o + part(min(i0 + 4 * k + wave, r.runs - 1)) * D + kPer * lane);
+      const float lse = i0 + lane < r.runs && lane < 4 * count ? part_lse[part(i0 + lane)] : -INFINITY;
+      float mm = lse;
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) o[e] += w * x[e];
-    }
+      for (int d = 32; d >= 1; d >>= 1) mm = fmaxf(mm, __shfl_xor(mm, d, 64));
+      mm = fmaxf(mm, top);
+      const float w = fast_exp2(lse - mm), former = fast_exp2(top - mm);
+      top = mm;
+      ll *= former;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) o[e] *= former;
+#pragma unroll
+      for (int k = 0; k < count; ++k) {
+        const float wk = lane_value(w, 4 * k + wave);   // (0 behind the last)
+        ll += wk;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) o[e] += wk * x[k][e];
+      }
+    };
+    if (r.runs > 0 && r.runs <= 16) some(0, std::integral_constant<int, 4>{});
+    else
+      for (int i0 = 0; i0 < r.runs; i0 += 64) some(i0, std::integral_constant<int, 16>{});
 #pragma unroll
     for (int e = 0; e < kPer; ++e) red[wave][kPer * lane + e] = o[e];
     if (lane == 0) red_l[wave] = ll;

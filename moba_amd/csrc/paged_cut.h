@@ -61,9 +61,11 @@ __device__ __forceinline__ uint32_t upto_sum(uint32_t x) {
 }
 __device__ __forceinline__ uint32_t wave_sum(uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)upto_sum(x), 63); }
 
-// Tiles of a run.  With work = sum of groups * tiles and n = sum of groups, runs of work / (target - n) tiles come to
-// at most `target` units (each group's last run may be short); where the groups alone are more than half the target,
-// runs of work / (target / 2), and where they fill the chip several times, whole sequences.
+__device__ __forceinline__ int runs_of(int tiles, int run) { return (tiles - 1) / run + 1; }
+
+// Tiles of a run.  With work = sum of groups * tiles and n = sum of groups: runs of work / target tiles, if they come to at
+// most `target` units (each group's last run may be short), else of work / (target - n), which always do; where the groups
+// alone are more than half the target, of work / (target / 2), and where they fill the chip several times, whole sequences.
 __device__ __forceinline__ int run_tiles(const Shape& p, const Cut& c, int lane, const Share& first) {
   int64_t work = 0, groups = 0;
   for (int b0 = 0; b0 < p.table.B; b0 += 64) {
@@ -74,11 +76,15 @@ __device__ __forceinline__ int run_tiles(const Shape& p, const Cut& c, int lane,
     groups += wave_sum(s.groups);
   }
   if (groups >= (int64_t)kWholeAt * c.target) return kWholeRun;
-  const int64_t left = max(max((int64_t)c.target - groups, (int64_t)c.target / 2), (int64_t)1);
-  if (work < 1LL << 31) return (int)(((uint32_t)work + (uint32_t)left - 1) / (uint32_t)left);   // (64-bit division is slow)
-  return (int)min((work + left - 1) / left, (int64_t)kWholeRun);
+  auto ceil_div = [](int64_t a, int64_t b) {   // (64-bit division is slow)
+    return a < 1LL << 31 ? (int)(((uint32_t)a + (uint32_t)b - 1) / (uint32_t)b) : (int)min((a + b - 1) / b, (int64_t)kWholeRun);
+  };
+  if (p.table.B <= 64 && groups <= c.target) {
+    const int run = max(ceil_div(work, c.target), 1);
+    if (wave_sum(first.groups ? first.groups * runs_of(first.tiles, run) : 0) <= (uint32_t)c.target) return work > 0 ? run : 0;
+  }
+  return ceil_div(work, max(max((int64_t)c.target - groups, (int64_t)c.target / 2), (int64_t)1));
 }
-__device__ __forceinline__ int runs_of(int tiles, int run) { return (tiles - 1) / run + 1; }
 
 struct Unit {
   Sequence seq;
