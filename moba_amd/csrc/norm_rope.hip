@@ -7,8 +7,9 @@
 //
 // Bound by memory: 4 bytes an element forward, 6 backward (x is read again: its mean square is a few instructions and
 // spares a saved copy).  A wave takes a token, makes the token's angles once for all of its heads, and goes through
-// them 4 or 8 rows at a time, two of those in flight; with few tokens several waves share a token's heads.
+// them 4 or 8 rows at a time, the next ones on their way meanwhile; with few tokens several waves share a token's heads.
 #include "rotary.h"
+#include <type_traits>
 
 namespace moba {
 
@@ -52,78 +53,153 @@ __device__ __forceinline__ double position_of(const NormRopeParams<E>& p, int64_
 }
 
 constexpr int kNormWaves = 4;
+constexpr int kNormResident = 8;  // workgroups of the forward kernel that a compute unit holds
+
+// A wave's way through its work: pieces (a token, or one of `parts` shares of its rows), and of each the steps of 64 / G rows,
+// first the queries', then the keys'.  The rows of the next step are requested before the present one is worked on, and with
+// a piece's first step the position of its token.
+template <class E, int G, bool kBackward>
+struct Walk {
+  static constexpr int kRows = 64 / G;
+  const NormRopeParams<E>& p;
+  const RowPlace& at;
+  const int lane, q_steps, steps;
+  const int64_t pieces;
+  struct Rows {
+    u32x4 x, d;   // backward: d of dy
+  };
+  struct Place {
+    int64_t piece, t;
+    int step;
+  };
+  __device__ Walk(const NormRopeParams<E>& p_, const RowPlace& at_, int lane_)
+      : p(p_), at(at_), lane(lane_), q_steps((p_.heads[0] + kRows - 1) / kRows),
+        steps((p_.heads[0] + kRows - 1) / kRows + (p_.heads[1] + kRows - 1) / kRows), pieces(p_.S * p_.parts) {}
+  __device__ __forceinline__ Place first(int64_t piece) const {
+    const int64_t t = p.parts == 1 ? piece : piece / p.parts;
+    return {piece, t, (int)(piece - t * p.parts)};
+  }
+  __device__ __forceinline__ int side(const Place& w) const { return w.step >= q_steps; }
+  __device__ __forceinline__ int head(const Place& w) const {
+    return (w.step - (w.step >= q_steps ? q_steps : 0)) * kRows + lane / G;
+  }
+  __device__ __forceinline__ Rows load(const Place& w) const {
+    Rows r = {};
+    const int s = side(w), h = head(w);
+    if (w.piece < pieces && at.active && h < p.heads[s]) {
+      auto raw = [&](const typename E::elem* row) {
+        const u32x2 a = *reinterpret_cast<const u32x2*>(row + at.a), b = *reinterpret_cast<const u32x2*>(row + at.b);
+        return u32x4{a[0], a[1], b[0], b[1]};
+      };
+      if (!kBackward || p.w[s]) r.x = raw(p.x[s] + w.t * p.tok_stride[s] + h * p.head_stride[s]);
+      if constexpr (kBackward) r.d = raw(p.dy[s] + (w.t * p.heads[s] + h) * p.D);
+    }
+    return r;
+  }
+  __device__ __forceinline__ double position(const Place& w) const { return w.piece < pieces ? position_of(p, w.t) : 0.; }
+};
+template <class E>
+__device__ __forceinline__ void unpack(const u32x4& w, float (&x)[8]) {
+  const typename E::elem8 v = __builtin_bit_cast(typename E::elem8, w);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = (float)v[i];
+}
+// Every lane makes one pair's angle (of up to 64) and the lanes of a row fetch theirs.
+__device__ __forceinline__ Turn lane_turn(double position, float inv_freq, int u, bool turned) {
+  float c, s;
+  turn_of(position, inv_freq, c, s);
+  Turn t;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    t.c[i] = __shfl(c, (4 * u + i) & 63, 64);
+    t.s[i] = __shfl(s, (4 * u + i) & 63, 64);
+  }
+  t.turned = turned;
+  return t;
+}
 
 template <class E, int G>
 __global__ __launch_bounds__(64 * kNormWaves) void norm_rope_kernel(const NormRopeParams<E> p) {
-  constexpr int kRows = 64 / G;
   const int lane = threadIdx.x & 63, u = lane % G;
-  const int64_t wave = (int64_t)blockIdx.x * kNormWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t t = wave / p.parts;
-  const int part = (int)(wave - t * p.parts);
-  if (t >= p.S) return;
   const RowPlace at = row_place(u, p.D, p.rotary, p.interleaved);
-  const Turn turn = lane_turn(position_of(p, t), p.inv_freq, p.rotary, lane, u, at.turned);
+  const Walk<E, G, false> walk(p, at, lane);
+  const int64_t stride = (int64_t)gridDim.x * kNormWaves;
+  auto here = walk.first((int64_t)blockIdx.x * kNormWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
+  if (here.piece >= walk.pieces) return;
+  auto rows = walk.load(here);
+  double position = walk.position(here);
+  const float inv_freq = 2 * lane < p.rotary ? p.inv_freq[lane] : 0.f;
+  float w[2][8];
+  load_weight(p, 0, at, w[0]);
+  load_weight(p, 1, at, w[1]);
   const float over = 1.f / p.D;
-#pragma unroll
-  for (int side = 0; side < 2; ++side) {
-    float w[8];
-    load_weight(p, side, at, w);
-    const typename E::elem* x = p.x[side] + t * p.tok_stride[side];
-    typename E::elem* y = p.y[side] + t * p.heads[side] * p.D;
-    const bool normed = p.w[side] != nullptr;
-    auto one = [&](float (&v)[8], int h) __attribute__((always_inline)) {
-      if (normed) {
+  while (here.piece < walk.pieces) {
+    const Turn turn = lane_turn(position, inv_freq, u, at.turned);
+    const int64_t piece = here.piece;
+    do {
+      auto next = here;
+      next.step += p.parts;
+      if (next.step >= walk.steps) next = walk.first(here.piece + stride);
+      const auto next_rows = walk.load(next);
+      if (next.piece != piece) position = walk.position(next);
+      const int side = walk.side(here), h = walk.head(here);
+      float v[8];
+      unpack<E>(rows.x, v);
+      if (p.w[side]) {
         float sq = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) sq += v[i] * v[i];
         const float r = 1.f / sqrtf(row_sum<G>(sq) * over + p.eps);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = v[i] * r * w[i];
+        for (int i = 0; i < 8; ++i) v[i] = v[i] * r * (side ? w[1][i] : w[0][i]);
       }
       turn_row(v, turn, p.interleaved);
-      if (at.active && h < p.heads[side]) store_row<E>(y + (int64_t)h * p.D, at, v);
-    };
-    for (int h0 = part * kRows; h0 < p.heads[side]; h0 += 2 * p.parts * kRows) {
-      const int h = h0 + lane / G, h2 = h + p.parts * kRows;
-      float v[8] = {}, v2[8] = {};
-      if (at.active && h < p.heads[side]) load_row<E>(x + h * p.head_stride[side], at, v);
-      if (at.active && h2 < p.heads[side]) load_row<E>(x + h2 * p.head_stride[side], at, v2);
-      one(v, h);
-      if (h0 + p.parts * kRows < p.heads[side]) one(v2, h2);
-    }
+      if (at.active && h < p.heads[side]) store_row<E>(p.y[side] + (here.t * p.heads[side] + h) * p.D, at, v);
+      rows = next_rows;
+      here = next;
+    } while (here.piece == piece);
   }
 }
 
-// The weights' gradients are sums over all tokens: a wave keeps its own in registers over the tokens it takes (every
-// p.parts-th wave's stride), a workgroup adds its waves' and writes them, and the kernel below adds the workgroups' in
-// order.  No atomics: the same bits every time.
+// The weights' gradients are sums over all tokens: a wave keeps its own in registers over the tokens it takes, a workgroup adds
+// its waves' and writes them, and the kernel below adds the workgroups' in order.  No atomics: the same bits every time.
 template <class E, int G>
 __global__ __launch_bounds__(64 * kNormWaves) void norm_rope_bwd_kernel(const NormRopeParams<E> p) {
-  constexpr int kRows = 64 / G;
   __shared__ float sums[kNormWaves][2][128];
   const int lane = threadIdx.x & 63, u = lane % G, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const RowPlace at = row_place(u, p.D, p.rotary, p.interleaved);
-  const float over = 1.f / p.D;
+  const Walk<E, G, true> walk(p, at, lane);
+  const int64_t stride = (int64_t)gridDim.x * kNormWaves;
+  // (two steps ahead: with one, four waves to a SIMD hold 32 KiB to a compute unit in flight, and the kernel ran at 4.3 TB/s)
+  auto advance = [&](const auto& w) __attribute__((always_inline)) {
+    auto n = w;
+    if (++n.step >= walk.steps) n = walk.first(w.piece + stride);
+    return n;
+  };
+  auto here = walk.first((int64_t)blockIdx.x * kNormWaves + wave), next = advance(here);
+  auto rows = walk.load(here), next_rows = walk.load(next);
+  double position = walk.position(here), next_position = walk.position(next);
+  const float inv_freq = 2 * lane < p.rotary ? p.inv_freq[lane] : 0.f;
   float w[2][8], dw[2][8] = {};
   load_weight(p, 0, at, w[0]);
   load_weight(p, 1, at, w[1]);
-  for (int64_t t = (int64_t)blockIdx.x * kNormWaves + wave; t < p.S; t += (int64_t)gridDim.x * kNormWaves) {
-    const Turn turn = lane_turn(position_of(p, t), p.inv_freq, p.rotary, lane, u, at.turned);
-#pragma unroll
-    for (int side = 0; side < 2; ++side) {
-      const typename E::elem* x = p.x[side] + t * p.tok_stride[side];
-      const int64_t packed = t * p.heads[side] * p.D;
-      const bool normed = p.w[side] != nullptr;
-      for (int h0 = 0; h0 < p.heads[side]; h0 += kRows) {
-        const int h = h0 + lane / G;
-        const bool here = at.active && h < p.heads[side];
-        float v[8] = {}, d[8] = {};
-        if (here) {
-          load_row<E>(p.dy[side] + packed + (int64_t)h * p.D, at, d);
-          if (normed) load_row<E>(x + h * p.head_stride[side], at, v);
-        }
+  const float over = 1.f / p.D;
+  while (here.piece < walk.pieces) {
+    const Turn turn = lane_turn(position, inv_freq, u, at.turned);
+    const int64_t piece = here.piece;
+    do {
+      const auto after = advance(next);
+      const auto after_rows = walk.load(after);
+      const double after_position = after.piece != next.piece ? walk.position(after) : next_position;
+      auto work = [&](auto side) __attribute__((always_inline)) {
+        const int h = walk.head(here);
+        const bool there = at.active && h < p.heads[side];
+        float d[8];
+        unpack<E>(rows.d, d);
         turn_row<true>(d, turn, p.interleaved);
-        if (normed) {
+        if (p.w[side]) {
+          float v[8];
+          unpack<E>(rows.x, v);
           float sq = 0.f, dot = 0.f;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
@@ -135,13 +211,21 @@ __global__ __launch_bounds__(64 * kNormWaves) void norm_rope_bwd_kernel(const No
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const float n = v[i] * r;
-            if (here) dw[side][i] += d[i] * n;
+            if (there) dw[side][i] += d[i] * n;
             d[i] = r * (d[i] * w[side][i] - n * m);
           }
         }
-        if (here) store_row<E>(p.y[side] + packed + (int64_t)h * p.D, at, d);
-      }
-    }
+        if (there) store_row<E>(p.y[side] + (here.t * p.heads[side] + h) * p.D, at, d);
+      };
+      if (walk.side(here)) work(std::integral_constant<int, 1>{});
+      else work(std::integral_constant<int, 0>{});
+      rows = next_rows;
+      here = next;
+      position = next_position;
+      next_rows = after_rows;
+      next = after;
+      next_position = after_position;
+    } while (here.piece == piece);
   }
   if (!p.partials) return;
 #pragma unroll
@@ -162,18 +246,23 @@ __global__ __launch_bounds__(64 * kNormWaves) void norm_rope_bwd_kernel(const No
 }
 
 // dw[side][e] = sum of the workgroups' parts, 16 columns to a workgroup, 64 rows at a time; in 64 bits, rounded once
-constexpr int kSumCols = 16, kSumRows = 64;
+constexpr int kSumCols = 16, kSumRows = 64, kSumWaves = kSumCols * kSumRows / 64;
 template <class E>
 __global__ __launch_bounds__(kSumCols * kSumRows) void norm_rope_sum_kernel(const float* __restrict__ partials, int n, int D,
                                                                             void* dq_weight, void* dk_weight, int w32) {
-  __shared__ double sums[kSumRows][kSumCols];
+  __shared__ double sums[kSumWaves][kSumCols];
   const int c = threadIdx.x % kSumCols, r = threadIdx.x / kSumCols, col = blockIdx.x * kSumCols + c;
   double s = 0.;
+#pragma unroll 8
   for (int i = r; i < n; i += kSumRows) s += (double)partials[(int64_t)i * 2 * D + col];
-  sums[r][c] = s;
+  s += __shfl_xor(s, 16, 64);
+  s += __shfl_xor(s, 32, 64);
+  if ((threadIdx.x & 63) < kSumCols) sums[threadIdx.x >> 6][c] = s;
   __syncthreads();
   if (r != 0) return;
-  for (int i = 1; i < kSumRows; ++i) s += sums[i][c];
+  s = 0.;
+#pragma unroll
+  for (int i = 0; i < kSumWaves; ++i) s += sums[i][c];
   void* dw = col < D ? dq_weight : dk_weight;
   const int e = col < D ? col : col - D;
   if (!dw) return;
@@ -229,12 +318,15 @@ template <class E>
 static int launch_norm_rope(NormRopeParams<E> p, hipStream_t st) {
   LaunchCheck launch_check;
   const int rows = p.D > 64 ? 4 : 8;
-  // with few tokens, as many waves to a token as it has groups of rows, up to sixteen waves to a compute unit
-  const int most = ((p.heads[0] > p.heads[1] ? p.heads[0] : p.heads[1]) + rows - 1) / rows;
+  // with few tokens, as many waves to a token as it has steps, up to sixteen waves to a compute unit
+  const int most = (p.heads[0] + rows - 1) / rows + (p.heads[1] + rows - 1) / rows;
   const int cus = compute_units() > 0 ? compute_units() : 256;
   const int64_t want = (16LL * cus + p.S - 1) / p.S;
   p.parts = (int)(want < most ? want : most);
-  const int64_t wgs = (p.S * p.parts + kNormWaves - 1) / kNormWaves;
+  // A wave for every token, but for up to a few tokens to each wave that the chip holds, where new waves cost more than they
+  // balance: 20480 tokens, 10 heads: 27.7 us, 24.6 so; 131072 tokens, 40 heads: 489, 534 so
+  const int64_t need = (p.S * p.parts + kNormWaves - 1) / kNormWaves, held = (int64_t)kNormResident * cus;
+  const int64_t wgs = need > held && need <= 4 * held ? held : need;
   if (p.D > 64) hipLaunchKernelGGL((norm_rope_kernel<E, 16>), dim3((unsigned)wgs), dim3(64 * kNormWaves), 0, st, p);
   else hipLaunchKernelGGL((norm_rope_kernel<E, 8>), dim3((unsigned)wgs), dim3(64 * kNormWaves), 0, st, p);
   return launch_check.result();

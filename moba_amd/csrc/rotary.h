@@ -33,25 +33,11 @@ __device__ __forceinline__ void turn_of(double position, float inv_freq, float& 
   sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
 }
 
-// The angles of a lane's four pairs: every lane makes one pair's (of up to 64) and the lanes of a row fetch theirs.
+// The angles of a lane's four pairs.
 struct Turn {
   float c[4], s[4];
   bool turned;  // (not turned: c and s mean nothing; a turn by 0 would spread an infinity or a NaN to the element beside it)
 };
-__device__ __forceinline__ Turn lane_turn(double position, const float* __restrict__ inv_freq, int rotary, int lane, int u,
-                                          bool turned) {
-  float c = 1.f, s = 0.f;
-  if (2 * lane < rotary) turn_of(position, inv_freq[lane], c, s);
-  Turn t;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    t.c[i] = __shfl(c, (4 * u + i) & 63, 64);
-    t.s[i] = __shfl(s, (4 * u + i) & 63, 64);
-  }
-  t.turned = turned;
-  return t;
-}
-
 // x[0..3], x[4..7]: a lane's two groups.  kBack: by the angles' negatives, which is the transpose.
 template <bool kBack = false>
 __device__ __forceinline__ void turn_row(float (&x)[8], const Turn& t, bool interleaved) {
