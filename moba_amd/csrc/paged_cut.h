@@ -63,8 +63,8 @@ __device__ __forceinline__ uint32_t wave_sum(uint32_t x) { return (uint32_t)__bu
 
 __device__ __forceinline__ int runs_of(int tiles, int run) { return (tiles - 1) / run + 1; }
 
-// Tiles of a run.  With work = sum of groups * tiles and n = sum of groups: runs of work / target tiles, if they come to at
-// most `target` units (each group's last run may be short), else of work / (target - n), which always do; where the groups
+// Tiles of a run.  With work = sum of groups * tiles and n = sum of groups: the shortest runs, of work / target tiles or some
+// more, that come to at most `target` units (each group's last run may be short); runs of work / (target - n) always do.  Where the groups
 // alone are more than half the target, of work / (target / 2), and where they fill the chip several times, whole sequences.
 __device__ __forceinline__ int run_tiles(const Shape& p, const Cut& c, int lane, const Share& first) {
   int64_t work = 0, groups = 0;
@@ -79,11 +79,11 @@ __device__ __forceinline__ int run_tiles(const Shape& p, const Cut& c, int lane,
   auto ceil_div = [](int64_t a, int64_t b) {   // (64-bit division is slow)
     return a < 1LL << 31 ? (int)(((uint32_t)a + (uint32_t)b - 1) / (uint32_t)b) : (int)min((a + b - 1) / b, (int64_t)kWholeRun);
   };
-  if (p.table.B <= 64 && groups <= c.target) {
-    const int run = max(ceil_div(work, c.target), 1);
-    if (wave_sum(first.groups ? first.groups * runs_of(first.tiles, run) : 0) <= (uint32_t)c.target) return work > 0 ? run : 0;
-  }
-  return ceil_div(work, max(max((int64_t)c.target - groups, (int64_t)c.target / 2), (int64_t)1));
+  const int safe = ceil_div(work, max(max((int64_t)c.target - groups, (int64_t)c.target / 2), (int64_t)1));
+  if (p.table.B <= 64 && groups <= c.target)
+    for (int run = max(ceil_div(work, c.target), 1); run < safe; run += run / 16 + 1)
+      if (wave_sum(first.groups ? first.groups * runs_of(first.tiles, run) : 0) <= (uint32_t)c.target) return run;
+  return safe;
 }
 
 struct Unit {
