@@ -7,9 +7,10 @@
 // and where s grew, the elements that the page holds are rounded again.  A power of two makes that exact but for elements
 // that fall below e4m3's normal numbers (2^-15 of the page's range), and the division exact always.
 //
-// Bound by memory for prompts (each element is read once from memory; the second reading, after the page's maximum is known,
-// comes from L2; held in registers instead, two heads to a workgroup, a 131072-token prompt took 863 us instead of 640), by latency for single tokens: the angles of the page's tokens are made once for all heads, by all
-// waves, and wait in LDS.
+// Bound by memory for prompts, by latency for single tokens.  The angles of the page's tokens are made once for all heads, by
+// all waves, and wait in LDS; the rows go by groups of heads, two rows to a lane, which stay in registers, turned, until the
+// group's maxima are known, while the next group's are on their way (read again instead, from L2 or memory, a prompt of
+// 131072 tokens took 640 us).
 #include "paged.h"
 #include "rotary.h"
 
@@ -19,7 +20,7 @@ constexpr int kAppendWaves = 8;
 constexpr int kAngleTokens = 64;   // tokens whose angles lie in LDS at a time
 constexpr int kQueryTokens = 16;   // tokens of a workgroup that rotates queries, at most
 constexpr int kMostHeads = 256;    // key/value heads
-constexpr int kKeep = 1;           // rows of a lane that stay in registers between the two passes: those of single tokens
+constexpr int kKeep = 2;           // rows of a lane that stay in registers between the two passes
 
 template <class E>
 struct AppendParams {
@@ -43,16 +44,28 @@ __device__ __forceinline__ float page_scale(float a) {
   return __builtin_bit_cast(float, (uint32_t)(max(k, kLeastScaleExponent) + 127) << 23);
 }
 
-__device__ __forceinline__ float to_e4m3_range(float x) {
-  return x != x ? x : __builtin_amdgcn_fmed3f(x, -kE4m3Max, kE4m3Max);
-}
+// four numbers of that range, or NaN, to e4m3 (the instruction makes NaN of what lies beyond it)
 __device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d) {
-  int w = __builtin_amdgcn_cvt_pk_fp8_f32(to_e4m3_range(a), to_e4m3_range(b), 0, false);
-  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(to_e4m3_range(c), to_e4m3_range(d), w, true);
+  const int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
 }
 __device__ __forceinline__ void store_row8(char* row, const RowPlace& p, const float (&x)[8], float over) {
   *reinterpret_cast<uint32_t*>(row + p.a) = pack_e4m3(x[0] * over, x[1] * over, x[2] * over, x[3] * over);
   *reinterpret_cast<uint32_t*>(row + p.b) = pack_e4m3(x[4] * over, x[5] * over, x[6] * over, x[7] * over);
+}
+// the largest finite magnitude of a lane's elements, and whether there is an infinity among them (then clamped to the type's largest
+// number, which no finite element's quotient by its scale exceeds).  (The maximum passes over NaN.)
+__device__ __forceinline__ float largest(const float (&x)[8], bool& infinite) {
+  float m = fabsf(x[0]);
+#pragma unroll
+  for (int e = 1; e < 8; ++e) m = fmaxf(m, fabsf(x[e]));
+  infinite = m == INFINITY;
+  if (__builtin_expect(infinite, 0)) {
+    m = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(x[e]) < INFINITY ? fabsf(x[e]) : 0.f);
+  }
+  return m == m ? m : 0.f;
 }
 // the elements of a word as they would be with a scale 1 / by times as large
 __device__ __forceinline__ uint32_t rescaled(uint32_t w, float by) {
@@ -101,7 +114,7 @@ __device__ __forceinline__ void unpack(const u32x4& w, float (&x)[8]) {
 }
 
 template <class E, int D, bool k8>
-__global__ __launch_bounds__(64 * kAppendWaves, 6) void paged_append_kernel(const AppendParams<E> p) {
+__global__ __launch_bounds__(64 * kAppendWaves, 4) void paged_append_kernel(const AppendParams<E> p) {
   constexpr int G = D / 8, kRows = 64 / G;       // lanes of a row, rows of a wave
   constexpr int kStep = kAppendWaves * kRows;    // rows of the workgroup
   __shared__ Angles angles;
@@ -163,16 +176,23 @@ __global__ __launch_bounds__(64 * kAppendWaves, 6) void paged_append_kernel(cons
   auto raw = [&](int half, int i, int h) __attribute__((always_inline)) {   // token `from` + i, head h
     return load_raw<E>(source[half] + i * p.tok_stride[half] + h * p.head_stride[half], at);
   };
-  // the lane's first row is on their way while the page is looked up and the angles are made
-  u32x4 kept[kKeep][2];
+  // Pages with up to kAngleTokens new tokens go by groups of heads whose rows stay in registers, the next group's on their way
+  // (the first while the page is looked up and the angles are made).
+  const bool in_pieces = !k8 || count > kAngleTokens;
+  const int group = in_pieces ? heads : min(heads, max(kKeep * kStep / count, 1));
+  u32x4 coming[kKeep][2];
+  auto load_group = [&](int h0) __attribute__((always_inline)) {
+    const int n = min(group, heads - h0);
 #pragma unroll
-  for (int s = 0; s < kKeep; ++s) {
-    const int r = row0 + s * kStep, i = r / heads;
-    if (r < piece0 * heads) {
-      kept[s][0] = raw(0, i, r - i * heads);
-      kept[s][1] = raw(1, i, r - i * heads);
+    for (int s = 0; s < kKeep; ++s) {
+      const int r = row0 + s * kStep, i = r / n;
+      if (r < count * n) {
+        coming[s][0] = raw(0, i, h0 + r - i * n);
+        coming[s][1] = raw(1, i, h0 + r - i * n);
+      }
     }
-  }
+  };
+  if (!in_pieces) load_group(0);
   const int id = page_id(table, b, page);
   if (id < 0) return;
   constexpr int kBytes = k8 ? 1 : 2;
@@ -190,77 +210,108 @@ __global__ __launch_bounds__(64 * kAppendWaves, 6) void paged_append_kernel(cons
       most[half][h] = 0;
     }
   }
-  const bool in_pieces = count > kAngleTokens;
-  for (int pass = k8 ? 0 : 1; pass < 2; ++pass) {
-    for (int c0 = 0; c0 < count; c0 += kAngleTokens) {
-      const int piece = min(kAngleTokens, count - c0);
-      if (pass == (k8 ? 0 : 1) || in_pieces) {
-        __syncthreads();   // (the angles before have been read; the maxima are cleared)
-        if (p.rotary) make_angles(piece, [&](int i) { return first + from + c0 + i; });
-        __syncthreads();
-      }
-      auto row = [&](const u32x4 (&w)[2], int i, int h) __attribute__((always_inline)) {
-        float x[2][8];
-        unpack<E>(w[0], x[0]);
-        unpack<E>(w[1], x[1]);
-        if (at.turned) turn_row(x[0], turn_from(angles, i, u, true), p.interleaved);
+  auto turned = [&](const u32x4 (&w)[2], int i, float (&x)[2][8]) __attribute__((always_inline)) {
+    unpack<E>(w[0], x[0]);
+    unpack<E>(w[1], x[1]);
+    if (at.turned) turn_row(x[0], turn_from(angles, i, u, true), p.interleaved);
+  };
+  auto add_most = [&](const float (&x)[2][8], int h) __attribute__((always_inline)) {   // whether there are infinities
+    bool infinite[2];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          if (k8 && pass == 0) {
-            float m = 0.f;
+    for (int half = 0; half < 2; ++half) {
+      const float m = row_max<G>(largest(x[half], infinite[half]));
+      if (u == 0) atomicMax(&most[half][h], float_bits(m));
+    }
+    return infinite[0] || infinite[1];
+  };
+  auto put = [&](float (&x)[2][8], int token, int h, bool infinite) __attribute__((always_inline)) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float a = fabsf(x[half][e]);
-              m = fmaxf(m, a < INFINITY ? a : 0.f);
-            }
-            m = row_max<G>(m);
-            if (u == 0) atomicMax(&most[half][h], float_bits(m));
-          } else if constexpr (k8) {
-            store_row8(row_at(half, from + c0 + i, h), at, x[half], over[half][h]);
-          } else {
-            store_row<E>((typename E::elem*)row_at(half, from + c0 + i, h), at, x[half]);
-          }
+    for (int half = 0; half < 2; ++half) {
+      if constexpr (k8) {
+        float by = over[half][h];
+        if (__builtin_expect(infinite, 0)) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            x[half][e] = fabsf(x[half][e]) == INFINITY ? copysignf(kE4m3Max, x[half][e]) : x[half][e] * by;
+          by = 1.f;
         }
-      };
-      int done = 0;
-      if (c0 == 0) {
-#pragma unroll
-        for (int s = 0; s < kKeep; ++s) {
-          const int r = row0 + s * kStep, i = r / heads;
-          if (r < piece * heads) row(kept[s], i, r - i * heads);
-        }
-        done = kKeep * kStep;
-      }
-      for (int r = row0 + done; r < piece * heads; r += kStep) {
-        const int i = r / heads, h = r - i * heads;
-        const u32x4 w[2] = {raw(0, c0 + i, h), raw(1, c0 + i, h)};
-        row(w, i, h);
+        store_row8(row_at(half, token, h), at, x[half], by);
+      } else {
+        store_row<E>((typename E::elem*)row_at(half, token, h), at, x[half]);
       }
     }
-    if (pass == 1) break;
+  };
+  // the scales of n heads from h0 on, from the maxima; the tokens that the page holds, where a scale grew
+  auto set_scales = [&](int h0, int n) __attribute__((always_inline)) {
     __syncthreads();   // the maxima are complete
-    if (scale) {
-      const int half = tid >= heads, h = half ? tid - heads : tid;
+    const int half = tid >= heads, h = half ? tid - heads : tid;
+    if (scale && h >= h0 && h < h0 + n) {
       const float s = fmaxf(page_scale(__builtin_bit_cast(float, most[half][h])), former);
       over[half][h] = 1.f / s;
       again[half][h] = former > 0.f && s > former ? former / s : 0.f;
       *scale = s;
     }
     __syncthreads();
-    // tokens that the page holds, where a scale grew
-    for (int r = row0; r < from * heads; r += kStep) {
-      const int i = r / heads, h = r - i * heads;
+    for (int r = row0; r < from * n; r += kStep) {
+      const int i = r / n, hr = h0 + r - i * n;
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const float by = again[half][h];
+      for (int v = 0; v < 2; ++v) {
+        const float by = again[v][hr];
         if (by == 0.f) continue;
-        u32x2* w = reinterpret_cast<u32x2*>(row_at(half, i, h) + 8 * u);
-        u32x2 v = *w;
-        v[0] = rescaled(v[0], by);
-        v[1] = rescaled(v[1], by);
-        *w = v;
+        u32x2* w = reinterpret_cast<u32x2*>(row_at(v, i, hr) + 8 * u);
+        u32x2 bytes = *w;
+        bytes[0] = rescaled(bytes[0], by);
+        bytes[1] = rescaled(bytes[1], by);
+        *w = bytes;
       }
     }
+  };
+
+  if (!in_pieces) {
+    __syncthreads();   // (the maxima are cleared)
+    if (p.rotary) make_angles(count, [&](int i) { return first + from + i; });
+    __syncthreads();
+    for (int h0 = 0; h0 < heads; h0 += group) {
+      const int n = min(group, heads - h0);
+      float x[kKeep][2][8];
+      bool infinite[kKeep];
+#pragma unroll
+      for (int s = 0; s < kKeep; ++s) {
+        const int r = row0 + s * kStep;
+        if (r < count * n) turned(coming[s], r / n, x[s]);
+      }
+      if (h0 + group < heads) load_group(h0 + group);
+#pragma unroll
+      for (int s = 0; s < kKeep; ++s) {
+        const int r = row0 + s * kStep;
+        if (r < count * n) infinite[s] = add_most(x[s], h0 + r % n);
+      }
+      set_scales(h0, n);
+#pragma unroll
+      for (int s = 0; s < kKeep; ++s) {
+        const int r = row0 + s * kStep;
+        if (r < count * n) put(x[s], from + r / n, h0 + r % n, infinite[s]);
+      }
+    }
+    return;
+  }
+  // 16-bit pages: once through the rows.  Larger 8-bit pages: twice, the angles again for every piece
+  for (int pass = k8 ? 0 : 1; pass < 2; ++pass) {
+    for (int c0 = 0; c0 < count; c0 += kAngleTokens) {
+      const int piece = min(kAngleTokens, count - c0);
+      __syncthreads();   // (the angles before have been read; the maxima are cleared)
+      if (p.rotary) make_angles(piece, [&](int i) { return first + from + c0 + i; });
+      __syncthreads();
+      for (int r = row0; r < piece * heads; r += kStep) {
+        const int i = r / heads, h = r - i * heads;
+        const u32x4 w[2] = {raw(0, c0 + i, h), raw(1, c0 + i, h)};
+        float x[2][8];
+        turned(w, i, x);
+        if (k8 && pass == 0) add_most(x, h);
+        else put(x, from + c0 + i, h, k8);
+      }
+    }
+    if (k8 && pass == 0) set_scales(0, heads);
   }
 }
 

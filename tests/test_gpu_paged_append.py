@@ -74,6 +74,7 @@ def test_values_at_the_ends():
         v[:16, 1] = v[:16, 1].sign() * tiny
         v[3, 2, 7], v[20, 1, 0] = huge, -huge
         v[17, 0, 5], v[18, 1, 6], v[21, 2, 1] = float("inf"), float("-inf"), float("nan")
+        v[5, 2, 9], v[6, 2, 9], v[7, 2] = float("inf"), float("-inf"), float("nan")   # beside the largest number
         k[2, 0] = 0
         k[:16, 1] = 0
         k[19, 2, 40] = float("nan")
