@@ -47,19 +47,6 @@ __device__ __forceinline__ int page_id(const PageTable& t, int b, int64_t page) 
   return id >= 0 && id < t.num_pages ? id : -1;
 }
 
-// The number of entries i < n with value(i) <= x, for ascending values, found by the 64 lanes of a wave together.
-template <class Value>
-__device__ __forceinline__ int count_up_to(int n, int64_t x, int lane, Value value) {
-  int count = 0;
-  for (int i0 = 0; i0 < n; i0 += 64) {
-    const int i = i0 + lane;
-    const uint64_t m = __ballot(i < n && value(i < n ? i : n - 1) <= x);
-    count += __popcll(m);
-    if (~m) break;
-  }
-  return count;
-}
-
 // The last sequence b with start(b, cu_new[b]) <= x, for ascending starts, its row range and length, found by the lanes of a
 // wave together with one round of loads for every 64 sequences; b = -1 if there is none.
 template <class Start>

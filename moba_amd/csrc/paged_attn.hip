@@ -73,6 +73,19 @@ __device__ __forceinline__ f16x8 widened(uint32_t a, uint32_t b, F16) {
   return f16x8{p[0], p[1], q[0], q[1], r[0], r[1], s[0], s[1]};
 }
 
+// ... times any other factor, rounded
+__device__ __forceinline__ bf16x8 widened_by(uint32_t a, uint32_t b, float by) {
+  const u32x4 w = {pack2<Bf16>(__builtin_amdgcn_cvt_f32_fp8(a, 0) * by, __builtin_amdgcn_cvt_f32_fp8(a, 1) * by),
+                   pack2<Bf16>(__builtin_amdgcn_cvt_f32_fp8(a, 2) * by, __builtin_amdgcn_cvt_f32_fp8(a, 3) * by),
+                   pack2<Bf16>(__builtin_amdgcn_cvt_f32_fp8(b, 0) * by, __builtin_amdgcn_cvt_f32_fp8(b, 1) * by),
+                   pack2<Bf16>(__builtin_amdgcn_cvt_f32_fp8(b, 2) * by, __builtin_amdgcn_cvt_f32_fp8(b, 3) * by)};
+  return __builtin_bit_cast(bf16x8, w);
+}
+__device__ __forceinline__ bool power_of_two(float x) {   // (a normal one, not negative)
+  const uint32_t bits = float_bits(x);
+  return !(bits & 0x807fffff) && bits - 1 < 0x7f7fffff;
+}
+
 // fp16 probabilities are kept 2^7 times larger (the running maximum may lag by 2^8: they stay below 2^15), so that
 // those far below the maximum stay above the type's smallest number; the factor cancels
 template <class V> struct ProbShift { static constexpr float value = 0.f; };
@@ -503,6 +516,13 @@ constexpr int kManyWaves = 4;
 constexpr int kManyRows = 32 * kManyWaves;
 constexpr int kManyKeys = 64;
 
+// A tile lies in LDS in the order in which its fragments are read, so that a read's address is a constant of the lane and a
+// constant of the instruction, and no two lanes meet in a bank:
+//   K  for each block of 32 keys and step of 16 elements the 64 lanes' 16 bytes, lane (n, hh): elements 8hh .. of key n
+//   V  for each 16 elements and 4 keys (16 such in a row) 128 bytes, the keys one behind the other, which a transposing read of
+//      16 lanes takes
+// (Rows instead, their columns swizzled by exclusive or, took 13 address registers more; rows with 32 bytes between them, three times the
+// bank conflicts.)
 template <int D>
 constexpr int many_lds_bytes() { return 2 * 2 * kManyKeys * D * 2; }
 
@@ -518,10 +538,9 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(const Pa
   typedef typename V::elem4 velem4;
   typedef typename V::elem8 velem8;
   constexpr int kParts = ProbParts<E, V>::value;
-  constexpr int kRowBytes = D * 2, kCols = kRowBytes / 16;           // in LDS
-  constexpr int kTileBytes = kManyKeys * kRowBytes, kStage = 2 * kTileBytes;
-  constexpr int kFromRow = D * (k8 ? 1 : 2), kFromCols = kFromRow / 16;   // in the pages
-  constexpr int kPieces = kManyKeys * kFromCols / (64 * kManyWaves);      // 16-byte pieces of a tile of K (or V) of a thread
+  constexpr int kTileBytes = kManyKeys * D * 2, kStage = 2 * kTileBytes;
+  constexpr int kRow = D * (k8 ? 1 : 2);                                   // in the pages
+  constexpr int kPieces = kManyKeys * kRow / 16 / (64 * kManyWaves);       // 16-byte pieces of a tile of K (or V) of a thread
   constexpr int kSteps = D / 16, kDb = D / 32;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -556,26 +575,31 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(const Pa
   const int tiles = (key_hi - key_lo + kManyKeys - 1) / kManyKeys;
   const bool works = wave_row < rows;
 
-  // ---- copies.  Thread i's piece c of a tile is 16 bytes of key (c * 256 + i) / kFromCols.  A run begins at a multiple of 64 keys,
-  // so where in its page a piece lies is a constant of the thread and, in pages of more than 64 tokens, the tile's place.  Keys
-  // behind the run's last are masked, and read its page again; where the table names no page, page 0 is read
-  const uint32_t page_bytes = (uint32_t)shape.Hkv * kFromRow << table.page_log2;
-  const int64_t head_bytes = ((int64_t)hkv << table.page_log2) * kFromRow;
+  // ---- copies.  A run begins at a multiple of 64 keys, so where in its page a piece lies is a constant of the thread and, in
+  // pages of more than 64 tokens, the tile's place.  Keys behind the run's last are masked, and read its page again; where the table
+  // names no page, page 0 is read.
+  //   8-bit: piece c of a thread is 16 elements, `col`, of the key key_of(c), of K and of V
+  //   16-bit: piece c of a wave is the 1 KiB copy 4c + wave of the tile; of K step (4c + wave) % kSteps of a block of 32 keys, of V
+  //   the half wave % 2 of the keys and 16 elements
+  constexpr int kKeysAtOnce = k8 ? 64 * kManyWaves * 16 / kRow : 32;
+  const uint32_t page_bytes = (uint32_t)shape.Hkv * kRow << table.page_log2;
+  const int64_t head_bytes = ((int64_t)hkv << table.page_log2) * kRow;
   const int page_mask = (1 << table.page_log2) - 1;
   const int32_t* const page_row = table.pages + b * table.stride;
   const uint32_t lds = lds_addr(smem);
-  auto key_of = [&](int c) { return (c * 64 * kManyWaves + tid) / kFromCols; };
-  uint32_t in_page[kPieces];
+  constexpr int kLookups = k8 ? kPieces : 2;
+  const int col = k8 ? tid / kKeysAtOnce : 0;
+  auto key_of = [&](int c) { return (k8 ? tid % kKeysAtOnce : n) + c * kKeysAtOnce; };
+  const int v_key = 32 * (wave & 1) + 4 * (lane >> 3) + ((lane & 7) >> 1);   // 16-bit: of V
+  uint32_t in_page[kLookups];
 #pragma unroll
-  for (int c = 0; c < kPieces; ++c) {
-    const int col = k8 ? tid % kFromCols : swizzled<kRowBytes>(key_of(c), tid % kCols);
-    in_page[c] = (key_of(c) & page_mask) * kFromRow + col * 16;
-  }
+  for (int c = 0; c < kLookups; ++c) in_page[c] = (key_of(c) & page_mask) * kRow + (k8 ? col : hh) * 16;
+  const uint32_t v_in_page = (v_key & page_mask) * kRow + (lane & 1) * 16;
   auto look_up = [&](int key) __attribute__((always_inline)) {   // the page of a key of the run, -1 where there is none
     const int id = page_row[(uint32_t)min(key, key_hi - 1) >> table.page_log2];
     return (uint32_t)id < (uint32_t)table.num_pages ? id : -1;
   };
-  int ids[kPieces];            // of the tile to be fetched next
+  int ids[kLookups], v_id = 0; // of the tile to be fetched next
   float k_scale[4] = {};       // 8-bit: K's scales of the tile's four slots of 16 keys, times the softmax scale
   uint32_t there = 0;          // the tile's slots that have a page
   // lane i: slot i % 4's page and K scale: of the tile that is brought to LDS, of the one that fetch has asked for (8-bit:
@@ -583,27 +607,35 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(const Pa
   int taken_id = -1, slot_id = -1, slot_id2 = -1;
   float taken_scale = 0.f, slot_scale = 0.f;
   auto fetch_ids = [&](int t) __attribute__((always_inline)) {
+    const int key0 = key_lo + t * kManyKeys;
 #pragma unroll
-    for (int c = 0; c < kPieces; ++c) ids[c] = max(look_up(key_lo + t * kManyKeys + key_of(c)), 0);
-    const int key = key_lo + t * kManyKeys + (lane & 3) * kSlot, id = look_up(key);
+    for (int c = 0; c < kLookups; ++c) ids[c] = max(look_up(key0 + key_of(c)), 0);
+    if constexpr (!k8) v_id = max(look_up(key0 + v_key), 0);
+    const int key = key0 + (lane & 3) * kSlot, id = look_up(key);
     slot_id2 = key < key_hi ? id : -1;
   };
   u32x4 raw[2][k8 ? kPieces : 1];
-  float raw_scale[kPieces];    // V's of the pieces
+  float raw_scale[k8 ? kPieces : 1];   // V's of the pieces
   auto fetch = [&](int t) __attribute__((always_inline)) {
-    const int64_t at = head_bytes + (int64_t)((key_lo + t * kManyKeys) & page_mask & -kManyKeys) * kFromRow;
+    const int64_t at = head_bytes + (int64_t)((key_lo + t * kManyKeys) & page_mask & -kManyKeys) * kRow;
     const char *const k_from = p.pages[0] + at, *const v_from = p.pages[1] + at;
+    if constexpr (k8) {
 #pragma unroll
-    for (int c = 0; c < kPieces; ++c) {
-      const uint64_t off = (uint64_t)(uint32_t)ids[c] * page_bytes + in_page[c];
-      if constexpr (k8) {
+      for (int c = 0; c < kPieces; ++c) {
+        const uint64_t off = (uint64_t)(uint32_t)ids[c] * page_bytes + in_page[c];
         raw[0][c] = *reinterpret_cast<const u32x4*>(k_from + off);
         raw[1][c] = *reinterpret_cast<const u32x4*>(v_from + off);
         raw_scale[c] = p.scales[1][(uint32_t)ids[c] * (uint64_t)(uint32_t)shape.Hkv + hkv];
-      } else {
-        const uint32_t to = lds + (t & 1) * kStage + (c * kManyWaves + wave) * 1024;
-        async_copy16(k_from + off, to);
-        async_copy16(v_from + off, to + kTileBytes);
+      }
+    } else {
+      const char* const v_row = v_from + ((uint64_t)(uint32_t)v_id * page_bytes + v_in_page);
+#pragma unroll
+      for (int c = 0; c < kPieces; ++c) {
+        const int copy = c * kManyWaves + wave, blk = c * kManyWaves / kSteps;
+        const char* const k_row = k_from + ((uint64_t)(uint32_t)ids[blk] * page_bytes + in_page[blk]);
+        const uint32_t to = lds + (t & 1) * kStage + copy * 1024;
+        async_copy16(k_row + copy % kSteps * 32, to);
+        async_copy16(v_row + (copy >> 1) * 32, to + kTileBytes);
       }
     }
     slot_id = slot_id2;
@@ -612,31 +644,37 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(const Pa
       slot_scale = p.scales[0][place];
     }
   };
-  // V's rows of keys that nobody sees hold whatever lies there, and become zeros: whether there are such among the tile's
-  auto unseen = [&](int t) { return key_lo + (t + 1) * kManyKeys > key_hi || (uint32_t)(__ballot(taken_id >= 0) & 15) != 15; };
-  auto piece_unseen = [&](int t, int c) {
-    const int key = key_lo + t * kManyKeys + key_of(c);
-    return key >= key_hi || !((__ballot(taken_id >= 0) >> (key_of(c) >> 4)) & 1);
+  // V's rows of keys that nobody sees hold whatever lies there, and become zeros
+  auto taken = [&]() { return (uint32_t)__ballot(taken_id >= 0) & 15; };   // (asked by the whole wave)
+  auto unseen = [&](int t, uint32_t has) { return key_lo + (t + 1) * kManyKeys > key_hi || has != 15; };
+  auto key_unseen = [&](int t, uint32_t has, int key) {
+    return key_lo + t * kManyKeys + key >= key_hi || !((has >> (key >> 4)) & 1);
   };
-  // 8-bit: what fetch has brought goes to the tile's stage, 16 elements to two places of 8
+  // 8-bit: what fetch has brought goes to the tile's stage
   auto store = [&](int t, auto st) __attribute__((always_inline)) {
     if constexpr (k8) {
-      if (__builtin_expect(unseen(t), 0)) {
+      const uint32_t has = taken();
+      if (__builtin_expect(unseen(t, has), 0)) {
         asm volatile("");
 #pragma unroll
         for (int c = 0; c < kPieces; ++c)
-          if (piece_unseen(t, c)) raw[1][c] = u32x4{0, 0, 0, 0};
+          if (key_unseen(t, has, key_of(c))) raw[1][c] = u32x4{0, 0, 0, 0};
       }
 #pragma unroll
       for (int c = 0; c < kPieces; ++c) {
-        const int key = key_of(c), col = 2 * (tid % kFromCols);
-        const uint32_t to0 = lds + key * kRowBytes + (swizzled<kRowBytes>(key, col) << 4);
-        const uint32_t to1 = lds + key * kRowBytes + (swizzled<kRowBytes>(key, col + 1) << 4);
+        const int key = key_of(c);
+        const uint32_t k_to = lds + (((key >> 5) * kSteps + col) * 64 + (key & 31)) * 16;
+        const uint32_t v_to = lds + (col * 16 + (key >> 2)) * 128 + (key & 3) * 32;
         const u32x4 kw = raw[0][c], vw = raw[1][c];
-        *lds_ptr<elem8>(to0 + st * kStage) = widened(kw[0], kw[1], E{});
-        *lds_ptr<elem8>(to1 + st * kStage) = widened(kw[2], kw[3], E{});
-        *lds_ptr<bf16x8>(to0 + (st * kStage + kTileBytes)) = widened(vw[0], vw[1], Bf16{}, raw_scale[c]);
-        *lds_ptr<bf16x8>(to1 + (st * kStage + kTileBytes)) = widened(vw[2], vw[3], Bf16{}, raw_scale[c]);
+        *lds_ptr<elem8>(k_to + st * kStage) = widened(kw[0], kw[1], E{});
+        *lds_ptr<elem8>(k_to + (st * kStage + 512)) = widened(kw[2], kw[3], E{});
+        bf16x8 v0 = widened(vw[0], vw[1], Bf16{}, raw_scale[c]), v1 = widened(vw[2], vw[3], Bf16{}, raw_scale[c]);
+        if (__builtin_expect(!power_of_two(raw_scale[c]), 0)) {   // (no scale of paged_append's)
+          v0 = widened_by(vw[0], vw[1], raw_scale[c]);
+          v1 = widened_by(vw[2], vw[3], raw_scale[c]);
+        }
+        *lds_ptr<bf16x8>(v_to + (st * kStage + kTileBytes)) = v0;
+        *lds_ptr<bf16x8>(v_to + (st * kStage + kTileBytes + 16)) = v1;
       }
     }
   };
@@ -644,11 +682,14 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(const Pa
   auto landed = [&](int t, auto st) __attribute__((always_inline)) {
     if constexpr (!k8) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      if (__builtin_expect(unseen(t), 0)) {
+      const uint32_t has = taken();
+      if (__builtin_expect(unseen(t, has), 0)) {
         asm volatile("");
+        if (key_unseen(t, has, v_key)) {
 #pragma unroll
-        for (int c = 0; c < kPieces; ++c)
-          if (piece_unseen(t, c)) *lds_ptr<u32x4>(lds + (st * kStage + kTileBytes + c * 64 * kManyWaves * 16) + tid * 16) = u32x4{0, 0, 0, 0};
+          for (int c = 0; c < kPieces; ++c)
+            *lds_ptr<u32x4>(lds + (st * kStage + kTileBytes + c * 64 * kManyWaves * 16) + tid * 16) = u32x4{0, 0, 0, 0};
+        }
       }
     }
   };
@@ -665,20 +706,8 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(const Pa
     }
   }
   const float scale = fabsf(p.scale_log2);
-  // fragment addresses inside stage 0
-  uint32_t koff[kSteps], voff[2][kDb];
-#pragma unroll
-  for (int i = 0; i < kSteps; ++i) koff[i] = lds + n * kRowBytes + (swizzled<kRowBytes>(n, 2 * i + hh) << 4);
-  {
-    const int g16 = lane >> 4, l16 = lane & 15, i0 = l16 >> 2, i1 = l16 & 3, sub = (i1 & 1) * 8;
-#pragma unroll
-    for (int db = 0; db < kDb; ++db)
-#pragma unroll
-      for (int eight = 0; eight < 2; ++eight) {
-        const int key = 4 * hh + i0 + 8 * eight, c16 = 4 * db + 2 * (g16 & 1) + (i1 >> 1);
-        voff[eight][db] = lds + kTileBytes + key * kRowBytes + (swizzled<kRowBytes>(key, c16) << 4) + sub;
-      }
-  }
+  const uint32_t k_lane = lds + lane * 16;
+  const uint32_t v_lane = lds + kTileBytes + ((lane >> 4) & 1) * 2048 + hh * 128 + (lane & 15) * 8;
   f32x16 oacc[kDb];
 #pragma unroll
   for (int db = 0; db < kDb; ++db)
@@ -687,8 +716,8 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(const Pa
   float m_run = kNoMax, l_run = 0.f;
 
   // ---- a block of 32 keys: scores, then the largest of each row (masked where keys are not seen), then probabilities times V.
-  // The scores of a block are computed between the exponentials of the one before it: two chains for the matrix and the
-  // vector pipe where a wave alone would wait for one, then for the other.
+  // A wave's chain is serial; two waves of a SIMD fill each other's gaps, the one in its products first (s_setprio: 8 % of the
+  // kernel's time).  The scores of the next block between the exponentials of this one, in one wave, were no faster.
   constexpr std::integral_constant<int, 0> k0;
   constexpr std::integral_constant<int, 1> k1;
   velem8 va[2][kDb];           // V^T of the block whose probabilities are next
@@ -697,8 +726,8 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(const Pa
     for (int j2 = 0; j2 < 2; ++j2)
 #pragma unroll
       for (int db = 0; db < kDb; ++db) {
-        const uint32_t at = st * kStage + (32 * blk + kSlot * j2) * kRowBytes;
-        const velem4 x = lds_read_tr<velem4>(voff[0][db] + at), y = lds_read_tr<velem4>(voff[1][db] + at);
+        const int at = st * kStage + db * 4096 + (8 * blk + 4 * j2) * 128;   // keys 4hh .., and 8 + 4hh .. of 16
+        const velem4 x = lds_read_tr<velem4>(v_lane + at), y = lds_read_tr<velem4>(v_lane + (at + 256));
         va[j2][db] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
       }
   };
@@ -706,7 +735,7 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(const Pa
 #pragma unroll
     for (int e = 0; e < 16; ++e) s[e] = 0.f;
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) s = mfma32(*lds_ptr<const elem8>(koff[i] + (st * kStage + blk * 32 * kRowBytes)), bq[i], s);
+    for (int i = 0; i < kSteps; ++i) s = mfma32(*lds_ptr<const elem8>(k_lane + (st * kStage + (blk * kSteps + i) * 1024)), bq[i], s);
   };
   // f: the factors of the scores' halves (of 16 keys; not negative: see bq)
   auto mask_and_max = [&](int key0, auto blk, f32x16& s, float (&f)[2]) __attribute__((always_inline)) {
@@ -768,17 +797,9 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(const Pa
         for (int db = 0; db < kDb; ++db) oacc[db] = mfma32(va[j2][db], lo[j2], oacc[db]);
     }
   };
-  auto interleave = [&]() __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);            // a matrix instruction,
-      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);            // LDS reads,
-      __builtin_amdgcn_sched_group_barrier(0x002, 64 / kSteps, 0);  // vector instructions
-    }
-  };
   // the slots of the tile that has been brought to LDS are those of the tile at hand
   auto take_slots = [&]() __attribute__((always_inline)) {
-    there = (uint32_t)__ballot(taken_id >= 0) & 15;
+    there = taken();
     if constexpr (k8) {
 #pragma unroll
       for (int slot = 0; slot < 4; ++slot) k_scale[slot] = lane_value(taken_scale, slot) * scale;

@@ -171,6 +171,8 @@ def attended(batch, query, scaling=None):
         length, table = o + c, batch.table[b]
         rounded = c * rep > 32 and not (batch.quantized and query.dtype == torch.float16)
         part = torch.finfo(query.dtype).eps / 2 if rounded else 0.0
+        if batch.quantized and c * rep > 32 and not all(bool((torch.frexp(s)[0] == 0.5).all()) for s in batch.scales):
+            part += 2.0 ** -8       # (values times a scale that is no power of two are rounded to bf16)
         pages = [int(table[i]) if i < table.shape[0] else -1 for i in range(-(-length // batch.page))]
         good = [0 <= p < batch.pages[0].shape[0] for p in pages]
         there = torch.tensor(good).repeat_interleave(batch.page)[:length]

@@ -63,7 +63,7 @@ def test_either_type_on_8_bit_pages():
 def test_large_scores_and_scales(quantized, d):
     """Scores of hundreds, scales of every size beside each other, negative and zero softmax scales."""
     from moba_amd import paged_attention
-    batch = Batch([700, 40], [1, 3], 16, 2, d, BF16, quantized, seed=2)
+    batch = Batch([700, 40, 200], [1, 3, 35], 16, 2, d, BF16, quantized, seed=2)
     if quantized:
         batch.scales[1] *= 2.0 ** torch.randint(-60, 60, batch.scales[1].shape, generator=batch.g).float()
     else:
@@ -73,12 +73,26 @@ def test_large_scores_and_scales(quantized, d):
         check_attention(batch, paged_attention(q.cuda(), batch.cache(), *batch.index(), scaling=scaling), q, scaling)
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_any_scales(dtype):
+    """Scales that paged_append does not make: no powers of two, negative ones, zero."""
+    from moba_amd import paged_attention
+    batch = Batch([300, 40, 90], [1, 3, 70], 16, 2, 128, dtype, True, seed=7)
+    for s in batch.scales:
+        s *= torch.rand(s.shape, generator=batch.g) + 0.5
+        s[::5] *= -1
+        s[3::7] = 0
+    q, = batch.tensors(8)
+    for scaling in (None, -0.05):
+        check_attention(batch, paged_attention(q.cuda(), batch.cache(), *batch.index(), scaling=scaling), q, scaling)
+
+
 @pytest.mark.parametrize("quantized", [True, False])
 def test_values_that_are_not_finite(quantized):
     """They reach the rows that see them; what lies behind a sequence's end, or in other sequences' pages, reaches nobody."""
     from moba_amd import paged_attention
     for d, dtype in ((128, BF16), (64, FP16)):
-        batch = Batch([200, 70, 9], [1, 6, 1], 32, 2, d, dtype, quantized, seed=3)
+        batch = Batch([200, 70, 9, 33], [1, 6, 1, 40], 32, 2, d, dtype, quantized, seed=3)
         nan, pages = float("nan"), batch.pages
         for b, (o, c) in enumerate(zip(batch.old, batch.new)):                     # behind the end, all sequences
             last = int(batch.table[b, (o + c) // 32])
@@ -96,16 +110,20 @@ def test_values_that_are_not_finite(quantized):
         check_attention(batch, paged_attention(q.cuda(), batch.cache(), *batch.index()), q)
         # and one of its keys, other head
         pages[0][page, 0, slot, 7] = nan
+        # the same among many rows: sequence 3's eleventh new token
+        page, slot = int(batch.table[3, 43 // 32]), 43 % 32
+        pages[1][page, 0, slot, 9], pages[0][page, 1, slot, 60] = nan, nan
         got = paged_attention(q.cuda(), batch.cache(), *batch.index())
         check_attention(batch, got, q)
-        assert got[4:7, :3].isnan().all() and got[:4, :3].isfinite().all()
+        assert got[4:7, :3].isnan().all() and got[:4, :3].isfinite().all() and got[7:18].isfinite().all() and got[18:, 3:].isnan().all()
 
 
 @pytest.mark.parametrize("quantized", [True, False])
 def test_tables_that_do_not_fit(quantized):
     """Entries that are no page, lengths beyond the table or below the number of new tokens, row ranges that are none."""
     from moba_amd import paged_attention
-    batch = Batch([100, 0, 300, 40], [2, 20, 1, 3], 16, 2, 64, BF16, quantized, seed=4)
+    batch = Batch([100, 0, 300, 40, 200], [2, 20, 1, 3, 50], 16, 2, 64, BF16, quantized, seed=4)
+    batch.table[4, 3], batch.table[4, 9] = -7, 2 ** 30
     batch.table[0, 1], batch.table[0, 4], batch.table[1], batch.table[2, 5:] = -1, batch.pages[0].shape[0], 2 ** 31 - 1, -2 ** 31
     q, = batch.tensors(4)
     got = paged_attention(q.cuda(), batch.cache(), *batch.index())
