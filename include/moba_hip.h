@@ -406,8 +406,8 @@ int moba_qk_norm_rope_bwd(const void* dyq, const void* dyk, const void* q, const
  *
  * moba_paged_append: the new tokens' k and v [T,Hkv,D] go to their pages, k, and q [T,H,D] -> yq [T,H,D] (packed; both
  * NULL: none), turned by their positions as in moba_qk_norm_rope (rotary = 0: not turned).  Rows of yq that belong to no
- * sequence are zeros.  A token without a valid page is not written.  A page that receives tokens must be named by one sequence
- * only.  cache8: scales are powers of two, 2^k with the smallest k >= -100 for which the page's largest magnitude is at most
+ * sequence are zeros.  A token without a valid page is not written.  A page that receives tokens must be named once
+ * in the whole table.  cache8: scales are powers of two, 2^k with the smallest k >= -100 for which the page's largest magnitude is at most
  * 448 * 2^k, and not less than that of the tokens the page already holds, which are rounded again where it grows.
  *   strides {q token, q head, k token, k head, v token, v head, page_table row} in elements, multiples of 4 (the last: any);
  *   q, k, v and the pages 8-byte aligned; T < 2^30 */
@@ -425,7 +425,7 @@ int moba_paged_append(const void* k, const void* v, const void* q, void* yq, voi
  *   workspace: moba_paged_attention_workspace_bytes(T, B, H, Hkv, D, cache8, max_new) bytes; calls that may run at
  *   the same time need their own
  *   max_new: the most new tokens that a sequence has, or -1: a hint that spares a launch for sequences of many
- *   T < 2^24, T * H < 2^31 */
+ *   T < 2^24, T * H < 2^31, and fewer than 2^24 units of work (about B * Hkv, or T * H / 128 of long pieces; MOBA_ERR_LIMIT) */
 size_t moba_paged_attention_workspace_bytes(int64_t T, int B, int H, int Hkv, int D, int cache8, int max_new);
 int moba_paged_attention(const void* q, void* out, const void* k_pages, const void* v_pages, const float* k_scales,
                          const float* v_scales, const int32_t* page_table, const int32_t* lengths, const int32_t* cu_new,

@@ -156,6 +156,7 @@ PyMethodDef methods[] = {
     {"tail", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_tail)), METH_FASTCALL, nullptr},
     {"in_place", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_in_place)), METH_FASTCALL, nullptr},
     {"norm_rope", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_norm_rope)), METH_FASTCALL, nullptr},
+    {"check_leaves", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_check_leaves)), METH_FASTCALL, nullptr},
     {"paged_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_paged_append)), METH_FASTCALL, nullptr},
     {"paged_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_paged_attention)), METH_FASTCALL, nullptr},
     {"bind_layer", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_bind_layer)), METH_FASTCALL, nullptr},

@@ -9,11 +9,13 @@
 #include <ATen/ATen.h>
 #include <Python.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include "../../include/moba_hip.h"
 #include "host_layer.h"
@@ -66,6 +68,21 @@ hipStream_t stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.
 bool frequencies_fit(const Tensor& f, const at::Device& device, int64_t d) {
   return f.scalar_type() == at::kFloat && f.dim() == 1 && f.is_contiguous() && f.device() == device && f.numel() % 4 == 0 &&
          f.numel() > 0 && 2 * f.numel() <= d && aligned(f, 4);
+}
+
+// A leaf's gradient arrives on the stream that its node was made on.  A node that an eager graph keeps alive has another stream than
+// a capture, whose backward pass would have that stream wait for the captured one, and end the process: refused beforehand.
+void check_leaves(std::initializer_list<const Tensor*> leaves, const at::Device& device) {
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  const c10::hip::HIPStream captured = c10::hip::getCurrentHIPStream(device.index());
+  for (const Tensor* t : leaves) {
+    if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+    const auto stream = node ? node->stream() : std::nullopt;
+    TORCH_CHECK(!stream || (stream->id() == captured.id() && stream->device_index() == captured.device_index()),
+                "qk_norm_rope: an eager graph with the same leaves is alive, whose gradients belong to another stream than "
+                "the one being captured: let go of its outputs first");
+  }
 }
 
 void check(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " failed with code ", rc, ": ", str_error(rc)); }
@@ -178,6 +195,18 @@ struct NormRope : torch::autograd::Function<NormRope> {
 
 }  // namespace
 
+// check_leaves(q, k, q_weight, k_weight), for the caller's own path
+PyObject* py_check_leaves(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 4 && THPVariable_Check(args[0]), "check_leaves takes four tensors");
+  Tensor t[4];
+  for (int i = 0; i < 4; ++i)
+    if (THPVariable_Check(args[i])) t[i] = THPVariable_Unpack(args[i]);
+  check_leaves({&t[0], &t[1], &t[2], &t[3]}, t[0].device());
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
 // norm_rope(q, k, positions, inv_freq, q_weight, k_weight, eps, interleaved)
 PyObject* py_norm_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -198,6 +227,7 @@ PyObject* py_norm_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
   {
     const NoGil no_gil;
     if (at::GradMode::is_enabled() && (wants(a.q) || wants(a.k) || wants(a.q_weight) || wants(a.k_weight))) {
+      check_leaves({&a.q, &a.k, &a.q_weight, &a.k_weight}, a.q.device());
       auto given = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
       const auto out =
           NormRope::apply(a.q, a.k, a.positions, a.inv_freq, given(a.q_weight), given(a.k_weight), a.eps, a.interleaved);
@@ -234,8 +264,8 @@ struct Cache {
     v = plain_tensor(args[1]);
     return k && v && optional_tensor(args[2], k_scales) && optional_tensor(args[3], v_scales) && k->is_cuda() && k->dim() == 4;
   }
-  bool takes_rows(const Tensor& x) const {
-    return half_type(x) && (k_scales.defined() || x.scalar_type() == k->scalar_type()) && x.dim() == 3 && x.size(2) == k->size(3) &&
+  bool takes_rows(const Tensor& x) const {   // (none that a gradient is wanted for: there is none)
+    return !(x.requires_grad() && at::GradMode::is_enabled()) && half_type(x) && (k_scales.defined() || x.scalar_type() == k->scalar_type()) && x.dim() == 3 && x.size(2) == k->size(3) &&
            x.device() == k->device();
   }
 };

@@ -136,7 +136,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_
             head before the rotation; None: that side is rotated only
     Returns:
         the new q and k, packed.  Differentiable once in q, k and the weights; the weights' gradients are summed in a fixed
-        order (the same bits on every run).
+        order (the same bits on every run).  A call that is being captured into a graph is refused while an eager graph of the
+        same leaves is alive (its backward pass could not be captured).
     """
     y = _lib.host().norm_rope(q, k, positions, inv_freq, q_weight, k_weight, eps, interleaved)
     if y is not NotImplemented:
@@ -146,5 +147,6 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_
     positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
     tensors = (q, k, q_weight, k_weight)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        _lib.host().check_leaves(*tensors)
         return _QkNormRope.apply(q, k, positions, inv_freq, q_weight, k_weight, eps, interleaved)
     return _forward(_readable(q), _readable(k), positions, inv_freq, q_weight, k_weight, eps, interleaved)

@@ -21,7 +21,7 @@ MAX_KV_HEADS = 256
 MAX_TOKENS = (1 << 30) - 1   # packed rows of a call
 
 
-@dataclass(frozen=True)
+@dataclass(frozen=True, eq=False)
 class PagedKVCache:
     """The pages of one layer.
 
@@ -31,7 +31,7 @@ class PagedKVCache:
         page and head.  ``paged_append`` keeps them powers of two.
 
     Which pages belong to which sequence is the caller's affair (the ``page_table`` of the calls).  Pages may be shared by
-    sequences that only read them; a page that receives tokens in a call must be named by one sequence only.
+    sequences that only read them; a page that receives tokens in a call must be named once in the whole table.
     """
 
     k_pages: torch.Tensor
@@ -104,6 +104,8 @@ def _check_rows(cache, name, x, heads=None):
         raise ValueError(f"{name} must be [tokens, heads, head_dim] with the cache's head_dim (and, keys and values, its heads)")
     if x.shape[0] > MAX_TOKENS:
         raise ValueError(f"at most {MAX_TOKENS} tokens")
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("the operators on the paged cache have no gradients: call them under torch.no_grad()")
 
 
 def paged_append(cache: PagedKVCache, key: torch.Tensor, value: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
@@ -122,7 +124,8 @@ def paged_append(cache: PagedKVCache, key: torch.Tensor, value: torch.Tensor, pa
         inv_freq, interleaved: the rotation, as for ``qk_norm_rope``; without inv_freq nothing is rotated
         query: [tokens, heads, head_dim] of key's dtype, or None
     Returns:
-        the rotated queries (rows that belong to no sequence: zeros), or None without ``query``.
+        the rotated queries (rows that belong to no sequence: zeros), or None without ``query``.  No gradients: rows that
+        require one are refused outside ``torch.no_grad()``.
 
     The three index tensors stay on the device, and a captured call follows their contents.  A token whose position has no
     page (beyond the table's row, or an entry that is no page) is not written.  Elements of 8-bit pages are rounded from
@@ -187,7 +190,8 @@ def paged_attention(query: torch.Tensor, cache: PagedKVCache, page_table: torch.
             with many (results do not depend on it)
     Returns:
         [tokens, heads, head_dim] in query's dtype.  Rows that see no token (those of no sequence, of a sequence without
-        pages) are zeros; a page that the table names wrongly (no page of the pool) holds no tokens.
+        pages) are zeros; a page that the table names wrongly (no page of the pool) holds no tokens.  No gradients: a query that
+        requires one is refused outside ``torch.no_grad()``.
     """
     out = _lib.host().paged_attention(cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales, query, page_table, lengths,
                                       cu_new, scaling, max_new)

@@ -239,6 +239,36 @@ def test_same_bits_every_time_on_every_stream_and_in_a_graph():
         assert all(torch.equal(a, b) for a, b in zip(both(), want))
 
 
+@pytest.mark.parametrize("native", [True, False])
+def test_a_capture_beside_a_living_graph_of_the_same_leaves_is_refused(native, monkeypatch):
+    """Its backward pass would join the captured stream to the one that the leaves' gradients belong to.  No backward pass runs
+    before the eager graph has gone."""
+    from moba_amd import _lib, qk_norm_rope
+    q, k, dq, dk, positions, weights = make(20, 4, 2, 64, BF16, seed=5)
+    inv_freq, leaves = frequencies(32, "cuda"), [x.detach().requires_grad_() for x in (q, k, *weights)]
+    if not native:
+        monkeypatch.setattr(_lib.host(), "norm_rope", lambda *a: NotImplemented)
+    alive = qk_norm_rope(*leaves[:2], positions, inv_freq, *leaves[2:])
+    want = [y.detach().clone() for y in alive]
+    torch.cuda.synchronize()
+    graph, held = torch.cuda.CUDAGraph(), torch.zeros(4, device="cuda")
+    for a, b in (((leaves[0], k), ()), ((q, leaves[1]), weights), ((q, k), (leaves[2], weights[1])), ((q, k), (None, leaves[3]))):
+        with pytest.raises(RuntimeError, match="eager graph"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                held.add_(1)
+                qk_norm_rope(*a, positions, inv_freq, *b)
+    with torch.cuda.graph(torch.cuda.CUDAGraph()), torch.no_grad():   # (no backward pass: not refused)
+        qk_norm_rope(*leaves[:2], positions, inv_freq, *leaves[2:])
+    del alive
+    with torch.cuda.graph(graph):
+        y = qk_norm_rope(*leaves[:2], positions, inv_freq, *leaves[2:])
+        g = torch.autograd.grad(y, leaves, (dq, dk))
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(y, want)) and all(x.isfinite().all() for x in g)
+
+
 def test_before_the_attention():
     """Training as it is used: norm and rotation, the packed attention behind them, one backward through both."""
     from moba_amd import moba_attn_varlen_gqa, qk_norm_rope

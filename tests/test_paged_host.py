@@ -138,3 +138,25 @@ def test_attention_entry_point_refuses():
         need, less = sizes(*args, -1), sizes(*args, 1)
         runs = (args[1] * 12 + 15) // 16 * 16
         assert (need - runs) % (32 * (args[4] + 1) * 4) == 0 and 0 < less <= need < 2 << 30, args
+
+
+def test_rows_that_want_a_gradient():
+    """There are none: refused, but for calls that record no graph (which go on to the next check)."""
+    from moba_amd import paged_append, paged_attention
+    rest = {k: v for k, v in append_args().items() if k in ("query", "cache", "page_table", "lengths", "cu_new")}
+    for name in ("key", "value", "query"):
+        args = append_args(**{name: append_args()[name].requires_grad_()})
+        with pytest.raises(RuntimeError, match="no gradients"):
+            paged_append(**args)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="AMD GPU"):
+            paged_append(**args)
+    rest["query"] = rest["query"].requires_grad_()
+    with pytest.raises(RuntimeError, match="no gradients"):
+        paged_attention(**rest)
+    with torch.inference_mode(), pytest.raises(RuntimeError, match="AMD GPU"):
+        paged_attention(**rest)
+
+
+def test_caches_compare_by_identity():
+    a, b = make(), make()
+    assert a == a and a != b and len({a, b}) == 2
