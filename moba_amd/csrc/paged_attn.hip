@@ -509,12 +509,15 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void paged_few_kernel(const Page
   }
 }
 
-// ---- many rows: bound by the products.  A workgroup of four waves takes 128 rows, 32 to a wave; a tile of 64 keys is brought into
-// LDS once for all of them, two stages, one barrier a tile.  8-bit tiles come through registers, where they become 16-bit
-// elements once for the four waves; 16-bit tiles are copied global -> LDS.  Two workgroups fit a compute unit.
-constexpr int kManyWaves = 4;
-constexpr int kManyRows = 32 * kManyWaves;
+// ---- many rows: bound by the products and, beside them, by the vector instructions of the softmax and of the 8-bit elements.  A
+// workgroup takes 32 rows to a wave; tiles of 64 keys are brought into LDS once for all of them, in rings of three K and two V
+// tiles, one barrier a tile.  16-bit tiles are copied global -> LDS, four waves to a workgroup and two workgroups to a compute unit, so
+// that one's lookups and barriers run under the other's products.  8-bit tiles come through registers, where they become 16-bit
+// elements: eight waves share that work where heads have 128 elements, one workgroup to a compute unit (2048 tokens against 34816
+// keys, 32 and 8 heads: 998 us, with four waves 1076; 16-bit pages: 1037 with eight, 1040 with four, but prompts without a cache 70
+// and 65).  Priority for the products gives 4 % with four waves and takes 2 % with eight.
 constexpr int kManyKeys = 64;
+template <int D, bool k8> constexpr int kManyWaves = D == 128 && k8 ? 8 : 4;
 
 // A tile lies in LDS in the order in which its fragments are read, so that a read's address is a constant of the lane and a
 // constant of the instruction, and no two lanes meet in a bank:
@@ -524,23 +527,24 @@ constexpr int kManyKeys = 64;
 // (Rows instead, their columns swizzled by exclusive or, took 13 address registers more; rows with 32 bytes between them, three times the
 // bank conflicts.)
 template <int D>
-constexpr int many_lds_bytes() { return 2 * 2 * kManyKeys * D * 2; }
+constexpr int many_lds_bytes() { return 5 * kManyKeys * D * 2; }
 
 // Elements of a probability: one, rounded, of the queries' own precision; where queries are fp16 and the products bf16, two.
 template <class E, class V> struct ProbParts { static constexpr int value = 2; };
 template <class E> struct ProbParts<E, E> { static constexpr int value = 1; };
 
 template <class E, int D, bool k8>
-__global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(const PagedParams<E> p) {
+__global__ __launch_bounds__(64 * (kManyWaves<D, k8>), 2) void paged_many_kernel(const PagedParams<E> p) {
   MOBA_ELEM_TYPES(E)
   using V = std::conditional_t<k8, Bf16, E>;
   typedef typename V::elem velem;
   typedef typename V::elem4 velem4;
   typedef typename V::elem8 velem8;
+  constexpr int kWaves = kManyWaves<D, k8>, kRows = 32 * kWaves;
   constexpr int kParts = ProbParts<E, V>::value;
-  constexpr int kTileBytes = kManyKeys * D * 2, kStage = 2 * kTileBytes;
+  constexpr int kTileBytes = kManyKeys * D * 2;
   constexpr int kRow = D * (k8 ? 1 : 2);                                   // in the pages
-  constexpr int kPieces = kManyKeys * kRow / 16 / (64 * kManyWaves);       // 16-byte pieces of a tile of K (or V) of a thread
+  constexpr int kPieces = kManyKeys * kRow / 16 / (64 * kWaves);       // 16-byte pieces of a tile of K (or V) of a thread
   constexpr int kSteps = D / 16, kDb = D / 32;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -560,10 +564,10 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(const Pa
   const int keys = keys_of(shape, seq);
   if (u == unit.first && hkv == 0 && tid == 0) p.runs[b] = {unit.first, unit.runs, unit.groups};
   // (the group with the most keys first)
-  const int count = seq.hi - seq.lo, rows = count * shape.rep, row0 = (unit.groups - 1 - unit.group) * kManyRows;
+  const int count = seq.hi - seq.lo, rows = count * shape.rep, row0 = (unit.groups - 1 - unit.group) * kRows;
   const int per = (unit.tiles + unit.runs - 1) / unit.runs;
   const int before = (int)seq.length - count;
-  const int last_row = min(row0 + kManyRows, rows) - 1;
+  const int last_row = min(row0 + kRows, rows) - 1;
   const int seen = min(keys, max(before + last_row / shape.rep + 1, 0));      // keys that the group's last row sees
   const int key_lo = (int)min((int64_t)unit.run * per * kManyKeys, (int64_t)seen);
   const int key_hi = (int)min((int64_t)(unit.run + 1) * per * kManyKeys, (int64_t)seen);
@@ -581,7 +585,7 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(const Pa
   //   8-bit: piece c of a thread is 16 elements, `col`, of the key key_of(c), of K and of V
   //   16-bit: piece c of a wave is the 1 KiB copy 4c + wave of the tile; of K step (4c + wave) % kSteps of a block of 32 keys, of V
   //   the half wave % 2 of the keys and 16 elements
-  constexpr int kKeysAtOnce = k8 ? 64 * kManyWaves * 16 / kRow : 32;
+  constexpr int kKeysAtOnce = k8 ? 64 * kWaves * 16 / kRow : 32;
   const uint32_t page_bytes = (uint32_t)shape.Hkv * kRow << table.page_log2;
   const int64_t head_bytes = ((int64_t)hkv << table.page_log2) * kRow;
   const int page_mask = (1 << table.page_log2) - 1;
@@ -599,13 +603,14 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(const Pa
     const int id = page_row[(uint32_t)min(key, key_hi - 1) >> table.page_log2];
     return (uint32_t)id < (uint32_t)table.num_pages ? id : -1;
   };
-  int ids[kLookups], v_id = 0; // of the tile to be fetched next
-  float k_scale[4] = {};       // 8-bit: K's scales of the tile's four slots of 16 keys, times the softmax scale
-  uint32_t there = 0;          // the tile's slots that have a page
-  // lane i: slot i % 4's page and K scale: of the tile that is brought to LDS, of the one that fetch has asked for (8-bit:
-  // a tile later), and the page of the one behind that
-  int taken_id = -1, slot_id = -1, slot_id2 = -1;
-  float taken_scale = 0.f, slot_scale = 0.f;
+  int ids[kLookups], v_ids[k8 ? kPieces : 1], v_id = 0;   // of the tiles of which K and V are fetched next (v_id: 16-bit, V of K's tile)
+  // Of the tile at hand, the next and the one behind it: the place of its K, the slots of 16 keys that have a page, and in lane i K's
+  // scale of slot i % 4.
+  uint32_t place[3], there[3] = {};
+  float k_scale[3] = {};
+  uint32_t v_place[2];               // V of the tile at hand and of the next
+  int slot_id = -1, slot_id2 = -1;   // lane i: the page of slot i % 4 of the tile whose K has been asked for, and of the next
+  float slot_scale = 0.f;
   auto fetch_ids = [&](int t) __attribute__((always_inline)) {
     const int key0 = key_lo + t * kManyKeys;
 #pragma unroll
@@ -616,79 +621,96 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(const Pa
   };
   u32x4 raw[2][k8 ? kPieces : 1];
   float raw_scale[k8 ? kPieces : 1];   // V's of the pieces
-  auto fetch = [&](int t) __attribute__((always_inline)) {
-    const int64_t at = head_bytes + (int64_t)((key_lo + t * kManyKeys) & page_mask & -kManyKeys) * kRow;
-    const char *const k_from = p.pages[0] + at, *const v_from = p.pages[1] + at;
-    if constexpr (k8) {
+  auto in_tile = [&](int t) { return head_bytes + (int64_t)((key_lo + t * kManyKeys) & page_mask & -kManyKeys) * kRow; };
+  auto fetch_k = [&](int t, uint32_t to) __attribute__((always_inline)) {
+    const char* const from = p.pages[0] + in_tile(t);
 #pragma unroll
-      for (int c = 0; c < kPieces; ++c) {
-        const uint64_t off = (uint64_t)(uint32_t)ids[c] * page_bytes + in_page[c];
-        raw[0][c] = *reinterpret_cast<const u32x4*>(k_from + off);
-        raw[1][c] = *reinterpret_cast<const u32x4*>(v_from + off);
-        raw_scale[c] = p.scales[1][(uint32_t)ids[c] * (uint64_t)(uint32_t)shape.Hkv + hkv];
-      }
-    } else {
-      const char* const v_row = v_from + ((uint64_t)(uint32_t)v_id * page_bytes + v_in_page);
-#pragma unroll
-      for (int c = 0; c < kPieces; ++c) {
-        const int copy = c * kManyWaves + wave, blk = c * kManyWaves / kSteps;
-        const char* const k_row = k_from + ((uint64_t)(uint32_t)ids[blk] * page_bytes + in_page[blk]);
-        const uint32_t to = lds + (t & 1) * kStage + copy * 1024;
-        async_copy16(k_row + copy % kSteps * 32, to);
-        async_copy16(v_row + (copy >> 1) * 32, to + kTileBytes);
+    for (int c = 0; c < kPieces; ++c) {
+      if constexpr (k8) {
+        raw[0][c] = *reinterpret_cast<const u32x4*>(from + ((uint64_t)(uint32_t)ids[c] * page_bytes + in_page[c]));
+      } else {
+        const int copy = c * kWaves + wave, blk = c * kWaves / kSteps;
+        async_copy16(from + ((uint64_t)(uint32_t)ids[blk] * page_bytes + in_page[blk]) + copy % kSteps * 32, lds + to + copy * 1024);
       }
     }
     slot_id = slot_id2;
+    if constexpr (k8) slot_scale = p.scales[0][(uint32_t)max(slot_id, 0) * (uint64_t)(uint32_t)shape.Hkv + hkv];
+  };
+  auto fetch_v = [&](int t, uint32_t to) __attribute__((always_inline)) {
+    const char* const from = p.pages[1] + in_tile(t);
     if constexpr (k8) {
-      const uint64_t place = (uint32_t)max(slot_id, 0) * (uint64_t)(uint32_t)shape.Hkv + hkv;
-      slot_scale = p.scales[0][place];
+#pragma unroll
+      for (int c = 0; c < kPieces; ++c) {
+        raw[1][c] = *reinterpret_cast<const u32x4*>(from + ((uint64_t)(uint32_t)v_ids[c] * page_bytes + in_page[c]));
+        raw_scale[c] = p.scales[1][(uint32_t)v_ids[c] * (uint64_t)(uint32_t)shape.Hkv + hkv];
+      }
+    } else {
+      const char* const row = from + ((uint64_t)(uint32_t)v_ids[0] * page_bytes + v_in_page);
+#pragma unroll
+      for (int c = 0; c < kPieces; ++c) {
+        const int copy = c * kWaves + wave;
+        async_copy16(row + (copy >> 1) * 32, lds + to + copy * 1024);
+      }
     }
   };
   // V's rows of keys that nobody sees hold whatever lies there, and become zeros
-  auto taken = [&]() { return (uint32_t)__ballot(taken_id >= 0) & 15; };   // (asked by the whole wave)
   auto unseen = [&](int t, uint32_t has) { return key_lo + (t + 1) * kManyKeys > key_hi || has != 15; };
   auto key_unseen = [&](int t, uint32_t has, int key) {
     return key_lo + t * kManyKeys + key >= key_hi || !((has >> (key >> 4)) & 1);
   };
-  // 8-bit: what fetch has brought goes to the tile's stage
-  auto store = [&](int t, auto st) __attribute__((always_inline)) {
+  // 8-bit: what the fetches have brought goes to its place
+  auto store_k = [&](uint32_t to) __attribute__((always_inline)) {
     if constexpr (k8) {
-      const uint32_t has = taken();
-      if (__builtin_expect(unseen(t, has), 0)) {
-        asm volatile("");
-#pragma unroll
-        for (int c = 0; c < kPieces; ++c)
-          if (key_unseen(t, has, key_of(c))) raw[1][c] = u32x4{0, 0, 0, 0};
-      }
 #pragma unroll
       for (int c = 0; c < kPieces; ++c) {
         const int key = key_of(c);
-        const uint32_t k_to = lds + (((key >> 5) * kSteps + col) * 64 + (key & 31)) * 16;
-        const uint32_t v_to = lds + (col * 16 + (key >> 2)) * 128 + (key & 3) * 32;
-        const u32x4 kw = raw[0][c], vw = raw[1][c];
-        *lds_ptr<elem8>(k_to + st * kStage) = widened(kw[0], kw[1], E{});
-        *lds_ptr<elem8>(k_to + (st * kStage + 512)) = widened(kw[2], kw[3], E{});
-        bf16x8 v0 = widened(vw[0], vw[1], Bf16{}, raw_scale[c]), v1 = widened(vw[2], vw[3], Bf16{}, raw_scale[c]);
-        if (__builtin_expect(!power_of_two(raw_scale[c]), 0)) {   // (no scale of paged_append's)
-          v0 = widened_by(vw[0], vw[1], raw_scale[c]);
-          v1 = widened_by(vw[2], vw[3], raw_scale[c]);
-        }
-        *lds_ptr<bf16x8>(v_to + (st * kStage + kTileBytes)) = v0;
-        *lds_ptr<bf16x8>(v_to + (st * kStage + kTileBytes + 16)) = v1;
+        const uint32_t at = lds + to + (((key >> 5) * kSteps + col) * 64 + (key & 31)) * 16;
+        const u32x4 w = raw[0][c];
+        *lds_ptr<elem8>(at) = widened(w[0], w[1], E{});
+        *lds_ptr<elem8>(at + 512) = widened(w[2], w[3], E{});
       }
     }
   };
+  auto store_v = [&](int t, uint32_t to, uint32_t has) __attribute__((always_inline)) {
+    if constexpr (k8) {
+      bool odd = false;   // (no scale of paged_append's)
+#pragma unroll
+      for (int c = 0; c < kPieces; ++c) odd |= !power_of_two(raw_scale[c]);
+      auto put = [&](auto plain) __attribute__((always_inline)) {
+#pragma unroll
+        for (int c = 0; c < kPieces; ++c) {
+          const int key = key_of(c);
+          const uint32_t at = lds + to + (col * 16 + (key >> 2)) * 128 + (key & 3) * 32;
+          u32x4 w = raw[1][c];
+          bf16x8 v0, v1;
+          if constexpr (plain) {
+            v0 = widened(w[0], w[1], Bf16{}, raw_scale[c]);
+            v1 = widened(w[2], w[3], Bf16{}, raw_scale[c]);
+          } else {
+            const bool none = key_unseen(t, has, key);
+            if (none) w = u32x4{0, 0, 0, 0};
+            const float by = none ? 1.f : raw_scale[c];
+            v0 = widened_by(w[0], w[1], by);
+            v1 = widened_by(w[2], w[3], by);
+          }
+          *lds_ptr<bf16x8>(at) = v0;
+          *lds_ptr<bf16x8>(at + 16) = v1;
+        }
+      };
+      if (__builtin_expect(unseen(t, has) || __any(odd), 0)) put(std::false_type{});
+      else put(std::true_type{});
+    }
+  };
   // 16-bit: the thread's own copies have landed
-  auto landed = [&](int t, auto st) __attribute__((always_inline)) {
+  auto landed = [&](int t, uint32_t to, uint32_t has) __attribute__((always_inline)) {
     if constexpr (!k8) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      const uint32_t has = taken();
       if (__builtin_expect(unseen(t, has), 0)) {
         asm volatile("");
         if (key_unseen(t, has, v_key)) {
 #pragma unroll
           for (int c = 0; c < kPieces; ++c)
-            *lds_ptr<u32x4>(lds + (st * kStage + kTileBytes + c * 64 * kManyWaves * 16) + tid * 16) = u32x4{0, 0, 0, 0};
+            *lds_ptr<u32x4>(lds + to + c * 64 * kWaves * 16 + tid * 16) = u32x4{0, 0, 0, 0};
         }
       }
     }
@@ -707,50 +729,62 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(const Pa
   }
   const float scale = fabsf(p.scale_log2);
   const uint32_t k_lane = lds + lane * 16;
-  const uint32_t v_lane = lds + kTileBytes + ((lane >> 4) & 1) * 2048 + hh * 128 + (lane & 15) * 8;
+  const uint32_t v_lane = lds + ((lane >> 4) & 1) * 2048 + hh * 128 + (lane & 15) * 8;
   f32x16 oacc[kDb];
-#pragma unroll
-  for (int db = 0; db < kDb; ++db)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) oacc[db][e] = 0.f;
   float m_run = kNoMax, l_run = 0.f;
 
-  // ---- a block of 32 keys: scores, then the largest of each row (masked where keys are not seen), then probabilities times V.
-  // A wave's chain is serial; two waves of a SIMD fill each other's gaps, the one in its products first (s_setprio: 8 % of the
-  // kernel's time).  The scores of the next block between the exponentials of this one, in one wave, were no faster.
-  constexpr std::integral_constant<int, 0> k0;
-  constexpr std::integral_constant<int, 1> k1;
-  velem8 va[2][kDb];           // V^T of the block whose probabilities are next
-  auto read_v = [&](auto st, auto blk) __attribute__((always_inline)) {
-#pragma unroll
-    for (int j2 = 0; j2 < 2; ++j2)
-#pragma unroll
-      for (int db = 0; db < kDb; ++db) {
-        const int at = st * kStage + db * 4096 + (8 * blk + 4 * j2) * 128;   // keys 4hh .., and 8 + 4hh .. of 16
-        const velem4 x = lds_read_tr<velem4>(v_lane + at), y = lds_read_tr<velem4>(v_lane + (at + 256));
-        va[j2][db] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-      }
+  // At the beginning of tile t's work K of tile t + 2 and V of tile t + 1 go to LDS, and are complete long before the barrier at its end:
+  // 8-bit tiles from registers, which the fetches fill again with the tiles behind; 16-bit ones from memory.
+  auto bring_k = [&](int t, int at) __attribute__((always_inline)) {
+    if constexpr (!k8) fetch_k(t, place[at]);
+    there[at] = (uint32_t)__ballot(slot_id >= 0) & 15;
+    k_scale[at] = slot_scale;
+    store_k(place[at]);
+    if constexpr (k8) fetch_k(t + 1, 0);
   };
-  auto score = [&](auto st, auto blk, f32x16& s) __attribute__((always_inline)) {
-#pragma unroll
-    for (int e = 0; e < 16; ++e) s[e] = 0.f;
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i) s = mfma32(*lds_ptr<const elem8>(k_lane + (st * kStage + (blk * kSteps + i) * 1024)), bq[i], s);
+  auto bring_v = [&](int t, int at) __attribute__((always_inline)) {
+    if constexpr (!k8) fetch_v(t, v_place[at]);
+    store_v(t, v_place[at], there[at]);
+    if constexpr (k8) fetch_v(t + 1, 0);
   };
-  // f: the factors of the scores' halves (of 16 keys; not negative: see bq)
-  auto mask_and_max = [&](int key0, auto blk, f32x16& s, float (&f)[2]) __attribute__((always_inline)) {
-    f[0] = k8 ? k_scale[2 * blk] : scale;
-    f[1] = k8 ? k_scale[2 * blk + 1] : scale;
-    const uint32_t has = (there >> (2 * blk)) & 3;
-    if (__builtin_expect(key0 + 31 > first_masked || has != 3, 0)) {
+  auto next_ids = [&](int t) __attribute__((always_inline)) {
+    if constexpr (k8) {
+#pragma unroll
+      for (int c = 0; c < kPieces; ++c) v_ids[c] = ids[c];
+    } else {
+      v_ids[0] = v_id;
+    }
+    fetch_ids(t);
+  };
+  auto barrier = [&]() __attribute__((always_inline)) {
+    // (the wave's LDS instructions are done; loads to registers may be on their way)
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  };
+
+  auto k_frag = [&](uint32_t st, int blk, int i) __attribute__((always_inline)) {
+    return *lds_ptr<const elem8>(k_lane + st + (blk * kSteps + i) * 1024);
+  };
+  auto v_frag = [&](uint32_t st, int blk, int j2, int db) __attribute__((always_inline)) {
+    const uint32_t at = v_lane + st + (db * 4096 + (8 * blk + 4 * j2) * 128);   // keys 4hh .., and 8 + 4hh .. of 16
+    const velem4 x = lds_read_tr<velem4>(at), y = lds_read_tr<velem4>(at + 256);
+    return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  // masks what a row does not see of a block's scores; f: the factors of their halves (of 16 keys)
+  auto mask = [&](int key0, int blk, int tile, f32x16& s, float (&f)[2]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) f[half] = k8 ? lane_value(k_scale[tile], 2 * blk + half) * scale : scale;
+    const uint32_t has = (there[tile] >> (2 * blk)) & 3;
+    if (__builtin_expect(key0 + 32 * blk + 31 > first_masked || has != 3, 0)) {
       asm volatile("");   // (a branch, not sixteen comparisons in every block)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         s[e] *= f[e >> 3];
-        if (key0 + 8 * (e >> 2) + 4 * hh + (e & 3) > limit || !(has & (1 << (e >> 3)))) s[e] = -INFINITY;
+        if (key0 + 32 * blk + 8 * (e >> 2) + 4 * hh + (e & 3) > limit || !(has & (1 << (e >> 3)))) s[e] = -INFINITY;
       }
       f[0] = f[1] = 1.f;
     }
+  };
+  auto largest = [&](const f32x16& s, const float (&f)[2]) __attribute__((always_inline)) {   // of a row's scores
     float mx[2];
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
@@ -758,119 +792,183 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(const Pa
 #pragma unroll
       for (int e = 1; e < 8; ++e) mx[half] = fmaxf(mx[half], s[8 * half + e]);
     }
-    const float m = max_xhalf(fmaxf(mx[0] * f[0], mx[1] * f[1]));
-    if (__any(m > m_run + kMaxLag)) {
-      const float m_new = m > m_run + kMaxLag ? m : m_run;
-      const float alpha = fast_exp2(m_run - m_new);
-      m_run = m_new;
-      l_run *= alpha;
-#pragma unroll
-      for (int db = 0; db < kDb; ++db)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) oacc[db][e] *= alpha;
-    }
+    return max_xhalf(fmaxf(mx[0] * f[0], mx[1] * f[1]));
   };
-  velem8 hi[2], lo[2];
-  auto probabilities = [&](f32x16& s, const float (&f)[2]) __attribute__((always_inline)) {
+  velem8 hi[2], lo[2];   // a block's probabilities
+  auto exponentials = [&](f32x16& s, const float (&f)[2], int from, int to) __attribute__((always_inline)) {
     const float ref = m_run - ProbShift<V>::value;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
+    for (int e = from; e < to; ++e) {
       s[e] = fast_exp2(fmaf(s[e], f[e >> 3], -ref));
       l_run += s[e];
-    }
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const velem h = (velem)s[e];
-      hi[e >> 3][e & 7] = h;
-      if constexpr (kParts == 2) lo[e >> 3][e & 7] = (velem)(s[e] - (float)h);
+      asm volatile("" : "+v"(s[e]), "+v"(l_run));
     }
   };
-  auto add_values = [&]() __attribute__((always_inline)) {
+  auto pack = [&](const f32x16& s, int half) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j2 = 0; j2 < 2; ++j2)
-#pragma unroll
-      for (int db = 0; db < kDb; ++db) oacc[db] = mfma32(va[j2][db], hi[j2], oacc[db]);
-    if constexpr (kParts == 2) {
-#pragma unroll
-      for (int j2 = 0; j2 < 2; ++j2)
-#pragma unroll
-        for (int db = 0; db < kDb; ++db) oacc[db] = mfma32(va[j2][db], lo[j2], oacc[db]);
+    for (int e = 0; e < 8; ++e) {
+      const velem h = (velem)s[8 * half + e];
+      hi[half][e] = h;
+      if constexpr (kParts == 2) lo[half][e] = (velem)(s[8 * half + e] - (float)h);
     }
   };
-  // the slots of the tile that has been brought to LDS are those of the tile at hand
-  auto take_slots = [&]() __attribute__((always_inline)) {
-    there = taken();
-    if constexpr (k8) {
+
+  // All keys of the run, in blocks of 32, by hand in slots of one matrix instruction and the vector instructions beside it: the
+  // scores of the next block under the second half of this one's exponentials, this one's probabilities times V under
+  // the first half of the next one's.  kFixed: relative to the maximum of the first block (false where a row has none);
+  // otherwise with a running maximum.
+  auto all_keys = [&](auto fixed) __attribute__((always_inline)) {
+    constexpr bool kFixed = fixed;
 #pragma unroll
-      for (int slot = 0; slot < 4; ++slot) k_scale[slot] = lane_value(taken_scale, slot) * scale;
-    }
-  };
-  f32x16 s0, s1;
-  float f0[2], f1[2];
-  // Tile t + 1 goes to LDS at the beginning of tile t's work, and is complete long before the barrier at its end: 8-bit tiles
-  // from registers, which fetch fills again with the tile behind it; 16-bit ones from memory.  (Stored just before the barrier, 8-bit tiles
-  // took 1.39 ms for 2048 tokens against 34816 keys.)
-  auto bring = [&](int t, auto st) __attribute__((always_inline)) {
-    if constexpr (!k8) fetch(t);
-    taken_id = slot_id;
-    taken_scale = slot_scale;
-    store(t, st);
-    if constexpr (k8) fetch(t + 1);
-    fetch_ids(t + (k8 ? 2 : 1));
-  };
-  auto barrier = [&]() __attribute__((always_inline)) {
-    // (the wave's LDS instructions are done; loads to registers may be on their way)
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-  };
-  if (tiles > 0) {
+    for (int i = 0; i < 3; ++i) place[i] = i * kTileBytes;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) v_place[i] = (3 + i) * kTileBytes;
     fetch_ids(0);
     if constexpr (k8) {
-      fetch(0);
-      fetch_ids(1);
+      fetch_k(0, 0);
+      next_ids(1);
+      fetch_v(0, 0);
     }
-    bring(0, k0);
-    landed(0, k0);
+    bring_k(0, 0);
+    next_ids(k8 ? 2 : 1);
+    bring_v(0, 0);
+    landed(0, v_place[0], there[0]);
+    bring_k(1, 1);
+    next_ids(k8 ? 3 : 2);
     barrier();
-  }
-  // (the stage is a constant of each copy of the body, and part of its LDS instructions)
-  auto tile = [&](int t, auto st, auto more) __attribute__((always_inline)) {
-    constexpr std::integral_constant<int, 1 - st> other;
-    const int key0 = key_lo + t * kManyKeys;
-    take_slots();
-    if constexpr (more) bring(t + 1, other);
-    __builtin_amdgcn_s_setprio(1);
-    score(st, k0, s0);
-    __builtin_amdgcn_s_setprio(0);
-    mask_and_max(key0, k0, s0, f0);
-    read_v(st, k0);
-    probabilities(s0, f0);
-    __builtin_amdgcn_s_setprio(1);
-    add_values();
-    score(st, k1, s1);
-    __builtin_amdgcn_s_setprio(0);
-    mask_and_max(key0 + 32, k1, s1, f1);
-    read_v(st, k1);
-    probabilities(s1, f1);
-    __builtin_amdgcn_s_setprio(1);
-    add_values();
-    __builtin_amdgcn_s_setprio(0);
-    if constexpr (more) {
-      landed(t + 1, other);
-      barrier();        // tile t + 1 is complete, and nobody reads tile t any more
+#pragma unroll
+    for (int db = 0; db < kDb; ++db)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) oacc[db][e] = 0.f;
+    l_run = 0.f;
+    f32x16 s0, s1;
+    float f0[2], f1[2];
+    elem8 ahead[kSteps / 2];   // the first K fragments of the next scores
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s0[e] = 0.f;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) s0 = mfma32(k_frag(0, 0, i), bq[i], s0);
+#pragma unroll
+    for (int i = 0; i < kSteps / 2; ++i) ahead[i] = k_frag(0, 1, i);
+    mask(key_lo, 0, 0, s0, f0);
+    const float m = largest(s0, f0);
+    const bool found = m > kNoMax;
+    m_run = found ? m : kFixed ? 0.f : kNoMax;
+    exponentials(s0, f0, 0, 8);
+    pack(s0, 0);
+
+    // sc: the scores of block blk of the tile at hand, of which the first half is in hi[0]; sn takes those of the next block, in
+    // tile `next` of the three; then, K fragments of block `blk` of tile 1 are next
+    auto step = [&](f32x16& sc, float (&fc)[2], f32x16& sn, float (&fn)[2], auto blk, auto has_next, int key0, bool more)
+        __attribute__((always_inline)) {
+      constexpr int kNext = blk;   // tile of the next block
+      velem8 va[2][kDb];
+      elem8 ka[kSteps];
+      if constexpr (has_next) {
+#pragma unroll
+        for (int i = 0; i < kSteps / 2; ++i) ka[i] = ahead[i];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sn[e] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        if constexpr (has_next) {
+          if (i + kSteps / 2 < kSteps) ka[i + kSteps / 2] = k_frag(place[kNext], 1 - blk, i + kSteps / 2);
+          sn = mfma32(ka[i], bq[i], sn);
+        }
+        exponentials(sc, fc, 8 + 8 * i / kSteps, 8 + 8 * (i + 1) / kSteps);
+        if (i >= kSteps / 2) {
+#pragma unroll
+          for (int db = (i - kSteps / 2) * kDb * 2 / kSteps; db < (i - kSteps / 2 + 1) * kDb * 2 / kSteps; ++db)
+            va[0][db] = v_frag(v_place[0], blk, 0, db);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      pack(sc, 1);
+      if constexpr (has_next) mask(key0 + kNext * kManyKeys, 1 - blk, kNext, sn, fn);
+#pragma unroll
+      for (int k = 0; k < 2 * kDb; ++k) {
+        if (k < kDb) va[1][k] = v_frag(v_place[0], blk, 1, k);
+        if constexpr (has_next) {
+          if (k >= kDb && more) {
+#pragma unroll
+            for (int i = (k - kDb) * kSteps / (2 * kDb); i < (k - kDb + 1) * kSteps / (2 * kDb); ++i) ahead[i] = k_frag(place[1], blk, i);
+          }
+        }
+        oacc[k % kDb] = mfma32(va[k / kDb][k % kDb], hi[k / kDb], oacc[k % kDb]);
+        if constexpr (kParts == 2) oacc[k % kDb] = mfma32(va[k / kDb][k % kDb], lo[k / kDb], oacc[k % kDb]);
+        if constexpr (has_next && kFixed) {   // (the first slot is left to the last score product's result)
+          const int from = k == 0 ? 0 : 8 * (k - 1) / (2 * kDb - 1), to = k == 0 ? 0 : 8 * k / (2 * kDb - 1);
+          exponentials(sn, fn, from, to);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if constexpr (has_next && !kFixed) {
+        const float mm = largest(sn, fn);
+        if (__any(mm > m_run + kMaxLag)) {
+          const float m_new = mm > m_run + kMaxLag ? mm : m_run;
+          const float alpha = fast_exp2(m_run - m_new);
+          m_run = m_new;
+          l_run *= alpha;
+#pragma unroll
+          for (int db = 0; db < kDb; ++db)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) oacc[db][e] *= alpha;
+        }
+        exponentials(sn, fn, 0, 8);
+      }
+      if constexpr (has_next) pack(sn, 0);
+    };
+    constexpr std::integral_constant<int, 0> k0;
+    constexpr std::integral_constant<int, 1> k1;
+    int key0 = key_lo;
+    for (int t = 0; t + 1 < tiles; ++t, key0 += kManyKeys) {
+      const bool two_more = t + 2 < tiles;
+      if (two_more) bring_k(t + 2, 2);
+      bring_v(t + 1, 1);
+      next_ids(t + (k8 ? 4 : 3));
+      if constexpr (kWaves == 4) __builtin_amdgcn_s_setprio(1);
+      step(s0, f0, s1, f1, k0, std::true_type{}, key0, true);
+      step(s1, f1, s0, f0, k1, std::true_type{}, key0, true);
+      if constexpr (kWaves == 4) __builtin_amdgcn_s_setprio(0);
+      landed(t + 1, v_place[1], there[1]);
+      barrier();   // what was brought is complete, and nobody reads tile t any more
+      const uint32_t free = place[0];
+      place[0] = place[1]; place[1] = place[2]; place[2] = free;
+      const uint32_t v_free = v_place[0];
+      v_place[0] = v_place[1]; v_place[1] = v_free;
+      there[0] = there[1]; there[1] = there[2];
+      k_scale[0] = k_scale[1]; k_scale[1] = k_scale[2];
     }
+    step(s0, f0, s1, f1, k0, std::true_type{}, key0, false);
+    step(s1, f1, s0, f0, k1, std::false_type{}, key0, false);
+    return found;
   };
-  constexpr std::integral_constant<bool, true> more;
-  constexpr std::integral_constant<bool, false> last;
-  int t = 0;
-  for (; t + 2 < tiles; t += 2) {
-    tile(t, k0, more);
-    tile(t + 1, k1, more);
-  }
-  if (t + 1 < tiles) {
-    tile(t, k0, more);
-    tile(t + 1, k1, last);
-  } else if (t < tiles) {
-    tile(t, k0, last);
+  if (tiles > 0) {
+    constexpr bool kFixed = std::is_same_v<V, Bf16>;
+    bool again = !kFixed;
+    if constexpr (kFixed) {
+      const bool found = all_keys(std::true_type{});
+      const float sum = sum_xhalf(l_run);
+      // (a row whose first keys have no page has no reference)
+      const bool bad = wave_row + n < rows && (float_bits(sum) >= float_bits(0x1p96f) || any_not_finite(oacc) || (!found && limit >= key_lo));
+      __syncthreads();   // (everybody has read the last tile)
+      volatile int* const flags = reinterpret_cast<volatile int*>(smem);
+      const bool any_bad = __any(bad);
+      if (lane == 0) flags[wave] = any_bad;
+      __syncthreads();
+      int some = 0;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) some |= flags[w];
+      again = __builtin_amdgcn_readfirstlane(some) != 0;
+      __syncthreads();   // (everybody has read the flags)
+    }
+    if (__builtin_expect(again, 0)) all_keys(std::false_type{});
+  } else {
+#pragma unroll
+    for (int db = 0; db < kDb; ++db)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) oacc[db][e] = 0.f;
   }
   if (!works) return;   // (no barrier follows)
   if (__builtin_expect(__any(any_not_finite(oacc)), 0))
@@ -887,7 +985,7 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(const Pa
       *reinterpret_cast<u32x2*>(to + 8 * i) = u32x2{pack2<E>(o[e] * inv, o[e + 1] * inv), pack2<E>(o[e + 2] * inv, o[e + 3] * inv)};
     }
   } else {
-    const int64_t prow = (int64_t)blockIdx.x * kManyRows + 32 * wave + n;
+    const int64_t prow = (int64_t)blockIdx.x * kRows + 32 * wave + n;
 #pragma unroll
     for (int i = 0; i < 4 * kDb; ++i) {
       const f32x16& o = oacc[i >> 2];
@@ -1009,7 +1107,10 @@ static Cuts paged_cuts(int64_t T, int B, int rep, int Hkv, int D, bool cache8, i
   const bool many = most_new * rep > kFewRows;
   c.few = bounded_cut({kFewRows, kFewTile, 0, many ? kFewRows : 0x7fffffff, target(D == 128 && !cache8 ? 1 : 2), 0, 0}, T, B, rep);
   c.many = {};
-  if (many) c.many = bounded_cut({kManyRows, kManyKeys, kFewRows, 0x7fffffff, target(2), 0, 0}, T, B, rep);
+  if (many) {
+    const int waves = D == 128 && cache8 ? kManyWaves<128, true> : kManyWaves<64, false>;
+    c.many = bounded_cut({32 * waves, kManyKeys, kFewRows, 0x7fffffff, target(8 / waves), 0, 0}, T, B, rep);
+  }
   return c;
 }
 
@@ -1035,7 +1136,7 @@ static int launch_paged(const PagedParams<E>& p, hipStream_t st) {
   if (p.many.most > 0) {
     const auto many = paged_many_kernel<E, D, k8>;
     if (!allow_dynamic_lds((const void*)many, many_lds_bytes<D>(), allowed[1])) return MOBA_ERR_LAUNCH;
-    hipLaunchKernelGGL(many, dim3((unsigned)p.many.most * p.shape.Hkv), dim3(64 * kManyWaves), many_lds_bytes<D>(), st, p);
+    hipLaunchKernelGGL(many, dim3((unsigned)p.many.most * p.shape.Hkv), dim3(64 * (kManyWaves<D, k8>)), many_lds_bytes<D>(), st, p);
   }
   const int64_t rows = (int64_t)p.shape.table.T * p.shape.H;
   const int heads = rows <= 8192 ? 1 : p.shape.H;

@@ -87,6 +87,26 @@ def test_any_scales(dtype):
         check_attention(batch, paged_attention(q.cuda(), batch.cache(), *batch.index(), scaling=scaling), q, scaling)
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("quantized", [True, False])
+@pytest.mark.parametrize("d", [64, 128])
+def test_first_keys_that_say_nothing_of_the_others(d, quantized, dtype):
+    """Many rows whose first keys have no page, or scores far above or below those that follow."""
+    from moba_amd import paged_attention
+    for change in ("none", "above", "below"):
+        batch = Batch([150, 0, 300], [40, 90, 17], 16, 2, d, dtype, quantized, seed=9)
+        q, = batch.tensors(8)
+        q, keys = q.abs() * 40, batch.pages[0]
+        if change == "none":
+            batch.table[0, :3], batch.table[1, :2], batch.table[2, 0] = -1, -1, -1
+        else:
+            first = [int(batch.table[b, i]) for b in range(3) for i in range(2)]
+            for page in range(keys.shape[0]):     # scores of some hundreds of either sign, or small
+                sign = 1 if change == "above" else -1
+                keys[page] = (keys[page].float().abs() * (sign if page in first else 0.05)).to(keys.dtype)
+        check_attention(batch, paged_attention(q.cuda(), batch.cache(), *batch.index()), q)
+
+
 @pytest.mark.parametrize("quantized", [True, False])
 def test_values_that_are_not_finite(quantized):
     """They reach the rows that see them; what lies behind a sequence's end, or in other sequences' pages, reaches nobody."""
