@@ -523,7 +523,8 @@ template <int D, bool k8> constexpr int kManyWaves = D == 128 && k8 ? 8 : 4;
 // constant of the instruction, and no two lanes meet in a bank:
 //   K  for each block of 32 keys and step of 16 elements the 64 lanes' 16 bytes, lane (n, hh): elements 8hh .. of key n
 //   V  for each 16 elements and 4 keys (16 such in a row) 128 bytes, the keys one behind the other, which a transposing read of
-//      16 lanes takes
+//      16 lanes takes; of odd 16 elements every two of these have changed places, so that the even and the odd that are read
+//      together lie in different banks
 // (Rows instead, their columns swizzled by exclusive or, took 13 address registers more; rows with 32 bytes between them, three times the
 // bank conflicts.)
 template <int D>
@@ -594,7 +595,7 @@ __global__ __launch_bounds__(64 * (kManyWaves<D, k8>), 2) void paged_many_kernel
   constexpr int kLookups = k8 ? kPieces : 2;
   const int col = k8 ? tid / kKeysAtOnce : 0;
   auto key_of = [&](int c) { return (k8 ? tid % kKeysAtOnce : n) + c * kKeysAtOnce; };
-  const int v_key = 32 * (wave & 1) + 4 * (lane >> 3) + ((lane & 7) >> 1);   // 16-bit: of V
+  const int v_key = 32 * (wave & 1) + 4 * ((lane >> 3) ^ ((wave >> 1) & 1)) + ((lane & 7) >> 1);   // 16-bit: of V
   uint32_t in_page[kLookups];
 #pragma unroll
   for (int c = 0; c < kLookups; ++c) in_page[c] = (key_of(c) & page_mask) * kRow + (k8 ? col : hh) * 16;
@@ -680,7 +681,7 @@ __global__ __launch_bounds__(64 * (kManyWaves<D, k8>), 2) void paged_many_kernel
 #pragma unroll
         for (int c = 0; c < kPieces; ++c) {
           const int key = key_of(c);
-          const uint32_t at = lds + to + (col * 16 + (key >> 2)) * 128 + (key & 3) * 32;
+          const uint32_t at = lds + to + (col * 16 + ((key >> 2) ^ (col & 1))) * 128 + (key & 3) * 32;
           u32x4 w = raw[1][c];
           bf16x8 v0, v1;
           if constexpr (plain) {
@@ -729,7 +730,7 @@ __global__ __launch_bounds__(64 * (kManyWaves<D, k8>), 2) void paged_many_kernel
   }
   const float scale = fabsf(p.scale_log2);
   const uint32_t k_lane = lds + lane * 16;
-  const uint32_t v_lane = lds + ((lane >> 4) & 1) * 2048 + hh * 128 + (lane & 15) * 8;
+  const uint32_t v_lane = lds + ((lane >> 4) & 1) * 2048 + (hh ^ ((lane >> 4) & 1)) * 128 + (lane & 15) * 8;
   f32x16 oacc[kDb];
   float m_run = kNoMax, l_run = 0.f;
 
