@@ -8,6 +8,8 @@
 // Bound by memory: 4 bytes an element forward, 6 backward (x is read again: its mean square is a few instructions and
 // spares a saved copy).  A wave takes a token, makes the token's angles once for all of its heads, and goes through
 // them 4 or 8 rows at a time, the next ones on their way meanwhile; with few tokens several waves share a token's heads.
+// 131072 tokens, 40 heads of 128: 2.68 GB in 0.49 ms, 5.5 TB/s, what a copy reaches; 20480 tokens, 10 heads: 105 MB in 24.6 us
+// forward, 157 MB in 38.2 backward and 3.9 for the weights' sums; one token: 3.6.
 #include "rotary.h"
 #include <type_traits>
 

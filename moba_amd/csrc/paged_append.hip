@@ -10,7 +10,8 @@
 // Bound by memory for prompts, by latency for single tokens.  The angles of the page's tokens are made once for all heads, by
 // all waves, and wait in LDS; the rows go by groups of heads, two rows to a lane, which stay in registers, turned, until the
 // group's maxima are known, while the next group's are on their way (read again instead, from L2 or memory, a prompt of
-// 131072 tokens took 640 us).
+// 131072 tokens took 640 us).  That prompt, 32 and 8 heads, with its queries: 2.95 GB in 595 us, 5.0 TB/s; sixteen sequences of
+// one new token: 6.9 us, a chain of lookup, row, maxima, the page's earlier tokens.
 #include "paged.h"
 #include "rotary.h"
 
