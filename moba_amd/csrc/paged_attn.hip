@@ -24,7 +24,7 @@
 // hold whatever was there.)
 //
 //   paged_few_kernel    one run of keys: out itself; several: the run's rows (normalised) and their log-sum-exps (base 2)
-//   paged_many_kernel   the same for sequences of more than 32 rows
+//   paged_many_kernel   the same for sequences of more rows
 //   paged_merge_kernel  the runs of a row together; zeros where there is nothing to see
 #include "attn_common.h"
 #include "paged_cut.h"
@@ -932,10 +932,12 @@ __global__ __launch_bounds__(64 * (kManyWaves<D, k8>), 2) void paged_many_kernel
       if (two_more) bring_k(t + 2, 2);
       bring_v(t + 1, 1);
       next_ids(t + (k8 ? 4 : 3));
-      if constexpr (kWaves == 4) __builtin_amdgcn_s_setprio(1);
-      step(s0, f0, s1, f1, k0, std::true_type{}, key0, true);
-      step(s1, f1, s0, f0, k1, std::true_type{}, key0, true);
-      if constexpr (kWaves == 4) __builtin_amdgcn_s_setprio(0);
+      if (works) {
+        if constexpr (kWaves == 4) __builtin_amdgcn_s_setprio(1);
+        step(s0, f0, s1, f1, k0, std::true_type{}, key0, true);
+        step(s1, f1, s0, f0, k1, std::true_type{}, key0, true);
+        if constexpr (kWaves == 4) __builtin_amdgcn_s_setprio(0);
+      }
       landed(t + 1, v_place[1], there[1]);
       barrier();   // what was brought is complete, and nobody reads tile t any more
       const uint32_t free = place[0];
@@ -1100,8 +1102,8 @@ static Cut bounded_cut(Cut c, int64_t T, int B, int rep) {
   return c;
 }
 
-// One round of workgroups, two to a compute unit (one where a wave's blocks are large).  Sequences of more than 32 rows per
-// key/value head go to the many-row kernel, if it is launched: if there may be any.
+// One round of workgroups, two to a compute unit (one where a wave's blocks are large).  Sequences of many rows per key/value head
+// go to the many-row kernel, if it is launched: if there may be any.
 struct Cuts {
   Cut few, many;
 };
@@ -1110,12 +1112,17 @@ static Cuts paged_cuts(int64_t T, int B, int rep, int Hkv, int D, bool cache8, i
   auto target = [&](int per_cu) { return per_cu * cus / Hkv > 0 ? per_cu * cus / Hkv : 1; };
   const int64_t most_new = max_new >= 0 && max_new < T ? max_new : T;
   Cuts c;
-  const bool many = most_new * rep > kFewRows;
-  c.few = bounded_cut({kFewRows, kFewTile, 0, many ? kFewRows : 0x7fffffff, target(D == 128 && !cache8 ? 1 : 2), 0, 0}, T, B, rep);
+  // 8-bit pages: up to 64 rows are few, in two groups of which the second finds the keys in L2.  16 sequences of 64 rows against 8192
+  // keys, 8 heads: 100 us, as many rows 112; 64 of 40 against 2048: 86 and 101; one of 64 against 131072, one head: 30 and 32.  128
+  // rows would be faster for 8 heads (one sequence, 4096 keys: 21 and 27) and slower for one (16 sequences, 8192 keys: 42 and 33).
+  // 16-bit pages are twice the bytes: up to 32 rows (16 of 64 rows, one head: 30 us as many rows, 35 as few; 64 of 40: 110 and 135).
+  const int few_rows = cache8 ? 2 * kFewRows : kFewRows;
+  const bool many = most_new * rep > few_rows;
+  c.few = bounded_cut({kFewRows, kFewTile, 0, many ? few_rows : 0x7fffffff, target(D == 128 && !cache8 ? 1 : 2), 0, 0}, T, B, rep);
   c.many = {};
   if (many) {
     const int waves = D == 128 && cache8 ? kManyWaves<128, true> : kManyWaves<64, false>;
-    c.many = bounded_cut({32 * waves, kManyKeys, kFewRows, 0x7fffffff, target(8 / waves), 0, 0}, T, B, rep);
+    c.many = bounded_cut({32 * waves, kManyKeys, few_rows, 0x7fffffff, target(8 / waves), 0, 0}, T, B, rep);
   }
   return c;
 }
