@@ -837,9 +837,9 @@ __global__ __launch_bounds__(64 * (kManyWaves<D, k8>), 2) void paged_many_kernel
     bring_k(0, 0);
     next_ids(k8 ? 2 : 1);
     bring_v(0, 0);
-    landed(0, v_place[0], there[0]);
     bring_k(1, 1);
     next_ids(k8 ? 3 : 2);
+    landed(0, v_place[0], there[0]);   // (16-bit: K of tile 1 among what is waited for)
     barrier();
 #pragma unroll
     for (int db = 0; db < kDb; ++db)
