@@ -1003,21 +1003,24 @@ __global__ __launch_bounds__(64 * (kManyWaves<D, k8>), 2) void paged_many_kernel
   }
 }
 
-// A workgroup takes `heads` heads of a token, one after the other: four waves take a quarter of the runs each, a lane owns
-// D / 64 elements; the four sums meet in LDS.  Rows of one run are there already.  Bound by its chain of reads (sequence, its
-// number of runs, log-sum-exps and rows): 4.7 us.
-template <class E, int D>
+// `heads` heads of a token, one after the other, for kShare waves, a lane for D / 64 elements.  Four waves (few tokens, which may
+// have many runs) take a quarter of the runs each, their sums meet in LDS; one wave needs neither.  Rows of one run are there already.
+// Bound by its chain of reads (sequence, its number of runs, log-sum-exps and rows): 4.7 us for one token.
+template <class E, int D, int kShare>
 __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams<E> p, int heads) {
   typedef typename E::elem elem;
   constexpr int kPer = D / 64;
   typedef float fvec __attribute__((ext_vector_type(kPer)));
   __shared__ float red[4][D];
   __shared__ float red_l[4];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave_in_group = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = kShare == 4 ? wave_in_group : 0;
   const Shape& shape = p.shape;
   const PageTable& table = shape.table;
-  const int per_token = shape.H / heads;
-  const int t = (int)blockIdx.x / per_token, h0 = ((int)blockIdx.x - t * per_token) * heads;
+  const int per_token = (shape.H + heads - 1) / heads;
+  const int item = kShare == 4 ? (int)blockIdx.x : (int)blockIdx.x * 4 + wave_in_group;
+  const int t = item / per_token, h0 = (item - t * per_token) * heads;
+  if (t >= table.T) return;
   Sequence seq = {0, 0, 0};
   const int b = last_up_to(table, t, lane, seq, [](int, int lo) { return (int64_t)lo; });
   Runs r = {0, 0, 0};
@@ -1034,22 +1037,22 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams<E> p
   const float* const part_lse = is_many ? p.many_lse : p.few_lse;
   // (numbers that no unit has left, where the row ranges are none)
   if (r.first < 0 || r.runs < 0 || r.groups < 1 || r.first + (int64_t)r.runs * r.groups > cut.parts) r.runs = 0;
-  for (int h = h0; h < h0 + heads; ++h) {
+  for (int h = h0; h < min(h0 + heads, shape.H); ++h) {
     const int hkv = h / shape.rep, row = row_in_seq + h - hkv * shape.rep;
     int group = row / cut.group_rows;
     const int rr = row - group * cut.group_rows;
     if (is_many) group = r.groups - 1 - group;
     if (group < 0 || group >= r.groups) r.runs = 0;
     auto part = [&](int i) { return ((r.first + (int64_t)i * r.groups + group) * shape.Hkv + hkv) * cut.group_rows + rr; };
-    // Rows and log-sum-exps of up to 64 runs are asked for together, a wave's quarter of the rows and, lane by lane, all of
-    // the others; more runs come 64 at a time, with a running maximum.
+    // Rows and log-sum-exps of some runs are asked for together, a wave's share of the rows and, lane by lane, all of
+    // the others; more runs come as many at a time, with a running maximum.
     float top = kNoMax, ll = 0.f, o[kPer] = {};
-    auto some = [&](int i0, auto count) __attribute__((always_inline)) {   // runs i0 .., 4 * count of them
+    auto some = [&](int i0, auto count) __attribute__((always_inline)) {   // runs i0 .., kShare * count of them
       fvec x[count];
 #pragma unroll
       for (int k = 0; k < count; ++k)
-        x[k] = *reinterpret_cast<const fvec*>(part_o + part(min(i0 + 4 * k + wave, r.runs - 1)) * D + kPer * lane);
-      const float lse = i0 + lane < r.runs && lane < 4 * count ? part_lse[part(i0 + lane)] : -INFINITY;
+        x[k] = *reinterpret_cast<const fvec*>(part_o + part(min(i0 + kShare * k + wave, r.runs - 1)) * D + kPer * lane);
+      const float lse = i0 + lane < r.runs && lane < kShare * count ? part_lse[part(i0 + lane)] : -INFINITY;
       float mm = lse;
 #pragma unroll
       for (int d = 32; d >= 1; d >>= 1) mm = fmaxf(mm, __shfl_xor(mm, d, 64));
@@ -1061,25 +1064,33 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams<E> p
       for (int e = 0; e < kPer; ++e) o[e] *= former;
 #pragma unroll
       for (int k = 0; k < count; ++k) {
-        const float wk = lane_value(w, 4 * k + wave);   // (0 behind the last)
+        const float wk = lane_value(w, kShare * k + wave);   // (0 behind the last)
         ll += wk;
 #pragma unroll
         for (int e = 0; e < kPer; ++e) o[e] += wk * x[k][e];
       }
     };
-    if (r.runs > 0 && r.runs <= 16) some(0, std::integral_constant<int, 4>{});
+    if (r.runs > 0 && r.runs <= 4 * kShare) some(0, std::integral_constant<int, 4>{});
+    else if (kShare == 1 && r.runs > 0 && r.runs <= 8) some(0, std::integral_constant<int, 8>{});
     else
-      for (int i0 = 0; i0 < r.runs; i0 += 64) some(i0, std::integral_constant<int, 16>{});
+      for (int i0 = 0; i0 < r.runs; i0 += 16 * kShare) some(i0, std::integral_constant<int, 16>{});
+    if constexpr (kShare == 1) {
+      const float inv = ll == 0.f ? 0.f : 1.f / ll;
+      elem* const to = p.out + ((int64_t)t * shape.H + h) * D + kPer * lane;
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) red[wave][kPer * lane + e] = o[e];
-    if (lane == 0) red_l[wave] = ll;
-    __syncthreads();
-    if (threadIdx.x < D) {
-      const int d = threadIdx.x;
-      const float l4 = red_l[0] + red_l[1] + red_l[2] + red_l[3];
-      p.out[((int64_t)t * shape.H + h) * D + d] = (elem)(l4 == 0.f ? 0.f : (red[0][d] + red[1][d] + red[2][d] + red[3][d]) / l4);
+      for (int e = 0; e < kPer; ++e) to[e] = (elem)(o[e] * inv);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) red[wave][kPer * lane + e] = o[e];
+      if (lane == 0) red_l[wave] = ll;
+      __syncthreads();
+      if (threadIdx.x < D) {
+        const int d = threadIdx.x;
+        const float l4 = red_l[0] + red_l[1] + red_l[2] + red_l[3];
+        p.out[((int64_t)t * shape.H + h) * D + d] = (elem)(l4 == 0.f ? 0.f : (red[0][d] + red[1][d] + red[2][d] + red[3][d]) / l4);
+      }
+      __syncthreads();
     }
-    __syncthreads();
   }
 }
 
@@ -1152,8 +1163,16 @@ static int launch_paged(const PagedParams<E>& p, hipStream_t st) {
     hipLaunchKernelGGL(many, dim3((unsigned)p.many.most * p.shape.Hkv), dim3(64 * (kManyWaves<D, k8>)), many_lds_bytes<D>(), st, p);
   }
   const int64_t rows = (int64_t)p.shape.table.T * p.shape.H;
-  const int heads = rows <= 8192 ? 1 : p.shape.H;
-  hipLaunchKernelGGL((paged_merge_kernel<E, D>), dim3((unsigned)(rows / heads)), dim3(256), 0, st, p, heads);
+  // (a wave to a row from some thousand rows on: 774 tokens of 16 heads, five runs each, 29.7 us with four, 9.8 so; 136 of 8, up to 60
+  // runs: 5.3 and 4.0; 69 of 8 and less are equal, 37 of 8, up to 256 runs: 9 with four, 16 so)
+  if (rows <= 1024) {
+    hipLaunchKernelGGL((paged_merge_kernel<E, D, 4>), dim3((unsigned)rows), dim3(256), 0, st, p, 1);
+  } else {
+    const int64_t want = (rows + 16383) / 16384;
+    const int heads = (int)(want < p.shape.H ? want : p.shape.H), per_token = (p.shape.H + heads - 1) / heads;
+    const int64_t waves = (int64_t)p.shape.table.T * per_token;
+    hipLaunchKernelGGL((paged_merge_kernel<E, D, 1>), dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, st, p, heads);
+  }
   return launch_check.result();
 }
 
