@@ -1129,11 +1129,13 @@ static Cuts paged_cuts(int64_t T, int B, int rep, int Hkv, int D, bool cache8, i
   // 16-bit pages are twice the bytes: up to 32 rows (16 of 64 rows, one head: 30 us as many rows, 35 as few; 64 of 40: 110 and 135).
   const int few_rows = cache8 ? 2 * kFewRows : kFewRows;
   const bool many = most_new * rep > few_rows;
-  c.few = bounded_cut({kFewRows, kFewTile, 0, many ? few_rows : 0x7fffffff, target(D == 128 && !cache8 ? 1 : 2), 0, 0}, T, B, rep);
+  c.few = bounded_cut({kFewRows, kFewTile, 1, 0, many ? few_rows : 0x7fffffff, target(D == 128 && !cache8 ? 1 : 2), 0, 0}, T, B, rep);
   c.many = {};
   if (many) {
     const int waves = D == 128 && cache8 ? kManyWaves<128, true> : kManyWaves<64, false>;
-    c.many = bounded_cut({32 * waves, kManyKeys, few_rows, 0x7fffffff, target(8 / waves), 0, 0}, T, B, rep);
+    // (695 tokens and 204 against 883 and 151, 5 heads on one: 30.0 us with runs of any length, 24.4 with at least four tiles, 24.6 with
+    // six; 609 tokens of 8 heads: 27.5, 21, 21)
+    c.many = bounded_cut({32 * waves, kManyKeys, 4, few_rows, 0x7fffffff, target(8 / waves), 0, 0}, T, B, rep);
   }
   return c;
 }

@@ -13,7 +13,8 @@ namespace moba {
 // Of sequences with more than rows_over and at most rows_up_to query rows per key/value head:
 struct Cut {
   int group_rows;  // query rows of a unit
-  int tile_keys;   // a run of keys is a number of tiles
+  int tile_keys;   // a run of keys is a number of tiles,
+  int least_tiles; // no fewer than this
   int rows_over, rows_up_to;
   int target;      // units per key/value head that fill the chip
   int most;        // no more units per key/value head than this, whatever the batch
@@ -65,7 +66,8 @@ __device__ __forceinline__ int runs_of(int tiles, int run) { return (tiles - 1) 
 
 // Tiles of a run.  With work = sum of groups * tiles and n = sum of groups: the shortest runs, of work / target tiles or some
 // more, that come to at most `target` units (each group's last run may be short); runs of work / (target - n) always do.  Where the groups
-// alone are more than half the target, of work / (target / 2), and where they fill the chip several times, whole sequences.
+// alone are more than half the target, of work / (target / 2), and where they fill the chip several times, whole sequences.  No runs of
+// fewer than least_tiles: where a unit's start outweighs a tile, short runs cost more in the merge than they save.
 __device__ __forceinline__ int run_tiles(const Shape& p, const Cut& c, int lane, const Share& first) {
   int64_t work = 0, groups = 0;
   for (int b0 = 0; b0 < p.table.B; b0 += 64) {
@@ -79,9 +81,9 @@ __device__ __forceinline__ int run_tiles(const Shape& p, const Cut& c, int lane,
   auto ceil_div = [](int64_t a, int64_t b) {   // (64-bit division is slow)
     return a < 1LL << 31 ? (int)(((uint32_t)a + (uint32_t)b - 1) / (uint32_t)b) : (int)min((a + b - 1) / b, (int64_t)kWholeRun);
   };
-  const int safe = ceil_div(work, max(max((int64_t)c.target - groups, (int64_t)c.target / 2), (int64_t)1));
+  const int safe = max(ceil_div(work, max(max((int64_t)c.target - groups, (int64_t)c.target / 2), (int64_t)1)), work > 0 ? c.least_tiles : 0);
   if (p.table.B <= 64 && groups <= c.target)
-    for (int run = max(ceil_div(work, c.target), 1); run < safe; run += run / 16 + 1)
+    for (int run = max(ceil_div(work, c.target), c.least_tiles); run < safe; run += run / 16 + 1)
       if (wave_sum(first.groups ? first.groups * runs_of(first.tiles, run) : 0) <= (uint32_t)c.target) return run;
   return safe;
 }
