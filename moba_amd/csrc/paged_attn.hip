@@ -11,8 +11,8 @@
 //   V  ds_read_b64_tr_b8 transposes 8 keys x 16 elements
 // A page's key scale multiplies the scores, its value scale the probabilities, both in 32 bits.  One token of 32 heads on 8
 // against 131072 keys in 8 bits: 268 MB in 47 us, 5.7 TB/s; 16 sequences of up to 24001 keys in fp16 on 8 bits: 128 MB in
-// 26.9; four times five tokens against 12345 to 20480 keys in 16 bits: 294 MB in 51, 5.8 TB/s; one token against 4096
-// keys: 8.7, most of it finding the unit, the pages, and the first copies.
+// 26.8; four times five tokens against 12345 to 20480 keys in 16 bits: 294 MB in 51, 5.8 TB/s; one token against 4096
+// keys: 7.6, most of it finding the unit, the pages, and the first copies.
 //
 // Precision: the scores' products are exact, their sums 32 bits.  With few rows a probability (times the value scale) goes to the second
 // product as the sum of two elements, its rounded value and the rounded rest (16 bits of it in bf16, 22 in fp16): the products are not
@@ -1129,7 +1129,8 @@ static Cuts paged_cuts(int64_t T, int B, int rep, int Hkv, int D, bool cache8, i
   // 16-bit pages are twice the bytes: up to 32 rows (16 of 64 rows, one head: 30 us as many rows, 35 as few; 64 of 40: 110 and 135).
   const int few_rows = cache8 ? 2 * kFewRows : kFewRows;
   const bool many = most_new * rep > few_rows;
-  c.few = bounded_cut({kFewRows, kFewTile, 1, 0, many ? few_rows : 0x7fffffff, target(D == 128 && !cache8 ? 1 : 2), 0, 0}, T, B, rep);
+  // (runs of at least two tiles: one token against 4096 keys, with the merge 13.5 us with runs of one, 12.3 of two, 13.4 of three)
+  c.few = bounded_cut({kFewRows, kFewTile, 2, 0, many ? few_rows : 0x7fffffff, target(D == 128 && !cache8 ? 1 : 2), 0, 0}, T, B, rep);
   c.many = {};
   if (many) {
     const int waves = D == 128 && cache8 ? kManyWaves<128, true> : kManyWaves<64, false>;
