@@ -160,7 +160,7 @@ def attended(batch, query, scaling=None):
     """[rows, heads, d] in 64 bits: every new token against its sequence's tokens up to itself; rows that see nothing: zeros.
     Returns also how far a result in 32 bits may be off, [rows, heads, 1]: with e the error of a score, a probability is off by
     2e of itself (its own and the sum's), and by 2^-15 for the exponential, the two elements it is split into and the sums, or by half a step of its type
-    where a sequence has more than 32 rows and it is one element (all but fp16 queries on 8-bit pages); all of it times the largest finite value that the row sees.  e: D roundings of a sum of products, and 2^-22 of the score in the base-2 domain."""
+    where a sequence has more than 32 rows, or 64 with 8-bit pages, and it is one element (all but fp16 queries on 8-bit pages); all of it times the largest finite value that the row sees.  e: D roundings of a sum of products, and 2^-22 of the score in the base-2 domain."""
     d, hkv = query.shape[2], batch.pages[0].shape[1]
     rep = query.shape[1] // hkv
     scale = d ** -0.5 if scaling is None else scaling
@@ -169,9 +169,10 @@ def attended(batch, query, scaling=None):
         if not c:
             continue
         length, table = o + c, batch.table[b]
-        rounded = c * rep > 32 and not (batch.quantized and query.dtype == torch.float16)
+        many = c * rep > (64 if batch.quantized else 32)
+        rounded = many and not (batch.quantized and query.dtype == torch.float16)
         part = torch.finfo(query.dtype).eps / 2 if rounded else 0.0
-        if batch.quantized and c * rep > 32 and not all(bool((torch.frexp(s)[0] == 0.5).all()) for s in batch.scales):
+        if batch.quantized and many and not all(bool((torch.frexp(s)[0] == 0.5).all()) for s in batch.scales):
             part += 2.0 ** -8       # (values times a scale that is no power of two are rounded to bf16)
         pages = [int(table[i]) if i < table.shape[0] else -1 for i in range(-(-length // batch.page))]
         good = [0 <= p < batch.pages[0].shape[0] for p in pages]
