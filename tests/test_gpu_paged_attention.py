@@ -33,6 +33,7 @@ CASES = [  # old, new, page, heads, kv heads, head_dim, dtype, quantized, rows b
     ([3000], [40], 16, 4, 1, 128, FP16, True, 0),                           # many rows, few groups: several runs each
     ([3001, 2222], [33, 70], 128, 5, 5, 128, BF16, False, 0),
     ([63], [65], 16, 1, 1, 128, BF16, True, 0),
+    ([40, 10], [560, 45], 64, 30, 2, 64, BF16, True, 1),                    # more rows than the merge has waves for, an odd share of heads
 ]
 
 
@@ -234,6 +235,30 @@ def test_graph_and_streams():
         torch.cuda.synchronize()
         assert torch.equal(out, paged_attention(q, cache, table, lengths, cu)), i
         assert torch.equal(out_other, want_other) and torch.equal(eager_other, want_other), i
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+def test_graph_of_many_rows(quantized):
+    """Pieces of prompts and single tokens change places between replays."""
+    from moba_amd import paged_attention
+    batch = Batch([900, 300, 0], [150, 40, 1], 16, 2, 128, BF16, quantized, seed=13, pad_rows=9)
+    q = batch.tensors(8)[0]
+    cache, (table, lengths, cu) = batch.cache(), batch.index()
+    given = q.cuda()
+    paged_attention(given, cache, table, lengths, cu)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = paged_attention(given, cache, table, lengths, cu)
+    for old, new in (([900, 300, 0], [150, 40, 1]), ([1049, 0, 0], [1, 190, 1]), ([0, 339, 0], [0, 1, 0]), ([849, 100, 1], [200, 0, 0])):
+        batch.old, batch.new = old, new
+        rows = [0, new[0], new[0] + new[1], sum(new)]
+        lengths.copy_(torch.tensor([o + n for o, n in zip(old, new)]))
+        cu.copy_(torch.tensor(rows))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, paged_attention(given, cache, table, lengths, cu))
+        check_attention(batch, out, q)
 
 
 @pytest.mark.parametrize("quantized", [False, True])
