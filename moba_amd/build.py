@@ -62,7 +62,7 @@ def _host_module(force: bool) -> None:
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
            f'-DMOBA_TORCH_VERSION="{torch.__version__}"',
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *("-I" + d for d in include), *srcs, "-o", HOST,
-           "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python"]
+           "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_hip", "-ltorch_hip", "-ltorch_cpu", "-ltorch_python"]
     stamp = os.path.join(OBJ, "host.cmd")   # the command the module was built with: PyTorch's version and place are in it
     same = os.path.exists(stamp) and open(stamp).read() == "\n".join(cmd)
     if not force and same and os.path.exists(HOST) and all(os.path.getmtime(HOST) > os.path.getmtime(d) for d in deps):

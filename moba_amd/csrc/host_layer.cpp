@@ -7,6 +7,7 @@
 // Every function takes the ordinary call -- tensors of the right kind that are read where they lie -- and answers
 // NotImplemented to any other, which the caller's own path then checks, copies or refuses.
 #include <ATen/ATen.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <Python.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
@@ -70,6 +71,13 @@ bool frequencies_fit(const Tensor& f, const at::Device& device, int64_t d) {
          f.numel() > 0 && 2 * f.numel() <= d && aligned(f, 4);
 }
 
+// A new tensor, without the way through the dispatcher (which is a third of what at::empty takes).
+Tensor fresh(at::IntArrayRef size, at::ScalarType type, const at::Device& device) {
+  return Tensor(at::detail::empty_cuda(size, type, device, std::nullopt));
+}
+Tensor fresh_like(const Tensor& t) { return fresh(t.sizes(), t.scalar_type(), t.device()); }   // (packed, whatever t's strides)
+Tensor bytes(size_t count, const at::Device& device) { return fresh({(int64_t)count}, at::kByte, device); }
+
 // A leaf's gradient arrives on the stream that its node was made on.  A node that an eager graph keeps alive has another stream than
 // a capture, whose backward pass would have that stream wait for the captured one, and end the process: refused beforehand.
 void check_leaves(std::initializer_list<const Tensor*> leaves, const at::Device& device) {
@@ -121,7 +129,7 @@ void* mutable_pointer(Tensor& t) { return t.defined() ? t.mutable_data_ptr() : n
 
 std::pair<Tensor, Tensor> norm_forward(const NormArgs& a, const int64_t* strides) {
   const c10::OptionalDeviceGuard guard(a.q.device());
-  Tensor yq = at::empty(a.q.sizes(), a.q.options()), yk = at::empty(a.k.sizes(), a.k.options());
+  Tensor yq = fresh_like(a.q), yk = fresh_like(a.k);
   check(norm_call(pointer(a.q), pointer(a.k), mutable_pointer(yq), mutable_pointer(yk), pointer(a.q_weight), pointer(a.k_weight),
                   pointer(a.positions), (const float*)pointer(a.inv_freq), a.q.size(0), (int)a.q.size(1), (int)a.k.size(1),
                   (int)a.q.size(2), (int)(2 * a.inv_freq.numel()), strides, a.positions.scalar_type() == at::kLong ? 64 : 32,
@@ -160,12 +168,12 @@ struct NormRope : torch::autograd::Function<NormRope> {
         return aligned(t, 16) ? t : t.clone();
       };
       const Tensor dyq = packed(dy[0]), dyk = packed(dy[1]);
-      Tensor dq = at::empty(a.q.sizes(), a.q.options()), dk = at::empty(a.k.sizes(), a.k.options()), dqw, dkw, space;
+      Tensor dq = fresh_like(a.q), dk = fresh_like(a.k), dqw, dkw, space;
       // (the graph's edges are numbered by the tensors there are: a side without a weight has none)
-      if (a.q_weight.defined() && ctx->needs_input_grad(4)) dqw = at::empty_like(a.q_weight);
-      if (a.k_weight.defined() && ctx->needs_input_grad(a.q_weight.defined() ? 5 : 4)) dkw = at::empty_like(a.k_weight);
+      if (a.q_weight.defined() && ctx->needs_input_grad(4)) dqw = fresh_like(a.q_weight);
+      if (a.k_weight.defined() && ctx->needs_input_grad(a.q_weight.defined() ? 5 : 4)) dkw = fresh_like(a.k_weight);
       if (dqw.defined() || dkw.defined())
-        space = at::empty({(int64_t)norm_bwd_bytes(a.q.size(0), (int)a.q.size(2))}, a.q.options().dtype(at::kByte));
+        space = bytes(norm_bwd_bytes(a.q.size(0), (int)a.q.size(2)), a.q.device());
       check(norm_bwd_call(pointer(dyq), pointer(dyk), pointer(a.q), pointer(a.k), mutable_pointer(dq), mutable_pointer(dk),
                           pointer(a.q_weight), pointer(a.k_weight), mutable_pointer(dqw), mutable_pointer(dkw),
                           mutable_pointer(space), pointer(a.positions), (const float*)pointer(a.inv_freq), a.q.size(0),
@@ -317,7 +325,7 @@ PyObject* py_paged_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const Tensor k = *key, v = *value, kp = *cache.k, vp = *cache.v, table = *index.table, lengths = *index.lengths, cu = *index.cu;
     const NoGil no_gil;
     const c10::OptionalDeviceGuard guard(k.device());
-    if (query.defined()) out = at::empty(query.sizes(), query.options());
+    if (query.defined()) out = fresh_like(query);
     check(append_call(pointer(k), pointer(v), pointer(query), mutable_pointer(out), kp.mutable_data_ptr(), vp.mutable_data_ptr(),
                       (float*)mutable_pointer(cache.k_scales), (float*)mutable_pointer(cache.v_scales), (const int32_t*)pointer(table),
                       (const int32_t*)pointer(lengths), (const int32_t*)pointer(cu), (const float*)pointer(inv_freq), k.size(0),
@@ -361,10 +369,9 @@ PyObject* py_paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const Tensor q = *query, kp = *cache.k, vp = *cache.v, table = *index.table, lengths = *index.lengths, cu = *index.cu;
     const NoGil no_gil;
     const c10::OptionalDeviceGuard guard(q.device());
-    out = at::empty(q.sizes(), q.options());
+    out = fresh_like(q);
     const int b = (int)table.size(0);
-    Tensor space = at::empty({(int64_t)attention_bytes(tokens, b, (int)heads, (int)hkv, (int)d, cache.k_scales.defined(), (int)max_new)},
-                             q.options().dtype(at::kByte));
+    Tensor space = bytes(attention_bytes(tokens, b, (int)heads, (int)hkv, (int)d, cache.k_scales.defined(), (int)max_new), q.device());
     check(attention_call(pointer(q), mutable_pointer(out), pointer(kp), pointer(vp), (const float*)pointer(cache.k_scales),
                          (const float*)pointer(cache.v_scales), (const int32_t*)pointer(table), (const int32_t*)pointer(lengths),
                          (const int32_t*)pointer(cu), mutable_pointer(space), tokens, b, (int)heads, (int)hkv, (int)d, (int)kp.size(2),
