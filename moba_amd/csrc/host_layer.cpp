@@ -273,8 +273,9 @@ struct Cache {
     return k && v && optional_tensor(args[2], k_scales) && optional_tensor(args[3], v_scales) && k->is_cuda() && k->dim() == 4;
   }
   bool takes_rows(const Tensor& x) const {   // (none that a gradient is wanted for: there is none)
-    return !(x.requires_grad() && at::GradMode::is_enabled()) && half_type(x) && (k_scales.defined() || x.scalar_type() == k->scalar_type()) && x.dim() == 3 && x.size(2) == k->size(3) &&
-           x.device() == k->device();
+    const bool wants_gradient = x.requires_grad() && at::GradMode::is_enabled();
+    return !wants_gradient && half_type(x) && (k_scales.defined() || x.scalar_type() == k->scalar_type()) && x.dim() == 3 &&
+           x.size(2) == k->size(3) && x.device() == k->device();
   }
 };
 

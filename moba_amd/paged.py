@@ -1,6 +1,7 @@
 """A paged key/value cache on MI355X, with 16-bit elements or 8-bit ones and a scale for every page and head, and the operators on
 it: ``paged_append`` writes the keys and values of new tokens, rotated by position on the way, and ``paged_attention`` attends
-them.  Sequences of any lengths and any numbers of new tokens are served together.  (The reference keeps transformers' contiguous cache, one length for the whole batch, moba/wrapper.py:76-82.)"""
+them.  Sequences of any lengths and any numbers of new tokens are served together.  (The reference keeps transformers' contiguous
+cache, one length for the whole batch, moba/wrapper.py:76-82.)"""
 
 from __future__ import annotations
 
@@ -190,7 +191,7 @@ def paged_attention(query: torch.Tensor, cache: PagedKVCache, page_table: torch.
             with many (results do not depend on it)
     Returns:
         [tokens, heads, head_dim] in query's dtype.  Rows that see no token (those of no sequence, of a sequence without
-        pages) are zeros; a page that the table names wrongly (no page of the pool) holds no tokens.  No gradients: a query that
+        pages), or whose scores are all minus infinity, are zeros; a page that the table names wrongly (no page of the pool) holds no tokens.  No gradients: a query that
         requires one is refused outside ``torch.no_grad()``.
     """
     out = _lib.host().paged_attention(cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales, query, page_table, lengths,

@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from paged_reference import Batch, check_append, check_attention
+from paged_reference import Batch, attended, check_append, check_attention
 from rotary_reference import frequencies
 
 pytestmark = pytest.mark.gpu
@@ -137,6 +137,27 @@ def test_values_that_are_not_finite(quantized):
         got = paged_attention(q.cuda(), batch.cache(), *batch.index())
         check_attention(batch, got, q)
         assert got[4:7, :3].isnan().all() and got[:4, :3].isfinite().all() and got[7:18].isfinite().all() and got[18:, 3:].isnan().all()
+
+
+@pytest.mark.parametrize("d,dtype", [(128, BF16), (64, BF16), (128, FP16), (64, FP16)])
+def test_scores_that_are_not_finite(d, dtype):
+    """Infinite keys and queries, NaN among the queries: NaN in the rows whose softmax is none, and in no others; a key with the
+    score minus infinity counts for nothing."""
+    from moba_amd import paged_attention
+    batch = Batch([300, 50, 7], [6, 60, 1], 16, 2, d, dtype, False, seed=14)
+    q, = batch.tensors(6)
+    for b, position, head, sign in ((0, 303, 0, 1), (1, 80, 1, -1), (0, 17, 1, 1), (2, 3, 0, -1)):
+        batch.pages[0][int(batch.table[b, position // 16]), head, position % 16, 9] = sign * float("inf")
+    q[2, 1, 4], q[20, 5, 0], q[40, 2, 3], q[41, 0, 8] = float("nan"), float("inf"), float("nan"), -float("inf")
+    got = paged_attention(q.cuda(), batch.cache(), *batch.index())
+    want = attended(batch, q)[0]
+    assert want.isnan().any() and not want.isnan().all((1, 2)).any()
+    got, fine = got.cpu().double(), want.isfinite()
+    assert torch.equal(got.isnan(), want.isnan())
+    # half a step of the result and of a probability, of many rows one element; 2^-10: 2 * (d + 12) * 2^-24 of a score's size, at
+    # most 11 or so, and 2^-15, of the largest value
+    tolerance = torch.finfo(dtype).eps / 2 * 1.001 * (want[fine].abs().max() + batch.pages[1].abs().max().double()) + 2.0 ** -10
+    assert ((got - want).abs()[fine] <= tolerance).all()
 
 
 @pytest.mark.parametrize("quantized", [True, False])
