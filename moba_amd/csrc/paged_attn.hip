@@ -1103,8 +1103,9 @@ using namespace moba;
 static Cut bounded_cut(Cut c, int64_t T, int B, int rep) {
   // (of a cut with rows_over, at most T * rep / (rows_over + 1) sequences)
   const int64_t with_rows = c.rows_over ? T * rep / (c.rows_over + 1) : T, sequences = with_rows < B ? with_rows : B;
-  // (one group each where no sequence has more rows than a group)
-  const int64_t groups = sequences + (c.rows_up_to > c.group_rows ? T * rep / c.group_rows : 0);
+  // (no sequence has more groups than rows_up_to rows make)
+  const int64_t by_rows = sequences + T * rep / c.group_rows, by_sequences = sequences * ((c.rows_up_to - 1) / c.group_rows + 1);
+  const int64_t groups = by_rows < by_sequences ? by_rows : by_sequences;
   const int64_t several = groups < (int64_t)kWholeAt * c.target ? groups : (int64_t)kWholeAt * c.target;
   const int64_t parts = c.target / 2 + 1 + several > c.target ? c.target / 2 + 1 + several : c.target;
   const int64_t most = groups > parts ? groups : parts;

@@ -160,3 +160,26 @@ def test_rows_that_want_a_gradient():
 def test_caches_compare_by_identity():
     a, b = make(), make()
     assert a == a and a != b and len({a, b}) == 2
+
+
+def attention_code(T, B, H, Hkv, D, cache8=1, hint=-1):
+    """What the entry point answers for sizes that it takes: here, where there is no GPU, that nothing could be launched."""
+    from moba_amd import _lib
+    some = 256   # (never read)
+    return _lib.load().moba_paged_attention(*[some] * 10, T, B, H, Hkv, D, 16, 3, 1, hint, (ctypes.c_int64 * 3)(H * D, D, 1), cache8,
+                                            0.125, 0, None)
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the addresses are none")
+def test_long_pieces_on_8_bit_pages():
+    """Up to 64 rows of a sequence are few with 8-bit pages, two groups of 32: a long piece asks for no more of them than that, neither
+    workgroups nor workspace."""
+    from moba_amd import _lib
+    sizes = _lib.load().moba_paged_attention_workspace_bytes
+    for T, B in ((2048, 1), (131072, 1), (131072, 20), (1 << 22, 1)):
+        # units of 256 compute units, two workgroups to each (many rows: one), 8 key/value heads: few rows and many
+        few = max(64, 33 + 2 * B)
+        many = 17 + min(128, B + T * 4 // 256)
+        assert sizes(T, B, 32, 8, 128, 1, -1) <= (few * 32 + many * 256) * 8 * 129 * 4 + 16 * B, (T, B)
+    for args in ((1 << 22, 1, 128, 8, 128), (1 << 22, 1, 128, 8, 64), (1 << 23, 4, 128, 16, 128)):
+        assert attention_code(*args) == attention_code(*args, cache8=0) == -3, args
