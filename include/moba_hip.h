@@ -425,7 +425,8 @@ int moba_paged_append(const void* k, const void* v, const void* q, void* yq, voi
  *   workspace: moba_paged_attention_workspace_bytes(T, B, H, Hkv, D, cache8, max_new) bytes; calls that may run at
  *   the same time need their own
  *   max_new: the most new tokens that a sequence has, or -1: a hint that spares a launch for sequences of many
- *   T < 2^24, T * H < 2^31, and fewer than 2^24 units of work (about B * Hkv, or T * H / 128 of long pieces; MOBA_ERR_LIMIT) */
+ *   T < 2^24, T * H < 2^31, and fewer than 2^32 threads to a launch (MOBA_ERR_LIMIT otherwise): at most 256 * Hkv for a sequence with
+ *   rows, 512 * Hkv with e4m3 pages, and 2 * T * H for long pieces (8 * T * H where max_new says that there are none) */
 size_t moba_paged_attention_workspace_bytes(int64_t T, int B, int H, int Hkv, int D, int cache8, int max_new);
 int moba_paged_attention(const void* q, void* out, const void* k_pages, const void* v_pages, const float* k_scales,
                          const float* v_scales, const int32_t* page_table, const int32_t* lengths, const int32_t* cu_new,

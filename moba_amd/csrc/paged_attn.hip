@@ -1190,8 +1190,10 @@ static int paged_attention(const void* q, void* out, const void* k_pages, const 
   const Cuts cuts = paged_cuts(table.T, table.B, p.shape.rep, Hkv, D, cache8 != 0, max_new);
   p.few = cuts.few;
   p.many = cuts.many;
-  const int64_t most = p.few.most > p.many.most ? p.few.most : p.many.most;
-  if (most * Hkv >= 1LL << 24 || table.T >= 1 << 24) return MOBA_ERR_LIMIT;   // (threads of a launch: 32 bits)
+  // (threads of a launch: 32 bits)
+  const int64_t many_threads = 64 * (D == 128 && cache8 ? kManyWaves<128, true> : kManyWaves<64, false>);
+  if ((int64_t)p.few.most * Hkv * 64 * kFewWaves >= 1LL << 32 || (int64_t)p.many.most * Hkv * many_threads >= 1LL << 32 || table.T >= 1 << 24)
+    return MOBA_ERR_LIMIT;
   p.q = (const elem*)q; p.out = (elem*)out;
   p.pages[0] = (const char*)k_pages; p.pages[1] = (const char*)v_pages;
   p.scales[0] = k_scales; p.scales[1] = v_scales;

@@ -183,3 +183,14 @@ def test_long_pieces_on_8_bit_pages():
         assert sizes(T, B, 32, 8, 128, 1, -1) <= (few * 32 + many * 256) * 8 * 129 * 4 + 16 * B, (T, B)
     for args in ((1 << 22, 1, 128, 8, 128), (1 << 22, 1, 128, 8, 64), (1 << 23, 4, 128, 16, 128)):
         assert attention_code(*args) == attention_code(*args, cache8=0) == -3, args
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the addresses are none")
+def test_launches_of_too_many_threads():
+    """Refused as a limit before anything is launched, by the threads of each kernel's own workgroups: 512 of the many-row one
+    for 128-element heads on 8-bit pages."""
+    T = 1 << 21
+    assert attention_code(T, T // 65, 256, 256, 128) == -4          # 40448 units of many rows a head: 5.3e9 threads
+    assert attention_code(T, T // 65, 256, 256, 64) == -3           # 256 threads each, 48640 units: 3.2e9
+    assert attention_code(1 << 22, 1 << 12, 256, 256, 128, cache8=0, hint=0) == -4   # few rows, says the hint: 8.9e9
+    assert attention_code(1 << 22, 1 << 12, 256, 256, 128, cache8=0) == -3           # 2.4e9
