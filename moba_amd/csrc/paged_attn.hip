@@ -1064,10 +1064,11 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams<E> p
       for (int e = 0; e < kPer; ++e) o[e] *= former;
 #pragma unroll
       for (int k = 0; k < count; ++k) {
-        const float wk = lane_value(w, kShare * k + wave);   // (0 behind the last)
+        const float wk = lane_value(w, kShare * k + wave);   // (0 behind the last, whose row is the last one's again)
         ll += wk;
+        const bool there = i0 + kShare * k + wave < r.runs;   // (0 times an infinity is not 0)
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) o[e] += wk * x[k][e];
+        for (int e = 0; e < kPer; ++e) o[e] += there ? wk * x[k][e] : 0.f;
       }
     };
     if (r.runs > 0 && r.runs <= 4 * kShare) some(0, std::integral_constant<int, 4>{});
