@@ -247,9 +247,11 @@ __global__ __launch_bounds__(64 * kAppendWaves, 4) void paged_append_kernel(cons
     __syncthreads();   // the maxima are complete
     const int half = tid >= heads, h = half ? tid - heads : tid;
     if (scale && h >= h0 && h < h0 + n) {
-      const float s = fmaxf(page_scale(__builtin_bit_cast(float, most[half][h])), former);
+      // (a former scale that is none of page_scale()'s may have either sign)
+      const float least = page_scale(__builtin_bit_cast(float, most[half][h]));
+      const float s = fabsf(former) >= least ? former : least;
       over[half][h] = 1.f / s;
-      again[half][h] = former > 0.f && s > former ? former / s : 0.f;
+      again[half][h] = former / s;   // 1: as they are; 0: the least magnitude, or a former scale of 0
       *scale = s;
     }
     __syncthreads();
@@ -258,7 +260,7 @@ __global__ __launch_bounds__(64 * kAppendWaves, 4) void paged_append_kernel(cons
 #pragma unroll
       for (int v = 0; v < 2; ++v) {
         const float by = again[v][hr];
-        if (by == 0.f) continue;
+        if (by == 1.f) continue;
         u32x2* w = reinterpret_cast<u32x2*>(row_at(v, i, hr) + 8 * u);
         u32x2 bytes = *w;
         bytes[0] = rescaled(bytes[0], by);

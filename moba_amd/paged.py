@@ -29,7 +29,8 @@ class PagedKVCache:
     k_pages, v_pages: [num_pages, kv_heads, page_size, head_dim], bf16, fp16 or e4m3 (``torch.float8_e4m3fn``); page_size
         16, 32, 64, 128 or 256, head_dim 64 or 128
     k_scales, v_scales: [num_pages, kv_heads] float32, for e4m3 only: an element stands for its value times the scale of its
-        page and head.  ``paged_append`` keeps them powers of two.
+        page and head.  Those that ``paged_append`` sets are powers of two; of a page that holds tokens it keeps one of any value
+        that is large enough for the new ones as well.
 
     Which pages belong to which sequence is the caller's affair (the ``page_table`` of the calls).  Pages may be shared by
     sequences that only read them; a page that receives tokens in a call must be named once in the whole table.

@@ -209,3 +209,38 @@ def test_graph_and_streams():
             for t in (lengths, steps):
                 t[1] = 1
     assert lengths.tolist() == steps.tolist()
+
+
+@pytest.mark.parametrize("page", [16, 128])
+def test_scales_that_held_tokens_may_have(page):
+    """Far smaller than the new tokens need, so that their ratio is no 32-bit number; and others than paged_append's own: zero,
+    negative, no power of two, smaller and larger than the new tokens'.  What the page holds stands for the same values as before."""
+    from moba_amd import paged_append
+    held = page - 5
+    batch = Batch([held], [3], page, 8, 64, BF16, True, seed=17)
+    page_id = int(batch.table[0, 0])
+    # head:                       0          1          2       3    4       5      6       7
+    scales = torch.tensor([2.0 ** -100, 2.0 ** -60, 2.0 ** -7, 0.0, -0.01, -300.0, 0.013, 77.7])
+    grown = [True, True, False, True, True, False, True, False]
+    for s in batch.scales:
+        s[page_id] = scales
+    for codes in batch.pages:                             # (all of magnitude 1 to 448, so that none is lost without reason)
+        codes[page_id] = (codes[page_id].float().sign() * codes[page_id].float().abs().clamp(min=1)).to(E4M3)
+    k, v = (x.clamp(-4, 4) for x in batch.tensors(8, 8))
+    for x in (k, v):
+        x[:, 0], x[:, 1] = x[:, 0] * 2.0 ** 70, x[:, 1] * 2.0 ** 120
+        x[:, 2] = x[:, 2] * 0.1
+        x[:, 3:7] = x[:, 3:7] * 20
+    cache = batch.cache()
+    paged_append(cache, k.cuda(), v.cuda(), *batch.index())
+    for half, (pages, new, x) in enumerate(((cache.k_pages, cache.k_scales, k), (cache.v_pages, cache.v_scales, v))):
+        codes, new = pages[page_id].cpu(), new[page_id].cpu()
+        before, after = (c.double() * s[:, None, None].double() for c, s in ((batch.pages[half][page_id], scales), (codes, new)))
+        for h in range(8):
+            if not grown[h]:
+                assert new[h] == scales[h] and torch.equal(codes[h, :held].view(torch.uint8), batch.pages[half][page_id, h, :held].view(torch.uint8)), h
+            assert new[h].abs() * 448 * (1 + 2.0 ** -22) >= x[:, h].abs().max() and new[h].abs() >= scales[h].abs(), (h, new[h])
+            # half a step of e4m3 of a normal number or of the smallest, and of the factors' 32 bits
+            for got, want in ((after[h, :held], before[h, :held]), (after[h, held:held + 3], x[:, h].double())):
+                bound = torch.maximum(2.0 ** -4 * want.abs(), 2.0 ** -10 * new[h].double().abs()) * 1.001
+                assert ((got - want).abs() <= bound).all(), (half, h, new[h], ((got - want).abs() / bound).max())
