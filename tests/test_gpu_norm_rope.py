@@ -1,5 +1,7 @@
 """qk_norm_rope on the GPU against its formula in 64 bits, forward and backward."""
 
+import math
+
 import pytest
 import torch
 
@@ -351,3 +353,35 @@ def test_the_native_call_lets_other_threads_run():
             qk_norm_rope(q, k, positions, frequencies(32, "cuda"))
     finally:
         _lib.bind_layer(_lib.host())
+
+
+PI = 314159265358979323846264338327950288419716939937510582097494459230781640628620899  # * 10^-80
+
+
+def exact_turn(position, inv_freq):
+    """cos and sin of position * inv_freq, whose whole turns are taken off in whole numbers."""
+    top, bottom = inv_freq.as_integer_ratio()
+    top *= position
+    turn = 2 * PI * bottom
+    rest = (top * 10 ** 80) % turn                       # of an angle of rest / 10^80 / bottom
+    if 2 * rest > turn:
+        rest -= turn
+    angle = rest / (10 ** 80 * bottom)                    # (a quotient of whole numbers, rounded once)
+    return math.cos(angle), math.sin(angle)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_angles_of_far_positions(dtype):
+    """Up to the last position that a double tells from the next, at frequencies of 1 and more as well."""
+    from moba_amd import qk_norm_rope
+    g = torch.Generator().manual_seed(2)
+    positions = [s * (2 ** e + i) for e in (20, 30, 31, 34, 40, 45, 50, 52) for s, i in ((1, 0), (-1, 12345), (1, 777))] + [2 ** 53]
+    inv_freq = torch.cat([frequencies(24), torch.tensor([1.0, 3.0, 1000.0, 0.7, 2.0 ** -30, 1e-20, 0.0, 123456.789])])
+    x = torch.randn((len(positions), 2, 64), generator=g).to(dtype)
+    x[:, 1, :32], x[:, 1, 32:] = 1, 0                     # (the angle's cosine and sine themselves)
+    got, _ = qk_norm_rope(x.cuda(), x.cuda(), torch.tensor(positions).cuda(), inv_freq.cuda())
+    cs = torch.tensor([[exact_turn(p, f) for f in inv_freq.tolist()] for p in positions], dtype=torch.float64)
+    cos, sin = cs[:, None, :, 0], cs[:, None, :, 1]
+    a, b = x.double()[..., :32], x.double()[..., 32:]
+    want = torch.cat([a * cos - b * sin, b * cos + a * sin], -1)
+    check(got.cpu(), want, pair_size(x.double(), 32), dtype, forward_steps(0), "y")
