@@ -78,6 +78,9 @@ Tensor fresh(at::IntArrayRef size, at::ScalarType type, const at::Device& device
 Tensor fresh_like(const Tensor& t) { return fresh(t.sizes(), t.scalar_type(), t.device()); }   // (packed, whatever t's strides)
 Tensor bytes(size_t count, const at::Device& device) { return fresh({(int64_t)count}, at::kByte, device); }
 
+// whether a forward-mode tangent comes with it (there are no such derivatives)
+bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+
 // A leaf's gradient arrives on the stream that its node was made on.  A node that an eager graph keeps alive has another stream than
 // a capture, whose backward pass would have that stream wait for the captured one, and end the process: refused beforehand.
 void check_leaves(std::initializer_list<const Tensor*> leaves, const at::Device& device) {
@@ -158,6 +161,8 @@ struct NormRope : torch::autograd::Function<NormRope> {
     const NormArgs a = {saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], ctx->saved_data["eps"].toDouble(),
                         ctx->saved_data["interleaved"].toBool()};
     torch::autograd::variable_list grads(8);
+    TORCH_CHECK(!has_tangent(dy[0]) && !has_tangent(dy[1]),
+                "qk_norm_rope has no forward-mode derivatives: tensors with a tangent are refused");
     {
       const at::NoGradGuard no_grad;
       const c10::OptionalDeviceGuard guard(a.q.device());
@@ -228,6 +233,9 @@ PyObject* py_norm_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const int interleaved = PyObject_IsTrue(args[7]);
   if (interleaved < 0) return nullptr;
   a.interleaved = interleaved;
+  for (const Tensor* t : {&a.q, &a.k, &a.inv_freq, &a.q_weight, &a.k_weight})
+    if (has_tangent(*t)) Py_RETURN_NOTIMPLEMENTED;
+  if (a.inv_freq.requires_grad() && at::GradMode::is_enabled()) Py_RETURN_NOTIMPLEMENTED;
   int64_t strides[4];
   if (!norm_fits(a, strides)) Py_RETURN_NOTIMPLEMENTED;
   auto wants = [](const Tensor& t) { return t.defined() && t.requires_grad(); };

@@ -8,6 +8,7 @@ import ctypes
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from . import moba_efficient as E
@@ -24,6 +25,10 @@ def _strides_of(t: torch.Tensor):
 
 def _readable(t: torch.Tensor) -> torch.Tensor:
     return t if _strides_of(t) is not None else E._aligned(t)
+
+
+def _has_tangent(*tensors) -> bool:
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _check(q, k, positions, inv_freq, q_weight, k_weight, eps):
@@ -51,6 +56,10 @@ def _check(q, k, positions, inv_freq, q_weight, k_weight, eps):
         raise ValueError("all tensors must be on one device")
     if not eps >= 0:
         raise ValueError("eps must not be negative")
+    if _has_tangent(q, k, inv_freq, *weights):
+        raise RuntimeError("qk_norm_rope has no forward-mode derivatives: tensors with a tangent are refused")
+    if inv_freq.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("qk_norm_rope has no gradient of inv_freq: call it under torch.no_grad(), or with inv_freq.detach()")
     if not q.is_cuda:
         raise RuntimeError("qk_norm_rope needs tensors on an AMD GPU (there is no CPU path)")
 
@@ -99,6 +108,8 @@ class _QkNormRope(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dyq, dyk):
         q, k, positions, inv_freq, q_weight, k_weight = ctx.saved_tensors
+        if _has_tangent(dyq, dyk):
+            raise RuntimeError("qk_norm_rope has no forward-mode derivatives: tensors with a tangent are refused")
         q, k = _readable(q), _readable(k)
         dyq, dyk = E._aligned(dyq), E._aligned(dyk)
         dq, dk = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
@@ -135,8 +146,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_
         q_weight, k_weight: [head_dim], of q's dtype or float32: ``x * weight / sqrt(mean(x^2) + eps)`` over the elements of a
             head before the rotation; None: that side is rotated only
     Returns:
-        the new q and k, packed.  Differentiable once in q, k and the weights; the weights' gradients are summed in a fixed
-        order (the same bits on every run).  A call that is being captured into a graph is refused while an eager graph of the
+        the new q and k, packed.  Differentiable once in q, k and the weights, backward (tensors with forward-mode tangents
+        are refused, and an inv_freq that requires a gradient outside ``torch.no_grad()``); the weights' gradients are summed in
+        a fixed order (the same bits on every run).  A call that is being captured into a graph is refused while an eager graph of the
         same leaves is alive (its backward pass could not be captured).
     """
     y = _lib.host().norm_rope(q, k, positions, inv_freq, q_weight, k_weight, eps, interleaved)

@@ -385,3 +385,31 @@ def test_angles_of_far_positions(dtype):
     a, b = x.double()[..., :32], x.double()[..., 32:]
     want = torch.cat([a * cos - b * sin, b * cos + a * sin], -1)
     check(got.cpu(), want, pair_size(x.double(), 32), dtype, forward_steps(0), "y")
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_derivatives_that_there_are_none_of(native, monkeypatch):
+    import torch.autograd.forward_ad as fwd
+    from moba_amd import _lib, qk_norm_rope
+    q, k, dq, dk, positions, w = make(20, 4, 2, 64, BF16, seed=6)
+    f = frequencies(32, "cuda")
+    if not native:
+        monkeypatch.setattr(_lib.host(), "norm_rope", lambda *a: NotImplemented)
+    args, leaf = [q, k, positions, f, *w], q.clone().requires_grad_()
+    want = qk_norm_rope(*args)
+    y = qk_norm_rope(leaf, *args[1:])
+    with fwd.dual_level():
+        for i in (0, 1, 3, 4, 5):
+            for where in (torch.enable_grad, torch.no_grad):
+                with where(), pytest.raises(RuntimeError, match="forward-mode"):
+                    qk_norm_rope(*[fwd.make_dual(x, torch.ones_like(x)) if i == j else x for j, x in enumerate(args)])
+        for dy in ((fwd.make_dual(dq, dq), dk), (dq, fwd.make_dual(dk, dk))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(y, leaf, dy, retain_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(qk_norm_rope(*args), want))
+        assert torch.autograd.grad(y, leaf, (dq, dk))[0].isfinite().all()
+    learned = f.clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="gradient of inv_freq"):
+        qk_norm_rope(q, k, positions, learned)
+    with torch.no_grad():
+        assert all(torch.equal(a, b) for a, b in zip(qk_norm_rope(q, k, positions, learned, *w), want))

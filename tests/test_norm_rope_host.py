@@ -57,3 +57,26 @@ def test_entry_points_refuse():
         assert backward(**wrong) == -1, wrong
     assert lib.moba_qk_norm_rope_bwd_workspace_bytes(0, 64) == 0
     assert lib.moba_qk_norm_rope_bwd_workspace_bytes(5, 64) == 2 * 2 * 64 * 4
+
+
+def test_derivatives_that_there_are_none_of():
+    """Refused, rather than lost: forward-mode tangents of any input, and the gradient of inv_freq."""
+    import torch.autograd.forward_ad as fwd
+    from moba_amd import qk_norm_rope
+    q, k = torch.zeros((6, 4, 64), dtype=torch.bfloat16), torch.zeros((6, 2, 64), dtype=torch.bfloat16)
+    at, f, w = torch.arange(6), frequencies(32), torch.ones(64, dtype=torch.bfloat16)
+    args = [q, k, at, f, w, w]
+    with fwd.dual_level():
+        for i in (0, 1, 3, 4, 5):
+            for where in (torch.enable_grad, torch.no_grad):
+                with where(), pytest.raises(RuntimeError, match="forward-mode"):
+                    qk_norm_rope(*[fwd.make_dual(x, torch.ones_like(x)) if i == j else x for j, x in enumerate(args)])
+        with pytest.raises(RuntimeError, match="AMD GPU"):
+            qk_norm_rope(*args)
+    with pytest.raises(RuntimeError, match="forward-mode"):
+        torch.func.jvp(lambda x: qk_norm_rope(x, k, at, f)[0], (q,), (torch.ones_like(q),))
+    leaf = f.clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="gradient of inv_freq"):
+        qk_norm_rope(q, k, at, leaf)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="AMD GPU"):
+        qk_norm_rope(q, k, at, leaf)
