@@ -272,17 +272,21 @@ PyObject* py_norm_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
 namespace {
 
 // ---- the paged cache (whose tensors its class has checked)
+bool wants_derivative(const Tensor& t) {   // (there are none)
+  return t.defined() && ((t.requires_grad() && at::GradMode::is_enabled()) || has_tangent(t));
+}
+
 struct Cache {
   const Tensor *k, *v;
   Tensor k_scales, v_scales;
   bool take(PyObject* const* args) {
     k = plain_tensor(args[0]);
     v = plain_tensor(args[1]);
-    return k && v && optional_tensor(args[2], k_scales) && optional_tensor(args[3], v_scales) && k->is_cuda() && k->dim() == 4;
+    return k && v && optional_tensor(args[2], k_scales) && optional_tensor(args[3], v_scales) && k->is_cuda() && k->dim() == 4 &&
+           !wants_derivative(*k) && !wants_derivative(*v) && !wants_derivative(k_scales) && !wants_derivative(v_scales);
   }
-  bool takes_rows(const Tensor& x) const {   // (none that a gradient is wanted for: there is none)
-    const bool wants_gradient = x.requires_grad() && at::GradMode::is_enabled();
-    return !wants_gradient && half_type(x) && (k_scales.defined() || x.scalar_type() == k->scalar_type()) && x.dim() == 3 &&
+  bool takes_rows(const Tensor& x) const {
+    return !wants_derivative(x) && half_type(x) && (k_scales.defined() || x.scalar_type() == k->scalar_type()) && x.dim() == 3 &&
            x.size(2) == k->size(3) && x.device() == k->device();
   }
 };
@@ -324,6 +328,7 @@ PyObject* py_paged_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (query.defined() && (!cache.takes_rows(query) || query.scalar_type() != key->scalar_type() || query.size(0) != key->size(0) ||
                           query.size(1) < 1 || query.size(1) > kMostHeads || !rows_in_place(query, 4, 8, strides)))
     Py_RETURN_NOTIMPLEMENTED;
+  if (wants_derivative(inv_freq)) Py_RETURN_NOTIMPLEMENTED;
   if (inv_freq.defined() && !frequencies_fit(inv_freq, key->device(), d)) Py_RETURN_NOTIMPLEMENTED;
   if (!rows_in_place(*key, 4, 8, strides + 2) || !rows_in_place(*value, 4, 8, strides + 4)) Py_RETURN_NOTIMPLEMENTED;
   strides[6] = index.table->stride(0);

@@ -13,7 +13,7 @@ import torch
 
 from . import _lib
 from . import moba_efficient as E
-from .norm_rope import _check_inv_freq, _readable, _strides_of
+from .norm_rope import _check_inv_freq, _has_tangent, _readable, _strides_of
 
 E4M3 = torch.float8_e4m3fn
 PAGE_SIZES = (16, 32, 64, 128, 256)
@@ -106,8 +106,14 @@ def _check_rows(cache, name, x, heads=None):
         raise ValueError(f"{name} must be [tokens, heads, head_dim] with the cache's head_dim (and, keys and values, its heads)")
     if x.shape[0] > MAX_TOKENS:
         raise ValueError(f"at most {MAX_TOKENS} tokens")
-    if x.requires_grad and torch.is_grad_enabled():
+
+
+def _check_no_gradients(cache, *tensors):
+    tensors = [t for t in (cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales, *tensors) if t is not None]
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise RuntimeError("the operators on the paged cache have no gradients: call them under torch.no_grad()")
+    if _has_tangent(*tensors):
+        raise RuntimeError("the operators on the paged cache have no forward-mode derivatives: tensors with a tangent are refused")
 
 
 def paged_append(cache: PagedKVCache, key: torch.Tensor, value: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
@@ -126,8 +132,9 @@ def paged_append(cache: PagedKVCache, key: torch.Tensor, value: torch.Tensor, pa
         inv_freq, interleaved: the rotation, as for ``qk_norm_rope``; without inv_freq nothing is rotated
         query: [tokens, heads, head_dim] of key's dtype, or None
     Returns:
-        the rotated queries (rows that belong to no sequence: zeros), or None without ``query``.  No gradients: rows that
-        require one are refused outside ``torch.no_grad()``.
+        the rotated queries (rows that belong to no sequence: zeros), or None without ``query``.  No gradients: tensors that
+        require one, the cache's and inv_freq among them, are refused outside ``torch.no_grad()``, those with a forward-mode
+        tangent everywhere.
 
     The three index tensors stay on the device, and a captured call follows their contents.  A token whose position has no
     page (beyond the table's row, or an entry that is no page) is not written.  Elements of 8-bit pages are rounded from
@@ -141,6 +148,7 @@ def paged_append(cache: PagedKVCache, key: torch.Tensor, value: torch.Tensor, pa
         return out
     # tensors that have to be copied first, none at all, or wrong ones
     hkv, d = cache.k_pages.shape[1], cache.k_pages.shape[3]
+    _check_no_gradients(cache, key, value, query, inv_freq)
     for name, x in (("key", key), ("value", value)):
         _check_rows(cache, name, x, hkv)
     if value.shape != key.shape or value.dtype != key.dtype:
@@ -192,14 +200,16 @@ def paged_attention(query: torch.Tensor, cache: PagedKVCache, page_table: torch.
             with many (results do not depend on it)
     Returns:
         [tokens, heads, head_dim] in query's dtype.  Rows that see no token (those of no sequence, of a sequence without
-        pages), or whose scores are all minus infinity, are zeros; a page that the table names wrongly (no page of the pool) holds no tokens.  No gradients: a query that
-        requires one is refused outside ``torch.no_grad()``.
+        pages), or whose scores are all minus infinity, are zeros; a page that the table names wrongly (no page of the pool) holds
+        no tokens.  No gradients: a query or a cache that requires one is refused outside ``torch.no_grad()``, one with a
+        forward-mode tangent everywhere.
     """
     out = _lib.host().paged_attention(cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales, query, page_table, lengths,
                                       cu_new, scaling, max_new)
     if out is not NotImplemented:
         return out
     # tensors that have to be copied first, none at all, or wrong ones
+    _check_no_gradients(cache, query)
     _check_rows(cache, "query", query)
     hkv, d = cache.k_pages.shape[1], cache.k_pages.shape[3]
     tokens, heads = query.shape[:2]

@@ -244,3 +244,36 @@ def test_scales_that_held_tokens_may_have(page):
             for got, want in ((after[h, :held], before[h, :held]), (after[h, held:held + 3], x[:, h].double())):
                 bound = torch.maximum(2.0 ** -4 * want.abs(), 2.0 ** -10 * new[h].double().abs()) * 1.001
                 assert ((got - want).abs() <= bound).all(), (half, h, new[h], ((got - want).abs() / bound).max())
+
+
+@pytest.mark.parametrize("quantized", [True, False])
+def test_derivatives_that_there_are_none_of(quantized):
+    import torch.autograd.forward_ad as fwd
+    from moba_amd import PagedKVCache, paged_append, paged_attention
+    batch = Batch([10], [2], 16, 2, 64, BF16, quantized)
+    k, v, q = (x.cuda() for x in batch.tensors(2, 2, 4))
+    index, f = batch.index(), frequencies(32, "cuda")
+    names = ("k_scales", "v_scales") if quantized else ("k_pages", "v_pages")
+    changed = lambda name, change: PagedKVCache(**{  # noqa: E731
+        n: change(x) if n == name else x for n, x in vars(batch.cache()).items()})
+    for name in names:
+        cache = changed(name, lambda x: x.requires_grad_())
+        for call in (lambda: paged_append(cache, k, v, *index), lambda: paged_attention(q, cache, *index)):
+            with pytest.raises(RuntimeError, match="no gradients"):
+                call()
+            with torch.no_grad():
+                call()
+    with pytest.raises(RuntimeError, match="no gradients"):
+        paged_append(batch.cache(), k, v, *index, inv_freq=f.clone().requires_grad_())
+    with fwd.dual_level():
+        dual = lambda x: fwd.make_dual(x, torch.ones_like(x))  # noqa: E731
+        for name in names:
+            cache = changed(name, dual)
+            for call in (lambda: paged_append(cache, k, v, *index), lambda: paged_attention(q, cache, *index)):
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call()
+        for args in ((dual(k), v, q, f), (k, dual(v), q, f), (k, v, dual(q), f), (k, v, q, dual(f))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                paged_append(batch.cache(), *args[:2], *index, query=args[2], inv_freq=args[3])
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            paged_attention(dual(q), batch.cache(), *index)

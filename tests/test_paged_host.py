@@ -194,3 +194,39 @@ def test_launches_of_too_many_threads():
     assert attention_code(T, T // 65, 256, 256, 64) == -3           # 256 threads each, 48640 units: 3.2e9
     assert attention_code(1 << 22, 1 << 12, 256, 256, 128, cache8=0, hint=0) == -4   # few rows, says the hint: 8.9e9
     assert attention_code(1 << 22, 1 << 12, 256, 256, 128, cache8=0) == -3           # 2.4e9
+
+
+def test_derivatives_that_there_are_none_of():
+    """Refused, rather than lost: gradients of the cache and of inv_freq, and forward-mode tangents of anything."""
+    import torch.autograd.forward_ad as fwd
+    from moba_amd import PagedKVCache, paged_append, paged_attention
+    attend = lambda cache, **changes: paged_attention(**{  # noqa: E731
+        n: x for n, x in append_args(cache=cache, **changes).items() if n in ("query", "cache", "page_table", "lengths", "cu_new")})
+
+    def caches(change):
+        """The 16-bit and the 8-bit cache with one tensor changed."""
+        for dtype in (BF16, E4M3):
+            fields = {n: getattr(make(dtype), n) for n in ("k_pages", "v_pages", "k_scales", "v_scales")}
+            for name, x in fields.items():
+                if x is not None and x.dtype != E4M3:
+                    yield PagedKVCache(**{**fields, name: change(x)})
+
+    for cache in caches(lambda x: x.requires_grad_()):
+        for call in (lambda: paged_append(**append_args(cache=cache)), lambda: attend(cache)):
+            with pytest.raises(RuntimeError, match="no gradients"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="AMD GPU"):
+                call()
+    with pytest.raises(RuntimeError, match="no gradients"):
+        paged_append(**append_args(inv_freq=frequencies(32).requires_grad_()))
+    with fwd.dual_level(), torch.no_grad():
+        dual = lambda x: fwd.make_dual(x, torch.ones_like(x))  # noqa: E731
+        for cache in caches(dual):
+            for call in (lambda: paged_append(**append_args(cache=cache)), lambda: attend(cache)):
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call()
+        for name in ("key", "value", "query", "inv_freq"):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                paged_append(**append_args(**{name: dual(append_args()[name])}))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            attend(make(), query=dual(append_args()["query"]))
