@@ -276,6 +276,11 @@ bool wants_derivative(const Tensor& t) {   // (there are none)
   return t.defined() && ((t.requires_grad() && at::GradMode::is_enabled()) || has_tangent(t));
 }
 
+// autograd learns that a tensor has changed (an inference tensor keeps no such number)
+void written(const Tensor& t) {
+  if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 struct Cache {
   const Tensor *k, *v;
   Tensor k_scales, v_scales;
@@ -347,6 +352,7 @@ PyObject* py_paged_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
                       inv_freq.defined() ? (int)(2 * inv_freq.numel()) : 0, (int)kp.size(2), kp.size(0), table.size(1), strides,
                       cache.k_scales.defined(), interleaved, type_code(k), stream_of(k)),
           "moba_paged_append");
+    for (const Tensor& t : {kp, vp, cache.k_scales, cache.v_scales}) written(t);
   }
   if (!out.defined()) Py_RETURN_NONE;
   return THPVariable_Wrap(std::move(out));

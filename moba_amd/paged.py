@@ -183,6 +183,9 @@ def paged_append(cache: PagedKVCache, key: torch.Tensor, value: torch.Tensor, pa
             0 if inv_freq is None else 2 * inv_freq.numel(), cache.k_pages.shape[2], cache.k_pages.shape[0],
             page_table.shape[1], strides, int(cache.quantized), int(interleaved), E._dtype_code(key),
             E._stream(key.device)), "moba_paged_append")
+    # (autograd learns that they have changed, as after any operator that writes; an inference tensor keeps no such number)
+    changed = (cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales)
+    torch.autograd.graph.increment_version([t for t in changed if t is not None and not t.is_inference()])
     return out
 
 

@@ -277,3 +277,31 @@ def test_derivatives_that_there_are_none_of(quantized):
                 paged_append(batch.cache(), *args[:2], *index, query=args[2], inv_freq=args[3])
         with pytest.raises(RuntimeError, match="forward-mode"):
             paged_attention(dual(q), batch.cache(), *index)
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("quantized", [True, False])
+def test_autograd_learns_what_was_written(quantized, native, monkeypatch):
+    """A graph that kept the cache's tensors for its backward pass says that they have changed."""
+    from moba_amd import _lib, paged_append, paged_attention
+    if not native:
+        monkeypatch.setattr(_lib.host(), "paged_append", lambda *a: NotImplemented)
+    batch = Batch([10], [2], 16, 2, 64, BF16, quantized)
+    k, v, q = (x.cuda() for x in batch.tensors(2, 2, 4))
+    index, cache = batch.index(), batch.cache()
+    fields = [x for x in vars(cache).values() if x is not None]
+    kept = cache.v_scales if quantized else cache.v_pages
+    leaf = torch.ones_like(kept, requires_grad=True)
+    loss = (leaf * kept).sum()
+    before = [x._version for x in fields]
+    paged_attention(q, cache, *index)
+    assert [x._version for x in fields] == before
+    paged_append(cache, k, v, *index)
+    assert [x._version for x in fields] == [n + 1 for n in before]
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        cache = batch.cache()
+        paged_append(cache, k, v, *index)
+    paged_append(cache, k, v, *index)
+    check_append(batch, cache, k.cpu(), v.cpu(), None, False)
