@@ -93,3 +93,24 @@ def test_more_work_than_one_round(old, new, page, heads, kv_heads, d, dtype, qua
     got = paged_attention(q.cuda(), cache, *index)
     check_attention(batch, got, q)
     assert torch.equal(got, paged_attention(q.cuda(), cache, *index, max_new=max(new)))
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_scales_of_pages_that_nobody_names(dtype, bad):
+    """The first page of the pool, which is read in the place of pages that are none, and all others that no table names."""
+    from moba_amd import paged_attention
+    batch = Batch([200, 70, 9, 33, 0], [1, 6, 1, 40, 90], 32, 2, 128, dtype, True, seed=5, spare=4)
+    batch.table[0, 2], batch.table[3, 0], batch.table[4, 1] = -1, 10 ** 6, -1
+    free = sorted(set(range(batch.pages[0].shape[0])) - set(batch.table.flatten().tolist()))
+    if free[0] != 0:                                      # (page 0's part goes to a free one)
+        batch.table[batch.table == 0] = free[-1]
+        for x in (*batch.pages, *batch.scales):
+            x[free[-1]] = x[0]
+        free = [0] + free[:-1]
+    q, = batch.tensors(8)
+    for x in batch.scales:
+        x[free] = bad
+    for x in batch.pages:
+        x[free] = float("nan")
+    check_attention(batch, paged_attention(q.cuda(), batch.cache(), *batch.index()), q)
