@@ -1,9 +1,10 @@
 // The rotation by position, as the kernels before the attention and in front of the paged cache apply it.
 //
-// Pair i of a head is turned by the angle position * inv_freq[i].  The angle is a product in 64 bits and its rest, taken in turns by
-// 1 / (2 pi) in two parts of 64 bits, reduced to half a turn either way there, and only then a 32-bit number: its error stays
-// below 2^-24 of a turn for every position that 64 bits tell from the next (up to 2^53) and every angle up to 2^70 turns.
-// (In 32 bits a position of 10^6 is off by 0.06 rad; in 64 bits without the rests one of 2^40 by 2 * 10^-4, one of 2^52 by 0.8.)
+// Pair i of a head is turned by the angle position * inv_freq[i].  The angle is a product in 64 bits, taken in turns and
+// reduced to half a turn either way there, far angles with the rests that 64 bits leave of the product and of 1 / (2 pi), and
+// only then a 32-bit number: its error stays below 2^-24 of a turn for every position that 64 bits tell from the next (up to 2^53)
+// and every angle up to 2^70 turns.  (In 32 bits a position of 10^6 is off by 0.06 rad; in 64 bits without the rests one of 2^40 by
+// 2 * 10^-4, one of 2^52 by 0.8.)
 //
 // A row of D elements is the work of G lanes (8 up to 64 elements, 16 up to 128), 8 elements to a lane in two groups of
 // four: lane u < rotary / 8 holds pairs 4u to 4u+3, the lanes behind hold the elements 8u to 8u+7 that are not turned.
@@ -31,9 +32,13 @@ __device__ __forceinline__ RowPlace row_place(int u, int D, int rotary, bool int
 // cos and sin of the angle of a pair at a position
 __device__ __forceinline__ void turn_of(double position, float inv_freq, float& c, float& s) {
   constexpr double kOver2Pi = 0x1.45f306dc9c883p-3, kOver2PiRest = -0x1.6b01ec5417056p-57;
-  const double f = inv_freq, angle = position * f, rest = fma(position, f, -angle);
-  double turns = fma(angle, kOver2Pi, -rint(angle * kOver2Pi)) + fma(angle, kOver2PiRest, rest * kOver2Pi);
-  turns -= rint(turns);
+  const double f = inv_freq, angle = position * f, near = angle * kOver2Pi;
+  double turns = near - rint(near);
+  if (fabs(near) > 0x1p26) {   // (up to there the two roundings are off by 2^-26 of a turn; both rests everywhere: 1 % of an append)
+    const double rest = fma(position, f, -angle);
+    turns = fma(angle, kOver2Pi, -rint(near)) + fma(angle, kOver2PiRest, rest * kOver2Pi);
+    turns -= rint(turns);
+  }
   sincospif(2.f * (float)turns, &s, &c);
 }
 
