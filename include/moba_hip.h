@@ -410,7 +410,7 @@ int moba_qk_norm_rope_bwd(const void* dyq, const void* dyk, const void* q, const
  * in the whole table.  cache8: scales are powers of two, 2^k with the smallest k >= -100 for which the page's largest magnitude is at most
  * 448 * 2^k, and not less than that of the tokens the page already holds, which are rounded again where it grows.
  *   strides {q token, q head, k token, k head, v token, v head, page_table row} in elements, multiples of 4 (the last: any);
- *   q, k, v and the pages 8-byte aligned; T < 2^30 */
+ *   q, k, v and the pages 8-byte aligned; T < 2^30, and T / page_size + 2 * B, with q T / 16 more, below 2^23 (MOBA_ERR_LIMIT) */
 int moba_paged_append(const void* k, const void* v, const void* q, void* yq, void* k_pages, void* v_pages, float* k_scales,
                       float* v_scales, const int32_t* page_table, const int32_t* lengths, const int32_t* cu_new,
                       const float* inv_freq, int64_t T, int B, int H, int Hkv, int D, int rotary, int page_size,
@@ -424,7 +424,8 @@ int moba_paged_append(const void* k, const void* v, const void* q, void* yq, voi
  *   16-bit pages are of q's type; e4m3 pages (cache8) go with either.
  *   workspace: moba_paged_attention_workspace_bytes(T, B, H, Hkv, D, cache8, max_new) bytes; calls that may run at
  *   the same time need their own
- *   max_new: the most new tokens that a sequence has, or -1: a hint that spares a launch for sequences of many
+ *   max_new: the most new tokens that a sequence has, or -1: a hint that spares a launch for sequences of many.  One that is too
+ *   small costs time, and their last bits may differ
  *   T < 2^24, T * H < 2^31, and fewer than 2^32 threads to a launch (MOBA_ERR_LIMIT otherwise): at most 256 * Hkv for a sequence with
  *   rows, 512 * Hkv with e4m3 pages, and 2 * T * H for long pieces (8 * T * H where max_new says that there are none) */
 size_t moba_paged_attention_workspace_bytes(int64_t T, int B, int H, int Hkv, int D, int cache8, int max_new);

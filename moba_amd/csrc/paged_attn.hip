@@ -518,8 +518,8 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void paged_few_kernel(const Page
 // tiles, one barrier a tile.  16-bit tiles are copied global -> LDS, four waves to a workgroup and two workgroups to a compute unit, so
 // that one's lookups and barriers run under the other's products.  8-bit tiles come through registers, where they become 16-bit
 // elements: eight waves share that work where heads have 128 elements, one workgroup to a compute unit (2048 tokens against 34816
-// keys, 32 and 8 heads: 998 us, with four waves 1076; 16-bit pages: 1037 with eight, 1040 with four, but prompts without a cache 70
-// and 65).  Priority for the products gives 4 % with four waves and takes 2 % with eight.
+// keys, 32 and 8 heads, the whole call: 1067 us, with four waves 1145; 16-bit pages: 1129 with eight, 1111 with four, and 2048 tokens
+// without a cache 77 and 70).  Priority for the products gives 4 % with four waves and takes 2 % with eight.
 constexpr int kManyKeys = 64;
 template <int D, bool k8> constexpr int kManyWaves = D == 128 && k8 ? 8 : 4;
 

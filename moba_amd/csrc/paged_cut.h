@@ -2,8 +2,11 @@
 //
 // A unit is a group of query rows of one (sequence, key/value head) against a run of the sequence's keys.  The host knows
 // neither the sequences' lengths nor how their new tokens are divided (both may change between replays of a captured
-// call), so every workgroup finds its own unit: the runs are as long as fills the chip once with the whole batch's work,
-// and the units of the sequences are counted through.  A long sequence among short ones gets the units that its keys ask for.
+// call), so every workgroup finds its own unit, and the units of the sequences are counted through.  Up to as many groups as the
+// chip has places (half as many where there are more than 64 sequences), the runs are as long as fills the chip once with the
+// whole batch's work, so that a long sequence among short ones gets the units that its keys ask for.  With more they are the work
+// of two places each, however full the last round is, and from kWholeAt times as many on a sequence's keys are one run.  Every
+// group counts with all of its sequence's keys, those that no row of it sees included.
 // One wave looks at 64 sequences at a time: up to 64 of them the whole cut is one load and some hundred cycles.
 #pragma once
 #include "paged.h"
@@ -21,7 +24,9 @@ struct Cut {
   int parts;       // no more than this of them where there is a sequence of several runs
 };
 constexpr int kWholeRun = 0x3fffffff;  // tiles
-constexpr int kWholeAt = 4;            // with this many times `target` groups and more, a sequence's keys are one run
+// With this many times `target` groups and more, a sequence's keys are one run.  That is right for sequences of like lengths, and slow for one
+// long one among them: one token each for 255 sequences, 131072 keys and 254 of 513, 8 heads, 8 bits: 120 us; one more of these: 1135.
+constexpr int kWholeAt = 4;
 
 struct Shape {
   PageTable table;

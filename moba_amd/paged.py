@@ -19,7 +19,7 @@ E4M3 = torch.float8_e4m3fn
 PAGE_SIZES = (16, 32, 64, 128, 256)
 HEAD_DIMS = (64, 128)
 MAX_KV_HEADS = 256
-MAX_TOKENS = (1 << 30) - 1   # packed rows of a call
+MAX_TOKENS = (1 << 30) - 1   # packed rows of a call; paged_append's launch and paged_attention take fewer, see there
 
 
 @dataclass(frozen=True, eq=False)
@@ -140,7 +140,8 @@ def paged_append(cache: PagedKVCache, key: torch.Tensor, value: torch.Tensor, pa
     page (beyond the table's row, or an entry that is no page) is not written.  Elements of 8-bit pages are rounded from
     the rotated 32-bit values; the scale of a page and head is the smallest power of two that takes its largest
     magnitude into e4m3's range, and where new tokens raise the scale of a page, what it holds is rounded again.  An
-    infinite value is held as the largest number the page has.
+    infinite value is held as the largest number an 8-bit page has.  Fewer than 2^30 tokens, and tokens / page_size +
+    2 * sequences (with ``query`` tokens / 16 more) below 2^23.
     """
     out = _lib.host().paged_append(cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales, key, value, page_table, lengths,
                                    cu_new, inv_freq, query, interleaved)
@@ -200,12 +201,19 @@ def paged_attention(query: torch.Tensor, cache: PagedKVCache, page_table: torch.
             sequence b, and every row sees its sequence's tokens up to itself
         scaling: softmax scale, ``head_dim ** -0.5`` by default
         max_new: the most new tokens that a sequence has, if that is known: a hint that spares the search for sequences
-            with many (results do not depend on it)
+            with many.  Results do not depend on it; with one that is too small, sequences that have more than it says are slow,
+            and in the precision of few rows
     Returns:
         [tokens, heads, head_dim] in query's dtype.  Rows that see no token (those of no sequence, of a sequence without
         pages), or whose scores are all minus infinity, are zeros; a page that the table names wrongly (no page of the pool) holds
         no tokens.  No gradients: a query or a cache that requires one is refused outside ``torch.no_grad()``, one with a
         forward-mode tangent everywhere.
+
+    Scores, softmax statistics and sums are 32 bits.  A probability meets the values as the sum of two 16-bit elements (of the
+    values' products: query's type with 16-bit pages, bf16 with 8-bit ones) where a sequence has few rows, new tokens times heads on a
+    key/value head: up to 32, with 8-bit pages 64.  With more rows it is one element, rounded (fp16 queries on 8-bit pages: two of
+    bf16), and values of 8-bit pages whose scale is no power of two are rounded to bf16.  At most 2^24 - 1 tokens, fewer than 2^31
+    tokens times heads, and some million sequences times key/value heads.
     """
     out = _lib.host().paged_attention(cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales, query, page_table, lengths,
                                       cu_new, scaling, max_new)
