@@ -158,20 +158,24 @@ struct NormRope : torch::autograd::Function<NormRope> {
 
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list dy) {
     const auto saved = ctx->get_saved_variables();
-    const NormArgs a = {saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], ctx->saved_data["eps"].toDouble(),
-                        ctx->saved_data["interleaved"].toBool()};
+    NormArgs a = {saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], ctx->saved_data["eps"].toDouble(),
+                  ctx->saved_data["interleaved"].toBool()};
     torch::autograd::variable_list grads(8);
     TORCH_CHECK(!has_tangent(dy[0]) && !has_tangent(dy[1]),
                 "qk_norm_rope has no forward-mode derivatives: tensors with a tangent are refused");
     {
       const at::NoGradGuard no_grad;
       const c10::OptionalDeviceGuard guard(a.q.device());
-      int64_t strides[4];
-      TORCH_CHECK(norm_fits(a, strides), "qk_norm_rope: saved tensors that changed");
       auto packed = [](const Tensor& g) {
         Tensor t = g.contiguous();
         return aligned(t, 16) ? t : t.clone();
       };
+      int64_t strides[4];
+      if (!norm_fits(a, strides)) {   // (hooks on saved tensors may give back copies that lie otherwise)
+        for (Tensor* t : {&a.q, &a.k, &a.positions, &a.inv_freq, &a.q_weight, &a.k_weight})
+          if (t->defined()) *t = packed(*t);
+        TORCH_CHECK(norm_fits(a, strides), "qk_norm_rope: saved tensors that changed");
+      }
       const Tensor dyq = packed(dy[0]), dyk = packed(dy[1]);
       Tensor dq = fresh_like(a.q), dk = fresh_like(a.k), dqw, dkw, space;
       // (the graph's edges are numbered by the tensors there are: a side without a weight has none)

@@ -413,3 +413,28 @@ def test_derivatives_that_there_are_none_of(native, monkeypatch):
         qk_norm_rope(q, k, positions, learned)
     with torch.no_grad():
         assert all(torch.equal(a, b) for a, b in zip(qk_norm_rope(q, k, positions, learned, *w), want))
+
+
+@pytest.mark.parametrize("native", [True])
+def test_saved_tensors_that_come_back_otherwise(native, monkeypatch):
+    """Hooks on saved tensors keep values, not strides and alignment."""
+    from moba_amd import _lib, qk_norm_rope
+    q, k, dq, dk, positions, weights = make(30, 4, 2, 64, BF16, seed=8)
+    inv_freq = frequencies(32, "cuda")
+    if not native:
+        monkeypatch.setattr(_lib.host(), "norm_rope", lambda *a: NotImplemented)
+
+    def shifted(t):
+        return torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)[1:].view(t.shape).copy_(t)
+
+    def strided(t):
+        return torch.stack([t, t], -1)[..., 0]
+
+    def gradients():
+        leaves = [x.detach().clone().requires_grad_() for x in (q, k, *weights)]
+        return torch.autograd.grad(qk_norm_rope(*leaves[:2], positions, inv_freq, *leaves[2:]), leaves, (dq, dk))
+
+    want = gradients()
+    for back in (shifted, strided):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach().clone(), back):
+            assert all(torch.equal(a, b) for a, b in zip(gradients(), want)), back
