@@ -110,7 +110,7 @@ class _QkNormRope(torch.autograd.Function):
         q, k, positions, inv_freq, q_weight, k_weight = ctx.saved_tensors
         if _has_tangent(dyq, dyk):
             raise RuntimeError("qk_norm_rope has no forward-mode derivatives: tensors with a tangent are refused")
-        q, k = _readable(q), _readable(k)
+        q, k, positions, inv_freq = _readable(q), _readable(k), positions.contiguous(), inv_freq.contiguous()
         dyq, dyk = E._aligned(dyq), E._aligned(dyk)
         dq, dk = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
         need = [w is not None and ctx.needs_input_grad[4 + i] for i, w in enumerate((q_weight, k_weight))]

@@ -415,7 +415,7 @@ def test_derivatives_that_there_are_none_of(native, monkeypatch):
         assert all(torch.equal(a, b) for a, b in zip(qk_norm_rope(q, k, positions, learned, *w), want))
 
 
-@pytest.mark.parametrize("native", [True])
+@pytest.mark.parametrize("native", [True, False])
 def test_saved_tensors_that_come_back_otherwise(native, monkeypatch):
     """Hooks on saved tensors keep values, not strides and alignment."""
     from moba_amd import _lib, qk_norm_rope
