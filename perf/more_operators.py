@@ -416,7 +416,7 @@ def _run_prefix(s, case):
 def _run_sums(s, case):
     if own:
         from moba_amd import paged_key_sums
-        paged_key_sums(s["cache"], s["sums"], s["page_table"], s["lengths"], s["cu_new"])
+        paged_key_sums(s["cache"], s["sums"], s["page_table"], s["lengths"], s["cu_new"], s["query"].shape[0])
         return s["sums"]
     held = torch.arange(case["page"], device="cuda") < s["filled"][:, None]
     s["sums"][s["touched"]] = torch.where(held[:, None, :, None], _laid_out(s, "k", s["touched"]), 0).sum(2)
