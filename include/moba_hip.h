@@ -58,7 +58,7 @@ extern "C" {
 
 enum { MOBA_DTYPE_BF16 = 0, MOBA_DTYPE_F16 = 1 };
 
-#define MOBA_ABI_VERSION 121 /* the signatures below; moba_version() returns the number the library was built with */
+#define MOBA_ABI_VERSION 122 /* the signatures below; moba_version() returns the number the library was built with */
 int moba_version(void);
 const char* moba_strerror(int code);
 
@@ -434,6 +434,68 @@ int moba_paged_attention(const void* q, void* out, const void* k_pages, const vo
                          void* workspace, int64_t T, int B, int H, int Hkv, int D, int page_size, int64_t num_pages,
                          int64_t max_pages, int max_new, const int64_t* strides, int cache8, float scale, int dtype,
                          void* stream);
+
+/* moba_paged_prefix_attention: the result of moba_paged_attention where groups of neighbouring sequences begin with the same pages,
+ * which are read once for all of a group's rows.
+ *   cu_groups [G+1] int32: group g is sequences cu_groups[g] .. cu_groups[g+1]-1 (those outside of all groups share nothing);
+ *   shared [G] int32: leading tokens for which the table rows of a group's sequences name the same pages (the first one's are read;
+ *   rounded down to a multiple of 64).  Read on the device.
+ *   The rest as for moba_paged_attention; fewer than 2^32 threads to a launch: about twice as many as there. */
+size_t moba_paged_prefix_attention_workspace_bytes(int64_t T, int B, int G, int H, int Hkv, int D, int cache8);
+int moba_paged_prefix_attention(const void* q, void* out, const void* k_pages, const void* v_pages, const float* k_scales,
+                                const float* v_scales, const int32_t* page_table, const int32_t* lengths, const int32_t* cu_new,
+                                const int32_t* cu_groups, const int32_t* shared, void* workspace, int64_t T, int B, int G, int H,
+                                int Hkv, int D, int page_size, int64_t num_pages, int64_t max_pages, const int64_t* strides,
+                                int cache8, float scale, int dtype, void* stream);
+
+/* Blocks of the cache that a new token attends (of whole prompts in the reference: moba/moba_efficient.py:326-443).  A block is
+ * block_size tokens of a sequence, a multiple of page_size.
+ *
+ * moba_paged_key_sums: sums [num_pages, Hkv, D] fp32 of the keys that a page holds, for the pages that have received the new tokens
+ *   (of T packed rows); other pages' are left as they are.  k_pages 16-byte aligned.  table_stride: of the page table, in entries.
+ *   (T / page_size + 2 * B) * Hkv below 2^25.
+ * moba_paged_select_blocks: blocks [T,H,topk] int32: of every row the topk - 1 blocks in front of its token's own whose products
+ *   q . (sum of their pages' sums), in 64 bits, are largest (of equal ones the lowest; NaN as minus infinity), and its own, ascending;
+ *   -1 behind the last.  topk at most 64; the table at most 16384 blocks wide.  q, sums 16-byte aligned; strides {q token, q head,
+ *   page_table row}, the first two multiples of 8.  workspace (scores): 8-byte aligned.
+ * moba_paged_block_attention: softmax attention of every row over the keys of its blocks (any [T,H,topk] int32: an entry that is no
+ *   block of the sequence up to the token's own is none, the same block twice is once) up to its token.  Up to 32 rows
+ *   (tokens times heads) of a sequence and key/value head read the union of their blocks once.  Precision: that of few rows in
+ *   moba_paged_attention.  Rows without a key are zeros.  topk at most 64, block_size at most 2^24;
+ *   (T * H / Hkv / 32 + B) * Hkv below 2^24.  The rest as for moba_paged_attention. */
+int moba_paged_key_sums(const void* k_pages, const float* k_scales, float* sums, const int32_t* page_table, const int32_t* lengths,
+                        const int32_t* cu_new, int64_t T, int B, int Hkv, int D, int page_size, int64_t num_pages,
+                        int64_t max_pages, int64_t table_stride, int cache8, int dtype, void* stream);
+size_t moba_paged_select_blocks_workspace_bytes(int64_t T, int B, int H, int Hkv, int page_size, int64_t max_pages, int block_size);
+int moba_paged_select_blocks(const void* q, const float* sums, int32_t* blocks, const int32_t* page_table, const int32_t* lengths,
+                             const int32_t* cu_new, void* workspace, int64_t T, int B, int H, int Hkv, int D, int page_size,
+                             int64_t num_pages, int64_t max_pages, int block_size, int topk, const int64_t* strides, int dtype,
+                             void* stream);
+size_t moba_paged_block_attention_workspace_bytes(int64_t T, int B, int H, int Hkv, int D, int page_size, int64_t max_pages,
+                                                  int block_size, int topk, int cache8);
+int moba_paged_block_attention(const void* q, void* out, const void* k_pages, const void* v_pages, const float* k_scales,
+                               const float* v_scales, const int32_t* blocks, const int32_t* page_table, const int32_t* lengths,
+                               const int32_t* cu_new, void* workspace, int64_t T, int B, int H, int Hkv, int D, int page_size,
+                               int64_t num_pages, int64_t max_pages, int block_size, int topk, const int64_t* strides, int cache8,
+                               float scale, int dtype, void* stream);
+
+/* Pages from a pool and back, on the device.  The pool is a stack: free_pages [num_pages] int32, of which the first free_count [1]
+ * are free.  page_table [B, max_pages] int32 with rows of table_stride entries, lengths [B] int32.  B at most 8192, B * max_pages
+ * below 2^31.
+ *
+ * moba_paged_reserve: new_tokens [B] int32 more tokens for every sequence.  One whose tokens do not fit its row of the table gets none; of
+ *   the others one is served if its tokens and those asked for before it are at most `rows`, and the pages that it and those before
+ *   it need are there (or it needs none); otherwise it gets nothing.  Writes the entries of the new pages, lengths (the served
+ *   ones'), free_count, cu_new [B+1] (the running sum of the tokens given), and for each of the rows its sequence, position and slot
+ *   (page * page_size + place in it): owners, positions [rows] int32, slots [rows] int64; -1, 0, -1 behind cu_new[B], and slot -1 where
+ *   the table names no page of the pool.  rows < 2^30, 0 allowed.
+ * moba_paged_release: sequences keep their first keep[b] tokens; the pages behind go back to the pool (entries that name none of
+ *   it do not), so that a reserve that is taken back leaves the stack as it was, and their entries become -1. */
+int moba_paged_reserve(int32_t* free_pages, int32_t* free_count, int32_t* page_table, int32_t* lengths, const int32_t* new_tokens,
+                       int32_t* cu_new, int32_t* owners, int32_t* positions, int64_t* slots, int B, int64_t rows, int page_size,
+                       int64_t num_pages, int64_t max_pages, int64_t table_stride, void* stream);
+int moba_paged_release(int32_t* free_pages, int32_t* free_count, int32_t* page_table, int32_t* lengths, const int32_t* keep, int B,
+                       int page_size, int64_t num_pages, int64_t max_pages, int64_t table_stride, void* stream);
 
 /* Measurement aid, no counterpart in the reference: what the matrix pipes sustain when they do nothing else.
  * Launches `workgroups` workgroups (0: one per compute unit) of eight waves, two per SIMD as in the forward kernel;

@@ -7,10 +7,14 @@ from .config import MoBAConfig
 from .moba_efficient import moba_attn_varlen, moba_attn_varlen_gqa
 from .norm_rope import qk_norm_rope
 from .paged import PagedKVCache, paged_append, paged_attention
+from .paged_blocks import paged_block_attention, paged_key_sums, paged_select_blocks
+from .paged_prefix import paged_prefix_attention
+from .paged_tables import PagePool, paged_release, paged_reserve
 from .wrapper import moba_layer
 
 __all__ = ["MoBAConfig", "register_moba", "moba_attn_varlen", "moba_attn_varlen_gqa", "moba_layer", "qk_norm_rope", "PagedKVCache",
-           "paged_append", "paged_attention"]
+           "paged_append", "paged_attention", "paged_prefix_attention", "paged_key_sums", "paged_select_blocks", "paged_block_attention",
+           "PagePool", "paged_reserve", "paged_release"]
 
 
 def register_moba(cfg: MoBAConfig):

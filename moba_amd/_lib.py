@@ -67,6 +67,18 @@ _SIGNATURES = {
     "moba_paged_attention_workspace_bytes": (c_size_t, [c_int64] + [c_int] * 6),
     "moba_paged_attention": (c_int, [c_void_p] * 10 + [c_int64] + [c_int] * 5 + [c_int64] * 2 + [c_int, c_strides, c_int, c_float, c_int,
                                                                                                c_void_p]),
+    "moba_paged_prefix_attention_workspace_bytes": (c_size_t, [c_int64] + [c_int] * 6),
+    "moba_paged_prefix_attention": (c_int, [c_void_p] * 12 + [c_int64] + [c_int] * 6 + [c_int64] * 2 + [c_strides, c_int, c_float, c_int,
+                                                                                                       c_void_p]),
+    "moba_paged_key_sums": (c_int, [c_void_p] * 6 + [c_int64] + [c_int] * 4 + [c_int64] * 3 + [c_int] * 2 + [c_void_p]),
+    "moba_paged_select_blocks_workspace_bytes": (c_size_t, [c_int64] + [c_int] * 4 + [c_int64, c_int]),
+    "moba_paged_select_blocks": (c_int, [c_void_p] * 7 + [c_int64] + [c_int] * 5 + [c_int64] * 2 + [c_int] * 2
+                                        + [c_strides, c_int, c_void_p]),
+    "moba_paged_block_attention_workspace_bytes": (c_size_t, [c_int64] + [c_int] * 5 + [c_int64] + [c_int] * 3),
+    "moba_paged_block_attention": (c_int, [c_void_p] * 11 + [c_int64] + [c_int] * 5 + [c_int64] * 2 + [c_int] * 2
+                                          + [c_strides, c_int, c_float, c_int, c_void_p]),
+    "moba_paged_reserve": (c_int, [c_void_p] * 9 + [c_int, c_int64, c_int] + [c_int64] * 3 + [c_void_p]),
+    "moba_paged_release": (c_int, [c_void_p] * 5 + [c_int, c_int] + [c_int64] * 3 + [c_void_p]),
     "moba_mfma_probe": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p]),
     "moba_tail_splits": (c_int, [c_int] * 5),
     "moba_tail": (c_int, [c_void_p] * 6 + [c_int] * 6 + [c_strides, c_float, c_int, c_void_p]),
@@ -96,7 +108,7 @@ class SizesStruct(ctypes.Structure):
     _fields_ = [(n, c_int64) for n in ("kbar_elems", "chunk_mean_workspace_bytes", "sel_ints", "cnt_ints", "seg_off_ints",
                                        "seg_dest_ints", "fwd_hist_bound", "bwd_hist_bound", "part_rows", "redo_ints",
                                        "lse_floats", "delta_floats")]
-ABI_VERSION = 121  # MOBA_ABI_VERSION of include/moba_hip.h, the signatures above
+ABI_VERSION = 122  # MOBA_ABI_VERSION of include/moba_hip.h, the signatures above
 DTYPE_BF16, DTYPE_F16 = 0, 1
 
 
@@ -147,6 +159,7 @@ def host():
                                "`python -m moba_amd.build`")
         bind(module, lib.moba_tail)
         bind_layer(module)
+        bind_serving(module)
         _host = module
     return _host
 
@@ -163,6 +176,15 @@ def bind_layer(module, **instead):
     names = ("moba_qk_norm_rope", "moba_qk_norm_rope_bwd", "moba_qk_norm_rope_bwd_workspace_bytes", "moba_paged_append",
              "moba_paged_attention", "moba_paged_attention_workspace_bytes", "moba_strerror")
     module.bind_layer(*(ctypes.cast(instead.get(n, getattr(lib, n)), c_void_p).value for n in names))
+
+
+def bind_serving(module, **instead):
+    """Give the extension module the entry points of the operators of serving, `instead` in the place of some."""
+    lib = load()
+    names = ("moba_paged_prefix_attention", "moba_paged_prefix_attention_workspace_bytes", "moba_paged_block_attention",
+             "moba_paged_block_attention_workspace_bytes", "moba_paged_key_sums", "moba_paged_select_blocks",
+             "moba_paged_select_blocks_workspace_bytes", "moba_paged_reserve", "moba_paged_release")
+    module.bind_serving(*(ctypes.cast(instead.get(n, getattr(lib, n)), c_void_p).value for n in names))
 
 
 def exported_symbols():

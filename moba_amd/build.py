@@ -1,5 +1,5 @@
 """Builds the HIP kernels into ``moba_amd/libmoba_hip.so`` with hipcc for gfx950, and the extension module
-``moba_amd._host`` (csrc/host.cpp, csrc/host_layer.cpp, host code) with g++.
+``moba_amd._host`` (csrc/host*.cpp, host code) with g++.
 
 Run as ``python -m moba_amd.build``.  hipcc cross-compiles without a GPU.
 """
@@ -17,8 +17,8 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(CSRC, "build")
 LIB = os.path.join(HERE, "libmoba_hip.so")
 HOST = os.path.join(HERE, "_host" + sysconfig.get_config_var("EXT_SUFFIX"))   # extension module, see csrc/host.cpp
-SOURCES = ["chunk_mean.hip", "gate_topk.hip", "lists.hip", "fwd.hip", "fwd_tile.hip", "bwd.hip", "decode.hip", "norm_rope.hip", "paged_append.hip", "paged_attn.hip",
-           "plan.hip", "probe.hip", "capi.hip"]
+SOURCES = ["chunk_mean.hip", "gate_topk.hip", "lists.hip", "fwd.hip", "fwd_tile.hip", "bwd.hip", "decode.hip", "norm_rope.hip", "paged_append.hip", "paged_attn.hip", "paged_prefix.hip",
+           "paged_blocks.hip", "paged_select.hip", "paged_tables.hip", "plan.hip", "probe.hip", "capi.hip"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [
@@ -52,10 +52,10 @@ def _compile(src: str, force: bool) -> str:
 
 
 def _host_module(force: bool) -> None:
-    """csrc/host.cpp and csrc/host_layer.cpp against the installed PyTorch (host code only)."""
+    """csrc/host.cpp, csrc/host_layer.cpp and csrc/host_serving.cpp against the installed PyTorch (host code only)."""
     import torch
-    srcs = [os.path.join(CSRC, name) for name in ("host.cpp", "host_layer.cpp")]
-    deps = [*srcs, os.path.join(CSRC, "host_layer.h"), os.path.abspath(__file__), os.path.join(os.path.dirname(HERE), "include", "moba_hip.h")]
+    srcs = [os.path.join(CSRC, name) for name in ("host.cpp", "host_layer.cpp", "host_serving.cpp")]
+    deps = [*srcs, *(os.path.join(CSRC, name) for name in ("host_layer.h", "host_tensors.h")), os.path.abspath(__file__), os.path.join(os.path.dirname(HERE), "include", "moba_hip.h")]
     root = os.path.dirname(torch.__file__)
     include = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
                os.path.join(os.path.dirname(os.path.dirname(HIPCC)), "include"), sysconfig.get_paths()["include"]]

@@ -160,6 +160,13 @@ PyMethodDef methods[] = {
     {"paged_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_paged_append)), METH_FASTCALL, nullptr},
     {"paged_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_paged_attention)), METH_FASTCALL, nullptr},
     {"bind_layer", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_bind_layer)), METH_FASTCALL, nullptr},
+    {"paged_prefix_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_paged_prefix_attention)), METH_FASTCALL, nullptr},
+    {"paged_block_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_paged_block_attention)), METH_FASTCALL, nullptr},
+    {"paged_key_sums", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_paged_key_sums)), METH_FASTCALL, nullptr},
+    {"paged_select_blocks", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_paged_select_blocks)), METH_FASTCALL, nullptr},
+    {"paged_reserve", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_paged_reserve)), METH_FASTCALL, nullptr},
+    {"paged_release", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_paged_release)), METH_FASTCALL, nullptr},
+    {"bind_serving", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_bind_serving)), METH_FASTCALL, nullptr},
     {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_bind)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

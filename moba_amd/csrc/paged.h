@@ -26,16 +26,19 @@ struct PageTable {
   int num_pages, max_pages, page_log2;
 };
 
-// rows lo .. hi - 1 are the sequence's new tokens; token t of them is its position length - hi + t
+// rows lo .. hi - 1 are the sequence's new tokens; token t of them is its position length - hi + t.  begin: the first key that they
+// attend as this sequence's (where sequences share what lies before it, see paged_shared.h)
 struct Sequence {
   int lo, hi;
   int64_t length;
+  int begin;
 };
 __device__ __forceinline__ Sequence sequence_of(const PageTable& t, int b) {
   Sequence s;
   s.lo = min(max(t.cu_new[b], 0), t.T);
   s.hi = min(max(t.cu_new[b + 1], s.lo), t.T);
   s.length = max(t.lengths[b], 0);
+  s.begin = 0;
   return s;
 }
 // tokens that the sequence's row of the table has room for

@@ -28,19 +28,30 @@ constexpr int kWholeRun = 0x3fffffff;  // tiles
 // long one among them: one token each for 255 sequences, 131072 keys and 254 of 513, 8 heads, 8 bits: 120 us; one more of these: 1135.
 constexpr int kWholeAt = 4;
 
+// Table: PageTable, or another that has its own count_of(), sequence_of(), table_row() and `kShares`
+template <class Table>
 struct Shape {
-  PageTable table;
+  Table table;
   int H, Hkv, rep;
 };
+__device__ __forceinline__ int count_of(const PageTable& t) { return t.B; }                // sequences
+__device__ __forceinline__ int table_row(const PageTable& t, int b) { return b; }          // a sequence's row of the page table
+template <class Table>
+constexpr bool kShares = false;   // whether a token attends keys of more than one sequence
+template <class Table>
+constexpr bool kChooses = false;  // whether a row attends some of the keys only
 
 // A sequence's part in a cut: groups of rows (0: none of its units are of this cut), tiles of keys
 struct Share {
   Sequence seq;
   int groups, tiles;
 };
-__device__ __forceinline__ int keys_of(const Shape& p, const Sequence& s) { return (int)min(s.length, room(p.table)); }
-__device__ __forceinline__ Share share_of(const Shape& p, const Cut& c, const Sequence& s) {
-  const int rows = (s.hi - s.lo) * p.rep, keys = keys_of(p, s);
+// the end of a sequence's keys
+template <class Table>
+__device__ __forceinline__ int keys_of(const Shape<Table>& p, const Sequence& s) { return (int)min(s.length, room(p.table)); }
+template <class Table>
+__device__ __forceinline__ Share share_of(const Shape<Table>& p, const Cut& c, const Sequence& s) {
+  const int rows = (s.hi - s.lo) * p.rep, keys = keys_of(p, s) - s.begin;
   Share r;
   r.seq = s;
   r.tiles = keys > 0 ? (keys - 1) / c.tile_keys + 1 : 0;
@@ -48,8 +59,9 @@ __device__ __forceinline__ Share share_of(const Shape& p, const Cut& c, const Se
   return r;
 }
 // of sequence b, each lane its own
-__device__ __forceinline__ Share share_at(const Shape& p, const Cut& c, int b) {
-  if (b >= p.table.B) return {{0, 0, 0}, 0, 0};
+template <class Table>
+__device__ __forceinline__ Share share_at(const Shape<Table>& p, const Cut& c, int b) {
+  if (b >= count_of(p.table)) return {{0, 0, 0, 0}, 0, 0};
   return share_of(p, c, sequence_of(p.table, b));
 }
 
@@ -73,9 +85,10 @@ __device__ __forceinline__ int runs_of(int tiles, int run) { return (tiles - 1) 
 // more, that come to at most `target` units (each group's last run may be short); runs of work / (target - n) always do.  Where the groups
 // alone are more than half the target, of work / (target / 2), and where they fill the chip several times, whole sequences.  No runs of
 // fewer than least_tiles: where a unit's start outweighs a tile, short runs cost more in the merge than they save.
-__device__ __forceinline__ int run_tiles(const Shape& p, const Cut& c, int lane, const Share& first) {
+template <class Table>
+__device__ __forceinline__ int run_tiles(const Shape<Table>& p, const Cut& c, int lane, const Share& first) {
   int64_t work = 0, groups = 0;
-  for (int b0 = 0; b0 < p.table.B; b0 += 64) {
+  for (int b0 = 0; b0 < count_of(p.table); b0 += 64) {
     const Share s = b0 ? share_at(p, c, b0 + lane) : first;
     const int64_t w = (int64_t)s.groups * s.tiles;   // (below 2^56: in pieces of 24 bits a wave's sum fits 32)
     work += wave_sum((uint32_t)w & 0xffffff) + ((int64_t)wave_sum((uint32_t)(w >> 24) & 0xffffff) << 24) +
@@ -87,7 +100,7 @@ __device__ __forceinline__ int run_tiles(const Shape& p, const Cut& c, int lane,
     return a < 1LL << 31 ? (int)(((uint32_t)a + (uint32_t)b - 1) / (uint32_t)b) : (int)min((a + b - 1) / b, (int64_t)kWholeRun);
   };
   const int safe = max(ceil_div(work, max(max((int64_t)c.target - groups, (int64_t)c.target / 2), (int64_t)1)), work > 0 ? c.least_tiles : 0);
-  if (p.table.B <= 64 && groups <= c.target)
+  if (count_of(p.table) <= 64 && groups <= c.target)
     for (int run = max(ceil_div(work, c.target), c.least_tiles); run < safe; run += run / 16 + 1)
       if (wave_sum(first.groups ? first.groups * runs_of(first.tiles, run) : 0) <= (uint32_t)c.target) return run;
   return safe;
@@ -98,9 +111,10 @@ struct Unit {
   int b, group, run, runs, groups, tiles, first;  // tiles: of the sequence; first: number of the sequence's first unit
 };
 // unit number u: all groups of a sequence's first run, then of its second, ...  b = -1 past the last
-__device__ __forceinline__ Unit unit_at(const Shape& p, const Cut& c, int u, int run, int lane, const Share& first) {
+template <class Table>
+__device__ __forceinline__ Unit unit_at(const Shape<Table>& p, const Cut& c, int u, int run, int lane, const Share& first) {
   int64_t base = 0;
-  for (int b0 = 0; b0 < p.table.B; b0 += 64) {
+  for (int b0 = 0; b0 < count_of(p.table); b0 += 64) {
     const Share s = b0 ? share_at(p, c, b0 + lane) : first;
     const int runs = s.groups ? runs_of(s.tiles, run) : 0;
     const uint32_t mine = (uint32_t)s.groups * runs, upto = upto_sum(mine);
@@ -113,6 +127,7 @@ __device__ __forceinline__ Unit unit_at(const Shape& p, const Cut& c, int u, int
       r.seq.lo = of(s.seq.lo);
       r.seq.hi = of(s.seq.hi);
       r.seq.length = of((int)s.seq.length);
+      r.seq.begin = kShares<Table> ? of(s.seq.begin) : 0;
       r.runs = of(runs);
       r.groups = of(s.groups);
       r.tiles = of(s.tiles);
@@ -128,6 +143,20 @@ __device__ __forceinline__ Unit unit_at(const Shape& p, const Cut& c, int u, int
   Unit none = {};
   none.b = -1;
   return none;
+}
+
+// The unit of a workgroup, its key/value head, and the number under which it leaves what the merge has to know; false: none.  Workgroups
+// are numbered by unit and head.
+template <class Table>
+__device__ __forceinline__ bool find_unit(const Shape<Table>& p, const Cut& c, int lane, Unit& unit, int& hkv, int& item) {
+  const int u = (int)blockIdx.x / p.Hkv;
+  hkv = (int)blockIdx.x - u * p.Hkv;
+  const Share first = share_at(p, c, lane);
+  const int run = run_tiles(p, c, lane, first);
+  if (run == 0) return false;   // (no work at all)
+  unit = unit_at(p, c, u, run, lane, first);
+  item = unit.b;
+  return unit.b >= 0 && (unit.runs == 1 || u < c.parts);   // (the latter: row ranges that are none)
 }
 
 // What the merge has to know of a sequence, left for it by the sequence's first unit

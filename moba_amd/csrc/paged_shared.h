@@ -1,0 +1,82 @@
+// Sequences that begin with the same pages: what is common is attended once for all of them.
+//
+// cu_groups [G+1] cuts the sequences into groups of neighbours, shared [G] says how many leading tokens the tables of a group's
+// sequences name the same pages for.  The batch is attended as G + B sequences: number g < G has all new tokens of group g as its
+// rows and the first shared[g] tokens (rounded down to whole tiles) of the group's first table as its keys; number G + b has
+// sequence b's rows and the keys behind those.  Every row sees keys up to its own position in either, so that the result is that
+// of the sequences one by one, whatever `shared` says of equal tables.  A token's rows of both sides meet in the merge.
+#pragma once
+#include "paged_cut.h"
+
+namespace moba {
+
+constexpr int kSharedStep = 64;   // a run of keys begins at a multiple of this
+
+struct SharedTable : PageTable {
+  const int32_t* cu_groups;  // [G+1]
+  const int32_t* shared;     // [G]
+  int G;
+};
+template <>
+constexpr bool kShares<SharedTable> = true;
+
+__device__ __forceinline__ int first_member(const SharedTable& t, int g) { return min(max(t.cu_groups[g], 0), t.B); }
+// the end of the keys that a group attends together
+__device__ __forceinline__ int shared_keys(const SharedTable& t, int g) {
+  return (int)min((int64_t)(max(t.shared[g], 0) & -kSharedStep), room(t));
+}
+// group of sequence b, -1 if it is in none: the last g < G with cu_groups[g] <= b, if b < cu_groups[g + 1]
+__device__ __forceinline__ int group_of(const SharedTable& t, int b) {
+  int lo = 0, hi = t.G;   // cu_groups[lo] <= b < cu_groups[hi], but for the ends
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (t.cu_groups[mid] <= b) lo = mid; else hi = mid;
+  }
+  return t.cu_groups[lo] <= b && b < t.cu_groups[lo + 1] ? lo : -1;
+}
+
+__device__ __forceinline__ int count_of(const SharedTable& t) { return t.G + t.B; }
+__device__ __forceinline__ int table_row(const SharedTable& t, int v) {
+  return __builtin_amdgcn_readfirstlane(v < t.G ? min(first_member(t, v), t.B - 1) : v - t.G);
+}
+__device__ __forceinline__ Sequence sequence_of(const SharedTable& t, int v) {
+  Sequence s;
+  if (v < t.G) {
+    const int first = first_member(t, v), end = max(min(t.cu_groups[v + 1], t.B), first);
+    s.lo = min(max(t.cu_new[first], 0), t.T);
+    s.hi = min(max(t.cu_new[end], s.lo), t.T);
+    s.length = shared_keys(t, v);
+    s.begin = 0;
+  } else {
+    s = sequence_of(static_cast<const PageTable&>(t), v - t.G);
+    const int g = group_of(t, v - t.G);
+    s.begin = g >= 0 ? (int)min((int64_t)shared_keys(t, g), min(s.length, room(t))) : 0;
+  }
+  return s;
+}
+
+// Position of new token j of a unit's rows: in its own sequence, the last member of the group that begins no later.
+__device__ __forceinline__ int position_at(const SharedTable& t, const Unit& u, int j) {
+  if (u.b >= t.G) return (int)u.seq.length - (u.seq.hi - u.seq.lo) + j;
+  const int token = u.seq.lo + j, end = min(t.cu_groups[u.b + 1], t.B);
+  int lo = first_member(t, u.b), hi = end;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (t.cu_new[mid] <= token) lo = mid; else hi = mid;
+  }
+  lo = min(lo, t.B - 1);
+  const Sequence s = sequence_of(static_cast<const PageTable&>(t), lo);
+  return (int)min(s.length - s.hi + token, (int64_t)0x7fffffff);
+}
+// (a group's rows are of several sequences)
+__device__ __forceinline__ int least_position(const SharedTable& t, const Unit& u, int first, int position) {
+  if (u.b >= t.G) return position_at(t, u, first);
+#pragma unroll
+  for (int d = 16; d >= 1; d >>= 1) position = min(position, __shfl_xor(position, d, 64));
+  return __builtin_amdgcn_readfirstlane(position);
+}
+__device__ __forceinline__ int last_seen(const SharedTable& t, const Unit& u, int j) {
+  return u.b >= t.G ? position_at(t, u, j) : 0x7ffffffe;
+}
+
+}  // namespace moba

@@ -74,6 +74,11 @@ class PagedKVCache:
             return cls(*pages)
         return cls(*pages, *(torch.ones(shape[:2], dtype=torch.float32, device=device) for _ in range(2)))
 
+    def key_sums(self) -> torch.Tensor:
+        """Zeros for the sums of the pages' keys, [num_pages, kv_heads, head_dim] float32, that ``paged_key_sums`` keeps."""
+        pages, heads, _, d = self.k_pages.shape
+        return torch.zeros((pages, heads, d), dtype=torch.float32, device=self.k_pages.device)
+
     @property
     def quantized(self) -> bool:
         return self.k_scales is not None
@@ -97,6 +102,18 @@ def _check_table(cache, page_table, lengths, cu_new, device):
 def _table(page_table):
     """The page table with contiguous rows."""
     return page_table if page_table.stride(1) == 1 or page_table.shape[1] <= 1 else page_table.contiguous()
+
+
+def _plain(t):
+    """The tensor itself, without a subclass of torch.Tensor around it."""
+    return t if t is None or type(t) is torch.Tensor else t.as_subclass(torch.Tensor)
+
+
+def _taken(out, name):
+    """The answer of a native call that has to take its arguments."""
+    if out is NotImplemented:
+        raise RuntimeError(f"{name} cannot take these tensors")
+    return out
 
 
 def _check_rows(cache, name, x, heads=None):
