@@ -77,7 +77,7 @@ _SIGNATURES = {
     "moba_paged_block_attention_workspace_bytes": (c_size_t, [c_int64] + [c_int] * 5 + [c_int64] + [c_int] * 3),
     "moba_paged_block_attention": (c_int, [c_void_p] * 11 + [c_int64] + [c_int] * 5 + [c_int64] * 2 + [c_int] * 2
                                           + [c_strides, c_int, c_float, c_int, c_void_p]),
-    "moba_paged_reserve": (c_int, [c_void_p] * 9 + [c_int, c_int64, c_int] + [c_int64] * 3 + [c_void_p]),
+    "moba_paged_reserve": (c_int, [c_void_p] * 10 + [c_int, c_int64, c_int] + [c_int64] * 3 + [c_void_p]),
     "moba_paged_release": (c_int, [c_void_p] * 5 + [c_int, c_int] + [c_int64] * 3 + [c_void_p]),
     "moba_mfma_probe": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p]),
     "moba_tail_splits": (c_int, [c_int] * 5),
@@ -108,7 +108,7 @@ class SizesStruct(ctypes.Structure):
     _fields_ = [(n, c_int64) for n in ("kbar_elems", "chunk_mean_workspace_bytes", "sel_ints", "cnt_ints", "seg_off_ints",
                                        "seg_dest_ints", "fwd_hist_bound", "bwd_hist_bound", "part_rows", "redo_ints",
                                        "lse_floats", "delta_floats")]
-ABI_VERSION = 122  # MOBA_ABI_VERSION of include/moba_hip.h, the signatures above
+ABI_VERSION = 123  # MOBA_ABI_VERSION of include/moba_hip.h, the signatures above
 DTYPE_BF16, DTYPE_F16 = 0, 1
 
 

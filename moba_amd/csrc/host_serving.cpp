@@ -231,8 +231,9 @@ PyObject* py_paged_reserve(PyObject*, PyObject* const* args, Py_ssize_t n) {
     out[1] = fresh({rows}, at::kInt, device);
     out[2] = fresh({rows}, at::kInt, device);
     out[3] = fresh({rows}, at::kLong, device);
+    Tensor space = bytes((b + 1) * 4, device);
     check(reserve_call(t.of(t.free_pages), t.of(t.free_count), t.of(t.table), t.of(t.lengths), t.of(t.asked), t.of(out[0]), t.of(out[1]),
-                       t.of(out[2]), (int64_t*)out[3].mutable_data_ptr(), (int)b, rows, (int)t.page, t.free_pages.size(0), t.table.size(1),
+                       t.of(out[2]), (int64_t*)out[3].mutable_data_ptr(), (int32_t*)space.mutable_data_ptr(), (int)b, rows, (int)t.page, t.free_pages.size(0), t.table.size(1),
                        t.table.stride(0), stream_of(t.lengths)),
           "moba_paged_reserve");
     for (const Tensor& x : {t.free_count, t.table, t.lengths}) written(x);

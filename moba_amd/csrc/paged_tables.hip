@@ -8,11 +8,15 @@
 // Page number i that is given out (the served sequences' in order) is the i-th from the top.  Release is the inverse: the pages
 // of a sequence behind its first `keep` tokens go back so that the first sequence's first page is on top again.
 //
-// One workgroup decides (the sums over the sequences, in LDS), fills the table and, for up to kRowsAtOnce rows, says where they belong;
-// more rows are a second launch of as many workgroups as that takes.  Nothing here is floating point, and no order depends on
-// timing: sums are scans.  Bound by latency: loads of the lengths, two scans, a search in LDS and a load for every page and row.
+// One workgroup decides: the sums over the sequences are scans in registers (of 32 bits that saturate: what is compared with a limit
+// may stop there) with one number of every wave in LDS.  For up to kRowsAtOnce rows it also fills the table and says where the rows
+// belong; more are a second launch of as many workgroups as that takes, which finds ranks and rows in what the first has left.
+// A row's page is looked up where it comes from, the table or the pool's stack, and waits for no entry to be written.  Nothing here
+// is floating point, and no order depends on timing.  Bound by latency: 64 sequences with five tokens each 4.2 us, their way back 4.1
+// (with 64-bit sums by lane shuffles, and rows that waited for the table, 10.4 and 4.9); eight documents of 471000 tokens on 29000
+// pages of 16 tokens 3.1 + 7.5 us, and 16.3 back, whose places on the stack one workgroup counts.
 #include "common.h"
-#include "paged.h"
+#include "paged_cut.h"
 
 namespace moba {
 
@@ -33,34 +37,45 @@ struct TableParams {
   const int32_t* asked;  // [B]: new tokens, or those to keep
   int32_t *cu_new, *owners, *positions;   // [B+1], [rows], [rows]
   int64_t* slots;        // [rows]
+  int32_t* ranks;        // [B+1]: number of the first page given to a sequence, and of all of them
   int64_t stride;
   int B, rows, max_pages, page_log2;
 };
 
-// inclusive sums over the threads up to this one, and over all of them.  `red`: [2 * kTableWaves]; every thread calls it
-template <class T>
-struct Scan {
-  T upto, all;
+// Sums over the threads up to this one, and over all of them, of two numbers at a time
+struct Two {
+  uint32_t a, b;
 };
-template <class T>
-__device__ __forceinline__ Scan<T> scan(T x, T* red) {
+struct Scan {
+  Two upto, all;
+};
+__device__ __forceinline__ uint32_t add_sat(uint32_t x, uint32_t y) { return __builtin_elementwise_add_sat(x, y); }
+// the lanes' sums as upto_sum() has them, saturating
+__device__ __forceinline__ uint32_t upto_sat(uint32_t x) {
+#define MOBA_DPP_ADD(ctrl, rows) x = add_sat(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, ctrl, rows, 0xf, false))
+  MOBA_DPP_ADD(0x111, 0xf);
+  MOBA_DPP_ADD(0x112, 0xf);
+  MOBA_DPP_ADD(0x114, 0xf);
+  MOBA_DPP_ADD(0x118, 0xf);
+  MOBA_DPP_ADD(0x142, 0xa);
+  MOBA_DPP_ADD(0x143, 0xc);
+#undef MOBA_DPP_ADD
+  return x;
+}
+// red: [waves], another one than in the call before; every thread calls it
+__device__ __forceinline__ Scan scan(Two x, Two* red) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const T y = __shfl_up(x, d, 64);
-    if (lane >= d) x += y;
-  }
-  __syncthreads();   // (the former call's sums have been read)
+  x = {upto_sat(x.a), upto_sat(x.b)};
   if (lane == 63) red[wave] = x;
   __syncthreads();
-  T before = 0, all = 0;
+  Two before = {0, 0}, all = {0, 0};
 #pragma unroll
   for (int w = 0; w < kTableWaves; ++w) {
-    const T y = red[w];
-    before += w < wave ? y : 0;
-    all += y;
+    const Two y = red[w];
+    before = {w < wave ? add_sat(before.a, y.a) : before.a, w < wave ? add_sat(before.b, y.b) : before.b};
+    all = {add_sat(all.a, y.a), add_sat(all.b, y.b)};
   }
-  return {x + before, all};
+  return {{add_sat(x.a, before.a), add_sat(x.b, before.b)}, all};
 }
 
 // the last i in [0, n) with a[i] <= x, for ascending a with a[0] <= x
@@ -75,33 +90,43 @@ __device__ __forceinline__ int last_at_most(const int* a, int n, int x) {
 
 __device__ __forceinline__ int pages_of(int64_t tokens, int page_log2) { return (int)((tokens + (1 << page_log2) - 1) >> page_log2); }
 
-// Row t, whose sequence's rows are cu[b] .. cu[b+1] - 1 and end at its last token
-__device__ __forceinline__ void place_row(const TableParams& p, const int* cu, int t) {
+// Row t of a batch whose row ranges, given pages and former lengths are cu, rank [B+1] and old(b); top: free pages before the call
+template <class Old>
+__device__ __forceinline__ void place_row(const TableParams& p, const int* cu, const int* rank, Old old, int top, int t) {
   int b = -1, position = 0;
   int64_t slot = -1;
   if (t < cu[p.B]) {
     b = last_at_most(cu, p.B, t);
-    position = p.lengths[b] - (cu[b + 1] - t);
+    const int before = old(b), have = pages_of(before, p.page_log2);
+    position = before + t - cu[b];
     const int page = position >> p.page_log2;
-    const int id = position >= 0 && page < p.max_pages ? p.table[b * p.stride + page] : -1;
+    const int id = page < have ? p.table[b * p.stride + page] : p.pool.free_pages[top - 1 - (rank[b] + page - have)];
     if (id >= 0 && id < p.pool.num_pages) slot = ((int64_t)id << p.page_log2) + (position & ((1 << p.page_log2) - 1));
   }
   p.owners[t] = b;
   p.positions[t] = position;
   p.slots[t] = slot;
 }
+// Pages i .. of those that are given, up to `end`, go to their entries
+template <class Old>
+__device__ __forceinline__ void place_pages(const TableParams& p, const int* rank, Old old, int top, int i, int end) {
+  if (i >= end) return;
+  for (int b = last_at_most(rank, p.B, i); i < end; ++i) {
+    while (rank[b + 1] <= i) ++b;   // (some sequence has page i: i < rank[B])
+    p.table[b * p.stride + pages_of(old(b), p.page_log2) + i - rank[b]] = p.pool.free_pages[top - 1 - i];
+  }
+}
 
 __global__ __launch_bounds__(kTableThreads) void paged_reserve_kernel(const TableParams p) {
-  extern __shared__ __attribute__((aligned(8))) int lds[];
-  int64_t* const red = reinterpret_cast<int64_t*>(lds);
-  int* const rank = lds + 2 * kTableWaves;   // [B]: pages given to the sequences before
-  int* const have = rank + p.B;              // [B]: pages that a sequence had
-  int* const cu = have + p.B;                // [B+1]
+  __shared__ Two red[2][kTableWaves];
+  extern __shared__ int lds[];
+  int* const cu = lds;                       // [B+1]
+  int* const rank = cu + p.B + 1;            // [B+1]
+  int* const old_length = rank + p.B + 1;    // [B]
   const int tid = threadIdx.x;
-  const int free_count = min(max(*p.pool.free_count, 0), p.pool.num_pages);
+  const int top = min(max(*p.pool.free_count, 0), p.pool.num_pages);
   const int64_t most = min((int64_t)p.max_pages << p.page_log2, (int64_t)0x7fffffff);
-  int64_t asked = 0, asked_pages = 0;   // sums over the sequences of the steps before
-  int given = 0, given_pages = 0;
+  Two asked = {0, 0}, given = {0, 0};   // tokens and pages, of the sequences of the steps before
   for (int b0 = 0; b0 < p.B; b0 += kTableThreads) {
     const int b = b0 + tid;
     int64_t old = 0, n = 0;
@@ -110,61 +135,64 @@ __global__ __launch_bounds__(kTableThreads) void paged_reserve_kernel(const Tabl
       n = max(p.asked[b], 0);
       if (old + n > most) n = 0;
     }
-    const int held = pages_of(old, p.page_log2), need = pages_of(old + n, p.page_log2) - held;
-    const Scan<int64_t> tokens = scan<int64_t>(n, red), pages = scan<int64_t>(need, red);
-    const bool served = asked + tokens.upto <= p.rows && (need == 0 || asked_pages + pages.upto <= free_count);
-    asked += tokens.all;
-    asked_pages += pages.all;
-    // (of the served both sums fit 31 bits)
-    const Scan<int64_t> both = scan<int64_t>(served ? n << 32 | need : 0, red);
+    const uint32_t need = pages_of(old + n, p.page_log2) - pages_of(old, p.page_log2);
+    const Scan wanted = scan({(uint32_t)n, need}, red[0]);
+    const bool served = add_sat(asked.a, wanted.upto.a) <= (uint32_t)p.rows &&
+                        (need == 0 || add_sat(asked.b, wanted.upto.b) <= (uint32_t)top);
+    asked = {add_sat(asked.a, wanted.all.a), add_sat(asked.b, wanted.all.b)};
+    const Scan got = scan({served ? (uint32_t)n : 0, served ? need : 0}, red[1]);   // (below 2^31)
     if (b < p.B) {
-      cu[b + 1] = given + (int)(both.upto >> 32);
-      rank[b] = given_pages + (int)(uint32_t)both.upto - (served ? need : 0);
-      have[b] = held;
-      p.cu_new[b + 1] = cu[b + 1];
+      const int end = (int)(given.a + got.upto.a), pages = (int)(given.b + got.upto.b);
+      cu[b + 1] = end;
+      rank[b + 1] = pages;
+      old_length[b] = (int)old;
+      p.cu_new[b + 1] = end;
+      if (p.rows > kRowsAtOnce) p.ranks[b + 1] = pages;
       if (served && n) p.lengths[b] = (int)(old + n);
     }
-    given += (int)(both.all >> 32);
-    given_pages += (int)(uint32_t)both.all;
+    given = {given.a + got.all.a, given.b + got.all.b};
   }
   if (tid == 0) {
-    cu[0] = 0;
-    p.cu_new[0] = 0;
-    *p.pool.free_count = free_count - given_pages;
-  }
-  __syncthreads();
-  const int each = given_pages > kTableThreads ? kPagesOfThread : 1;
-  for (int64_t i0 = (int64_t)tid * each; i0 < given_pages; i0 += kTableThreads * each) {
-    int b = last_at_most(rank, p.B, (int)i0);
-    for (int i = (int)i0; i < min(i0 + each, (int64_t)given_pages); ++i) {
-      while (b + 1 < p.B && rank[b + 1] <= i) ++b;
-      p.table[b * p.stride + have[b] + i - rank[b]] = p.pool.free_pages[free_count - 1 - i];
-    }
+    cu[0] = rank[0] = p.cu_new[0] = 0;
+    if (p.rows > kRowsAtOnce) p.ranks[0] = 0;
+    *p.pool.free_count = top - (int)given.b;
   }
   if (p.rows > kRowsAtOnce) return;
-  __syncthreads();   // (the table and the lengths are written)
-  for (int t = tid; t < p.rows; t += kTableThreads) place_row(p, cu, t);
+  __syncthreads();
+  auto old = [&](int b) { return old_length[b]; };
+  for (int t = tid; t < p.rows; t += kTableThreads) place_row(p, cu, rank, old, top, t);
+  for (int i = tid; i < (int)given.b; i += kTableThreads) place_pages(p, rank, old, top, i, i + 1);
 }
 
+// the same for rows, and pages, that are many: each thread four of them (there are no more pages than rows)
 __global__ __launch_bounds__(256) void paged_rows_kernel(const TableParams p) {
-  extern __shared__ __attribute__((aligned(8))) int cu[];
-  for (int b = threadIdx.x; b <= p.B; b += 256) cu[b] = p.cu_new[b];
+  extern __shared__ int lds[];
+  int *const cu = lds, *const rank = lds + p.B + 1;
+  for (int b = threadIdx.x; b <= p.B; b += 256) {
+    cu[b] = p.cu_new[b];
+    rank[b] = p.ranks[b];
+  }
   __syncthreads();
+  const int top = *p.pool.free_count + rank[p.B];
+  auto old = [&](int b) { return max(p.lengths[b], 0) - (cu[b + 1] - cu[b]); };
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const int64_t t = (int64_t)blockIdx.x * 1024 + k * 256 + threadIdx.x;
-    if (t < p.rows) place_row(p, cu, (int)t);
+    if (t < p.rows) place_row(p, cu, rank, old, top, (int)t);
   }
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i < rank[p.B]) place_pages(p, rank, old, top, (int)i, (int)min(i + 4, (int64_t)rank[p.B]));
 }
 
 __global__ __launch_bounds__(kTableThreads) void paged_release_kernel(const TableParams p) {
-  extern __shared__ __attribute__((aligned(8))) int lds[];
-  int64_t* const red = reinterpret_cast<int64_t*>(lds);
-  int* const first = lds + 2 * kTableWaves;  // [B]: entries that go in the sequences before (their number is below 2^31)
+  __shared__ Two red[2][kTableWaves];
+  __shared__ int counts[2][kPagesOfThread * kTableWaves];
+  extern __shared__ int lds[];
+  int* const first = lds;                    // [B]: entries that go in the sequences before (their number is below 2^31)
   int* const stay = first + p.B;             // [B]: pages that stay
-  const int tid = threadIdx.x;
-  int free_count = min(max(*p.pool.free_count, 0), p.pool.num_pages), total = 0;
-  for (int b0 = 0; b0 < p.B; b0 += kTableThreads) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int free_count = min(max(*p.pool.free_count, 0), p.pool.num_pages), total = 0, parity = 0;
+  for (int b0 = 0; b0 < p.B; b0 += kTableThreads, parity ^= 1) {
     const int b = b0 + tid;
     int gone = 0, kept = 0;
     if (b < p.B) {
@@ -173,47 +201,56 @@ __global__ __launch_bounds__(kTableThreads) void paged_release_kernel(const Tabl
       gone = min(pages_of(old, p.page_log2), p.max_pages) - kept;
       if (keep < old) p.lengths[b] = keep;
     }
-    const Scan<int64_t> s = scan<int64_t>(gone, red);
+    const Scan s = scan({(uint32_t)gone, 0}, red[parity]);
     if (b < p.B) {
-      first[b] = total + (int)s.upto - gone;
+      first[b] = total + (int)s.upto.a - gone;
       stay[b] = kept;
     }
-    total += (int)s.all;
+    total += (int)s.all.a;
   }
   __syncthreads();
-  // from the last entry to the first, so that a place on the stack is the number of pages that have come before
-  const int each = total > kTableThreads ? kPagesOfThread : 1;
-  for (int64_t r0 = 0; r0 < total; r0 += kTableThreads * each) {
-    const int64_t mine = r0 + (int64_t)tid * each;
-    int id[kPagesOfThread], count = 0;
-    if (mine < total) {
-      int b = last_at_most(first, p.B, total - 1 - (int)mine);
+  // From the last entry to the first, so that a place on the stack is the number of pages that have come before.  Entry k * kTableThreads +
+  // thread of a step is number k of a thread.
+  for (int64_t r0 = 0; r0 < total; r0 += kTableThreads * kPagesOfThread, parity ^= 1) {
+    int id[kPagesOfThread], before[kPagesOfThread];
 #pragma unroll
-      for (int k = 0; k < kPagesOfThread; ++k) {
-        id[k] = -1;
-        if (k >= each || mine + k >= total) continue;
-        const int i = total - 1 - (int)(mine + k);
-        while (first[b] > i) --b;
+    for (int k = 0; k < kPagesOfThread; ++k) {
+      const int64_t r = r0 + k * kTableThreads + tid;
+      id[k] = -1;
+      if (r < total) {
+        const int i = total - 1 - (int)r, b = last_at_most(first, p.B, i);
         int32_t* const entry = p.table + b * p.stride + stay[b] + i - first[b];
-        const int x = *entry;
+        id[k] = *entry;
         *entry = -1;
-        if (x >= 0 && x < p.pool.num_pages) {
-          id[k] = x;
-          ++count;
-        }
       }
     }
-    const Scan<int64_t> s = scan<int64_t>(count, red);
-    if (mine < total) {
-      int64_t place = free_count + s.upto - count;
 #pragma unroll
-      for (int k = 0; k < kPagesOfThread; ++k)
-        if (k < each && id[k] >= 0) {
-          if (place < p.pool.num_pages) p.pool.free_pages[place] = id[k];   // (more than there are: named twice)
-          ++place;
-        }
+    for (int k = 0; k < kPagesOfThread; ++k) {
+      const uint64_t m = __ballot(id[k] >= 0 && id[k] < p.pool.num_pages);
+      before[k] = __builtin_popcountll(m & ((1ull << lane) - 1));
+      if (lane == 0) counts[parity][k * kTableWaves + wave] = __builtin_popcountll(m);
     }
-    free_count = (int)min(free_count + s.all, (int64_t)p.pool.num_pages);
+    __syncthreads();
+    // sums of the counts, each wave for itself
+    constexpr int kCounts = kPagesOfThread * kTableWaves, kEach = (kCounts + 63) / 64;
+    int x[kEach], sum = 0;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      x[j] = lane * kEach + j < kCounts ? counts[parity][lane * kEach + j] : 0;
+      sum += x[j];
+    }
+    const int upto = (int)upto_sum((uint32_t)sum), all = __builtin_amdgcn_readlane(upto, 63);
+#pragma unroll
+    for (int k = 0; k < kPagesOfThread; ++k) {
+      const int at = k * kTableWaves + wave, in_lane = at % kEach;
+      int place = __builtin_amdgcn_readlane(upto - sum, at / kEach);
+#pragma unroll
+      for (int j = 0; j < kEach; ++j)
+        if (j < in_lane) place += __builtin_amdgcn_readlane(x[j], at / kEach);
+      const int64_t to = (int64_t)free_count + place + before[k];
+      if (id[k] >= 0 && id[k] < p.pool.num_pages && to < p.pool.num_pages) p.pool.free_pages[to] = id[k];   // (more than there are: named twice)
+    }
+    free_count = (int)min((int64_t)free_count + all, (int64_t)p.pool.num_pages);
   }
   if (tid == 0) *p.pool.free_count = free_count;
 }
@@ -238,23 +275,25 @@ static int check_tables(TableParams& p, int32_t* free_pages, int32_t* free_count
 using namespace moba;
 
 extern "C" int moba_paged_reserve(int32_t* free_pages, int32_t* free_count, int32_t* page_table, int32_t* lengths,
-                                  const int32_t* new_tokens, int32_t* cu_new, int32_t* owners, int32_t* positions, int64_t* slots, int B,
-                                  int64_t rows, int page_size, int64_t num_pages, int64_t max_pages, int64_t table_stride, void* stream) {
+                                  const int32_t* new_tokens, int32_t* cu_new, int32_t* owners, int32_t* positions, int64_t* slots, int32_t* workspace,
+                                  int B, int64_t rows, int page_size, int64_t num_pages, int64_t max_pages, int64_t table_stride, void* stream) {
   TableParams p;
   const int rc = check_tables(p, free_pages, free_count, page_table, lengths, new_tokens, B, page_size, num_pages, max_pages, table_stride);
   if (rc != MOBA_OK) return rc;
-  if (!cu_new || rows < 0 || (rows && (!owners || !positions || !slots)) || ((uintptr_t)slots & 7)) return MOBA_ERR_ARG;
+  if (!cu_new || !workspace || rows < 0 || (rows && (!owners || !positions || !slots)) || ((uintptr_t)slots & 7)) return MOBA_ERR_ARG;
   if (rows >= 1LL << 30) return MOBA_ERR_LIMIT;
-  p.cu_new = cu_new; p.owners = owners; p.positions = positions; p.slots = slots;
+  p.cu_new = cu_new; p.owners = owners; p.positions = positions; p.slots = slots; p.ranks = workspace;
   p.rows = (int)rows;
-  static bool allowed[kMaxDevices];
-  const int most_lds = (2 * kTableWaves + 3 * kMostTableSequences + 1) * 4, need = (2 * kTableWaves + 3 * B + 1) * 4;
   LaunchCheck launch_check;
-  if (!allow_dynamic_lds((const void*)paged_reserve_kernel, most_lds, allowed)) return MOBA_ERR_LAUNCH;
   hipStream_t st = (hipStream_t)stream;
+  const int need = (3 * B + 2) * 4;
+  static bool allowed[2][kMaxDevices];
+  if (!allow_dynamic_lds((const void*)paged_reserve_kernel, (3 * kMostTableSequences + 2) * 4, allowed[0]) ||
+      !allow_dynamic_lds((const void*)paged_rows_kernel, (2 * kMostTableSequences + 2) * 4, allowed[1]))
+    return MOBA_ERR_LAUNCH;
   hipLaunchKernelGGL(paged_reserve_kernel, dim3(1), dim3(kTableThreads), need, st, p);
   if (rows > kRowsAtOnce)
-    hipLaunchKernelGGL(paged_rows_kernel, dim3((unsigned)((rows + 1023) / 1024)), dim3(256), (B + 1) * 4, st, p);
+    hipLaunchKernelGGL(paged_rows_kernel, dim3((unsigned)((rows + 1023) / 1024)), dim3(256), (2 * B + 2) * 4, st, p);
   return launch_check.result();
 }
 
@@ -263,10 +302,9 @@ extern "C" int moba_paged_release(int32_t* free_pages, int32_t* free_count, int3
   TableParams p;
   const int rc = check_tables(p, free_pages, free_count, page_table, lengths, keep, B, page_size, num_pages, max_pages, table_stride);
   if (rc != MOBA_OK) return rc;
-  static bool allowed[kMaxDevices];
-  const int most_lds = (2 * kTableWaves + 2 * kMostTableSequences) * 4, need = (2 * kTableWaves + 2 * B) * 4;
   LaunchCheck launch_check;
-  if (!allow_dynamic_lds((const void*)paged_release_kernel, most_lds, allowed)) return MOBA_ERR_LAUNCH;
-  hipLaunchKernelGGL(paged_release_kernel, dim3(1), dim3(kTableThreads), need, (hipStream_t)stream, p);
+  static bool allowed[kMaxDevices];
+  if (!allow_dynamic_lds((const void*)paged_release_kernel, 2 * kMostTableSequences * 4, allowed)) return MOBA_ERR_LAUNCH;
+  hipLaunchKernelGGL(paged_release_kernel, dim3(1), dim3(kTableThreads), 2 * B * 4, (hipStream_t)stream, p);
   return launch_check.result();
 }

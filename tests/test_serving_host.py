@@ -51,16 +51,16 @@ def test_tables_entry_points_refuse():
     lib = _lib.load()
     some = 256   # (never read)
 
-    def reserve(free=some, count=some, table=some, lengths=some, new=some, cu=some, owners=some, positions=some, slots=some, B=2, rows=4,
+    def reserve(free=some, count=some, table=some, lengths=some, new=some, cu=some, owners=some, positions=some, slots=some, space=some, B=2, rows=4,
                 page=16, pool=3, wide=1, stride=1):
-        return lib.moba_paged_reserve(free, count, table, lengths, new, cu, owners, positions, slots, B, rows, page, pool, wide, stride, None)
+        return lib.moba_paged_reserve(free, count, table, lengths, new, cu, owners, positions, slots, space, B, rows, page, pool, wide, stride, None)
 
     def release(free=some, count=some, table=some, lengths=some, new=some, B=2, page=16, pool=3, wide=1, stride=1):
         return lib.moba_paged_release(free, count, table, lengths, new, B, page, pool, wide, stride, None)
 
     common = [dict(free=None), dict(count=None), dict(table=None), dict(lengths=None), dict(new=None), dict(B=0), dict(pool=0), dict(wide=0),
               dict(stride=-1)]
-    for wrong in common + [dict(cu=None), dict(owners=None), dict(positions=None), dict(slots=None), dict(slots=some + 4), dict(rows=-1)]:
+    for wrong in common + [dict(cu=None), dict(owners=None), dict(positions=None), dict(slots=None), dict(space=None), dict(slots=some + 4), dict(rows=-1)]:
         assert reserve(**wrong) == -1, wrong
     for wrong in common:
         assert release(**wrong) == -1, wrong
