@@ -26,18 +26,18 @@ struct SumParams {
   const char* pages;
   const float* scales;   // 8-bit pages
   float* sums;           // [num_pages, Hkv, D]
-  int Hkv, items;
+  int Hkv, items;   // waves
 };
 
-// One wave to a page and head: 64 / L tokens at a time, L lanes of 16 bytes to a token.
-template <class E, int D, bool k8>
+// One wave to kHeads heads of a page: 64 / L tokens at a time, L lanes of 16 bytes to a token, the heads' steps on their way together.
+template <class E, int D, bool k8, int kHeads>
 __global__ __launch_bounds__(256) void paged_key_sums_kernel(const SumParams<E> p) {
   constexpr int kRow = D * (k8 ? 1 : 2), L = kRow / 16, kTokens = 64 / L, kElems = k8 ? 16 : 8, kAhead = 8;
   const int lane = threadIdx.x & 63;
   const int item = __builtin_amdgcn_readfirstlane((int)blockIdx.x * 4 + (threadIdx.x >> 6));
   if (item >= p.items) return;
   const PageTable& table = p.table;
-  const int u = item / p.Hkv, hkv = item - u * p.Hkv;
+  const int parts = (p.Hkv + kHeads - 1) / kHeads, u = item / parts, h0 = (item - u * parts) * kHeads;
   Sequence seq = {};
   auto start = [&](int b, int lo) { return (int64_t)(lo >> table.page_log2) + 2 * (int64_t)b; };
   const int b = last_up_to(table, u, lane, seq, start);
@@ -47,57 +47,76 @@ __global__ __launch_bounds__(256) void paged_key_sums_kernel(const SumParams<E> 
   const int held = (int)min(max(seq.length - (page << table.page_log2), (int64_t)0), (int64_t)1 << table.page_log2);
   const int id = __builtin_amdgcn_readfirstlane(page_id(table, b, page));
   if (held == 0 || id < 0) return;
-  const int64_t head = (int64_t)id * p.Hkv + hkv;
   const int r = lane / L, c = lane % L;
-  const char* const from = p.pages + ((head << table.page_log2) + r) * kRow + c * 16;
-  float acc[kElems];
+  const int64_t head0 = (int64_t)id * p.Hkv + h0;
+  const char* const from = p.pages + (head0 << table.page_log2) * kRow + c * 16;
+  const int64_t head_bytes = (int64_t)kRow << table.page_log2;
+  float by[kHeads];
+  float acc[kHeads][kElems];
 #pragma unroll
-  for (int e = 0; e < kElems; ++e) acc[e] = 0.f;
+  for (int h = 0; h < kHeads; ++h) {
+    by[h] = k8 ? p.scales[head0 + (h0 + h < p.Hkv ? h : 0)] : 1.f;
+#pragma unroll
+    for (int e = 0; e < kElems; ++e) acc[h][e] = 0.f;
+  }
   for (int t0 = 0; t0 < held; t0 += kTokens * kAhead) {
-    u32x4 w[kAhead];
+    u32x4 w[kHeads][kAhead];
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      w[k] = u32x4{0, 0, 0, 0};   // (what a page holds behind its sequence's end counts for nothing)
-      if (t0 + k * kTokens + r < held) w[k] = *reinterpret_cast<const u32x4*>(from + (int64_t)(t0 + k * kTokens) * kRow);
+    for (int h = 0; h < kHeads; ++h)
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k)   // (tokens behind the last held one, and heads behind the last, are others again)
+        w[h][k] = *reinterpret_cast<const u32x4*>(from + (h0 + h < p.Hkv ? h : 0) * head_bytes + min(t0 + k * kTokens + r, held - 1) * kRow);
+    if (t0 + kTokens * kAhead > held) {
+#pragma unroll
+      for (int h = 0; h < kHeads; ++h)
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k)
+          if (t0 + k * kTokens + r >= held) w[h][k] = u32x4{0, 0, 0, 0};
     }
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      if constexpr (k8) {
+    for (int h = 0; h < kHeads; ++h)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          acc[4 * i] += __builtin_amdgcn_cvt_f32_fp8(w[k][i], 0);
-          acc[4 * i + 1] += __builtin_amdgcn_cvt_f32_fp8(w[k][i], 1);
-          acc[4 * i + 2] += __builtin_amdgcn_cvt_f32_fp8(w[k][i], 2);
-          acc[4 * i + 3] += __builtin_amdgcn_cvt_f32_fp8(w[k][i], 3);
+      for (int k = 0; k < kAhead; ++k) {
+        if constexpr (k8) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            acc[h][4 * i] += __builtin_amdgcn_cvt_f32_fp8(w[h][k][i], 0);
+            acc[h][4 * i + 1] += __builtin_amdgcn_cvt_f32_fp8(w[h][k][i], 1);
+            acc[h][4 * i + 2] += __builtin_amdgcn_cvt_f32_fp8(w[h][k][i], 2);
+            acc[h][4 * i + 3] += __builtin_amdgcn_cvt_f32_fp8(w[h][k][i], 3);
+          }
+        } else {
+          const typename E::elem8 x = __builtin_bit_cast(typename E::elem8, w[h][k]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) acc[h][e] += (float)x[e];
         }
-      } else {
-        const typename E::elem8 x = __builtin_bit_cast(typename E::elem8, w[k]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) acc[e] += (float)x[e];
       }
-    }
   }
   // the lanes of a column: each keeps half of what it has and is given the other's of that half
-  int n = kElems, at = c * kElems;
 #pragma unroll
-  for (int m = 32; m >= L; m >>= 1) {
-    n /= 2;
-    const bool upper = lane & m;
+  for (int h = 0; h < kHeads; ++h) {
+    int n = kElems, at = c * kElems;
 #pragma unroll
-    for (int i = 0; i < kElems / 2; ++i) {
-      if (i >= n) break;
-      const float mine = upper ? acc[i + n] : acc[i], other = upper ? acc[i] : acc[i + n];
-      acc[i] = mine + __shfl_xor(other, m, 64);
+    for (int m = 32; m >= L; m >>= 1) {
+      n /= 2;
+      const bool upper = lane & m;
+#pragma unroll
+      for (int i = 0; i < kElems / 2; ++i) {
+        if (i >= n) break;
+        const float mine = upper ? acc[h][i + n] : acc[h][i], other = upper ? acc[h][i] : acc[h][i + n];
+        acc[h][i] = mine + __shfl_xor(other, m, 64);
+      }
+      at += upper ? n : 0;
     }
-    at += upper ? n : 0;
-  }
-  const float by = k8 ? p.scales[head] : 1.f;
+    if (h0 + h < p.Hkv) {
 #pragma unroll
-  for (int i = 0; i < D / 64; ++i) p.sums[head * D + at + i] = acc[i] * by;
+      for (int i = 0; i < D / 64; ++i) p.sums[(head0 + h) * D + at + i] = acc[h][i] * by[h];
+    }
+  }
 }
 
 // ---- scores
-constexpr int kScoreRows = 16;
+constexpr int kScoreRows = 32, kScoreSumsLog2 = 4, kScoreSums = 1 << kScoreSumsLog2;
 constexpr int kMostBlocks = 16384;   // of a sequence
 
 struct SelectShape {
@@ -115,18 +134,22 @@ struct SelectParams {
   int64_t q_tok_stride, q_head_stride;
   const float* sums;
   double* scores;       // [tokens, H, blocks]
-  int split_log2;       // threads of a block's column
+  int split_log2;       // sums that a block's pages are shared out to
 };
 __device__ __forceinline__ int64_t block_tokens(const SelectShape& s) { return (int64_t)s.each << s.table.page_log2; }
 
+// A workgroup forms the sums of up to 16 blocks (fewer where a block's pages are shared out among threads) in LDS, and their products
+// with its rows by v_mfma_f64_16x16x4, a quarter of the elements to a wave.
 template <class E, int D>
 __global__ __launch_bounds__(256) void paged_score_kernel(const SelectParams<E> p) {
-  constexpr int kQuads = D / 4, kSums = 256 / kQuads, kPitch = D + 2, kAhead = 8;
-  __shared__ double part[kSums][kPitch];
-  __shared__ float rows[kScoreRows][D + 1];
+  constexpr int kQuads = D / 4, kThreads = 256 / kQuads, kRounds = kScoreSums / kThreads, kAhead = 4;
+  typedef double f64x4 __attribute__((ext_vector_type(4)));
+  __shared__ double part[kScoreSums][D + 2];
+  __shared__ float rows[kScoreRows][D + 4];
+  __shared__ double red[4][kScoreRows][kScoreSums + 1];
   const SelectShape& s = p.s;
   const PageTable& table = s.table;
-  const int tid = threadIdx.x, lane = tid & 63, hkv = blockIdx.y;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hkv = blockIdx.y;
   Sequence seq = {};
   auto cut = [&](int row) { return min(max(row - s.t0, 0), s.tokens); };
   auto start = [&](int b, int lo) { return (int64_t)cut(lo) * s.rep / kScoreRows + b; };
@@ -138,7 +161,7 @@ __global__ __launch_bounds__(256) void paged_score_kernel(const SelectParams<E> 
   const int rows_here = (int)min(count - row0, (int64_t)kScoreRows);
   const int64_t last = seq.length - seq.hi + lo + (row0 + rows_here - 1) / s.rep;   // position of the last of them
   const int history = (int)min(max(last, (int64_t)0) / block_tokens(s), (int64_t)s.blocks);
-  const int split = 1 << p.split_log2, at_once = kSums >> p.split_log2;
+  const int split = 1 << p.split_log2, at_once = kScoreSums >> p.split_log2;
   if ((int)blockIdx.z * at_once >= history) return;
   for (int i = tid; i < rows_here * (D / 8); i += 256) {
     const int r = i / (D / 8), d = i % (D / 8) * 8, row = (int)row0 + r, j = row / s.rep;
@@ -147,26 +170,38 @@ __global__ __launch_bounds__(256) void paged_score_kernel(const SelectParams<E> 
 #pragma unroll
     for (int e = 0; e < 8; ++e) rows[r][d + e] = (float)x[e];
   }
-  const int quad = tid % kQuads, sum = tid / kQuads, mine = sum % at_once, part_of = sum / at_once;
+  const int quad = tid % kQuads;
   for (int j0 = blockIdx.z * at_once; j0 < history; j0 += gridDim.z * at_once) {
-    double acc[4] = {0., 0., 0., 0.};
-    const int64_t page0 = (int64_t)(j0 + mine) * s.each;
-    if (j0 + mine < history)
-      for (int i0 = part_of; i0 < s.each; i0 += split * kAhead) {
-        f32x4 x[kAhead];
+    // sum number i: of block i % at_once, its pages i / at_once, .. + split, ..
+    double acc[kRounds][4];
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k) {
-          const int i = i0 + k * split, id = i < s.each ? page_id(table, b, page0 + i) : -1;
-          x[k] = f32x4{0.f, 0.f, 0.f, 0.f};
-          if (id >= 0) x[k] = *reinterpret_cast<const f32x4*>(p.sums + ((int64_t)id * s.Hkv + hkv) * D + 4 * quad);
+    for (int k = 0; k < kRounds; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[k][e] = 0.;
+    for (int i0 = 0; i0 < s.each; i0 += split * kAhead) {
+      f32x4 x[kRounds][kAhead];
+#pragma unroll
+      for (int k = 0; k < kRounds; ++k) {
+        const int sum = tid / kQuads + k * kThreads, j = j0 + (sum & (at_once - 1));
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+          const int i = i0 + a * split + (sum >> (kScoreSumsLog2 - p.split_log2));
+          const int id = i < s.each && j < history ? page_id(table, b, (int64_t)j * s.each + i) : -1;
+          x[k][a] = f32x4{0.f, 0.f, 0.f, 0.f};
+          if (id >= 0) x[k][a] = *reinterpret_cast<const f32x4*>(p.sums + ((int64_t)id * s.Hkv + hkv) * D + 4 * quad);
         }
-#pragma unroll
-        for (int k = 0; k < kAhead; ++k)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[e] += (double)x[k][e];
       }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) part[sum][4 * quad + e] = acc[e];
+      for (int k = 0; k < kRounds; ++k)
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[k][e] += (double)x[k][a][e];
+    }
+#pragma unroll
+    for (int k = 0; k < kRounds; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) part[tid / kQuads + k * kThreads][4 * quad + e] = acc[k][e];
     __syncthreads();
     if (split > 1) {
       for (int i = tid; i < at_once * D; i += 256) {
@@ -176,17 +211,24 @@ __global__ __launch_bounds__(256) void paged_score_kernel(const SelectParams<E> 
       }
       __syncthreads();
     }
-    // 256 / (16 * at_once) threads to a row and block, at least one
-    const int threads = kSums == 16 && at_once == 16 ? 1 : 16 / at_once;
-    const int dot = tid / threads, k0 = tid - dot * threads, r = dot / at_once, j = dot - r * at_once;
-    double x = 0.;
-    for (int d = k0; d < D; d += threads) x = fma((double)rows[r < rows_here ? r : 0][d], part[j][d], x);
-    for (int m = threads / 2; m >= 1; m >>= 1) x += __shfl_xor(x, m, 64);
-    if (k0 == 0 && r < rows_here && j0 + j < history) {
-      const int row = (int)row0 + r, t = row / s.rep;
-      p.scores[((int64_t)(lo - s.t0 + t) * s.H + hkv * s.rep + row - t * s.rep) * s.blocks + j0 + j] = x;
+    // (rows and blocks that are none have columns and rows of their own)
+    for (int r0 = 0; r0 < rows_here; r0 += 16) {
+      f64x4 c = {0., 0., 0., 0.};
+#pragma unroll
+      for (int m = 0; m < D / 16; ++m) {
+        const int d = wave * (D / 4) + 4 * m + (lane >> 4);
+        c = __builtin_amdgcn_mfma_f64_16x16x4f64((double)rows[r0 + (lane & 15)][d], part[lane & 15][d], c, 0, 0, 0);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) red[wave][r0 + (lane >> 4) + 4 * e][lane & 15] = c[e];
     }
     __syncthreads();
+    for (int r = tid >> 4; r < rows_here; r += 16) {
+      const int j = tid & 15, row = (int)row0 + r, t = row / s.rep;
+      if (j < at_once && j0 + j < history)
+        p.scores[((int64_t)(lo - s.t0 + t) * s.H + hkv * s.rep + row - t * s.rep) * s.blocks + j0 + j] =
+            red[0][r][j] + red[1][r][j] + red[2][r][j] + red[3][r][j];
+    }
   }
 }
 
@@ -332,16 +374,19 @@ template <class E, int D>
 static int launch_select(SelectParams<E> p, int32_t* out, int64_t T, hipStream_t st) {
   LaunchCheck launch_check;
   SelectShape& s = p.s;
-  const int sums = 256 / (D / 4);
-  p.split_log2 = 0;
-  while ((2 << p.split_log2) <= sums && (16 << p.split_log2) <= s.each) ++p.split_log2;
-  const int chunks = (s.blocks - 1) / (sums >> p.split_log2) + 1;
   const int64_t step = tokens_at_once(T, s.H, s.blocks);
   for (int64_t t0 = 0; t0 < T; t0 += step) {
     s.t0 = (int)t0;
     s.tokens = (int)(T - t0 < step ? T - t0 : step);
-    const int64_t units = (int64_t)s.tokens * s.rep / kScoreRows + s.table.B, want = 4096 / (units * s.Hkv);
-    const int z = (int)(want < 1 ? 1 : want < chunks ? want : chunks);
+    const int64_t units = (int64_t)s.tokens * s.rep / kScoreRows + s.table.B;
+    // (a thread has up to eight pages of a block on its way; fewer where there are not enough blocks for the chip)
+    auto chunks = [&]() { return (s.blocks - 1) / (kScoreSums >> p.split_log2) + 1; };
+    p.split_log2 = 0;
+    while (p.split_log2 < kScoreSumsLog2 &&
+           (s.each > 8 << p.split_log2 || (s.each > 1 << p.split_log2 && units * s.Hkv * chunks() < 512)))
+      ++p.split_log2;
+    const int64_t want = 4096 / (units * s.Hkv);
+    const int z = (int)(want < 1 ? 1 : want < chunks() ? want : chunks());
     hipLaunchKernelGGL((paged_score_kernel<E, D>), dim3((unsigned)units, s.Hkv, z), dim3(256), 0, st, p);
     const int64_t rows = (int64_t)s.tokens * s.H;
     const PickParams pick = {s, p.scores, out};
@@ -375,14 +420,18 @@ extern "C" int moba_paged_key_sums(const void* k_pages, const float* k_scales, f
   const int page_log2 = page_log2_of(page_size);
   if ((D != 64 && D != 128) || page_log2 < 0 || (dtype != MOBA_DTYPE_BF16 && dtype != MOBA_DTYPE_F16)) return MOBA_ERR_UNSUPPORTED;
   if (((uintptr_t)k_pages & 15) || ((uintptr_t)sums & 3)) return MOBA_ERR_ARG;
-  const int64_t items = ((T >> page_log2) + 2 * (int64_t)B) * Hkv;
-  if (T >= 1LL << 30 || num_pages >= 1LL << 31 || max_pages >= 1LL << 31 || items >= 1LL << 25) return MOBA_ERR_LIMIT;   // (2^32 threads)
+  const int64_t units = (T >> page_log2) + 2 * (int64_t)B;   // (sequence b's pages are numbered from (its first row / page_size) + 2b on)
+  const int heads = Hkv > 1 && units * Hkv >= 8192 ? 2 : 1;
+  const int64_t items = units * ((Hkv + heads - 1) / heads);
+  if (units * Hkv >= 1LL << 31 || T >= 1LL << 30 || num_pages >= 1LL << 31 || max_pages >= 1LL << 31 || items >= 1LL << 25) return MOBA_ERR_LIMIT;   // (2^32 threads)
   LaunchCheck launch_check;
   auto launch = [&](auto e, auto d, auto c8) {
     typedef decltype(e) E;
     const SumParams<E> p = {table_of(page_table, lengths, cu_new, table_stride, T, B, num_pages, max_pages, page_log2), (const char*)k_pages,
                             k_scales, sums, Hkv, (int)items};
-    hipLaunchKernelGGL((paged_key_sums_kernel<E, d, c8>), dim3((unsigned)((items + 3) / 4)), dim3(256), 0, (hipStream_t)stream, p);
+    const dim3 grid((unsigned)((items + 3) / 4));
+    if (heads == 2) hipLaunchKernelGGL((paged_key_sums_kernel<E, d, c8, 2>), grid, dim3(256), 0, (hipStream_t)stream, p);
+    else hipLaunchKernelGGL((paged_key_sums_kernel<E, d, c8, 1>), grid, dim3(256), 0, (hipStream_t)stream, p);
   };
   constexpr std::integral_constant<int, 64> d64;
   constexpr std::integral_constant<int, 128> d128;
