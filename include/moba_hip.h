@@ -440,7 +440,8 @@ int moba_paged_attention(const void* q, void* out, const void* k_pages, const vo
  *   cu_groups [G+1] int32: group g is sequences cu_groups[g] .. cu_groups[g+1]-1 (those outside of all groups share nothing);
  *   shared [G] int32: leading tokens for which the table rows of a group's sequences name the same pages (the first one's are read;
  *   rounded down to a multiple of 64).  Read on the device.
- *   The rest as for moba_paged_attention; fewer than 2^32 threads to a launch: about twice as many as there. */
+ *   The rest as for moba_paged_attention; fewer than 2^32 threads to a launch: about twice as many as there.  Precision: that of few
+ *   rows up to 256 of a group or sequence (128 with 16-bit pages and D = 128). */
 size_t moba_paged_prefix_attention_workspace_bytes(int64_t T, int B, int G, int H, int Hkv, int D, int cache8);
 int moba_paged_prefix_attention(const void* q, void* out, const void* k_pages, const void* v_pages, const float* k_scales,
                                 const float* v_scales, const int32_t* page_table, const int32_t* lengths, const int32_t* cu_new,

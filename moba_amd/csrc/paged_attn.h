@@ -191,6 +191,8 @@ __device__ __forceinline__ void in_two(float a, float b, uint32_t& hi, uint32_t&
   lo = pack2<V>(a - (float)h[0], b - (float)h[1]);
 }
 
+template <class Table>
+constexpr int few_sets(int D) { return kShares<Table> && D == 64 ? 2 : 1; }
 template <int D, bool k8>
 constexpr int few_stage_bytes() { return 2 * kFewKeys * D * (k8 ? 1 : 2); }  // K and V of a step
 template <int D, bool k8>
@@ -206,8 +208,10 @@ __device__ __forceinline__ int least_position(const PageTable& t, const Unit& u,
 // the last key that new tokens up to j of a unit's rows see
 __device__ __forceinline__ int last_seen(const PageTable& t, const Unit& u, int j) { return position_at(t, u, j); }
 
-template <class E, int D, bool k8, class Table>
-__global__ __launch_bounds__(64 * kFewWaves, 2) void paged_few_kernel(const PagedParams<E, Table> p) {
+// kSets: sets of 32 rows to a workgroup, which read, and for 8-bit pages convert, K and V once for all of them
+template <class E, int D, bool k8, class Table, int kSets>
+__global__ __launch_bounds__(64 * kFewWaves, kSets > 1 && D == 128 ? 1 : 2) void paged_few_kernel(const PagedParams<E, Table> p) {
+  static_assert(kSets == 1 || !kChooses<Table>);
   MOBA_ELEM_TYPES(E)
   using V = std::conditional_t<k8, Bf16, E>;       // type of the second product
   typedef typename V::elem velem;
@@ -234,16 +238,23 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void paged_few_kernel(const Page
   if (unit.run == 0 && unit.group * !kChooses<Table> == 0 && hkv * !kChooses<Table> == 0 && tid == 0)
     p.runs[item] = {unit.first, unit.runs, unit.groups};
   const int b = table_row(table, unit.b);
-  const int count = seq.hi - seq.lo, rows = count * shape.rep, row0 = unit.group * kFewRows;
+  const int count = seq.hi - seq.lo, rows = count * shape.rep, row0 = unit.group * kFewRows * kSets;
   const int per = (unit.tiles + unit.runs - 1) / unit.runs;   // tiles of a run
   const int key_lo = __builtin_amdgcn_readfirstlane((int)min(seq.begin + (int64_t)unit.run * per * kFewTile, (int64_t)keys));
   const int key_hi = __builtin_amdgcn_readfirstlane((int)min(seq.begin + (int64_t)(unit.run + 1) * per * kFewTile, (int64_t)keys));
-  const int row = min(row0 + n, rows - 1);   // (rows past the last repeat it and are not written)
-  const int j = row / shape.rep, g = row - j * shape.rep;
-  const int position = position_at(table, unit, j);
-  const int limit = kChooses<Table> ? position : min(position, key_hi - 1);   // the row's last visible key (in this run)
-  int first_masked = least_position(table, unit, row0 / shape.rep, position);  // keys up to here: visible to every row
-  if constexpr (!kChooses<Table>) first_masked = min(first_masked, key_hi - 1);
+  const bool more = kSets > 1 && rows - row0 > kFewRows;   // than one set
+  int j[kSets], g[kSets];
+  int limit[kSets], first_masked[kSets];   // a row's last visible key (in this run); keys up to here are visible to every row of a set
+#pragma unroll
+  for (int q = 0; q < kSets; ++q) {
+    const int first = min(row0 + q * kFewRows, rows - 1), row = min(first + n, rows - 1);   // (rows past the last repeat it and are not written)
+    j[q] = row / shape.rep;
+    g[q] = row - j[q] * shape.rep;
+    const int position = position_at(table, unit, j[q]);
+    limit[q] = kChooses<Table> ? position : min(position, key_hi - 1);
+    first_masked[q] = least_position(table, unit, first / shape.rep, position);
+    if constexpr (!kChooses<Table>) first_masked[q] = min(first_masked[q], key_hi - 1);
+  }
   const int own_lo = key_lo + wave * kFewKeys;                         // the wave's first key
   const int mine = __builtin_amdgcn_readfirstlane(key_hi > own_lo ? (key_hi - own_lo - 1) / kFewTile + 1 : 0);
 
@@ -297,21 +308,22 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void paged_few_kernel(const Page
         const char* from = p.pages[half] + head_bytes + (id < 0 ? 0 : id * page_bytes + in_page * kRowBytes);
 #pragma unroll
         for (int i = 0; i < kSlotCopies; ++i)
-          async_copy16_sv<true>(from, ld_off[i], to + half * kBlockBytes + (slot * kSlotCopies + i) * 1024);
+          async_copy16_sv<!kShares<Table>>(from, ld_off[i], to + half * kBlockBytes + (slot * kSlotCopies + i) * 1024);
       }
   };
 
   // Q^T operands: of step s8, lane (n, hh) holds the 8 elements of row n that its 8 elements of a key meet
-  elem8 bq[kSteps];
-  {
-    const elem* src = p.q + (int64_t)(seq.lo + j) * p.q_tok_stride + (int64_t)(hkv * shape.rep + g) * p.q_head_stride;
+  elem8 bq[kSets][kSteps];
+#pragma unroll
+  for (int q = 0; q < kSets; ++q) {
+    const elem* src = p.q + (int64_t)(seq.lo + j[q]) * p.q_tok_stride + (int64_t)(hkv * shape.rep + g[q]) * p.q_head_stride;
 #pragma unroll
     for (int s8 = 0; s8 < kSteps; ++s8)
-      bq[s8] = *reinterpret_cast<const elem8*>(src + (k8 ? 32 * (s8 >> 1) + 16 * hh + 8 * (s8 & 1) : 16 * s8 + 8 * hh));
+      bq[q][s8] = *reinterpret_cast<const elem8*>(src + (k8 ? 32 * (s8 >> 1) + 16 * hh + 8 * (s8 & 1) : 16 * s8 + 8 * hh));
     // a negative softmax scale: the queries' signs turn, so that the largest product has the largest score
     if (p.scale_log2 < 0.f) {
 #pragma unroll
-      for (int s8 = 0; s8 < kSteps; ++s8) bq[s8] = -bq[s8];
+      for (int s8 = 0; s8 < kSteps; ++s8) bq[q][s8] = -bq[q][s8];
     }
   }
   const float scale = fabsf(p.scale_log2);
@@ -341,17 +353,23 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void paged_few_kernel(const Page
     }
   }
 
-  f32x16 oacc[kDb];
+  f32x16 oacc[kSets][kDb];
+  float m_run[kSets], l_run[kSets];
 #pragma unroll
-  for (int db = 0; db < kDb; ++db)
+  for (int q = 0; q < kSets; ++q) {
+    m_run[q] = kNoMax;
+    l_run[q] = 0.f;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) oacc[db][e] = 0.f;
-  float m_run = kNoMax, l_run = 0.f;
+    for (int db = 0; db < kDb; ++db)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) oacc[q][db][e] = 0.f;
+  }
   uint64_t there = 0;   // the slots of the batch that have a page
   const uint32_t everybody = rows - row0 >= 32 ? ~0u : (1u << (rows - row0)) - 1;
 
-  auto step = [&](int it, auto stage) __attribute__((always_inline)) {
+  auto step = [&](int it, auto stage, auto sets) __attribute__((always_inline)) {
     constexpr uint32_t st = stage * kStage;
+    constexpr int kHere = sets;
     // (the ids at hand are this batch's: the next batch's are fetched behind its last step but one)
     if (it % kBatch == 0) {
       there = __ballot(ids >= 0);
@@ -361,24 +379,31 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void paged_few_kernel(const Page
     // this block's copies have landed (the next block's may still be in flight)
     if (it + 1 < mine) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * kCopies) : "memory");
     else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    f32x16 s;
+    f32x16 s[kHere];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) s[e] = 0.f;
+    for (int q = 0; q < kHere; ++q)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[q][e] = 0.f;
     if constexpr (k8) {
       u32x4 raw[kKReads];
 #pragma unroll
       for (int i = 0; i < kKReads; ++i) raw[i] = *lds_ptr<const u32x4>(koff[i] + st);
 #pragma unroll
-      for (int i = 0; i < kKReads; ++i) {
-        s = mfma32(widened(raw[i][0], raw[i][1], E{}), bq[2 * i], s);
-        s = mfma32(widened(raw[i][2], raw[i][3], E{}), bq[2 * i + 1], s);
-      }
+      for (int i = 0; i < kKReads; ++i)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const elem8 ka = widened(raw[i][2 * half], raw[i][2 * half + 1], E{});
+#pragma unroll
+          for (int q = 0; q < kHere; ++q) s[q] = mfma32(ka, bq[q][2 * i + half], s[q]);
+        }
     } else {
       elem8 ka[kKReads];
 #pragma unroll
       for (int i = 0; i < kKReads; ++i) ka[i] = *lds_ptr<const elem8>(koff[i] + st);
 #pragma unroll
-      for (int i = 0; i < kKReads; ++i) s = mfma32(ka[i], bq[i], s);
+      for (int i = 0; i < kKReads; ++i)
+#pragma unroll
+        for (int q = 0; q < kHere; ++q) s[q] = mfma32(ka[i], bq[q][i], s[q]);
     }
     // the V^T fragments travel while the softmax runs
     velem8 va[2][kDb];
@@ -399,50 +424,57 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void paged_few_kernel(const Page
       }
     const int key0 = own_lo + it * kFewTile;
     // factors of the two slots' scores (not negative: see bq) and probabilities
-    float f[2] = {scale, scale}, vs[2] = {1.f, 1.f};
+    float f[kHere][2], vs[2] = {1.f, 1.f};
+#pragma unroll
+    for (int q = 0; q < kHere; ++q) f[q][0] = f[q][1] = scale;
     if constexpr (k8) {
       const uint32_t at = scale_base + ((it / kBatch) & 1) * (kScaleBytes / 2) + (it % kBatch) * 8;
       const f32x2 k2 = *lds_ptr<const f32x2>(at), v2 = *lds_ptr<const f32x2>(at + 256);
-      f[0] *= k2[0];
-      f[1] *= k2[1];
+#pragma unroll
+      for (int q = 0; q < kHere; ++q) {
+        f[q][0] *= k2[0];
+        f[q][1] *= k2[1];
+      }
       vs[0] = v2[0];
       vs[1] = v2[1];
     }
     const uint32_t has = (uint32_t)(there >> (2 * (it % kBatch))) & 3;
-    bool partly;   // whether somebody does not see all of the block
+    bool unseen;   // whether there are keys that nobody sees
     if constexpr (kChooses<Table>) {
-      bool whole[2];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const int slot = (it % kBatch) * 2 + half, first = __builtin_amdgcn_readlane(place_now, slot);
         const uint32_t who = (uint32_t)__builtin_amdgcn_readlane((int)chosen_now, slot);
-        whole[half] = (has >> half & 1) && (who & everybody) == everybody && first + kSlot - 1 <= first_masked;
-        if (!whole[half]) {
+        if (!(has >> half & 1) || (who & everybody) != everybody || first + kSlot - 1 > first_masked[0]) {
           asm volatile("");   // (a branch)
           const bool mine = (has >> half & 1) && (who >> n & 1);
 #pragma unroll
           for (int e = 8 * half; e < 8 * half + 8; ++e) {
-            s[e] *= f[half];
-            if (!mine || first + 8 * ((e >> 2) & 1) + 4 * hh + (e & 3) > limit) s[e] = -INFINITY;
+            s[0][e] *= f[0][half];
+            if (!mine || first + 8 * ((e >> 2) & 1) + 4 * hh + (e & 3) > limit[0]) s[0][e] = -INFINITY;
           }
-          f[half] = 1.f;
+          f[0][half] = 1.f;
         }
       }
-      partly = key0 + kFewKeys > key_hi || has != 3;
+      unseen = key0 + kFewKeys > key_hi || has != 3;
     } else {
-      partly = key0 + kFewKeys - 1 > first_masked || has != 3;
-    }
-    if (__builtin_expect(partly, 0)) {
-      asm volatile("");   // (a branch, not sixteen comparisons in every block)
-      if constexpr (!kChooses<Table>) {
+      unseen = false;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          s[e] *= f[e >> 3];
-          if (key0 + 8 * (e >> 2) + 4 * hh + (e & 3) > limit || !(has & (1 << (e >> 3)))) s[e] = -INFINITY;
+      for (int q = 0; q < kHere; ++q)
+        if (__builtin_expect(key0 + kFewKeys - 1 > first_masked[q] || has != 3, 0)) {
+          asm volatile("");   // (a branch, not sixteen comparisons in every block)
+          unseen = true;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            s[q][e] *= f[q][e >> 3];
+            if (key0 + 8 * (e >> 2) + 4 * hh + (e & 3) > limit[q] || !(has & (1 << (e >> 3)))) s[q][e] = -INFINITY;
+          }
+          f[q][0] = f[q][1] = 1.f;
         }
-        f[0] = f[1] = 1.f;
-      }
-      // values of keys that nobody sees: whatever lies there
+    }
+    if (__builtin_expect(unseen, 0)) {
+      asm volatile("");
+      // their values: whatever lies there
 #pragma unroll
       for (int j2 = 0; j2 < 2; ++j2)
 #pragma unroll
@@ -455,39 +487,42 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void paged_few_kernel(const Page
             }
           }
     }
-    float mx[2];
+    u32x4 hi[kHere][2], lo[kHere][2];
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      mx[half] = s[8 * half];
+    for (int q = 0; q < kHere; ++q) {
+      float mx[2];
 #pragma unroll
-      for (int e = 1; e < 8; ++e) mx[half] = fmaxf(mx[half], s[8 * half + e]);
-    }
-    mx[0] = max_xhalf(fmaxf(mx[0] * f[0], mx[1] * f[1]));
-    if (__any(mx[0] > m_run + kMaxLag)) {  // rare once the maximum has settled
-      const float m_new = mx[0] > m_run + kMaxLag ? mx[0] : m_run;
-      const float alpha = fast_exp2(m_run - m_new);
-      m_run = m_new;
-      l_run *= alpha;
+      for (int half = 0; half < 2; ++half) {
+        mx[half] = s[q][8 * half];
 #pragma unroll
-      for (int db = 0; db < kDb; ++db)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) oacc[db][e] *= alpha;
-    }
-    const float ref = m_run - ProbShift<V>::value;
-    u32x4 hi[2], lo[2];
-#pragma unroll
-    for (int e = 0; e < 16; e += 2) {
-      float p0 = fast_exp2(fmaf(s[e], f[e >> 3], -ref)), p1 = fast_exp2(fmaf(s[e + 1], f[e >> 3], -ref));
-      l_run += p0;
-      l_run += p1;
-      if constexpr (k8) {
-        p0 *= vs[e >> 3];
-        p1 *= vs[e >> 3];
+        for (int e = 1; e < 8; ++e) mx[half] = fmaxf(mx[half], s[q][8 * half + e]);
       }
-      uint32_t h, l;
-      in_two<V>(p0, p1, h, l);
-      hi[e >> 3][(e & 7) >> 1] = h;
-      lo[e >> 3][(e & 7) >> 1] = l;
+      mx[0] = max_xhalf(fmaxf(mx[0] * f[q][0], mx[1] * f[q][1]));
+      if (__any(mx[0] > m_run[q] + kMaxLag)) {  // rare once the maximum has settled
+        const float m_new = mx[0] > m_run[q] + kMaxLag ? mx[0] : m_run[q];
+        const float alpha = fast_exp2(m_run[q] - m_new);
+        m_run[q] = m_new;
+        l_run[q] *= alpha;
+#pragma unroll
+        for (int db = 0; db < kDb; ++db)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) oacc[q][db][e] *= alpha;
+      }
+      const float ref = m_run[q] - ProbShift<V>::value;
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) {
+        float p0 = fast_exp2(fmaf(s[q][e], f[q][e >> 3], -ref)), p1 = fast_exp2(fmaf(s[q][e + 1], f[q][e >> 3], -ref));
+        l_run[q] += p0;
+        l_run[q] += p1;
+        if constexpr (k8) {
+          p0 *= vs[e >> 3];
+          p1 *= vs[e >> 3];
+        }
+        uint32_t h, l;
+        in_two<V>(p0, p1, h, l);
+        hi[q][e >> 3][(e & 7) >> 1] = h;
+        lo[q][e >> 3][(e & 7) >> 1] = l;
+      }
     }
     if constexpr (k8) {
 #pragma unroll
@@ -496,80 +531,98 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void paged_few_kernel(const Page
         for (int db = 0; db < kDb; ++db) va[j2][db] = widened(vraw[j2][db][0], vraw[j2][db][1], Bf16{});
     }
 #pragma unroll
-    for (int j2 = 0; j2 < 2; ++j2)
+    for (int q = 0; q < kHere; ++q) {
 #pragma unroll
-      for (int db = 0; db < kDb; ++db) oacc[db] = mfma32(va[j2][db], __builtin_bit_cast(velem8, hi[j2]), oacc[db]);
+      for (int j2 = 0; j2 < 2; ++j2)
 #pragma unroll
-    for (int j2 = 0; j2 < 2; ++j2)
+        for (int db = 0; db < kDb; ++db) oacc[q][db] = mfma32(va[j2][db], __builtin_bit_cast(velem8, hi[q][j2]), oacc[q][db]);
 #pragma unroll
-      for (int db = 0; db < kDb; ++db) oacc[db] = mfma32(va[j2][db], __builtin_bit_cast(velem8, lo[j2]), oacc[db]);
+      for (int j2 = 0; j2 < 2; ++j2)
+#pragma unroll
+        for (int db = 0; db < kDb; ++db) oacc[q][db] = mfma32(va[j2][db], __builtin_bit_cast(velem8, lo[q][j2]), oacc[q][db]);
+    }
     if (it + 2 < mine) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // every fragment of this stage is in registers
       issue(it + 2);
     }
   };
   // (the stage is a constant of each copy of the body, and part of its LDS instructions)
-  for (int it = 0; it < mine; it += 2) {
-    step(it, std::integral_constant<int, 0>{});
-    if (it + 1 < mine) step(it + 1, std::integral_constant<int, 1>{});
+  auto all_steps = [&](auto sets) __attribute__((always_inline)) {
+    for (int it = 0; it < mine; it += 2) {
+      step(it, std::integral_constant<int, 0>{}, sets);
+      if (it + 1 < mine) step(it + 1, std::integral_constant<int, 1>{}, sets);
+    }
+  };
+  if constexpr (kSets > 1) {
+    if (more) all_steps(std::integral_constant<int, kSets>{});
+    else all_steps(std::integral_constant<int, 1>{});
+  } else {
+    all_steps(std::integral_constant<int, 1>{});
   }
-  if (__builtin_expect(__any(any_not_finite(oacc)), 0))  // (never for values of ordinary size)
-    one_by_one<E, V, D, k8, k8>(p, hkv, own_lo, kFewTile, key_hi, [&](int key, bool& sees) __attribute__((always_inline)) {
-      if constexpr (kChooses<Table>) {
-        uint32_t who;
-        const int page = chosen_page(table, item, key, who);
-        sees = (who >> n & 1) && ((int64_t)page << table.page_log2) + (key & page_mask) <= limit;
-        return page_id(table, b, page);
-      } else {
-        sees = key <= limit;
-        return page_id(table, b, key >> table.page_log2);
-      }
-    }, scale, bq, oacc, m_run, l_run);
-  l_run = sum_xhalf(l_run);
+#pragma unroll
+  for (int q = 0; q < kSets; ++q) {
+    if (__builtin_expect(__any(any_not_finite(oacc[q])), 0))  // (never for values of ordinary size)
+      one_by_one<E, V, D, k8, k8>(p, hkv, own_lo, kFewTile, key_hi, [&](int key, bool& sees) __attribute__((always_inline)) {
+        if constexpr (kChooses<Table>) {
+          uint32_t who;
+          const int page = chosen_page(table, item, key, who);
+          sees = (who >> n & 1) && ((int64_t)page << table.page_log2) + (key & page_mask) <= limit[q];
+          return page_id(table, b, page);
+        } else {
+          sees = key <= limit[q];
+          return page_id(table, b, key >> table.page_log2);
+        }
+      }, scale, bq[q], oacc[q], m_run[q], l_run[q]);
+    l_run[q] = sum_xhalf(l_run[q]);
+  }
 
   // ---- the waves meet in LDS.  Element e of lane (n, hh) is O[row n][32*db + 8*(e/4) + 4*hh + e%4].
-  __syncthreads();  // every wave has read its last fragments
   float* red = reinterpret_cast<float*>(smem);
   float* red_m = red + kFewWaves * 32 * kRedRow;
   float* red_l = red_m + kFewWaves * 32;
-  const int rows_here = min(kFewRows, rows - row0);
-  if (n < rows_here) {
 #pragma unroll
-    for (int db = 0; db < kDb; ++db)
+  for (int q = 0; q < kSets; ++q) {
+    const int first = row0 + q * kFewRows, rows_here = min(kFewRows, rows - first);
+    if (q && rows_here <= 0) break;
+    __syncthreads();  // every wave has read its last fragments, or the former set's rows
+    if (n < rows_here) {
 #pragma unroll
-      for (int g4 = 0; g4 < 4; ++g4)
-        *reinterpret_cast<f32x4*>(red + (wave * 32 + n) * kRedRow + 32 * db + 8 * g4 + 4 * hh) =
-            f32x4{oacc[db][4 * g4], oacc[db][4 * g4 + 1], oacc[db][4 * g4 + 2], oacc[db][4 * g4 + 3]};
-    if (hh == 0) {
-      red_m[wave * 32 + n] = m_run;
-      red_l[wave * 32 + n] = l_run;
+      for (int db = 0; db < kDb; ++db)
+#pragma unroll
+        for (int g4 = 0; g4 < 4; ++g4)
+          *reinterpret_cast<f32x4*>(red + (wave * 32 + n) * kRedRow + 32 * db + 8 * g4 + 4 * hh) =
+              f32x4{oacc[q][db][4 * g4], oacc[q][db][4 * g4 + 1], oacc[q][db][4 * g4 + 2], oacc[q][db][4 * g4 + 3]};
+      if (hh == 0) {
+        red_m[wave * 32 + n] = m_run[q];
+        red_l[wave * 32 + n] = l_run[q];
+      }
     }
-  }
-  __syncthreads();
-  for (int i = tid; i < rows_here * (D / 4); i += 64 * kFewWaves) {
-    const int rr = i / (D / 4), d = (i % (D / 4)) * 4;
-    float mm = red_m[rr];
+    __syncthreads();
+    for (int i = tid; i < rows_here * (D / 4); i += 64 * kFewWaves) {
+      const int rr = i / (D / 4), d = (i % (D / 4)) * 4;
+      float mm = red_m[rr];
 #pragma unroll
-    for (int w = 1; w < kFewWaves; ++w) mm = fmaxf(mm, red_m[w * 32 + rr]);
-    float ll = 0.f;
-    f32x4 oo = {0.f, 0.f, 0.f, 0.f};
+      for (int w = 1; w < kFewWaves; ++w) mm = fmaxf(mm, red_m[w * 32 + rr]);
+      float ll = 0.f;
+      f32x4 oo = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < kFewWaves; ++w) {
-      const float a = fast_exp2(red_m[w * 32 + rr] - mm);
-      ll += red_l[w * 32 + rr] * a;
-      const f32x4 x = *reinterpret_cast<const f32x4*>(red + (w * 32 + rr) * kRedRow + d);
+      for (int w = 0; w < kFewWaves; ++w) {
+        const float a = fast_exp2(red_m[w * 32 + rr] - mm);
+        ll += red_l[w * 32 + rr] * a;
+        const f32x4 x = *reinterpret_cast<const f32x4*>(red + (w * 32 + rr) * kRedRow + d);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) oo[e] += x[e] * a;
-    }
-    const float inv = ll == 0.f ? 0.f : 1.f / ll;   // (a row may see no key of its run, or none at all)
-    if (!kShares<Table> && unit.runs == 1) {
-      const int jj = (row0 + rr) / shape.rep, gg = row0 + rr - jj * shape.rep;
-      const int64_t orow = (int64_t)(seq.lo + jj) * shape.H + hkv * shape.rep + gg;
-      *reinterpret_cast<u32x2*>(p.out + orow * D + d) = u32x2{pack2<E>(oo[0] * inv, oo[1] * inv), pack2<E>(oo[2] * inv, oo[3] * inv)};
-    } else {
-      const int64_t prow = (int64_t)blockIdx.x * kFewRows + rr;
-      *reinterpret_cast<f32x4*>(p.few_o + prow * D + d) = f32x4{oo[0] * inv, oo[1] * inv, oo[2] * inv, oo[3] * inv};
-      if (d == 0) p.few_lse[prow] = ll == 0.f ? -INFINITY : mm - ProbShift<V>::value + fast_log2(ll);
+        for (int e = 0; e < 4; ++e) oo[e] += x[e] * a;
+      }
+      const float inv = ll == 0.f ? 0.f : 1.f / ll;   // (a row may see no key of its run, or none at all)
+      if (!kShares<Table> && unit.runs == 1) {
+        const int jj = (first + rr) / shape.rep, gg = first + rr - jj * shape.rep;
+        const int64_t orow = (int64_t)(seq.lo + jj) * shape.H + hkv * shape.rep + gg;
+        *reinterpret_cast<u32x2*>(p.out + orow * D + d) = u32x2{pack2<E>(oo[0] * inv, oo[1] * inv), pack2<E>(oo[2] * inv, oo[3] * inv)};
+      } else {
+        const int64_t prow = ((int64_t)blockIdx.x * kSets + q) * kFewRows + rr;
+        *reinterpret_cast<f32x4*>(p.few_o + prow * D + d) = f32x4{oo[0] * inv, oo[1] * inv, oo[2] * inv, oo[3] * inv};
+        if (d == 0) p.few_lse[prow] = ll == 0.f ? -INFINITY : mm - ProbShift<V>::value + fast_log2(ll);
+      }
     }
   }
 }
@@ -1099,15 +1152,19 @@ struct MergeToken {
     for (int s = 0; s < kSides; ++s) {
       r[s] = {0, 0, 0};
       is_many[s] = side[s].count * p.shape.rep > p.many.rows_over && p.many.most > 0;
-      if (side[s].keys) r[s] = p.runs[side[s].unit];   // (its units have left their numbers)
+      if (side[s].keys) {   // (its units have left their numbers)
+        const Runs x = p.runs[side[s].unit];
+        r[s] = {__builtin_amdgcn_readfirstlane(x.first), __builtin_amdgcn_readfirstlane(x.runs), __builtin_amdgcn_readfirstlane(x.groups)};
+      }
     }
   }
   __device__ __forceinline__ bool done() const { return kSides == 1 && r[0].runs == 1; }   // (the only run's unit has written the rows)
-  __device__ __forceinline__ Parts parts(const PagedParams<E, Table>& p, int h, int s) const {
+  // of query head g of key/value head hkv (group_rows is a power of two)
+  __device__ __forceinline__ Parts parts(const PagedParams<E, Table>& p, int hkv, int g, int s) const {
     const Cut& cut = is_many[s] ? p.many : p.few;
-    const int hkv = h / p.shape.rep, row = side[s].token * p.shape.rep + h - hkv * p.shape.rep;
-    int group = row / cut.group_rows;
-    const int rr = row - group * cut.group_rows;
+    const int row = side[s].token * p.shape.rep + g;
+    int group = row >> (31 - __builtin_clz(cut.group_rows));
+    const int rr = row & (cut.group_rows - 1);
     if (is_many[s]) group = r[s].groups - 1 - group;
     // (numbers that no unit has left, where the row ranges are none)
     const bool none = r[s].first < 0 || r[s].runs < 0 || r[s].groups < 1 || r[s].first + (int64_t)r[s].runs * r[s].groups > cut.parts ||
@@ -1139,51 +1196,53 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams<E, T
     // Rows and log-sum-exps of some runs are asked for together, a wave's share of the rows and, lane by lane, all of
     // the others; more runs come as many at a time, with a running maximum.
     float top = kNoMax, ll = 0.f, o[kPer] = {};
-    bool written = false;
+    const int hkv = h / shape.rep;
+    Parts parts[kSides];
 #pragma unroll
-    for (int s = 0; s < kSides; ++s) {
-      const Parts parts = token.parts(p, h, s);
-      if (kChooses<Table> && parts.runs == 1) {   // (is there already)
-        written = true;
-        break;
+    for (int s = 0; s < kSides; ++s) parts[s] = token.parts(p, hkv, h - hkv * shape.rep, s);
+    if (kChooses<Table> && parts[0].runs == 1) continue;   // (is there already)
+    // (the sides' runs one after the other)
+    const int runs = parts[0].runs + (kSides > 1 ? parts[kSides - 1].runs : 0);
+    auto row_of = [&](int i, const float*& lse) {
+      const Parts& side = kSides > 1 && i >= parts[0].runs ? parts[kSides - 1] : parts[0];
+      const int64_t row = side.first + (i - (kSides > 1 && i >= parts[0].runs ? parts[0].runs : 0)) * side.step;
+      lse = side.lse + row;
+      return side.o + row * D;
+    };
+    auto some = [&](int i0, auto count) __attribute__((always_inline)) {   // runs i0 .., kShare * count of them
+      fvec x[count];
+      const float* at = nullptr;
+#pragma unroll
+      for (int k = 0; k < count; ++k) x[k] = *reinterpret_cast<const fvec*>(row_of(min(i0 + kShare * k + wave, runs - 1), at) + kPer * lane);
+      row_of(min(i0 + lane, runs - 1), at);
+      const float lse = i0 + lane < runs && lane < kShare * count ? *at : -INFINITY;
+      float mm = lse;
+#pragma unroll
+      for (int d = 32; d >= 1; d >>= 1) mm = fmaxf(mm, __shfl_xor(mm, d, 64));
+      mm = fmaxf(mm, top);
+      const float w = fast_exp2(lse - mm), former = fast_exp2(top - mm);
+      top = mm;
+      ll *= former;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) o[e] *= former;
+#pragma unroll
+      for (int k = 0; k < count; ++k) {
+        const float wk = lane_value(w, kShare * k + wave);   // (0 behind the last, whose row is the last one's again)
+        ll += wk;
+        const bool there = i0 + kShare * k + wave < runs;   // (0 times an infinity is not 0)
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) o[e] += there ? wk * x[k][e] : 0.f;
       }
-      const int runs = parts.runs;
-      auto part = [&](int i) { return parts.first + i * parts.step; };
-      auto some = [&](int i0, auto count) __attribute__((always_inline)) {   // runs i0 .., kShare * count of them
-        fvec x[count];
-#pragma unroll
-        for (int k = 0; k < count; ++k)
-          x[k] = *reinterpret_cast<const fvec*>(parts.o + part(min(i0 + kShare * k + wave, runs - 1)) * D + kPer * lane);
-        const float lse = i0 + lane < runs && lane < kShare * count ? parts.lse[part(i0 + lane)] : -INFINITY;
-        float mm = lse;
-#pragma unroll
-        for (int d = 32; d >= 1; d >>= 1) mm = fmaxf(mm, __shfl_xor(mm, d, 64));
-        mm = fmaxf(mm, top);
-        const float w = fast_exp2(lse - mm), former = fast_exp2(top - mm);
-        top = mm;
-        ll *= former;
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) o[e] *= former;
-#pragma unroll
-        for (int k = 0; k < count; ++k) {
-          const float wk = lane_value(w, kShare * k + wave);   // (0 behind the last, whose row is the last one's again)
-          ll += wk;
-          const bool there = i0 + kShare * k + wave < runs;   // (0 times an infinity is not 0)
-#pragma unroll
-          for (int e = 0; e < kPer; ++e) o[e] += there ? wk * x[k][e] : 0.f;
-        }
-      };
-      if (runs > 0 && runs <= 4 * kShare) some(0, std::integral_constant<int, 4>{});
-      else if (kShare == 1 && runs > 0 && runs <= 8) some(0, std::integral_constant<int, 8>{});
-      else
-        for (int i0 = 0; i0 < runs; i0 += 16 * kShare) some(i0, std::integral_constant<int, 16>{});
-    }
-    if (written) continue;
+    };
+    if (runs > 0 && runs <= 4 * kShare) some(0, std::integral_constant<int, 4>{});
+    else if (kShare == 1 && runs > 0 && runs <= 8) some(0, std::integral_constant<int, 8>{});
+    else
+      for (int i0 = 0; i0 < runs; i0 += 16 * kShare) some(i0, std::integral_constant<int, 16>{});
     if constexpr (kShare == 1) {
       const float inv = ll == 0.f ? 0.f : 1.f / ll;
       elem* const to = p.out + ((int64_t)t * shape.H + h) * D + kPer * lane;
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) to[e] = (elem)(o[e] * inv);
+      if constexpr (kPer == 2) *reinterpret_cast<uint32_t*>(to) = pack2<E>(o[0] * inv, o[1] * inv);
+      else to[0] = (elem)(o[0] * inv);
     } else {
 #pragma unroll
       for (int e = 0; e < kPer; ++e) red[wave][kPer * lane + e] = o[e];
@@ -1222,25 +1281,19 @@ static Cut bounded_cut(Cut c, int64_t T, int B, int rep) {
 struct Cuts {
   Cut few, many;
 };
-static Cuts paged_cuts(int64_t T, int B, int rep, int Hkv, int D, bool cache8, int max_new) {
+// T: rows of the batch, counted as often as they are attended; few_per_cu: workgroups of few rows
+static Cuts paged_cuts(int64_t T, int sequences, int rep, int Hkv, int D, bool cache8, bool many, int group_rows, int few_rows, int few_per_cu) {
   const int cus = compute_units() > 0 ? compute_units() : 256;
   auto target = [&](int per_cu) { return per_cu * cus / Hkv > 0 ? per_cu * cus / Hkv : 1; };
-  const int64_t most_new = max_new >= 0 && max_new < T ? max_new : T;
   Cuts c;
-  // 8-bit pages: up to 64 rows are few, in two groups of which the second finds the keys in L2.  16 sequences of 64 rows against 8192
-  // keys, 8 heads: 100 us, as many rows 112; 64 of 40 against 2048: 86 and 101; one of 64 against 131072, one head: 30 and 32.  128
-  // rows would be faster for 8 heads (one sequence, 4096 keys: 21 and 27) and slower for one (16 sequences, 8192 keys: 42 and 33).
-  // 16-bit pages are twice the bytes: up to 32 rows (16 of 64 rows, one head: 30 us as many rows, 35 as few; 64 of 40: 110 and 135).
-  const int few_rows = cache8 ? 2 * kFewRows : kFewRows;
-  const bool many = most_new * rep > few_rows;
   // (runs of at least two tiles: one token against 4096 keys, with the merge 13.5 us with runs of one, 12.3 of two, 13.4 of three)
-  c.few = bounded_cut({kFewRows, kFewTile, 2, 0, many ? few_rows : 0x7fffffff, target(D == 128 && !cache8 ? 1 : 2), 0, 0}, T, B, rep);
+  c.few = bounded_cut({group_rows, kFewTile, 2, 0, many ? few_rows : 0x7fffffff, target(few_per_cu), 0, 0, false}, T, sequences, rep);
   c.many = {};
   if (many) {
     const int waves = D == 128 && cache8 ? kManyWaves<128, true> : kManyWaves<64, false>;
     // (695 tokens and 204 against 883 and 151, 5 heads on one: 30.0 us with runs of any length, 24.4 with at least four tiles, 24.6 with
     // six; 609 tokens of 8 heads: 27.5, 21, 21)
-    c.many = bounded_cut({32 * waves, kManyKeys, 4, few_rows, 0x7fffffff, target(8 / waves), 0, 0}, T, B, rep);
+    c.many = bounded_cut({32 * waves, kManyKeys, 4, few_rows, 0x7fffffff, target(8 / waves), 0, 0, false}, T, sequences, rep);
   }
   return c;
 }
@@ -1317,7 +1370,7 @@ template <class E, int D, bool k8, class Table>
 static int launch_paged(const PagedParams<E, Table>& p, hipStream_t st) {
   LaunchCheck launch_check;
   static bool allowed[2][kMaxDevices];
-  const auto few = paged_few_kernel<E, D, k8, Table>;
+  const auto few = paged_few_kernel<E, D, k8, Table, few_sets<Table>(D)>;
   if (!allow_dynamic_lds((const void*)few, few_lds_bytes<D, k8>(), allowed[0])) return MOBA_ERR_LAUNCH;
   hipLaunchKernelGGL(few, dim3((unsigned)p.few.most * p.shape.Hkv), dim3(64 * kFewWaves), (few_lds_bytes<D, k8>()), st, p);
   if (p.many.most > 0) {

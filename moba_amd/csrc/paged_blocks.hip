@@ -92,10 +92,10 @@ struct MergeToken<E, ChosenTable> {
     token = t - seq.lo;
   }
   __device__ __forceinline__ bool done() const { return false; }
-  __device__ __forceinline__ Parts parts(const PagedParams<E, ChosenTable>& p, int h, int) const {
+  __device__ __forceinline__ Parts parts(const PagedParams<E, ChosenTable>& p, int hkv, int g, int) const {
     const Shape<ChosenTable>& shape = p.shape;
     Runs r = {0, 0, 0};
-    const int hkv = h / shape.rep, row = token * shape.rep + h - hkv * shape.rep, group = row / kChosenRows;
+    const int row = token * shape.rep + g, group = row / kChosenRows;
     if (b >= 0) {
       const int64_t item = (first_group(seq.lo, shape.rep, b) + group) * shape.Hkv + hkv;
       if (item < shape.table.items) r = p.runs[item];
@@ -120,7 +120,7 @@ static bool chosen_sizes(ChosenSizes& s, int64_t T, int B, int H, int Hkv, int D
   s.items = (int)items;
   s.room_of_list = (int)room;
   const int64_t most = items >= (int64_t)kWholeAt * target ? items : target / 2 + items > target ? target / 2 + items : target;
-  s.cut = {kChosenRows, kFewTile, 2, 0, 0x7fffffff, target, (int)most, items >= (int64_t)kWholeAt * target ? 0 : (int)most};
+  s.cut = {kChosenRows, kFewTile, 2, 0, 0x7fffffff, target, (int)most, items >= (int64_t)kWholeAt * target ? 0 : (int)most, false};
   auto lines = [](int64_t n) { return (n + 15) / 16 * 16; };
   s.lists_at = lines(items * (int64_t)sizeof(Runs));
   s.keys_at = s.lists_at + lines(items * room * (int64_t)sizeof(Chosen));
@@ -133,7 +133,7 @@ template <class E, int D, bool k8>
 static int launch_chosen(const PagedParams<E, ChosenTable>& p, const UnionParams& u, hipStream_t st) {
   LaunchCheck launch_check;
   static bool allowed[kMaxDevices];
-  const auto few = paged_few_kernel<E, D, k8, ChosenTable>;
+  const auto few = paged_few_kernel<E, D, k8, ChosenTable, 1>;
   if (!allow_dynamic_lds((const void*)few, few_lds_bytes<D, k8>(), allowed)) return MOBA_ERR_LAUNCH;
   hipLaunchKernelGGL(paged_union_kernel, dim3(p.shape.table.items / p.shape.Hkv, p.shape.Hkv), dim3(kUnionThreads), 0, st, u);
   hipLaunchKernelGGL(few, dim3((unsigned)p.few.most), dim3(64 * kFewWaves), (few_lds_bytes<D, k8>()), st, p);

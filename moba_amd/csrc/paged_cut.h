@@ -22,6 +22,7 @@ struct Cut {
   int target;      // units per key/value head that fill the chip
   int most;        // no more units per key/value head than this, whatever the batch
   int parts;       // no more than this of them where there is a sequence of several runs
+  bool even;       // runs by even_run()
 };
 constexpr int kWholeRun = 0x3fffffff;  // tiles
 // With this many times `target` groups and more, a sequence's keys are one run.  That is right for sequences of like lengths, and slow for one
@@ -81,6 +82,47 @@ __device__ __forceinline__ uint32_t wave_sum(uint32_t x) { return (uint32_t)__bu
 
 __device__ __forceinline__ int runs_of(int tiles, int run) { return (tiles - 1) / run + 1; }
 
+// the largest of the lanes' x, none of them negative
+__device__ __forceinline__ int wave_max(int x) {
+#define MOBA_DPP_MAX(ctrl, rows) x = max(x, __builtin_amdgcn_update_dpp(0, x, ctrl, rows, 0xf, false))
+  MOBA_DPP_MAX(0x111, 0xf);
+  MOBA_DPP_MAX(0x112, 0xf);
+  MOBA_DPP_MAX(0x114, 0xf);
+  MOBA_DPP_MAX(0x118, 0xf);
+  MOBA_DPP_MAX(0x142, 0xa);
+  MOBA_DPP_MAX(0x143, 0xc);
+#undef MOBA_DPP_MAX
+  return __builtin_amdgcn_readlane(x, 63);
+}
+
+// Tiles of a run where units are long and of many lengths: a small part of the longest sequence, each lane its own, such that the rounds of
+// the long units, and all units shared out evenly, take least; a unit's start counts as least_tiles.  (Up to 64 sequences; `otherwise` where
+// every choice is more units than are launched.)  700 and 500 tokens behind 12288 shared ones, 8 heads: 8 bits 317 us, 349 with the runs of
+// run_tiles(); 16 bits 314 and 380; 4 times 64 behind 30000 153 and 148.
+__device__ __forceinline__ int even_run(const Cut& c, int lane, const Share& first, int sequences, int64_t work, int otherwise) {
+  constexpr int kParts = 32;
+  const int longest = wave_max(first.groups ? first.tiles : 0), run = max((longest - 1) / (min(lane, kParts - 1) + 1) + 1, c.least_tiles);
+  const float inv = 1.f / (float)run;
+  int units = 0, long_units = 0;
+  for (int b = 0; b < sequences; ++b) {
+    const int groups = __builtin_amdgcn_readlane(first.groups, b), tiles = __builtin_amdgcn_readlane(first.tiles, b);
+    if (groups == 0) continue;
+    int runs = (int)((float)(tiles - 1) * inv);
+    runs += (runs + 1) * run <= tiles - 1;
+    runs = runs - (runs * run > tiles - 1) + 1;
+    units += groups * runs;
+    long_units += 2 * tiles > run * runs ? groups * runs : 0;
+  }
+  const float rounds = (float)((long_units - 1) / c.target + 1) * (float)(run + c.least_tiles);
+  const float even = ((float)work + (float)units * (float)c.least_tiles) / (float)c.target;
+  float cost = units <= c.most ? fmaxf(rounds, even) : 1e30f;
+  const float mine = cost;
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) cost = fminf(cost, __shfl_xor(cost, d, 64));
+  const int at = __ffsll((unsigned long long)__ballot(mine == cost)) - 1;
+  return cost < 1e30f ? __builtin_amdgcn_readlane(run, at) : otherwise;
+}
+
 // Tiles of a run.  With work = sum of groups * tiles and n = sum of groups: the shortest runs, of work / target tiles or some
 // more, that come to at most `target` units (each group's last run may be short); runs of work / (target - n) always do.  Where the groups
 // alone are more than half the target, of work / (target / 2), and where they fill the chip several times, whole sequences.  No runs of
@@ -100,6 +142,7 @@ __device__ __forceinline__ int run_tiles(const Shape<Table>& p, const Cut& c, in
     return a < 1LL << 31 ? (int)(((uint32_t)a + (uint32_t)b - 1) / (uint32_t)b) : (int)min((a + b - 1) / b, (int64_t)kWholeRun);
   };
   const int safe = max(ceil_div(work, max(max((int64_t)c.target - groups, (int64_t)c.target / 2), (int64_t)1)), work > 0 ? c.least_tiles : 0);
+  if (c.even && groups > 0 && count_of(p.table) <= 64 && work < 1LL << 24) return even_run(c, lane, first, count_of(p.table), work, safe);
   if (count_of(p.table) <= 64 && groups <= c.target)
     for (int run = max(ceil_div(work, c.target), c.least_tiles); run < safe; run += run / 16 + 1)
       if (wave_sum(first.groups ? first.groups * runs_of(first.tiles, run) : 0) <= (uint32_t)c.target) return run;
@@ -110,15 +153,26 @@ struct Unit {
   Sequence seq;
   int b, group, run, runs, groups, tiles, first;  // tiles: of the sequence; first: number of the sequence's first unit
 };
-// unit number u: all groups of a sequence's first run, then of its second, ...  b = -1 past the last
+// unit number u: all groups of a sequence's first run, then of its second, ...; b = -1 past the last.  kShares, up to 64 sequences: those
+// with long runs first, so that none of these is left for the end (pieces of 200, 300, 301 and 97 tokens behind 12288 shared ones: 315 us
+// otherwise, 243 so; shorter steps between the lengths gain nothing, as workgroups start in the order of their numbers).
 template <class Table>
 __device__ __forceinline__ Unit unit_at(const Shape<Table>& p, const Cut& c, int u, int run, int lane, const Share& first) {
   int64_t base = 0;
   for (int b0 = 0; b0 < count_of(p.table); b0 += 64) {
     const Share s = b0 ? share_at(p, c, b0 + lane) : first;
     const int runs = s.groups ? runs_of(s.tiles, run) : 0;
-    const uint32_t mine = (uint32_t)s.groups * runs, upto = upto_sum(mine);
-    const uint64_t m = __ballot(base + upto > u && mine > 0);
+    const uint32_t mine = (uint32_t)s.groups * runs;
+    uint32_t upto = upto_sum(mine), all = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+    if constexpr (kShares<Table>) {
+      if (count_of(p.table) <= 64) {
+        const int per = runs ? (s.tiles - 1) / runs + 1 : 0;
+        const bool is_long = 2 * per > wave_max(per);
+        const uint32_t upto_long = upto_sum(is_long ? mine : 0), longs = (uint32_t)__builtin_amdgcn_readlane((int)upto_long, 63);
+        upto = is_long ? upto_long : longs + upto - upto_long;
+      }
+    }
+    const uint64_t m = __ballot(base + upto > u && base + upto - mine <= u && mine > 0);
     if (m) {
       const int at = __ffsll((unsigned long long)m) - 1;
       auto of = [&](int x) { return __builtin_amdgcn_readlane(x, at); };
@@ -138,7 +192,7 @@ __device__ __forceinline__ Unit unit_at(const Shape<Table>& p, const Cut& c, int
       if (rest < 0 || r.run >= r.runs) r.b = -1;   // (row ranges that are none: more units than 32 bits number)
       return r;
     }
-    base += (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+    base += all;
   }
   Unit none = {};
   none.b = -1;

@@ -5,27 +5,53 @@
 
 namespace moba {
 
-// a token's rows with its group's keys, and with its sequence's
+// A token's rows with its group's keys, and with its sequence's.  Up to 64 sequences and groups are asked for at once.
 __device__ __forceinline__ void sides_of(const Shape<SharedTable>& shape, int t, int lane, Side (&side)[2]) {
   const SharedTable& table = shape.table;
-  Sequence seq = {};
-  const int b = last_up_to(table, t, lane, seq, [](int, int lo) { return (int64_t)lo; });
-  const bool there = b >= 0 && t < seq.hi;
-  const int g = there ? __builtin_amdgcn_readfirstlane(group_of(table, b)) : -1;
-  side[0] = side[1] = {0, 0, 0, false};
-  int begin = 0;
-  const int keys = (int)min(seq.length, room(table));
-  if (g >= 0) {
-    const Sequence all = sequence_of(table, g);
-    side[0] = {g, t - all.lo, all.hi - all.lo, all.length > 0 && t >= all.lo && t < all.hi};
-    begin = min((int)all.length, keys);
+  Sequence seq = {}, all = {};
+  int b = -1, g = -1;
+  if (table.B <= 64 && table.G <= 64) {
+    const Sequence mine = sequence_of(static_cast<const PageTable&>(table), min(lane, table.B - 1));
+    const int group = min(lane, table.G - 1), first = table.cu_groups[group], end = table.cu_groups[group + 1];
+    const int keys = shared_keys(table, group);
+    const uint64_t begun = __ballot(lane < table.B && mine.lo <= t);
+    if (begun) {
+      b = 63 - __builtin_clzll(begun);
+      seq = {__builtin_amdgcn_readlane(mine.lo, b), __builtin_amdgcn_readlane(mine.hi, b), __builtin_amdgcn_readlane((int)mine.length, b), 0};
+      const uint64_t in = __ballot(lane < table.G && first <= b && b < end);
+      if (in) {
+        g = __ffsll((unsigned long long)in) - 1;
+        const int m0 = min(max(__builtin_amdgcn_readlane(first, g), 0), table.B), m1 = max(min(__builtin_amdgcn_readlane(end, g), table.B), m0);
+        all.lo = __builtin_amdgcn_readlane(mine.lo, min(m0, table.B - 1));     // (b is one of m0 .. m1 - 1)
+        all.hi = __builtin_amdgcn_readlane(mine.hi, max(m1 - 1, 0));
+        all.length = __builtin_amdgcn_readlane(keys, g);
+      }
+    }
+  } else {
+    b = last_up_to(table, t, lane, seq, [](int, int lo) { return (int64_t)lo; });
+    g = b >= 0 ? __builtin_amdgcn_readfirstlane(group_of(table, b)) : -1;
+    if (g >= 0) all = sequence_of(table, g);
   }
-  if (there) side[1] = {table.G + b, t - seq.lo, seq.hi - seq.lo, keys > begin};
+  const bool there = b >= 0 && t < seq.hi;
+  const int keys = (int)min(seq.length, room(table)), begin = g >= 0 ? min((int)all.length, keys) : 0;
+  side[0] = {max(g, 0), t - all.lo, all.hi - all.lo, there && g >= 0 && all.length > 0 && t >= all.lo && t < all.hi};
+  side[1] = {table.G + max(b, 0), t - seq.lo, seq.hi - seq.lo, there && keys > begin};
 }
 
 // Units of the batch: its tokens are rows of a group and of a sequence.  Every unit leaves parts.
 static Cuts shared_cuts(int64_t T, int B, int G, int rep, int Hkv, int D, bool cache8) {
-  Cuts c = paged_cuts(2 * T, B + G, rep, Hkv, D, cache8, -1);
+  // More rows are few than where nothing is shared: the groups of 32 read the same keys at the same time, from L2 all but one.  Single tokens
+  // of 24 sequences (96 rows) behind 16384 shared ones, 8 heads, 8 bits: 33 us as few rows, 49 as many; of 40 41 and 62, of 64 51 and
+  // 70, of 128 87 and 103, but two pieces of 128 tokens 88 and 83.  16-bit elements, heads of 128: 40 sequences 55 and 71, 64 76 and 82,
+  // but two pieces of 64 tokens 81 and 57.  Heads of 64: 64 rows to a workgroup (72 of four sequences behind 8208, fp16: 17.5 us with the
+  // others' launch gone, 22.4 as many; heads of 128 have no registers for it: 66 us for 64 rows behind 32768, 39.8 in two groups).
+  const int sets = few_sets<SharedTable>(D), few_rows = (D == 128 && !cache8 ? 4 : 8) * kFewRows;
+  Cuts c = paged_cuts(2 * T, B + G, rep, Hkv, D, cache8, T * rep > few_rows, sets * kFewRows, few_rows, D == 128 && !cache8 ? 1 : 2);
+  if (c.many.most > 0) {   // (pieces of prompts behind what is shared, among others: units of many lengths)
+    c.many.even = true;
+    const int64_t most = c.many.most + 2 * (int64_t)c.many.target;
+    c.many.most = (int)(most < 0x7fffffff ? most : 0x7fffffff);
+  }
   c.few.parts = c.few.most;
   c.many.parts = c.many.most;
   return c;

@@ -55,17 +55,57 @@ __device__ __forceinline__ Sequence sequence_of(const SharedTable& t, int v) {
   return s;
 }
 
-// Position of new token j of a unit's rows: in its own sequence, the last member of the group that begins no later.
+// Of sequence b, each lane its own, with the whole wave: groups and sequences that are 64 together at most are asked for at once, what they
+// say of each other goes from lane to lane.
+__device__ __forceinline__ Share share_at(const Shape<SharedTable>& p, const Cut& c, int b) {
+  const SharedTable& t = p.table;
+  if (count_of(t) > 64) return b < count_of(t) ? share_of(p, c, sequence_of(t, b)) : Share{{0, 0, 0, 0}, 0, 0};
+  const bool group = b < t.G;
+  const int first = t.cu_groups[min(b, t.G)], end = t.cu_groups[min(b + 1, t.G)], front = group ? shared_keys(t, b) : 0;
+  Sequence s = sequence_of(static_cast<const PageTable&>(t), min(max(b - t.G, 0), t.B - 1));
+  // a group's rows: from its first member's first to its last one's last
+  const int m0 = min(max(first, 0), t.B), m1 = max(min(end, t.B), m0);
+  const int lo = __shfl(s.lo, t.G + min(m0, t.B - 1), 64), hi = __shfl(s.hi, t.G + max(m1 - 1, 0), 64);
+  // a sequence's group: the last that begins no later
+  int g = 0;
+  for (int above = t.G; __any(above - g > 1);) {
+    const int mid = (g + above) >> 1, begins = __shfl(first, mid, 64);
+    if (above - g > 1) {
+      if (begins <= b - t.G) g = mid; else above = mid;
+    }
+  }
+  const int g_first = __shfl(first, g, 64), g_end = __shfl(end, g, 64), g_front = __shfl(front, g, 64);
+  if (b >= count_of(t)) return {{0, 0, 0, 0}, 0, 0};
+  if (group) {
+    s = {lo, m1 > m0 ? max(hi, lo) : lo, front, 0};
+  } else {
+    s.begin = g_first <= b - t.G && b - t.G < g_end ? (int)min((int64_t)g_front, min(s.length, room(t))) : 0;
+  }
+  return share_of(p, c, s);
+}
+
+// Position of new token j of a unit's rows: in its own sequence, the last member of the group that begins no later.  With the whole wave:
+// up to 64 members are asked for at once, and searched among the lanes.
 __device__ __forceinline__ int position_at(const SharedTable& t, const Unit& u, int j) {
   if (u.b >= t.G) return (int)u.seq.length - (u.seq.hi - u.seq.lo) + j;
-  const int token = u.seq.lo + j, end = min(t.cu_groups[u.b + 1], t.B);
-  int lo = first_member(t, u.b), hi = end;
+  const int token = u.seq.lo + j, first = first_member(t, u.b), end = min(t.cu_groups[u.b + 1], t.B);
+  int lo = 0, hi = end - first;
+  if (hi <= 64) {
+    const Sequence s = sequence_of(static_cast<const PageTable&>(t), min(first + ((int)threadIdx.x & 63), t.B - 1));
+    while (__any(hi - lo > 1)) {
+      const int mid = (lo + hi) >> 1, begins = __shfl(s.lo, mid, 64);
+      if (hi - lo > 1) {
+        if (begins <= token) lo = mid; else hi = mid;
+      }
+    }
+    const int ends = __shfl(s.hi, lo, 64), length = __shfl((int)s.length, lo, 64);
+    return (int)min((int64_t)length - ends + token, (int64_t)0x7fffffff);
+  }
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (t.cu_new[mid] <= token) lo = mid; else hi = mid;
+    if (t.cu_new[first + mid] <= token) lo = mid; else hi = mid;
   }
-  lo = min(lo, t.B - 1);
-  const Sequence s = sequence_of(static_cast<const PageTable&>(t), lo);
+  const Sequence s = sequence_of(static_cast<const PageTable&>(t), min(first + lo, t.B - 1));
   return (int)min(s.length - s.hi + token, (int64_t)0x7fffffff);
 }
 // (a group's rows are of several sequences)

@@ -37,8 +37,8 @@ def paged_prefix_attention(query: torch.Tensor, cache: PagedKVCache, page_table:
         what ``paged_attention`` does (with the sums in another order): every new token sees its sequence's tokens up to itself,
         also where ``shared`` says more than a sequence has.  Rows that see nothing are zeros.
 
-    Precision is that of ``paged_attention`` for as many rows as a group, and a sequence, has: what is shared is attended by the new
-    tokens of all of a group.  The index tensors stay on the device: a captured call follows them.  No gradients.
+    Precision is that of ``paged_attention`` for few rows where a group (for what it shares), or a sequence (for the rest), has up to 256
+    rows, new tokens times heads on a key/value head; 128 with 16-bit pages and heads of 128.  Otherwise it is that for many.  The index tensors stay on the device: a captured call follows them.  No gradients.
     """
     out = _prefix(query, cache, page_table, lengths, cu_new, cu_groups, shared, scaling)
     if out is not NotImplemented:
