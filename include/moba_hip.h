@@ -58,7 +58,7 @@ extern "C" {
 
 enum { MOBA_DTYPE_BF16 = 0, MOBA_DTYPE_F16 = 1 };
 
-#define MOBA_ABI_VERSION 123 /* the signatures below; moba_version() returns the number the library was built with */
+#define MOBA_ABI_VERSION 124 /* the signatures below; moba_version() returns the number the library was built with */
 int moba_version(void);
 const char* moba_strerror(int code);
 
@@ -489,11 +489,13 @@ int moba_paged_block_attention(const void* q, void* out, const void* k_pages, co
  *   it need are there (or it needs none); otherwise it gets nothing.  Writes the entries of the new pages, lengths (the served
  *   ones'), free_count, cu_new [B+1] (the running sum of the tokens given), and for each of the rows its sequence, position and slot
  *   (page * page_size + place in it): owners, positions [rows] int32, slots [rows] int64; -1, 0, -1 behind cu_new[B], and slot -1 where
- *   the table names no page of the pool.  rows < 2^30, 0 allowed.  workspace: B + 1 int32.
+ *   the table names no page of the pool.  rows < 2^30, 0 allowed.  workspace: moba_paged_reserve_workspace_bytes(B, rows) bytes, NULL
+ *   where these are none.
  * moba_paged_release: sequences keep their first keep[b] tokens; the pages behind go back to the pool (entries that name none of
  *   it do not), so that a reserve that is taken back leaves the stack as it was, and their entries become -1. */
+size_t moba_paged_reserve_workspace_bytes(int B, int64_t rows);
 int moba_paged_reserve(int32_t* free_pages, int32_t* free_count, int32_t* page_table, int32_t* lengths, const int32_t* new_tokens,
-                       int32_t* cu_new, int32_t* owners, int32_t* positions, int64_t* slots, int32_t* workspace, int B, int64_t rows,
+                       int32_t* cu_new, int32_t* owners, int32_t* positions, int64_t* slots, void* workspace, int B, int64_t rows,
                        int page_size, int64_t num_pages, int64_t max_pages, int64_t table_stride, void* stream);
 int moba_paged_release(int32_t* free_pages, int32_t* free_count, int32_t* page_table, int32_t* lengths, const int32_t* keep, int B,
                        int page_size, int64_t num_pages, int64_t max_pages, int64_t table_stride, void* stream);

@@ -77,6 +77,7 @@ _SIGNATURES = {
     "moba_paged_block_attention_workspace_bytes": (c_size_t, [c_int64] + [c_int] * 5 + [c_int64] + [c_int] * 3),
     "moba_paged_block_attention": (c_int, [c_void_p] * 11 + [c_int64] + [c_int] * 5 + [c_int64] * 2 + [c_int] * 2
                                           + [c_strides, c_int, c_float, c_int, c_void_p]),
+    "moba_paged_reserve_workspace_bytes": (c_size_t, [c_int, c_int64]),
     "moba_paged_reserve": (c_int, [c_void_p] * 10 + [c_int, c_int64, c_int] + [c_int64] * 3 + [c_void_p]),
     "moba_paged_release": (c_int, [c_void_p] * 5 + [c_int, c_int] + [c_int64] * 3 + [c_void_p]),
     "moba_mfma_probe": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p]),
@@ -108,7 +109,7 @@ class SizesStruct(ctypes.Structure):
     _fields_ = [(n, c_int64) for n in ("kbar_elems", "chunk_mean_workspace_bytes", "sel_ints", "cnt_ints", "seg_off_ints",
                                        "seg_dest_ints", "fwd_hist_bound", "bwd_hist_bound", "part_rows", "redo_ints",
                                        "lse_floats", "delta_floats")]
-ABI_VERSION = 123  # MOBA_ABI_VERSION of include/moba_hip.h, the signatures above
+ABI_VERSION = 124  # MOBA_ABI_VERSION of include/moba_hip.h, the signatures above
 DTYPE_BF16, DTYPE_F16 = 0, 1
 
 
@@ -183,7 +184,7 @@ def bind_serving(module, **instead):
     lib = load()
     names = ("moba_paged_prefix_attention", "moba_paged_prefix_attention_workspace_bytes", "moba_paged_block_attention",
              "moba_paged_block_attention_workspace_bytes", "moba_paged_key_sums", "moba_paged_select_blocks",
-             "moba_paged_select_blocks_workspace_bytes", "moba_paged_reserve", "moba_paged_release")
+             "moba_paged_select_blocks_workspace_bytes", "moba_paged_reserve", "moba_paged_reserve_workspace_bytes", "moba_paged_release")
     module.bind_serving(*(ctypes.cast(instead.get(n, getattr(lib, n)), c_void_p).value for n in names))
 
 

@@ -15,6 +15,7 @@ decltype(&moba_paged_key_sums) sums_call = nullptr;
 decltype(&moba_paged_select_blocks) select_call = nullptr;
 decltype(&moba_paged_select_blocks_workspace_bytes) select_bytes = nullptr;
 decltype(&moba_paged_reserve) reserve_call = nullptr;
+decltype(&moba_paged_reserve_workspace_bytes) reserve_bytes = nullptr;
 decltype(&moba_paged_release) release_call = nullptr;
 
 constexpr int64_t kMostTokens = 1 << 24;   // fewer than these
@@ -231,9 +232,11 @@ PyObject* py_paged_reserve(PyObject*, PyObject* const* args, Py_ssize_t n) {
     out[1] = fresh({rows}, at::kInt, device);
     out[2] = fresh({rows}, at::kInt, device);
     out[3] = fresh({rows}, at::kLong, device);
-    Tensor space = bytes((b + 1) * 4, device);
+    const size_t need = reserve_bytes((int)b, rows);
+    Tensor space;
+    if (need) space = bytes(need, device);
     check(reserve_call(t.of(t.free_pages), t.of(t.free_count), t.of(t.table), t.of(t.lengths), t.of(t.asked), t.of(out[0]), t.of(out[1]),
-                       t.of(out[2]), (int64_t*)out[3].mutable_data_ptr(), (int32_t*)space.mutable_data_ptr(), (int)b, rows, (int)t.page, t.free_pages.size(0), t.table.size(1),
+                       t.of(out[2]), (int64_t*)out[3].mutable_data_ptr(), mutable_pointer(space), (int)b, rows, (int)t.page, t.free_pages.size(0), t.table.size(1),
                        t.table.stride(0), stream_of(t.lengths)),
           "moba_paged_reserve");
     for (const Tensor& x : {t.free_count, t.table, t.lengths}) written(x);
@@ -273,13 +276,13 @@ PyObject* py_paged_release(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 // bind_serving(addresses of moba_paged_prefix_attention, .._workspace_bytes, moba_paged_block_attention, .._workspace_bytes,
-// moba_paged_key_sums, moba_paged_select_blocks, .._workspace_bytes, moba_paged_reserve, moba_paged_release), of the library whose
+// moba_paged_key_sums, moba_paged_select_blocks, .._workspace_bytes, moba_paged_reserve, .._workspace_bytes, moba_paged_release), of the library whose
 // version bind() has checked
 PyObject* py_bind_serving(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  TORCH_CHECK_TYPE(n == 9, "bind_serving takes nine addresses");
-  void* at[9];
-  for (int i = 0; i < 9; ++i) {
+  TORCH_CHECK_TYPE(n == 10, "bind_serving takes ten addresses");
+  void* at[10];
+  for (int i = 0; i < 10; ++i) {
     at[i] = PyLong_AsVoidPtr(args[i]);
     if (PyErr_Occurred()) return nullptr;
   }
@@ -291,7 +294,8 @@ PyObject* py_bind_serving(PyObject*, PyObject* const* args, Py_ssize_t n) {
   select_call = reinterpret_cast<decltype(select_call)>(at[5]);
   select_bytes = reinterpret_cast<decltype(select_bytes)>(at[6]);
   reserve_call = reinterpret_cast<decltype(reserve_call)>(at[7]);
-  release_call = reinterpret_cast<decltype(release_call)>(at[8]);
+  reserve_bytes = reinterpret_cast<decltype(reserve_bytes)>(at[8]);
+  release_call = reinterpret_cast<decltype(release_call)>(at[9]);
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }

@@ -274,15 +274,19 @@ static int check_tables(TableParams& p, int32_t* free_pages, int32_t* free_count
 
 using namespace moba;
 
+extern "C" size_t moba_paged_reserve_workspace_bytes(int B, int64_t rows) {
+  return B > 0 && rows > kRowsAtOnce ? ((size_t)B + 1) * sizeof(int32_t) : 0;
+}
+
 extern "C" int moba_paged_reserve(int32_t* free_pages, int32_t* free_count, int32_t* page_table, int32_t* lengths,
-                                  const int32_t* new_tokens, int32_t* cu_new, int32_t* owners, int32_t* positions, int64_t* slots, int32_t* workspace,
+                                  const int32_t* new_tokens, int32_t* cu_new, int32_t* owners, int32_t* positions, int64_t* slots, void* workspace,
                                   int B, int64_t rows, int page_size, int64_t num_pages, int64_t max_pages, int64_t table_stride, void* stream) {
   TableParams p;
   const int rc = check_tables(p, free_pages, free_count, page_table, lengths, new_tokens, B, page_size, num_pages, max_pages, table_stride);
   if (rc != MOBA_OK) return rc;
-  if (!cu_new || !workspace || rows < 0 || (rows && (!owners || !positions || !slots)) || ((uintptr_t)slots & 7)) return MOBA_ERR_ARG;
+  if (!cu_new || rows < 0 || (rows > kRowsAtOnce && !workspace) || (rows && (!owners || !positions || !slots)) || ((uintptr_t)slots & 7) || ((uintptr_t)workspace & 3)) return MOBA_ERR_ARG;
   if (rows >= 1LL << 30) return MOBA_ERR_LIMIT;
-  p.cu_new = cu_new; p.owners = owners; p.positions = positions; p.slots = slots; p.ranks = workspace;
+  p.cu_new = cu_new; p.owners = owners; p.positions = positions; p.slots = slots; p.ranks = (int32_t*)workspace;
   p.rows = (int)rows;
   LaunchCheck launch_check;
   hipStream_t st = (hipStream_t)stream;

@@ -30,7 +30,8 @@ def paged_key_sums(cache: PagedKVCache, sums: torch.Tensor, page_table: torch.Te
             of the keys of the tokens that the page holds up to its sequence's last.  Other pages' sums are left as they are.
         rows: the packed rows that cu_new counts in (its last number or more)
     """
-    if _sums(cache, sums, page_table, lengths, cu_new, rows) is not NotImplemented:
+    if _lib.host().paged_key_sums(cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales, sums, page_table, lengths, cu_new,
+                                  rows) is not NotImplemented:
         return
     _check_no_gradients(cache, sums)
     k = cache.k_pages
@@ -44,12 +45,8 @@ def paged_key_sums(cache: PagedKVCache, sums: torch.Tensor, page_table: torch.Te
     if not k.is_cuda:
         raise RuntimeError("paged_key_sums needs tensors on an AMD GPU (there is no CPU path)")
     if rows and page_table.shape[0]:
-        _taken(_sums(cache, sums, _table(page_table), lengths.contiguous(), cu_new.contiguous(), rows), "paged_key_sums")
-
-
-def _sums(cache, sums, page_table, lengths, cu_new, rows):
-    tensors = (cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales, sums, page_table, lengths, cu_new)
-    return _lib.host().paged_key_sums(*map(_plain, tensors), rows)
+        tensors = (k, cache.v_pages, cache.k_scales, cache.v_scales, sums, _table(page_table), lengths.contiguous(), cu_new.contiguous())
+        _taken(_lib.host().paged_key_sums(*map(_plain, tensors), rows), "paged_key_sums")
 
 
 def _check_blocks(block_size, page_size, topk):
@@ -82,7 +79,7 @@ def paged_select_blocks(query: torch.Tensor, sums: torch.Tensor, page_table: tor
     (``moba_attn_varlen`` rounds the blocks' means to the keys' type first, which can decide between blocks of nearly equal
     products otherwise.)  No gradients.
     """
-    out = _select(query, sums, page_table, lengths, cu_new, page_size, block_size, topk)
+    out = _lib.host().paged_select_blocks(query, sums, page_table, lengths, cu_new, page_size, block_size, topk)
     if out is not NotImplemented:
         return out
     if torch.is_grad_enabled() and (query.requires_grad or sums.requires_grad):
@@ -107,12 +104,8 @@ def paged_select_blocks(query: torch.Tensor, sums: torch.Tensor, page_table: tor
         return torch.full((*query.shape[:2], topk), -1, dtype=torch.int32, device=query.device)
     query = query if _addressable(query) else E._aligned(query)
     sums = sums if sums.is_contiguous() and sums.data_ptr() % 16 == 0 else E._aligned(sums)
-    return _taken(_select(query, sums, _table(page_table), lengths.contiguous(), cu_new.contiguous(), page_size, block_size, topk),
-                  "paged_select_blocks")
-
-
-def _select(query, sums, page_table, lengths, cu_new, *numbers):
-    return _lib.host().paged_select_blocks(*map(_plain, (query, sums, page_table, lengths, cu_new)), *numbers)
+    tensors = (query, sums, _table(page_table), lengths.contiguous(), cu_new.contiguous())
+    return _taken(_lib.host().paged_select_blocks(*map(_plain, tensors), page_size, block_size, topk), "paged_select_blocks")
 
 
 def paged_block_attention(query: torch.Tensor, cache: PagedKVCache, blocks: torch.Tensor, page_table: torch.Tensor,
@@ -134,7 +127,8 @@ def paged_block_attention(query: torch.Tensor, cache: PagedKVCache, blocks: torc
     Scores, softmax statistics and sums are 32 bits, a probability the sum of two 16-bit elements, as in ``paged_attention`` for few
     rows.
     """
-    out = _blocks(query, cache, page_table, lengths, cu_new, blocks, block_size, scaling)
+    out = _lib.host().paged_block_attention(cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales, query, page_table, lengths, cu_new,
+                                            blocks, block_size, scaling)
     if out is not NotImplemented:
         return out
     _check_no_gradients(cache, query)
@@ -152,10 +146,6 @@ def paged_block_attention(query: torch.Tensor, cache: PagedKVCache, blocks: torc
     if not query.shape[0] or not page_table.shape[0]:
         return torch.zeros(query.shape, dtype=query.dtype, device=query.device)
     query = query if _addressable(query) else E._aligned(query)
-    return _taken(_blocks(query, cache, _table(page_table), lengths.contiguous(), cu_new.contiguous(), blocks.contiguous(), block_size,
-                          scaling), "paged_block_attention")
-
-
-def _blocks(query, cache, page_table, lengths, cu_new, blocks, block_size, scaling):
-    tensors = (cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales, query, page_table, lengths, cu_new, blocks)
-    return _lib.host().paged_block_attention(*map(_plain, tensors), block_size, scaling)
+    tensors = (cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales, query, _table(page_table), lengths.contiguous(),
+               cu_new.contiguous(), blocks.contiguous())
+    return _taken(_lib.host().paged_block_attention(*map(_plain, tensors), block_size, scaling), "paged_block_attention")

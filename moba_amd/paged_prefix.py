@@ -40,7 +40,8 @@ def paged_prefix_attention(query: torch.Tensor, cache: PagedKVCache, page_table:
     Precision is that of ``paged_attention`` for few rows where a group (for what it shares), or a sequence (for the rest), has up to 256
     rows, new tokens times heads on a key/value head; 128 with 16-bit pages and heads of 128.  Otherwise it is that for many.  The index tensors stay on the device: a captured call follows them.  No gradients.
     """
-    out = _prefix(query, cache, page_table, lengths, cu_new, cu_groups, shared, scaling)
+    out = _lib.host().paged_prefix_attention(cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales, query, page_table, lengths, cu_new,
+                                             cu_groups, shared, scaling)
     if out is not NotImplemented:
         return out
     # tensors that have to be copied first, none at all, or wrong ones
@@ -61,10 +62,6 @@ def paged_prefix_attention(query: torch.Tensor, cache: PagedKVCache, page_table:
     if not query.shape[0] or not page_table.shape[0] or not shared.shape[0]:
         return paged_attention(query, cache, page_table, lengths, cu_new, scaling)
     query = query if _addressable(query) else E._aligned(query)
-    return _taken(_prefix(query, cache, _table(page_table), lengths.contiguous(), cu_new.contiguous(), cu_groups.contiguous(),
-                          shared.contiguous(), scaling), "paged_prefix_attention")
-
-
-def _prefix(query, cache, page_table, lengths, cu_new, cu_groups, shared, scaling):
-    tensors = (cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales, query, page_table, lengths, cu_new, cu_groups, shared)
-    return _lib.host().paged_prefix_attention(*map(_plain, tensors), scaling)
+    tensors = (cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales, query, _table(page_table), lengths.contiguous(),
+               cu_new.contiguous(), cu_groups.contiguous(), shared.contiguous())
+    return _taken(_lib.host().paged_prefix_attention(*map(_plain, tensors), scaling), "paged_prefix_attention")

@@ -93,7 +93,7 @@ def paged_reserve(pool: PagePool, page_table: torch.Tensor, lengths: torch.Tenso
     not fit aside), are more than ``rows``; or if it needs more pages and they, with those that the others before it need, are more
     than the pool has.  The index tensors stay on the device: a captured call follows them.  At most 8192 sequences.
     """
-    out = _reserve(pool, page_table, lengths, new_tokens, rows)
+    out = _lib.host().paged_reserve(pool.free_pages, pool.free_count, page_table, lengths, new_tokens, rows, pool.page_size)
     if out is not NotImplemented:
         return out
     _check(pool, page_table, lengths, "new_tokens", new_tokens)
@@ -104,11 +104,8 @@ def paged_reserve(pool: PagePool, page_table: torch.Tensor, lengths: torch.Tenso
     if not lengths.shape[0]:
         none = torch.full((rows,), -1, dtype=torch.int32, device=lengths.device)
         return torch.zeros(1, dtype=torch.int32, device=lengths.device), none, torch.zeros_like(none), none.long()
-    return _taken(_reserve(pool, page_table, lengths, new_tokens.contiguous(), rows), "paged_reserve")
-
-
-def _reserve(pool, page_table, lengths, new_tokens, rows):
-    return _lib.host().paged_reserve(*map(_plain, (pool.free_pages, pool.free_count, page_table, lengths, new_tokens)), rows, pool.page_size)
+    tensors = (pool.free_pages, pool.free_count, page_table, lengths, new_tokens.contiguous())
+    return _taken(_lib.host().paged_reserve(*map(_plain, tensors), rows, pool.page_size), "paged_reserve")
 
 
 def paged_release(pool: PagePool, page_table: torch.Tensor, lengths: torch.Tensor, keep: torch.Tensor) -> None:
@@ -124,14 +121,11 @@ def paged_release(pool: PagePool, page_table: torch.Tensor, lengths: torch.Tenso
     page of the pool do not go back.  A page that several sequences share would go back with each of them: keep the tokens that
     are shared, and release their pages once, with the sequence that they belong to.
     """
-    if _release(pool, page_table, lengths, keep) is not NotImplemented:
+    if _lib.host().paged_release(pool.free_pages, pool.free_count, page_table, lengths, keep, pool.page_size) is not NotImplemented:
         return
     _check(pool, page_table, lengths, "keep", keep)
     if not lengths.is_cuda:
         raise RuntimeError("paged_release needs tensors on an AMD GPU (there is no CPU path)")
     if lengths.shape[0]:
-        _taken(_release(pool, page_table, lengths, keep.contiguous()), "paged_release")
-
-
-def _release(pool, page_table, lengths, keep):
-    return _lib.host().paged_release(*map(_plain, (pool.free_pages, pool.free_count, page_table, lengths, keep)), pool.page_size)
+        tensors = (pool.free_pages, pool.free_count, page_table, lengths, keep.contiguous())
+        _taken(_lib.host().paged_release(*map(_plain, tensors), pool.page_size), "paged_release")
