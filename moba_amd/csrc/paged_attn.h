@@ -195,18 +195,24 @@ template <class Table>
 constexpr int few_sets(int D) { return kShares<Table> && D == 64 ? 2 : 1; }
 template <int D, bool k8>
 constexpr int few_stage_bytes() { return 2 * kFewKeys * D * (k8 ? 1 : 2); }  // K and V of a step
+constexpr int kListBytes = 8192;   // kChooses: a list that stays in LDS, behind the rest
 template <int D, bool k8>
-constexpr int few_lds_bytes() {
+constexpr int few_list_at() {
   const int loop = kFewWaves * (2 * few_stage_bytes<D, k8>() + kScaleBytes);
   const int end = kFewWaves * (32 * (D + 4) * 4 + 2 * 32 * 4);
   return loop > end ? loop : end;
 }
+template <int D, bool k8, class Table>
+constexpr int few_lds_bytes() { return few_list_at<D, k8>() + (kChooses<Table> ? kListBytes : 0); }
 
 // Position of new token j of a unit's rows, every lane its own; the least of a wave's 32 rows' (whose first is row0)
 __device__ __forceinline__ int position_at(const PageTable&, const Unit& u, int j) { return (int)u.seq.length - (u.seq.hi - u.seq.lo) + j; }
 __device__ __forceinline__ int least_position(const PageTable& t, const Unit& u, int first, int) { return position_at(t, u, first); }
 // the last key that new tokens up to j of a unit's rows see
 __device__ __forceinline__ int last_seen(const PageTable& t, const Unit& u, int j) { return position_at(t, u, j); }
+
+// kChooses: where a workgroup's list of blocks lies
+__device__ __forceinline__ int list_of(const PageTable&, char*) { return 0; }
 
 // kSets: sets of 32 rows to a workgroup, which read, and for 8-bit pages convert, K and V once for all of them
 template <class E, int D, bool k8, class Table, int kSets>
@@ -232,14 +238,18 @@ __global__ __launch_bounds__(64 * kFewWaves, kSets > 1 && D == 128 ? 1 : 2) void
   int hkv, item;
   if (!find_unit(shape, p.few, lane, unit, hkv, item)) return;
   const Sequence seq = unit.seq;
-  int keys;
-  if constexpr (kChooses<Table>) keys = __builtin_amdgcn_readfirstlane(table.keys[item]);   // (from here on: number in the list's keys)
-  else keys = keys_of(shape, seq);
-  if (unit.run == 0 && unit.group * !kChooses<Table> == 0 && hkv * !kChooses<Table> == 0 && tid == 0)
-    p.runs[item] = {unit.first, unit.runs, unit.groups};
+  if (unit.run == 0 && unit.group == 0 && hkv == 0 && tid == 0) p.runs[item] = {unit.first, unit.runs, unit.groups};
   const int b = table_row(table, unit.b);
   const int count = seq.hi - seq.lo, rows = count * shape.rep, row0 = unit.group * kFewRows * kSets;
-  const int per = (unit.tiles + unit.runs - 1) / unit.runs;   // tiles of a run
+  int keys, tiles = unit.tiles;   // kChooses: of the list
+  decltype(list_of(table, smem)) list = list_of(table, smem + few_list_at<D, k8>());
+  if constexpr (kChooses<Table>) {
+    keys = make_list(shape, seq, hkv, row0, min(rows - row0, kFewRows), smem, list);
+    tiles = (keys + kFewTile - 1) / kFewTile;
+  } else {
+    keys = keys_of(shape, seq);
+  }
+  const int per = (tiles + unit.runs - 1) / unit.runs;   // tiles of a run
   const int key_lo = __builtin_amdgcn_readfirstlane((int)min(seq.begin + (int64_t)unit.run * per * kFewTile, (int64_t)keys));
   const int key_hi = __builtin_amdgcn_readfirstlane((int)min(seq.begin + (int64_t)(unit.run + 1) * per * kFewTile, (int64_t)keys));
   const bool more = kSets > 1 && rows - row0 > kFewRows;   // than one set
@@ -280,7 +290,7 @@ __global__ __launch_bounds__(64 * kFewWaves, kSets > 1 && D == 128 ? 1 : 2) void
       ids = -1;
       chosen = 0;
       if (key < key_hi) {
-        const int page = chosen_page(table, item, (int)key, chosen);
+        const int page = chosen_page(table, list, (int)key, chosen);
         ids = page_id(table, b, page);
         place = (int)min((int64_t)page << table.page_log2, (int64_t)0x7fff0000) + ((int)key & page_mask);
       }
@@ -565,7 +575,7 @@ __global__ __launch_bounds__(64 * kFewWaves, kSets > 1 && D == 128 ? 1 : 2) void
       one_by_one<E, V, D, k8, k8>(p, hkv, own_lo, kFewTile, key_hi, [&](int key, bool& sees) __attribute__((always_inline)) {
         if constexpr (kChooses<Table>) {
           uint32_t who;
-          const int page = chosen_page(table, item, key, who);
+          const int page = chosen_page(table, list, key, who);
           sees = (who >> n & 1) && ((int64_t)page << table.page_log2) + (key & page_mask) <= limit[q];
           return page_id(table, b, page);
         } else {
@@ -1133,7 +1143,8 @@ struct Side {
   bool keys;
 };
 // of token t, found with the whole wave
-__device__ __forceinline__ void sides_of(const Shape<PageTable>& shape, int t, int lane, Side (&side)[1]) {
+template <class Table>
+__device__ __forceinline__ void sides_of(const Shape<Table>& shape, int t, int lane, Side (&side)[1]) {
   Sequence seq = {};
   const int b = last_up_to(shape.table, t, lane, seq, [](int, int lo) { return (int64_t)lo; });
   side[0] = {b, t - seq.lo, seq.hi - seq.lo, b >= 0 && t < seq.hi && keys_of(shape, seq) > 0};
@@ -1200,7 +1211,6 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams<E, T
     Parts parts[kSides];
 #pragma unroll
     for (int s = 0; s < kSides; ++s) parts[s] = token.parts(p, hkv, h - hkv * shape.rep, s);
-    if (kChooses<Table> && parts[0].runs == 1) continue;   // (is there already)
     // (the sides' runs one after the other)
     const int runs = parts[0].runs + (kSides > 1 ? parts[kSides - 1].runs : 0);
     auto row_of = [&](int i, const float*& lse) {
@@ -1235,7 +1245,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams<E, T
       }
     };
     if (runs > 0 && runs <= 4 * kShare) some(0, std::integral_constant<int, 4>{});
-    else if (kShare == 1 && runs > 0 && runs <= 8) some(0, std::integral_constant<int, 8>{});
+    else if ((kShare == 1 || kShares<Table>) && runs > 0 && runs <= 8 * kShare) some(0, std::integral_constant<int, 8>{});
     else
       for (int i0 = 0; i0 < runs; i0 += 16 * kShare) some(i0, std::integral_constant<int, 16>{});
     if constexpr (kShare == 1) {
@@ -1371,12 +1381,14 @@ static int launch_paged(const PagedParams<E, Table>& p, hipStream_t st) {
   LaunchCheck launch_check;
   static bool allowed[2][kMaxDevices];
   const auto few = paged_few_kernel<E, D, k8, Table, few_sets<Table>(D)>;
-  if (!allow_dynamic_lds((const void*)few, few_lds_bytes<D, k8>(), allowed[0])) return MOBA_ERR_LAUNCH;
-  hipLaunchKernelGGL(few, dim3((unsigned)p.few.most * p.shape.Hkv), dim3(64 * kFewWaves), (few_lds_bytes<D, k8>()), st, p);
-  if (p.many.most > 0) {
-    const auto many = paged_many_kernel<E, D, k8, Table>;
-    if (!allow_dynamic_lds((const void*)many, many_lds_bytes<D>(), allowed[1])) return MOBA_ERR_LAUNCH;
-    hipLaunchKernelGGL(many, dim3((unsigned)p.many.most * p.shape.Hkv), dim3(64 * (kManyWaves<D, k8>)), many_lds_bytes<D>(), st, p);
+  if (!allow_dynamic_lds((const void*)few, few_lds_bytes<D, k8, Table>(), allowed[0])) return MOBA_ERR_LAUNCH;
+  hipLaunchKernelGGL(few, dim3((unsigned)p.few.most * p.shape.Hkv), dim3(64 * kFewWaves), (few_lds_bytes<D, k8, Table>()), st, p);
+  if constexpr (!kChooses<Table>) {
+    if (p.many.most > 0) {
+      const auto many = paged_many_kernel<E, D, k8, Table>;
+      if (!allow_dynamic_lds((const void*)many, many_lds_bytes<D>(), allowed[1])) return MOBA_ERR_LAUNCH;
+      hipLaunchKernelGGL(many, dim3((unsigned)p.many.most * p.shape.Hkv), dim3(64 * (kManyWaves<D, k8>)), many_lds_bytes<D>(), st, p);
+    }
   }
   launch_merge<E, D>(p, st);
   return launch_check.result();

@@ -1,16 +1,24 @@
-// Rows that attend some blocks of their sequence's keys, each its own: how the blocks become units of work.
+// Rows that attend some blocks of their sequence's keys, each its own.
 //
 // A unit is up to 32 rows (tokens times heads) of one sequence and key/value head against a run of the keys of all blocks that at
-// least one of them has chosen: a list, in ascending order, of blocks with a bit for every row.  What a row has not chosen is masked, so
-// that a block is read once however many rows have it.  The list's keys are numbered through (all of its blocks are
-// whole but the last, which may be the sequence's last), and cut into runs as the whole keys of a sequence are (paged_cut.h).
+// least one of them has chosen.  Its workgroup makes a list of these, in ascending order, with a bit for every row: a mask of rows for
+// every block of the sequence, in LDS, a window at a time, into which the rows' entries are or-ed (whatever their order, one
+// result), and of which the blocks with a row are counted through.  What a row has not chosen is masked, so that a block is read once
+// however many rows have it.  The list's keys are numbered through (all of its blocks are whole but the last, which may be the
+// sequence's last) and cut into as many runs as the batch's cut says, which knows only how many blocks the rows may have chosen: as
+// many as if each had chosen its number at random.  (Lists made by a kernel before, and a cut by their lengths: 4.5 us for that
+// kernel, and another load before the first key: sixteen users' tokens on sixteen blocks of 512 53.3 us, 48.5 so;
+// one token on twelve of 4096 46.2 and 43.0.)
 #pragma once
 #include "attn_common.h"
 #include "paged_cut.h"
 
 namespace moba {
 
-constexpr int kChosenRows = 32;   // of a unit
+constexpr int kChosenRows = 32;    // of a unit
+constexpr int kWindow = 4096;      // blocks whose masks lie in LDS at a time
+constexpr int kLdsEntries = 1024;  // of a list that stays in LDS
+constexpr int kListThreads = 256;
 
 struct Chosen {
   int block;
@@ -18,95 +26,94 @@ struct Chosen {
 };
 struct ChosenTable : PageTable {
   const int32_t* blocks;  // [T, H, K], as they were given: any numbers
-  const Chosen* lists;    // [items, room_of_list]
-  const int32_t* keys;    // [items]: keys of the list's blocks
+  Chosen* lists;          // [workgroups, room_of_list] for lists that may be longer than kLdsEntries, or null
   int K, each;            // entries of a row; pages of a block
   Divisor by_each;
-  int room_of_list, items, target;  // items: (group of rows, key/value head), by the batch's bounds
+  int room_of_list;
 };
 template <>
 constexpr bool kChooses<ChosenTable> = true;
 
-// Groups of rows of the sequences, counted so that a sequence's first follows from where its rows begin (some numbers are nobody's):
-// sequence b's first is this many rows * rep / 32 + b
-__device__ __forceinline__ int64_t first_group(int lo, int rep, int b) { return (int64_t)lo * rep / kChosenRows + b; }
+__device__ __forceinline__ int block_keys(const ChosenTable& t) { return t.each << t.page_log2; }
 
-// The unit of a workgroup.  Runs as in run_tiles() and unit_at(), over items instead of sequences; with kWholeAt times as many items
-// as fill the chip an item's keys are one run.
-__device__ __forceinline__ bool find_unit(const Shape<ChosenTable>& shape, const Cut& c, int lane, Unit& unit, int& hkv, int& item) {
-  const ChosenTable& t = shape.table;
-  const int u = blockIdx.x;
-  unit = {};
-  auto tiles_of = [&](int i) { return i < t.items ? (t.keys[i] + c.tile_keys - 1) / c.tile_keys : 0; };
-  if (t.items >= kWholeAt * t.target) {
-    item = u;
-    unit.tiles = __builtin_amdgcn_readfirstlane(tiles_of(u));
-    unit.runs = 1;
-    unit.first = u;
-  } else {
-    constexpr int kKept = 8;   // of the items' tiles, 64 at a time
-    int kept[kKept];
-    int64_t work = 0;
-    int groups = 0;
-#pragma unroll
-    for (int k = 0; k < kKept; ++k) kept[k] = tiles_of(64 * k + lane);
-#pragma unroll
-    for (int k = 0; k < kKept; ++k) {
-      work += wave_sum(kept[k]);
-      groups += __builtin_popcountll(__ballot(kept[k] > 0));
-    }
-    for (int i0 = 64 * kKept; i0 < t.items; i0 += 64) {
-      const int tiles = tiles_of(i0 + lane);
-      work += wave_sum(tiles);
-      groups += __builtin_popcountll(__ballot(tiles > 0));
-    }
-    const int places = max(max(t.target - groups, t.target / 2), 1);
-    int run = max((int)min((work + places - 1) / places, (int64_t)kWholeRun), c.least_tiles);
-    if (t.items <= 64 * kKept && groups <= t.target) {   // the shortest runs that fit
-      const int safe = run;
-      for (int r = max((int)min((work + t.target - 1) / t.target, (int64_t)kWholeRun), c.least_tiles); r < safe; r += r / 16 + 1) {
-        int n = 0;
-#pragma unroll
-        for (int k = 0; k < kKept; ++k) n += kept[k] ? runs_of(kept[k], r) : 0;
-        if (wave_sum(n) <= (uint32_t)t.target) {
-          run = r;
-          break;
-        }
-      }
-    }
-    int base = 0;
-    item = -1;
-    auto look = [&](int i0, int tiles) __attribute__((always_inline)) {
-      const int runs = tiles ? runs_of(tiles, run) : 0, upto = (int)upto_sum(runs);
-      const uint64_t m = __ballot(base + upto > u && runs > 0);
-      if (m && item < 0) {
-        const int at = __ffsll((unsigned long long)m) - 1;
-        item = i0 + at;
-        unit.tiles = __builtin_amdgcn_readlane(tiles, at);
-        unit.runs = __builtin_amdgcn_readlane(runs, at);
-        unit.first = base + __builtin_amdgcn_readlane(upto - runs, at);
-        unit.run = u - unit.first;
-      }
-      base += __builtin_amdgcn_readlane(upto, 63);
-    };
-#pragma unroll
-    for (int k = 0; k < kKept; ++k) look(64 * k, kept[k]);
-    for (int i0 = 64 * kKept; i0 < t.items && item < 0; i0 += 64) look(i0, tiles_of(i0 + lane));
-  }
-  if (item < 0 || unit.tiles == 0) return false;
-  const int g = item / shape.Hkv;
-  hkv = item - g * shape.Hkv;
-  unit.b = last_up_to(t, g, lane, unit.seq, [&](int b, int lo) { return first_group(lo, shape.rep, b); });
-  if (unit.b < 0) return false;
-  unit.group = (int)(g - first_group(unit.seq.lo, shape.rep, unit.b));
-  unit.groups = 1;
-  return unit.group >= 0 && unit.group * kChosenRows < (unit.seq.hi - unit.seq.lo) * shape.rep;
+__device__ __forceinline__ Chosen* list_of(const ChosenTable& t, char* lds) {
+  return t.lists ? t.lists + (int64_t)blockIdx.x * t.room_of_list : reinterpret_cast<Chosen*>(lds);
 }
 
-// Of key `key` of an item's list: its page's number in the sequence, the rows that have chosen it
-__device__ __forceinline__ int chosen_page(const ChosenTable& t, int item, int key, uint32_t& rows) {
+// of blocks that `rows` rows have, K each at random
+__device__ __forceinline__ float chosen_blocks(float blocks, float k, float rows) {
+  return k < blocks ? blocks * (1.f - __builtin_amdgcn_exp2f(rows * __builtin_amdgcn_logf(1.f - k / blocks))) : blocks;
+}
+__device__ __forceinline__ Share share_of(const Shape<ChosenTable>& p, const Cut& c, const Sequence& s) {
+  const int rows = (s.hi - s.lo) * p.rep, keys = keys_of(p, s);
+  Share r = {s, 0, 0};
+  if (rows > 0 && keys > 0) {
+    const int all = block_keys(p.table);
+    const float some = chosen_blocks((float)((keys - 1) / all + 1), (float)p.table.K, (float)min(rows, kChosenRows)) * (float)all;
+    r.tiles = (min(keys, (int)fminf(some + 0.5f, 2e9f)) - 1) / c.tile_keys + 1;
+    r.groups = (rows - 1) / c.group_rows + 1;
+  }
+  return r;
+}
+
+// The list of a unit's rows row0 .. row0 + rows_here - 1, by the whole workgroup of kListThreads: the number of its keys.  `lds`: 4 * kWindow
+// + 64 bytes; `list`: in LDS or memory.
+__device__ __forceinline__ int make_list(const Shape<ChosenTable>& shape, const Sequence& seq, int hkv, int row0, int rows_here, char* lds,
+                                         Chosen* list) {
+  constexpr int kEach = kWindow / kListThreads, kWaves = kListThreads / 64;
+  uint32_t* const mask = reinterpret_cast<uint32_t*>(lds);
+  volatile int* const sums = reinterpret_cast<volatile int*>(lds + 4 * kWindow);   // [kWaves], and the last block
+  const ChosenTable& t = shape.table;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int keys = keys_of(shape, seq), all = block_keys(t), blocks = keys > 0 ? (keys - 1) / all + 1 : 0;
+  int total = 0;
+  for (int w0 = 0; w0 < blocks; w0 += kWindow) {
+    const int here = min(kWindow, blocks - w0);
+    for (int i = tid; i < (here + kEach - 1) / kEach * kEach; i += kListThreads) mask[i] = 0;
+    __syncthreads();
+    for (int i = tid; i < rows_here * t.K; i += kListThreads) {
+      const int r = i / t.K, row = row0 + r, j = row / shape.rep;
+      const int64_t position = seq.length - (seq.hi - seq.lo) + j;
+      const int block = t.blocks[((int64_t)(seq.lo + j) * shape.H + hkv * shape.rep + row - j * shape.rep) * t.K + i - r * t.K];
+      if (block >= w0 && block < w0 + here && (int64_t)block * all <= position) atomicOr(&mask[block - w0], 1u << r);
+    }
+    __syncthreads();
+    // each thread its neighbouring blocks
+    int mine = 0;
+    if (tid * kEach < here)
+#pragma unroll
+      for (int k = 0; k < kEach; ++k) mine += mask[tid * kEach + k] != 0;
+    int upto = (int)upto_sum(mine);
+    if (lane == 63) sums[wave] = upto;
+    __syncthreads();
+    int found = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      if (w < wave) upto += sums[w];
+      found += sums[w];
+    }
+    int at = total + upto - mine;
+    if (tid * kEach < here)
+#pragma unroll
+      for (int k = 0; k < kEach; ++k) {
+        const uint32_t who = mask[tid * kEach + k];
+        if (!who) continue;
+        list[at] = {w0 + tid * kEach + k, who};
+        if (++at == total + found) sums[kWaves] = w0 + tid * kEach + k;
+      }
+    total += found;
+    __syncthreads();   // (the list is written; masks and sums have been read)
+  }
+  if (total == 0) return 0;
+  const int last = sums[kWaves];
+  __syncthreads();   // (what comes next may lie here)
+  return __builtin_amdgcn_readfirstlane((total - 1) * all + min(all, keys - last * all));
+}
+
+// Of key `key` of a list: its page's number in the sequence, the rows that have chosen it
+__device__ __forceinline__ int chosen_page(const ChosenTable& t, const Chosen* list, int key, uint32_t& rows) {
   const int page = key >> t.page_log2, entry = quotient_or_same(page, t.by_each);
-  const Chosen c = t.lists[(int64_t)item * t.room_of_list + entry];
+  const Chosen c = list[entry];
   rows = c.rows;
   return c.block * t.each + page - entry * t.each;
 }
