@@ -6,9 +6,10 @@
 // result), and of which the blocks with a row are counted through.  What a row has not chosen is masked, so that a block is read once
 // however many rows have it.  The list's keys are numbered through (all of its blocks are whole but the last, which may be the
 // sequence's last) and cut into as many runs as the batch's cut says, which knows only how many blocks the rows may have chosen: as
-// many as if each had chosen its number at random.  (Lists made by a kernel before, and a cut by their lengths: 4.5 us for that
-// kernel, and another load before the first key: sixteen users' tokens on sixteen blocks of 512 53.3 us, 48.5 so;
-// one token on twelve of 4096 46.2 and 43.0.)
+// many as if each had chosen its number at random.  (Half way
+// to all of them choosing alike: sixteen users' tokens below 50.6 us.)  (Lists made by a kernel before, and a cut by their lengths: 4.5 us for that
+// kernel, and another load before the first key: sixteen users' tokens on sixteen blocks of 512 53.3 us, 47.8
+// so; one token on twelve of 4096 46.2 and 41.9.)
 #pragma once
 #include "attn_common.h"
 #include "paged_cut.h"
@@ -60,7 +61,7 @@ __device__ __forceinline__ Share share_of(const Shape<ChosenTable>& p, const Cut
 // + 64 bytes; `list`: in LDS or memory.
 __device__ __forceinline__ int make_list(const Shape<ChosenTable>& shape, const Sequence& seq, int hkv, int row0, int rows_here, char* lds,
                                          Chosen* list) {
-  constexpr int kEach = kWindow / kListThreads, kWaves = kListThreads / 64;
+  constexpr int kWaves = kListThreads / 64;
   uint32_t* const mask = reinterpret_cast<uint32_t*>(lds);
   volatile int* const sums = reinterpret_cast<volatile int*>(lds + 4 * kWindow);   // [kWaves], and the last block
   const ChosenTable& t = shape.table;
@@ -68,8 +69,8 @@ __device__ __forceinline__ int make_list(const Shape<ChosenTable>& shape, const 
   const int keys = keys_of(shape, seq), all = block_keys(t), blocks = keys > 0 ? (keys - 1) / all + 1 : 0;
   int total = 0;
   for (int w0 = 0; w0 < blocks; w0 += kWindow) {
-    const int here = min(kWindow, blocks - w0);
-    for (int i = tid; i < (here + kEach - 1) / kEach * kEach; i += kListThreads) mask[i] = 0;
+    const int here = min(kWindow, blocks - w0), each = (here + kListThreads - 1) / kListThreads;
+    for (int i = tid; i < each * kListThreads; i += kListThreads) mask[i] = 0;
     __syncthreads();
     for (int i = tid; i < rows_here * t.K; i += kListThreads) {
       const int r = i / t.K, row = row0 + r, j = row / shape.rep;
@@ -80,9 +81,7 @@ __device__ __forceinline__ int make_list(const Shape<ChosenTable>& shape, const 
     __syncthreads();
     // each thread its neighbouring blocks
     int mine = 0;
-    if (tid * kEach < here)
-#pragma unroll
-      for (int k = 0; k < kEach; ++k) mine += mask[tid * kEach + k] != 0;
+    for (int k = 0; k < each; ++k) mine += mask[tid * each + k] != 0;
     int upto = (int)upto_sum(mine);
     if (lane == 63) sums[wave] = upto;
     __syncthreads();
@@ -93,14 +92,12 @@ __device__ __forceinline__ int make_list(const Shape<ChosenTable>& shape, const 
       found += sums[w];
     }
     int at = total + upto - mine;
-    if (tid * kEach < here)
-#pragma unroll
-      for (int k = 0; k < kEach; ++k) {
-        const uint32_t who = mask[tid * kEach + k];
-        if (!who) continue;
-        list[at] = {w0 + tid * kEach + k, who};
-        if (++at == total + found) sums[kWaves] = w0 + tid * kEach + k;
-      }
+    for (int k = 0; k < each; ++k) {
+      const uint32_t who = mask[tid * each + k];
+      if (!who) continue;
+      list[at] = {w0 + tid * each + k, who};
+      if (++at == total + found) sums[kWaves] = w0 + tid * each + k;
+    }
     total += found;
     __syncthreads();   // (the list is written; masks and sums have been read)
   }

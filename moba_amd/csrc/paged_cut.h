@@ -80,7 +80,13 @@ __device__ __forceinline__ uint32_t upto_sum(uint32_t x) {
 }
 __device__ __forceinline__ uint32_t wave_sum(uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)upto_sum(x), 63); }
 
-__device__ __forceinline__ int runs_of(int tiles, int run) { return (tiles - 1) / run + 1; }
+// (a whole-number division is some forty instructions; this is exact up to 2^22 tiles, more go that way)
+__device__ __forceinline__ int runs_of(int tiles, int run) {
+  if (__any(tiles > 1 << 22)) return (tiles - 1) / run + 1;
+  int n = (int)((float)(tiles - 1) * __builtin_amdgcn_rcpf((float)run));
+  n += (n + 1) * run <= tiles - 1;
+  return n - (n * run > tiles - 1) + 1;
+}
 
 // the largest of the lanes' x, none of them negative
 __device__ __forceinline__ int wave_max(int x) {
@@ -102,14 +108,11 @@ __device__ __forceinline__ int wave_max(int x) {
 __device__ __forceinline__ int even_run(const Cut& c, int lane, const Share& first, int sequences, int64_t work, int otherwise) {
   constexpr int kParts = 32;
   const int longest = wave_max(first.groups ? first.tiles : 0), run = max((longest - 1) / (min(lane, kParts - 1) + 1) + 1, c.least_tiles);
-  const float inv = 1.f / (float)run;
   int units = 0, long_units = 0;
   for (int b = 0; b < sequences; ++b) {
     const int groups = __builtin_amdgcn_readlane(first.groups, b), tiles = __builtin_amdgcn_readlane(first.tiles, b);
     if (groups == 0) continue;
-    int runs = (int)((float)(tiles - 1) * inv);
-    runs += (runs + 1) * run <= tiles - 1;
-    runs = runs - (runs * run > tiles - 1) + 1;
+    const int runs = runs_of(tiles, run);
     units += groups * runs;
     long_units += 2 * tiles > run * runs ? groups * runs : 0;
   }
