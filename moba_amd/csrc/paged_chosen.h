@@ -5,11 +5,12 @@
 // every block of the sequence, in LDS, a window at a time, into which the rows' entries are or-ed (whatever their order, one
 // result), and of which the blocks with a row are counted through.  What a row has not chosen is masked, so that a block is read once
 // however many rows have it.  The list's keys are numbered through (all of its blocks are whole but the last, which may be the
-// sequence's last) and cut into as many runs as the batch's cut says, which knows only how many blocks the rows may have chosen: as
-// many as if each had chosen its number at random.  (Half way
-// to all of them choosing alike: sixteen users' tokens below 50.6 us.)  (Lists made by a kernel before, and a cut by their lengths: 4.5 us for that
-// kernel, and another load before the first key: sixteen users' tokens on sixteen blocks of 512 53.3 us, 47.8
-// so; one token on twelve of 4096 46.2 and 41.9.)
+// sequence's last) and cut into as many runs as the batch's cut says, which knows only how many blocks the rows may have: about as many
+// as if each had chosen its number at random.
+//
+// One token of 32 heads on 8, twelve blocks of 4096 behind 131072, 8 bits: 41.9 us, some 181 MB; sixteen users' tokens, sixteen blocks of
+// 512, fp16: 47.8.  A kernel before that makes the lists, and a cut by their lengths: 46.2 and 53.3; a cut half way between rows that
+// choose alike and at random: 41.9 and 50.6; more workgroups than fill the chip once: 50 and 54 and more.
 #pragma once
 #include "attn_common.h"
 #include "paged_cut.h"

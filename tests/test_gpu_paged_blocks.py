@@ -185,6 +185,8 @@ CASES = [  # old, new, page, block, n, heads, kv heads, head_dim, dtype, quantiz
     ([30000], [2], 16, 16, 64, 4, 4, 64, FP16, False, 0),
     ([90000], [1], 16, 16, 30, 4, 1, 64, BF16, True, 0),                            # more blocks than a window has
     ([100] * 300, [1] * 300, 16, 32, 2, 8, 8, 64, BF16, True, 0),                   # more units than the chip has places
+    ([20000, 70], [2, 1], 16, 16, 64, 16, 1, 128, BF16, True, 0),                   # longer lists than LDS has room for
+    ([20000], [2], 16, 16, 64, 16, 1, 64, FP16, False, 0),
 ]
 
 

@@ -121,6 +121,65 @@ def test_tables_that_do_not_fit(quantized):
     check_prefix(batch, [], paged_prefix_attention(q.cuda(), cache, table, lengths, cu, ints(2, 2), ints(64)), q)
 
 
+@pytest.mark.parametrize("quantized", [True, False])
+@pytest.mark.parametrize("d", [64, 128])
+def test_large_scores_and_scales(quantized, d):
+    """Scores of hundreds, scales of every size beside each other, negative and zero softmax scales."""
+    from moba_amd import paged_prefix_attention
+    batch = Batch([700, 640, 800, 200], [1, 3, 35, 4], 16, 2, d, BF16, quantized, seed=2)
+    index = share(batch, [(0, 3), (3, 4)], [640, 128])
+    if quantized:
+        batch.scales[1] *= 2.0 ** torch.randint(-60, 60, batch.scales[1].shape, generator=batch.g).float()
+    else:
+        batch.pages[1][::2] *= 2.0 ** 40
+    q = batch.tensors(4)[0] * 30
+    for scaling in (None, -0.1, 0.0, 1.0):
+        got = paged_prefix_attention(q.cuda(), batch.cache(), *batch.index(), *index, scaling=scaling)
+        check_prefix(batch, [(0, 3), (3, 4)], got, q, scaling)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_any_scales(dtype):
+    """Scales that paged_append does not make: no powers of two, negative ones, zero."""
+    from moba_amd import paged_prefix_attention
+    batch = Batch([300, 340, 390], [1, 3, 70], 16, 2, 128, dtype, True, seed=7)
+    index = share(batch, [(0, 3)], [256])
+    for s in batch.scales:
+        s *= torch.rand(s.shape, generator=batch.g) + 0.5
+        s[::5] *= -1
+        s[3::7] = 0
+    q, = batch.tensors(8)
+    for scaling in (None, -0.05):
+        got = paged_prefix_attention(q.cuda(), batch.cache(), *batch.index(), *index, scaling=scaling)
+        check_prefix(batch, [(0, 3)], got, q, scaling)
+
+
+@pytest.mark.parametrize("d,dtype,quantized", [(64, BF16, True), (64, FP16, False), (128, FP16, True), (128, BF16, False)])
+@pytest.mark.parametrize("members,new,heads", [(9, 4, 1), (33, 1, 1), (16, 1, 4), (100, 1, 2), (70, 3, 1), (130, 2, 2)])
+def test_members(members, new, heads, d, dtype, quantized):
+    """Groups of few and of more sequences than a wave has lanes, some without new tokens; rows around those that a workgroup takes."""
+    from moba_amd import paged_prefix_attention
+    count = [0 if i % 7 == 3 else new for i in range(members)]
+    batch = Batch([192 + 5 * (i % 9) for i in range(members)] + [30], count + [1], 16, 1, d, dtype, quantized, seed=members + d)
+    index = share(batch, [(0, members)], [192])
+    q, = batch.tensors(heads)
+    check_prefix(batch, [(0, members)], paged_prefix_attention(q.cuda(), batch.cache(), *batch.index(), *index), q)
+
+
+def test_a_cache_of_more_than_2_31_elements():
+    from moba_amd import PagedKVCache, paged_prefix_attention
+    E4M3 = torch.float8_e4m3fn
+    pages = 2 ** 31 // (8 * 256 * 128) + 2
+    zeros = lambda: torch.zeros((pages, 8, 256, 128), dtype=E4M3, device="cuda")  # noqa: E731
+    cache = PagedKVCache(zeros(), zeros(), *(torch.ones((pages, 8), device="cuda") for _ in range(2)))
+    for i, page in enumerate((pages - 1, 0, pages - 2)):
+        cache.v_pages[page] = torch.full((8, 256, 128), 2.0 + 2 * i, device="cuda").to(E4M3)
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    q = torch.ones((2, 8, 128), dtype=BF16, device="cuda")
+    got = paged_prefix_attention(q, cache, ints(pages - 1, 0, pages - 1, pages - 2).view(2, 2), ints(512, 512), ints(0, 1, 2), ints(0, 2), ints(256))
+    assert (got[0] == 3).all() and (got[1] == 4).all()
+
+
 def test_views_and_nothing():
     from moba_amd import paged_prefix_attention
     batch = Batch([100, 130], [1, 4], 16, 2, 128, BF16, True, seed=6)
