@@ -12,9 +12,10 @@
 // may stop there) with one number of every wave in LDS.  For up to kRowsAtOnce rows it also fills the table and says where the rows
 // belong; more are a second launch of as many workgroups as that takes, which finds ranks and rows in what the first has left.
 // A row's page is looked up where it comes from, the table or the pool's stack, and waits for no entry to be written.  Nothing here
-// is floating point, and no order depends on timing.  Bound by latency: 64 sequences with five tokens each 4.2 us, their way back 4.1
-// (with 64-bit sums by lane shuffles, and rows that waited for the table, 10.4 and 4.9); eight documents of 471000 tokens on 29000
-// pages of 16 tokens 3.1 + 7.5 us, and 16.3 back, whose places on the stack one workgroup counts.
+// is floating point, and no order depends on timing.  Bound by latency: 64 sequences with five tokens each 4.3 us, their way back 3.0
+// (with 64-bit sums by lane shuffles, and rows that waited for the table, 10.4; entries that each look for their sequence, 4.1 back);
+// eight documents of 471000 tokens on 29000 pages of 16 tokens 3.1 + 7.5 us, and 10.1 back (16.3), by one workgroup, as a page's place
+// on the stack is the number of those before it; more entries of a thread on their way at once, 16, are 20.8, four 12.1.
 #include "common.h"
 #include "paged_cut.h"
 
@@ -23,7 +24,7 @@ namespace moba {
 constexpr int kTableThreads = 1024, kTableWaves = kTableThreads / 64;
 constexpr int kMostTableSequences = 8192;   // whose sums fit a workgroup's LDS
 constexpr int kRowsAtOnce = 4096;
-constexpr int kPagesOfThread = 8;           // that a thread moves at a time, where there are more than threads
+constexpr int kPagesOfThread = 8;           // that a thread takes back at a time, where there are more than threads
 
 struct Pool {
   int32_t* free_pages;   // [num_pages]
@@ -186,11 +187,11 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(const TableParams p) {
 
 __global__ __launch_bounds__(kTableThreads) void paged_release_kernel(const TableParams p) {
   __shared__ Two red[2][kTableWaves];
-  __shared__ int counts[2][kPagesOfThread * kTableWaves];
+  __shared__ int counts[2][kTableWaves];
   extern __shared__ int lds[];
   int* const first = lds;                    // [B]: entries that go in the sequences before (their number is below 2^31)
   int* const stay = first + p.B;             // [B]: pages that stay
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int free_count = min(max(*p.pool.free_count, 0), p.pool.num_pages), total = 0, parity = 0;
   for (int b0 = 0; b0 < p.B; b0 += kTableThreads, parity ^= 1) {
     const int b = b0 + tid;
@@ -209,48 +210,50 @@ __global__ __launch_bounds__(kTableThreads) void paged_release_kernel(const Tabl
     total += (int)s.all.a;
   }
   __syncthreads();
-  // From the last entry to the first, so that a place on the stack is the number of pages that have come before.  Entry k * kTableThreads +
-  // thread of a step is number k of a thread.
-  for (int64_t r0 = 0; r0 < total; r0 += kTableThreads * kPagesOfThread, parity ^= 1) {
-    int id[kPagesOfThread], before[kPagesOfThread];
+  // From the last entry to the first, so that a place on the stack is the number of pages that have come before.  A wave has neighbouring
+  // entries, up to kPagesOfThread times its lanes of a step, and seldom has to look for their sequence.  (One compute unit's instructions are
+  // what bounds it.)
+  const int each = min((total + kTableThreads - 1) / kTableThreads, kPagesOfThread);
+  int begin = 0, end = 0;          // entries of the sequence at hand
+  int32_t* entries = nullptr;      // where entry 0 would be if all were its
+  for (int64_t r0 = 0; r0 < total; r0 += kTableThreads * each, parity ^= 1) {
+    int id[kPagesOfThread], found = 0;
+    uint64_t valid[kPagesOfThread];
+    const int last = (int)max(total - 1 - r0 - wave * each * 64 - lane, (int64_t)-1);
 #pragma unroll
     for (int k = 0; k < kPagesOfThread; ++k) {
-      const int64_t r = r0 + k * kTableThreads + tid;
+      if (k >= each) break;
+      const int i = last - k * 64;
       id[k] = -1;
-      if (r < total) {
-        const int i = total - 1 - (int)r, b = last_at_most(first, p.B, i);
-        int32_t* const entry = p.table + b * p.stride + stay[b] + i - first[b];
-        id[k] = *entry;
-        *entry = -1;
+      if (i >= 0) {
+        if (i < begin || i >= end) {
+          const int b = last_at_most(first, p.B, i);
+          begin = first[b];
+          end = b + 1 < p.B ? first[b + 1] : total;
+          entries = p.table + (b * p.stride + stay[b] - begin);
+        }
+        id[k] = entries[i];
+        entries[i] = -1;
       }
     }
 #pragma unroll
     for (int k = 0; k < kPagesOfThread; ++k) {
-      const uint64_t m = __ballot(id[k] >= 0 && id[k] < p.pool.num_pages);
-      before[k] = __builtin_popcountll(m & ((1ull << lane) - 1));
-      if (lane == 0) counts[parity][k * kTableWaves + wave] = __builtin_popcountll(m);
+      if (k >= each) break;
+      valid[k] = __ballot((uint32_t)id[k] < (uint32_t)p.pool.num_pages);
+      found += __builtin_popcountll(valid[k]);
     }
+    if (lane == 0) counts[parity][wave] = found;
     __syncthreads();
-    // sums of the counts, each wave for itself
-    constexpr int kCounts = kPagesOfThread * kTableWaves, kEach = (kCounts + 63) / 64;
-    int x[kEach], sum = 0;
-#pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-      x[j] = lane * kEach + j < kCounts ? counts[parity][lane * kEach + j] : 0;
-      sum += x[j];
-    }
-    const int upto = (int)upto_sum((uint32_t)sum), all = __builtin_amdgcn_readlane(upto, 63);
+    const int mine = lane < kTableWaves ? counts[parity][lane] : 0, upto = (int)upto_sum((uint32_t)mine);
+    int64_t place = (int64_t)free_count + __builtin_amdgcn_readlane(upto - mine, wave);
 #pragma unroll
     for (int k = 0; k < kPagesOfThread; ++k) {
-      const int at = k * kTableWaves + wave, in_lane = at % kEach;
-      int place = __builtin_amdgcn_readlane(upto - sum, at / kEach);
-#pragma unroll
-      for (int j = 0; j < kEach; ++j)
-        if (j < in_lane) place += __builtin_amdgcn_readlane(x[j], at / kEach);
-      const int64_t to = (int64_t)free_count + place + before[k];
-      if (id[k] >= 0 && id[k] < p.pool.num_pages && to < p.pool.num_pages) p.pool.free_pages[to] = id[k];   // (more than there are: named twice)
+      if (k >= each) break;
+      const int64_t to = place + __builtin_popcountll(valid[k] & ((1ull << lane) - 1));
+      if ((valid[k] >> lane & 1) && to < p.pool.num_pages) p.pool.free_pages[to] = id[k];   // (more than there are: named twice)
+      place += __builtin_popcountll(valid[k]);
     }
-    free_count = (int)min((int64_t)free_count + all, (int64_t)p.pool.num_pages);
+    free_count = (int)min((int64_t)free_count + __builtin_amdgcn_readlane(upto, 63), (int64_t)p.pool.num_pages);
   }
   if (tid == 0) *p.pool.free_count = free_count;
 }
@@ -279,12 +282,15 @@ extern "C" size_t moba_paged_reserve_workspace_bytes(int B, int64_t rows) {
 }
 
 extern "C" int moba_paged_reserve(int32_t* free_pages, int32_t* free_count, int32_t* page_table, int32_t* lengths,
-                                  const int32_t* new_tokens, int32_t* cu_new, int32_t* owners, int32_t* positions, int64_t* slots, void* workspace,
-                                  int B, int64_t rows, int page_size, int64_t num_pages, int64_t max_pages, int64_t table_stride, void* stream) {
+                                  const int32_t* new_tokens, int32_t* cu_new, int32_t* owners, int32_t* positions, int64_t* slots,
+                                  void* workspace, int B, int64_t rows, int page_size, int64_t num_pages, int64_t max_pages,
+                                  int64_t table_stride, void* stream) {
   TableParams p;
   const int rc = check_tables(p, free_pages, free_count, page_table, lengths, new_tokens, B, page_size, num_pages, max_pages, table_stride);
   if (rc != MOBA_OK) return rc;
-  if (!cu_new || rows < 0 || (rows > kRowsAtOnce && !workspace) || (rows && (!owners || !positions || !slots)) || ((uintptr_t)slots & 7) || ((uintptr_t)workspace & 3)) return MOBA_ERR_ARG;
+  if (!cu_new || rows < 0 || (rows > kRowsAtOnce && !workspace) || (rows && (!owners || !positions || !slots)) || ((uintptr_t)slots & 7) ||
+      ((uintptr_t)workspace & 3))
+    return MOBA_ERR_ARG;
   if (rows >= 1LL << 30) return MOBA_ERR_LIMIT;
   p.cu_new = cu_new; p.owners = owners; p.positions = positions; p.slots = slots; p.ranks = (int32_t*)workspace;
   p.rows = (int)rows;
