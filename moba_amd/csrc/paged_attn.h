@@ -205,11 +205,11 @@ constexpr int few_list_at() {
 template <int D, bool k8, class Table>
 constexpr int few_lds_bytes() { return few_list_at<D, k8>() + (kChooses<Table> ? kListBytes : 0); }
 
-// Position of new token j of a unit's rows, every lane its own; the least of a wave's 32 rows' (whose first is row0)
-__device__ __forceinline__ int position_at(const PageTable&, const Unit& u, int j) { return (int)u.seq.length - (u.seq.hi - u.seq.lo) + j; }
-__device__ __forceinline__ int least_position(const PageTable& t, const Unit& u, int first, int) { return position_at(t, u, first); }
+// Position of new token j of a unit's rows, every lane its own (mine: the lane's sequence of find_unit()); the least of a wave's 32 rows'
+__device__ __forceinline__ int position_at(const PageTable&, const Unit& u, int j, const Sequence&) { return (int)u.seq.length - (u.seq.hi - u.seq.lo) + j; }
+__device__ __forceinline__ int least_position(const PageTable& t, const Unit& u, int first, int) { return position_at(t, u, first, u.seq); }
 // the last key that new tokens up to j of a unit's rows see
-__device__ __forceinline__ int last_seen(const PageTable& t, const Unit& u, int j) { return position_at(t, u, j); }
+__device__ __forceinline__ int last_seen(const PageTable& t, const Unit& u, int j) { return position_at(t, u, j, u.seq); }
 
 // kChooses: where a workgroup's list of blocks lies
 __device__ __forceinline__ int list_of(const PageTable&, char*) { return 0; }
@@ -236,10 +236,11 @@ __global__ __launch_bounds__(64 * kFewWaves, kSets > 1 && D == 128 ? 1 : 2) void
   const auto& table = shape.table;
   Unit unit;
   int hkv, item;
-  if (!find_unit(shape, p.few, lane, unit, hkv, item)) return;
+  Share share;
+  if (!find_unit(shape, p.few, lane, unit, hkv, item, share)) return;
   const Sequence seq = unit.seq;
   if (unit.run == 0 && unit.group == 0 && hkv == 0 && tid == 0) p.runs[item] = {unit.first, unit.runs, unit.groups};
-  const int b = table_row(table, unit.b);
+  const int b = unit.row;
   const int count = seq.hi - seq.lo, rows = count * shape.rep, row0 = unit.group * kFewRows * kSets;
   int keys, tiles = unit.tiles;   // kChooses: of the list
   decltype(list_of(table, smem)) list = list_of(table, smem + few_list_at<D, k8>());
@@ -260,7 +261,7 @@ __global__ __launch_bounds__(64 * kFewWaves, kSets > 1 && D == 128 ? 1 : 2) void
     const int first = min(row0 + q * kFewRows, rows - 1), row = min(first + n, rows - 1);   // (rows past the last repeat it and are not written)
     j[q] = row / shape.rep;
     g[q] = row - j[q] * shape.rep;
-    const int position = position_at(table, unit, j[q]);
+    const int position = position_at(table, unit, j[q], share.seq);
     limit[q] = kChooses<Table> ? position : min(position, key_hi - 1);
     first_masked[q] = least_position(table, unit, first / shape.rep, position);
     if constexpr (!kChooses<Table>) first_masked[q] = min(first_masked[q], key_hi - 1);
@@ -683,11 +684,12 @@ __global__ __launch_bounds__(64 * (kManyWaves<D, k8>), 2) void paged_many_kernel
   const auto& table = shape.table;
   Unit unit;
   int hkv, item;
-  if (!find_unit(shape, p.many, lane, unit, hkv, item)) return;
+  Share share;
+  if (!find_unit(shape, p.many, lane, unit, hkv, item, share)) return;
   const Sequence seq = unit.seq;
   const int keys = keys_of(shape, seq);
   if (unit.run == 0 && unit.group == 0 && hkv == 0 && tid == 0) p.runs[item] = {unit.first, unit.runs, unit.groups};
-  const int b = table_row(table, unit.b);
+  const int b = unit.row;
   // (the group with the most keys first)
   const int count = seq.hi - seq.lo, rows = count * shape.rep, row0 = (unit.groups - 1 - unit.group) * kRows;
   const int per = (unit.tiles + unit.runs - 1) / unit.runs;
@@ -698,7 +700,7 @@ __global__ __launch_bounds__(64 * (kManyWaves<D, k8>), 2) void paged_many_kernel
   const int wave_row = row0 + 32 * wave;
   const int row = min(wave_row + n, rows - 1);
   const int j = row / shape.rep, g = row - j * shape.rep;
-  const int position = position_at(table, unit, j);
+  const int position = position_at(table, unit, j, share.seq);
   const int limit = min(position, key_hi - 1);
   const int first_masked = min(least_position(table, unit, min(wave_row, rows - 1) / shape.rep, position), key_hi - 1);
   const int tiles = (key_hi - key_lo + kManyKeys - 1) / kManyKeys;
@@ -1126,9 +1128,6 @@ __global__ __launch_bounds__(64 * (kManyWaves<D, k8>), 2) void paged_many_kernel
   }
 }
 
-// `heads` heads of a token, one after the other, for kShare waves, a lane for D / 64 elements.  Four waves (few tokens, which may
-// have many runs) take a quarter of the runs each, their sums meet in LDS; one wave needs neither.  Rows of one run are there already.
-// Bound by its chain of reads (sequence, its number of runs, log-sum-exps and rows): 4.7 us for one token.
 // Where the parts of a row lie: `runs` of them, row `first` + i * `step` of part_o and part_lse each
 struct Parts {
   const float *o, *lse;
@@ -1185,6 +1184,9 @@ struct MergeToken {
   }
 };
 
+// `heads` heads of a token, one after the other, for kShare waves, a lane for D / 64 elements.  Four waves (few tokens, which may
+// have many runs) take a quarter of the runs each, their sums meet in LDS; one wave needs neither.  Rows of one run are there already.
+// Bound by its chain of reads (sequence, its number of runs, log-sum-exps and rows): 4.7 us for one token.
 template <class E, int D, int kShare, class Table>
 __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams<E, Table> p, int heads) {
   typedef typename E::elem elem;

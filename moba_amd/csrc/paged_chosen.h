@@ -48,7 +48,7 @@ __device__ __forceinline__ float chosen_blocks(float blocks, float k, float rows
 }
 __device__ __forceinline__ Share share_of(const Shape<ChosenTable>& p, const Cut& c, const Sequence& s) {
   const int rows = (s.hi - s.lo) * p.rep, keys = keys_of(p, s);
-  Share r = {s, 0, 0};
+  Share r = {s, 0, 0, 0};
   if (rows > 0 && keys > 0) {
     const int all = block_keys(p.table);
     const float some = chosen_blocks((float)((keys - 1) / all + 1), (float)p.table.K, (float)min(rows, kChosenRows)) * (float)all;

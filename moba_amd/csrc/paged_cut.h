@@ -29,23 +29,22 @@ constexpr int kWholeRun = 0x3fffffff;  // tiles
 // long one among them: one token each for 255 sequences, 131072 keys and 254 of 513, 8 heads, 8 bits: 120 us; one more of these: 1135.
 constexpr int kWholeAt = 4;
 
-// Table: PageTable, or another that has its own count_of(), sequence_of(), table_row() and `kShares`
+// Table: PageTable, or another that has its own count_of(), sequence_of() and share_at(), and kShares or kChooses
 template <class Table>
 struct Shape {
   Table table;
   int H, Hkv, rep;
 };
 __device__ __forceinline__ int count_of(const PageTable& t) { return t.B; }                // sequences
-__device__ __forceinline__ int table_row(const PageTable& t, int b) { return b; }          // a sequence's row of the page table
 template <class Table>
 constexpr bool kShares = false;   // whether a token attends keys of more than one sequence
 template <class Table>
 constexpr bool kChooses = false;  // whether a row attends some of the keys only
 
-// A sequence's part in a cut: groups of rows (0: none of its units are of this cut), tiles of keys
+// A sequence's part in a cut: groups of rows (0: none of its units are of this cut), tiles of keys; kShares: its row of the page table
 struct Share {
   Sequence seq;
-  int groups, tiles;
+  int groups, tiles, row;
 };
 // the end of a sequence's keys
 template <class Table>
@@ -53,7 +52,7 @@ __device__ __forceinline__ int keys_of(const Shape<Table>& p, const Sequence& s)
 template <class Table>
 __device__ __forceinline__ Share share_of(const Shape<Table>& p, const Cut& c, const Sequence& s) {
   const int rows = (s.hi - s.lo) * p.rep, keys = keys_of(p, s) - s.begin;
-  Share r;
+  Share r = {};
   r.seq = s;
   r.tiles = keys > 0 ? (keys - 1) / c.tile_keys + 1 : 0;
   r.groups = rows > c.rows_over && rows <= c.rows_up_to && keys > 0 ? (rows - 1) / c.group_rows + 1 : 0;
@@ -62,7 +61,7 @@ __device__ __forceinline__ Share share_of(const Shape<Table>& p, const Cut& c, c
 // of sequence b, each lane its own
 template <class Table>
 __device__ __forceinline__ Share share_at(const Shape<Table>& p, const Cut& c, int b) {
-  if (b >= count_of(p.table)) return {{0, 0, 0, 0}, 0, 0};
+  if (b >= count_of(p.table)) return {};
   return share_of(p, c, sequence_of(p.table, b));
 }
 
@@ -154,7 +153,7 @@ __device__ __forceinline__ int run_tiles(const Shape<Table>& p, const Cut& c, in
 
 struct Unit {
   Sequence seq;
-  int b, group, run, runs, groups, tiles, first;  // tiles: of the sequence; first: number of the sequence's first unit
+  int b, row, group, run, runs, groups, tiles, first;  // row: of the page table; tiles: of the sequence; first: number of the sequence's first unit
 };
 // unit number u: all groups of a sequence's first run, then of its second, ...; b = -1 past the last.  kShares, up to 64 sequences: those
 // with long runs first, so that none of these is left for the end (pieces of 200, 300, 301 and 97 tokens behind 12288 shared ones: 315 us
@@ -181,6 +180,7 @@ __device__ __forceinline__ Unit unit_at(const Shape<Table>& p, const Cut& c, int
       auto of = [&](int x) { return __builtin_amdgcn_readlane(x, at); };
       Unit r;
       r.b = b0 + at;
+      r.row = kShares<Table> ? of(s.row) : r.b;
       r.seq.lo = of(s.seq.lo);
       r.seq.hi = of(s.seq.hi);
       r.seq.length = of((int)s.seq.length);
@@ -203,12 +203,12 @@ __device__ __forceinline__ Unit unit_at(const Shape<Table>& p, const Cut& c, int
 }
 
 // The unit of a workgroup, its key/value head, and the number under which it leaves what the merge has to know; false: none.  Workgroups
-// are numbered by unit and head.
+// are numbered by unit and head.  first: share_at() of the lanes.
 template <class Table>
-__device__ __forceinline__ bool find_unit(const Shape<Table>& p, const Cut& c, int lane, Unit& unit, int& hkv, int& item) {
+__device__ __forceinline__ bool find_unit(const Shape<Table>& p, const Cut& c, int lane, Unit& unit, int& hkv, int& item, Share& first) {
   const int u = (int)blockIdx.x / p.Hkv;
   hkv = (int)blockIdx.x - u * p.Hkv;
-  const Share first = share_at(p, c, lane);
+  first = share_at(p, c, lane);
   const int run = run_tiles(p, c, lane, first);
   if (run == 0) return false;   // (no work at all)
   unit = unit_at(p, c, u, run, lane, first);

@@ -36,9 +36,6 @@ __device__ __forceinline__ int group_of(const SharedTable& t, int b) {
 }
 
 __device__ __forceinline__ int count_of(const SharedTable& t) { return t.G + t.B; }
-__device__ __forceinline__ int table_row(const SharedTable& t, int v) {
-  return __builtin_amdgcn_readfirstlane(v < t.G ? min(first_member(t, v), t.B - 1) : v - t.G);
-}
 __device__ __forceinline__ Sequence sequence_of(const SharedTable& t, int v) {
   Sequence s;
   if (v < t.G) {
@@ -59,7 +56,12 @@ __device__ __forceinline__ Sequence sequence_of(const SharedTable& t, int v) {
 // say of each other goes from lane to lane.
 __device__ __forceinline__ Share share_at(const Shape<SharedTable>& p, const Cut& c, int b) {
   const SharedTable& t = p.table;
-  if (count_of(t) > 64) return b < count_of(t) ? share_of(p, c, sequence_of(t, b)) : Share{{0, 0, 0, 0}, 0, 0};
+  if (count_of(t) > 64) {
+    if (b >= count_of(t)) return {};
+    Share r = share_of(p, c, sequence_of(t, b));
+    r.row = b < t.G ? min(first_member(t, b), t.B - 1) : b - t.G;
+    return r;
+  }
   const bool group = b < t.G;
   const int first = t.cu_groups[min(b, t.G)], end = t.cu_groups[min(b + 1, t.G)], front = group ? shared_keys(t, b) : 0;
   Sequence s = sequence_of(static_cast<const PageTable&>(t), min(max(b - t.G, 0), t.B - 1));
@@ -75,32 +77,35 @@ __device__ __forceinline__ Share share_at(const Shape<SharedTable>& p, const Cut
     }
   }
   const int g_first = __shfl(first, g, 64), g_end = __shfl(end, g, 64), g_front = __shfl(front, g, 64);
-  if (b >= count_of(t)) return {{0, 0, 0, 0}, 0, 0};
+  if (b >= count_of(t)) return {};
   if (group) {
     s = {lo, m1 > m0 ? max(hi, lo) : lo, front, 0};
   } else {
     s.begin = g_first <= b - t.G && b - t.G < g_end ? (int)min((int64_t)g_front, min(s.length, room(t))) : 0;
   }
-  return share_of(p, c, s);
+  Share r = share_of(p, c, s);
+  r.row = group ? min(m0, t.B - 1) : b - t.G;
+  return r;
 }
 
-// Position of new token j of a unit's rows: in its own sequence, the last member of the group that begins no later.  With the whole wave:
-// up to 64 members are asked for at once, and searched among the lanes.
-__device__ __forceinline__ int position_at(const SharedTable& t, const Unit& u, int j) {
+// Position of new token j of a unit's rows: in its own sequence, the last that begins no later.  With the whole wave, whose lanes have
+// groups and sequences that are 64 together at most.
+__device__ __forceinline__ int position_at(const SharedTable& t, const Unit& u, int j, const Sequence& mine) {
   if (u.b >= t.G) return (int)u.seq.length - (u.seq.hi - u.seq.lo) + j;
-  const int token = u.seq.lo + j, first = first_member(t, u.b), end = min(t.cu_groups[u.b + 1], t.B);
-  int lo = 0, hi = end - first;
-  if (hi <= 64) {
-    const Sequence s = sequence_of(static_cast<const PageTable&>(t), min(first + ((int)threadIdx.x & 63), t.B - 1));
-    while (__any(hi - lo > 1)) {
-      const int mid = (lo + hi) >> 1, begins = __shfl(s.lo, mid, 64);
-      if (hi - lo > 1) {
-        if (begins <= token) lo = mid; else hi = mid;
+  const int token = u.seq.lo + j;
+  if (count_of(t) <= 64) {
+    int lo = 0;
+    for (int above = t.B; __any(above - lo > 1);) {
+      const int mid = (lo + above) >> 1, begins = __shfl(mine.lo, t.G + mid, 64);
+      if (above - lo > 1) {
+        if (begins <= token) lo = mid; else above = mid;
       }
     }
-    const int ends = __shfl(s.hi, lo, 64), length = __shfl((int)s.length, lo, 64);
+    const int ends = __shfl(mine.hi, t.G + lo, 64), length = __shfl((int)mine.length, t.G + lo, 64);
     return (int)min((int64_t)length - ends + token, (int64_t)0x7fffffff);
   }
+  const int first = first_member(t, u.b), end = min(t.cu_groups[u.b + 1], t.B);
+  int lo = 0, hi = end - first;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (t.cu_new[first + mid] <= token) lo = mid; else hi = mid;
@@ -110,13 +115,13 @@ __device__ __forceinline__ int position_at(const SharedTable& t, const Unit& u, 
 }
 // (a group's rows are of several sequences)
 __device__ __forceinline__ int least_position(const SharedTable& t, const Unit& u, int first, int position) {
-  if (u.b >= t.G) return position_at(t, u, first);
+  if (u.b >= t.G) return position_at(t, u, first, u.seq);
 #pragma unroll
   for (int d = 16; d >= 1; d >>= 1) position = min(position, __shfl_xor(position, d, 64));
   return __builtin_amdgcn_readfirstlane(position);
 }
 __device__ __forceinline__ int last_seen(const SharedTable& t, const Unit& u, int j) {
-  return u.b >= t.G ? position_at(t, u, j) : 0x7ffffffe;
+  return u.b >= t.G ? position_at(t, u, j, u.seq) : 0x7ffffffe;
 }
 
 }  // namespace moba
