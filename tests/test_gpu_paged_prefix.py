@@ -38,6 +38,8 @@ CASES = [  # groups (first, end), shared, old, new, page, heads, kv heads, head_
      BF16, True, 0),                                                                               # more sequences than a wave has lanes
     ([(0, 2)], [40000], [40000, 40100], [1, 2], 64, 8, 2, 128, BF16, True, 0),                     # several runs of the shared keys
     ([(0, 2)], [48], [48, 60], [1, 1], 16, 4, 2, 64, BF16, True, 0),                               # less than a tile is shared
+    ([(0, 3), (3, 5)], [640, 128], [700, 640, 900, 128, 4000], [300, 40, 1, 170, 12], 64, 33, 3, 128, BF16, True, 4),   # rows of many runs
+    ([(0, 3), (3, 5)], [640, 128], [700, 640, 900, 128, 9000], [300, 40, 1, 170, 12], 64, 33, 3, 64, FP16, False, 4),
 ]
 
 
