@@ -236,8 +236,8 @@ PyObject* py_paged_reserve(PyObject*, PyObject* const* args, Py_ssize_t n) {
     Tensor space;
     if (need) space = bytes(need, device);
     check(reserve_call(t.of(t.free_pages), t.of(t.free_count), t.of(t.table), t.of(t.lengths), t.of(t.asked), t.of(out[0]), t.of(out[1]),
-                       t.of(out[2]), (int64_t*)out[3].mutable_data_ptr(), mutable_pointer(space), (int)b, rows, (int)t.page, t.free_pages.size(0), t.table.size(1),
-                       t.table.stride(0), stream_of(t.lengths)),
+                       t.of(out[2]), (int64_t*)out[3].mutable_data_ptr(), mutable_pointer(space), (int)b, rows, (int)t.page,
+                       t.free_pages.size(0), t.table.size(1), t.table.stride(0), stream_of(t.lengths)),
           "moba_paged_reserve");
     for (const Tensor& x : {t.free_count, t.table, t.lengths}) written(x);
   }
@@ -276,8 +276,8 @@ PyObject* py_paged_release(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 // bind_serving(addresses of moba_paged_prefix_attention, .._workspace_bytes, moba_paged_block_attention, .._workspace_bytes,
-// moba_paged_key_sums, moba_paged_select_blocks, .._workspace_bytes, moba_paged_reserve, .._workspace_bytes, moba_paged_release), of the library whose
-// version bind() has checked
+// moba_paged_key_sums, moba_paged_select_blocks, .._workspace_bytes, moba_paged_reserve, .._workspace_bytes, moba_paged_release), of the
+// library whose version bind() has checked
 PyObject* py_bind_serving(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   TORCH_CHECK_TYPE(n == 10, "bind_serving takes ten addresses");

@@ -26,6 +26,9 @@
 //   paged_few_kernel    one run of keys: out itself; several: the run's rows (normalised) and their log-sum-exps (base 2)
 //   paged_many_kernel   the same for sequences of more rows
 //   paged_merge_kernel  the runs of a row together; zeros where there is nothing to see
+//
+// Table says what a sequence attends: PageTable all of its keys, SharedTable (paged_shared.h) what it has in common with its neighbours
+// together with them, ChosenTable (paged_chosen.h) some blocks.
 #pragma once
 #include "attn_common.h"
 #include "paged_cut.h"

@@ -9,11 +9,15 @@
 // should not depend on the order in which a sum is formed: products of 24 and 11 bits are exact, and blocks of equal sums have equal
 // scores.
 //
-// All three kernels are bound by memory or latency.  Sums: the keys of the pages that have received tokens, once.  Scores: the
-// sums of the history's pages once for up to 16 rows (tokens times heads) of a key/value head; a workgroup's threads take 16 bytes of
-// a page each, so that a whole block of many pages is on its way at once.  Selection: the scores of a row stay in registers, as whole
-// numbers in the same order, of which the (topk - 1)-th largest is found bit by bit: a comparison and a count for each of a lane's
-// scores and bit, until the count is right (some 20 bits).
+// All three kernels are bound by memory or latency.
+//   Sums       the keys of the pages that have received tokens, once: 131072 tokens, 8 heads, 8 bits: 143 MB in 23.3 us, 6.1 TB/s; the next
+//              token of 16 sequences 6.0.
+//   Scores     the sums of the history's pages once for up to 32 rows (tokens times heads) of a key/value head; a workgroup's threads
+//              take 16 bytes of a page each, so that a whole block of many pages is on its way at once.  32 heads on 8, blocks of 4096
+//              behind 131072: 6.4 us; 16 sequences of five tokens, blocks of 512, 15 MB: 12.9.
+//   Selection  the scores of a row stay in registers, as whole numbers in the same order, of which the (topk - 1)-th largest is found
+//              bit by bit: a comparison and a count for each of a lane's scores and bit, until the count is right (some 20 bits).
+//              3.9 and 5.8 us of these.
 #include "attn_common.h"
 #include "paged_cut.h"
 
@@ -26,10 +30,12 @@ struct SumParams {
   const char* pages;
   const float* scales;   // 8-bit pages
   float* sums;           // [num_pages, Hkv, D]
-  int Hkv, items;   // waves
+  int Hkv, items;        // waves
 };
 
-// One wave to kHeads heads of a page: 64 / L tokens at a time, L lanes of 16 bytes to a token, the heads' steps on their way together.
+// One wave to kHeads heads of a page: 64 / L tokens at a time, L lanes of 16 bytes to a token, the heads' steps on their way together.  Two
+// heads where that leaves the chip enough waves (131072 tokens as above: 30 us with one); loads of the next step before the sums of this
+// one took 52.
 template <class E, int D, bool k8, int kHeads>
 __global__ __launch_bounds__(256) void paged_key_sums_kernel(const SumParams<E> p) {
   constexpr int kRow = D * (k8 ? 1 : 2), L = kRow / 16, kTokens = 64 / L, kElems = k8 ? 16 : 8, kAhead = 8;
@@ -361,7 +367,7 @@ __global__ __launch_bounds__(kWaves == 1 ? 256 : 64 * kWaves) void paged_pick_ke
   if (tid < s.topk && tid >= count) out[tid] = tid == count && own < s.blocks ? (int)own : -1;
 }
 
-static constexpr int64_t kScoreBytes = 1LL << 29;   // of a launch's scores
+static constexpr int64_t kScoreBytes = 1LL << 29;   // of a launch's scores: more tokens are several launches
 constexpr int kMostTopk = 64;
 
 static int blocks_of(int64_t max_pages, int each) { return (int)((max_pages + each - 1) / each); }
@@ -423,7 +429,8 @@ extern "C" int moba_paged_key_sums(const void* k_pages, const float* k_scales, f
   const int64_t units = (T >> page_log2) + 2 * (int64_t)B;   // (sequence b's pages are numbered from (its first row / page_size) + 2b on)
   const int heads = Hkv > 1 && units * Hkv >= 8192 ? 2 : 1;
   const int64_t items = units * ((Hkv + heads - 1) / heads);
-  if (units * Hkv >= 1LL << 31 || T >= 1LL << 30 || num_pages >= 1LL << 31 || max_pages >= 1LL << 31 || items >= 1LL << 25) return MOBA_ERR_LIMIT;   // (2^32 threads)
+  if (units * Hkv >= 1LL << 31 || T >= 1LL << 30 || num_pages >= 1LL << 31 || max_pages >= 1LL << 31 || items >= 1LL << 25)
+    return MOBA_ERR_LIMIT;   // (2^32 threads)
   LaunchCheck launch_check;
   auto launch = [&](auto e, auto d, auto c8) {
     typedef decltype(e) E;
