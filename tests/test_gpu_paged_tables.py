@@ -85,6 +85,51 @@ def test_long_prompts():
     check_release(free, 20000, table, [80000, 77, 31999], [17, 80, 0], 16)
 
 
+@pytest.mark.parametrize("lengths,keep", [([144000, 143999, 144000], [0, 0, 0]), ([144000, 0, 9, 130000], [17, 0, 0, 16]), ([16] * 5000 + [100000], [0] * 5001),
+                                          ([1, 0, 33] * 2000 + [100000], [0, 0, 17] * 2000 + [99])])
+def test_many_pages_back(lengths, keep):
+    """More than one step takes, of long sequences, of many short ones, and of both; some entries name no page."""
+    rng = random.Random(len(lengths))
+    wide = max(-(-n // 16) for n in lengths)
+    held = [-(-n // 16) for n in lengths]
+    ids = rng.sample(range(30000), sum(held))
+    table = []
+    for n in held:
+        row = [ids.pop() if rng.random() < 0.9 else rng.choice((-1, 30000, 2 ** 31 - 1, -2 ** 31)) for _ in range(n)]
+        table.append(row + [-1] * (wide - n))
+    check_release([5] * 30000, 100, table, lengths, keep, 16)
+    check_release([5] * 30000, 29000, table, lengths, keep, 16)
+
+
+def test_no_rows():
+    """Without rows nobody gets tokens; sequences that want none are as they were."""
+    check_reserve([3, 2, 1, 0], 4, [[-1, -1], [9, -1]], [0, 16], [1, 0], 0, 16)
+    check_reserve([3, 2, 1, 0], 4, [[-1, -1], [9, -1]], [0, 16], [0, 0], 0, 16)
+
+
+def test_a_captured_prompt():
+    """Many rows: the second launch's workspace is the graph's own."""
+    from moba_amd import paged_release, paged_reserve
+    free, count, table, lengths, _, _ = case(3, 1000, 16, 2500, 5)
+    pool, t, n, wanted = pool_of(free, count, 16), ints(table), ints(lengths), ints([0, 0, 0])
+    kept = n.clone()
+    paged_reserve(pool_of(free, count, 16), t.clone(), n.clone(), wanted, 9000)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = paged_reserve(pool, t, n, wanted, 9000)
+        full = t.clone()
+        paged_release(pool, t, n, kept)
+    for new in ([5000, 16, 3000], [0, 0, 0], [1, 9000, 1], [4095, 2, 0]):
+        wanted.copy_(torch.tensor(new))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        _, after, _, *want = reserved(free, count, table, lengths, new, 9000, 16)
+        assert all(x.tolist() == w for x, w in zip(out, want)) and full.tolist() == after, new
+        assert t.tolist() == table and n.tolist() == lengths and pool.free_count.tolist() == [count], new
+
+
 def test_what_does_not_fit():
     free = list(range(20))
     row = [3, -1, 99, 4]
