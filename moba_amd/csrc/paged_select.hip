@@ -10,8 +10,8 @@
 // scores.
 //
 // All three kernels are bound by memory or latency.
-//   Sums       the keys of the pages that have received tokens, once: 131072 tokens, 8 heads, 8 bits: 143 MB in 23.3 us, 6.1 TB/s; the next
-//              token of 16 sequences 6.0.
+//   Sums       the keys of the pages that have received tokens, once: 131072 tokens, 8 heads, 8 bits: 143 MB in 22.7 us where they are in
+//              the last-level cache, 30 where they are not; the next token of 16 sequences 3.8.
 //   Scores     the sums of the history's pages once for up to 32 rows (tokens times heads) of a key/value head; a workgroup's threads
 //              take 16 bytes of a page each, so that a whole block of many pages is on its way at once.  32 heads on 8, blocks of 4096
 //              behind 131072: 6.4 us; 16 sequences of five tokens, blocks of 512, 15 MB: 12.9.
@@ -33,17 +33,17 @@ struct SumParams {
   int Hkv, items;        // waves
 };
 
-// One wave to kHeads heads of a page: 64 / L tokens at a time, L lanes of 16 bytes to a token, the heads' steps on their way together.  Two
-// heads where that leaves the chip enough waves (131072 tokens as above: 30 us with one); loads of the next step before the sums of this
-// one took 52.
-template <class E, int D, bool k8, int kHeads>
+// One wave to a page and head: 64 / L tokens at a time, L lanes of 16 bytes to a token, kAhead such steps on their way together.  (Eight of
+// them: 22.4 us for 131072 tokens as above, 22.7 so, but 8192 on pages of 16 6.3 and 5.0.  Two heads to a wave: 23.6 and 4.9, and the next
+// token of 16 sequences 4.3.)
+template <class E, int D, bool k8>
 __global__ __launch_bounds__(256) void paged_key_sums_kernel(const SumParams<E> p) {
-  constexpr int kRow = D * (k8 ? 1 : 2), L = kRow / 16, kTokens = 64 / L, kElems = k8 ? 16 : 8, kAhead = 8;
+  constexpr int kRow = D * (k8 ? 1 : 2), L = kRow / 16, kTokens = 64 / L, kElems = k8 ? 16 : 8, kAhead = 4;
   const int lane = threadIdx.x & 63;
   const int item = __builtin_amdgcn_readfirstlane((int)blockIdx.x * 4 + (threadIdx.x >> 6));
   if (item >= p.items) return;
   const PageTable& table = p.table;
-  const int parts = (p.Hkv + kHeads - 1) / kHeads, u = item / parts, h0 = (item - u * parts) * kHeads;
+  const int u = item / p.Hkv, hkv = item - u * p.Hkv;
   Sequence seq = {};
   auto start = [&](int b, int lo) { return (int64_t)(lo >> table.page_log2) + 2 * (int64_t)b; };
   const int b = last_up_to(table, u, lane, seq, start);
@@ -54,71 +54,71 @@ __global__ __launch_bounds__(256) void paged_key_sums_kernel(const SumParams<E> 
   const int id = __builtin_amdgcn_readfirstlane(page_id(table, b, page));
   if (held == 0 || id < 0) return;
   const int r = lane / L, c = lane % L;
-  const int64_t head0 = (int64_t)id * p.Hkv + h0;
-  const char* const from = p.pages + (head0 << table.page_log2) * kRow + c * 16;
-  const int64_t head_bytes = (int64_t)kRow << table.page_log2;
-  float by[kHeads];
-  float acc[kHeads][kElems];
+  const int64_t head = (int64_t)id * p.Hkv + hkv;
+  const char* const from = p.pages + (head << table.page_log2) * kRow + c * 16;
+  const float by = k8 ? p.scales[head] : 1.f;
+  float acc[kElems];
 #pragma unroll
-  for (int h = 0; h < kHeads; ++h) {
-    by[h] = k8 ? p.scales[head0 + (h0 + h < p.Hkv ? h : 0)] : 1.f;
-#pragma unroll
-    for (int e = 0; e < kElems; ++e) acc[h][e] = 0.f;
-  }
+  for (int e = 0; e < kElems; ++e) acc[e] = 0.f;
   for (int t0 = 0; t0 < held; t0 += kTokens * kAhead) {
-    u32x4 w[kHeads][kAhead];
+    u32x4 w[kAhead];
 #pragma unroll
-    for (int h = 0; h < kHeads; ++h)
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k)   // (tokens behind the last held one, and heads behind the last, are others again)
-        w[h][k] = *reinterpret_cast<const u32x4*>(from + (h0 + h < p.Hkv ? h : 0) * head_bytes + min(t0 + k * kTokens + r, held - 1) * kRow);
+    for (int k = 0; k < kAhead; ++k)   // (those behind the last held one are it again)
+      w[k] = *reinterpret_cast<const u32x4*>(from + min(t0 + k * kTokens + r, held - 1) * kRow);
     if (t0 + kTokens * kAhead > held) {
 #pragma unroll
-      for (int h = 0; h < kHeads; ++h)
-#pragma unroll
-        for (int k = 0; k < kAhead; ++k)
-          if (t0 + k * kTokens + r >= held) w[h][k] = u32x4{0, 0, 0, 0};
+      for (int k = 0; k < kAhead; ++k)
+        if (t0 + k * kTokens + r >= held) w[k] = u32x4{0, 0, 0, 0};
     }
 #pragma unroll
-    for (int h = 0; h < kHeads; ++h)
+    for (int k = 0; k < kAhead; ++k) {
+      if constexpr (k8) {
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        if constexpr (k8) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            acc[h][4 * i] += __builtin_amdgcn_cvt_f32_fp8(w[h][k][i], 0);
-            acc[h][4 * i + 1] += __builtin_amdgcn_cvt_f32_fp8(w[h][k][i], 1);
-            acc[h][4 * i + 2] += __builtin_amdgcn_cvt_f32_fp8(w[h][k][i], 2);
-            acc[h][4 * i + 3] += __builtin_amdgcn_cvt_f32_fp8(w[h][k][i], 3);
-          }
-        } else {
-          const typename E::elem8 x = __builtin_bit_cast(typename E::elem8, w[h][k]);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) acc[h][e] += (float)x[e];
+        for (int i = 0; i < 4; ++i) {
+          acc[4 * i] += __builtin_amdgcn_cvt_f32_fp8(w[k][i], 0);
+          acc[4 * i + 1] += __builtin_amdgcn_cvt_f32_fp8(w[k][i], 1);
+          acc[4 * i + 2] += __builtin_amdgcn_cvt_f32_fp8(w[k][i], 2);
+          acc[4 * i + 3] += __builtin_amdgcn_cvt_f32_fp8(w[k][i], 3);
         }
+      } else {
+        const typename E::elem8 x = __builtin_bit_cast(typename E::elem8, w[k]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[e] += (float)x[e];
       }
+    }
   }
   // the lanes of a column: each keeps half of what it has and is given the other's of that half
+  int at = c * kElems;
+  auto halve = [&](auto step) __attribute__((always_inline)) {
+    constexpr int m = 32 >> step, n = kElems >> (step + 1);
+    if constexpr (m >= L) {
 #pragma unroll
-  for (int h = 0; h < kHeads; ++h) {
-    int n = kElems, at = c * kElems;
-#pragma unroll
-    for (int m = 32; m >= L; m >>= 1) {
-      n /= 2;
-      const bool upper = lane & m;
-#pragma unroll
-      for (int i = 0; i < kElems / 2; ++i) {
-        if (i >= n) break;
-        const float mine = upper ? acc[h][i + n] : acc[h][i], other = upper ? acc[h][i] : acc[h][i + n];
-        acc[h][i] = mine + __shfl_xor(other, m, 64);
+      for (int i = 0; i < n; ++i) {
+        const uint32_t x = float_bits(acc[i]), y = float_bits(acc[i + n]);
+        uint32_t mine, other;   // what the lane has of its half, and what the other one has
+        if constexpr (m == 32) {
+          const auto z = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+          mine = z[0], other = z[1];
+        } else if constexpr (m == 16) {
+          const auto z = __builtin_amdgcn_permlane16_swap(x, y, false, false);
+          mine = z[0], other = z[1];
+        } else {
+          // (a choice of bits: one of elements becomes one of their numbers, and a search among all: 5.9 us for 16 sequences' next tokens)
+          const uint32_t upper = -(uint32_t)((lane & m) != 0);
+          mine = (x & ~upper) | (y & upper);
+          other = (uint32_t)__shfl_xor((int)((x & upper) | (y & ~upper)), m, 64);
+        }
+        acc[i] = __builtin_bit_cast(float, mine) + __builtin_bit_cast(float, other);
       }
-      at += upper ? n : 0;
+      at += lane & m ? n : 0;
     }
-    if (h0 + h < p.Hkv) {
+  };
+  halve(std::integral_constant<int, 0>{});
+  halve(std::integral_constant<int, 1>{});
+  halve(std::integral_constant<int, 2>{});
+  halve(std::integral_constant<int, 3>{});
 #pragma unroll
-      for (int i = 0; i < D / 64; ++i) p.sums[(head0 + h) * D + at + i] = acc[h][i] * by[h];
-    }
-  }
+  for (int i = 0; i < D / 64; ++i) p.sums[head * D + at + i] = acc[i] * by;
 }
 
 // ---- scores
@@ -385,7 +385,8 @@ static int launch_select(SelectParams<E> p, int32_t* out, int64_t T, hipStream_t
     s.t0 = (int)t0;
     s.tokens = (int)(T - t0 < step ? T - t0 : step);
     const int64_t units = (int64_t)s.tokens * s.rep / kScoreRows + s.table.B;
-    // (a thread has up to eight pages of a block on its way; fewer where there are not enough blocks for the chip)
+    // (a thread has up to eight pages of a block on its way; fewer where there are not enough blocks for the chip.  Blocks of 64 pages behind
+    // 131072 tokens 6.2 us, 7.5 without the latter, 30 with a thread to a block; of 8 pages behind 20000 5.0 and 7.2)
     auto chunks = [&]() { return (s.blocks - 1) / (kScoreSums >> p.split_log2) + 1; };
     p.split_log2 = 0;
     while (p.split_log2 < kScoreSumsLog2 &&
@@ -427,18 +428,15 @@ extern "C" int moba_paged_key_sums(const void* k_pages, const float* k_scales, f
   if ((D != 64 && D != 128) || page_log2 < 0 || (dtype != MOBA_DTYPE_BF16 && dtype != MOBA_DTYPE_F16)) return MOBA_ERR_UNSUPPORTED;
   if (((uintptr_t)k_pages & 15) || ((uintptr_t)sums & 3)) return MOBA_ERR_ARG;
   const int64_t units = (T >> page_log2) + 2 * (int64_t)B;   // (sequence b's pages are numbered from (its first row / page_size) + 2b on)
-  const int heads = Hkv > 1 && units * Hkv >= 8192 ? 2 : 1;
-  const int64_t items = units * ((Hkv + heads - 1) / heads);
-  if (units * Hkv >= 1LL << 31 || T >= 1LL << 30 || num_pages >= 1LL << 31 || max_pages >= 1LL << 31 || items >= 1LL << 25)
-    return MOBA_ERR_LIMIT;   // (2^32 threads)
+  const int64_t items = units * Hkv;
+  if (T >= 1LL << 30 || num_pages >= 1LL << 31 || max_pages >= 1LL << 31 || items >= 1LL << 25) return MOBA_ERR_LIMIT;   // (2^31 threads)
   LaunchCheck launch_check;
   auto launch = [&](auto e, auto d, auto c8) {
     typedef decltype(e) E;
     const SumParams<E> p = {table_of(page_table, lengths, cu_new, table_stride, T, B, num_pages, max_pages, page_log2), (const char*)k_pages,
                             k_scales, sums, Hkv, (int)items};
     const dim3 grid((unsigned)((items + 3) / 4));
-    if (heads == 2) hipLaunchKernelGGL((paged_key_sums_kernel<E, d, c8, 2>), grid, dim3(256), 0, (hipStream_t)stream, p);
-    else hipLaunchKernelGGL((paged_key_sums_kernel<E, d, c8, 1>), grid, dim3(256), 0, (hipStream_t)stream, p);
+    hipLaunchKernelGGL((paged_key_sums_kernel<E, d, c8>), grid, dim3(256), 0, (hipStream_t)stream, p);
   };
   constexpr std::integral_constant<int, 64> d64;
   constexpr std::integral_constant<int, 128> d128;

@@ -80,6 +80,8 @@ def test_long_prompts():
     check_reserve(free, count, table, lengths, new, sum(new) + 3, 16)
     check_reserve(free, 1200, table, lengths, new, sum(new), 16)
     check_reserve(free, count, table, lengths, [1, 2, 4094], 4097, 16)
+    check_reserve(free, count, table, lengths, [1, 2, 8190], 8193, 16)
+    check_reserve(free, count, table, lengths, [1, 2, 8189], 8192, 16)
     for row in table:
         row[:5000] = random.Random(1).sample(range(30000), 5000)
     check_release(free, 20000, table, [80000, 77, 31999], [17, 80, 0], 16)

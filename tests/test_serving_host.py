@@ -60,7 +60,8 @@ def test_tables_entry_points_refuse():
 
     common = [dict(free=None), dict(count=None), dict(table=None), dict(lengths=None), dict(new=None), dict(B=0), dict(pool=0), dict(wide=0),
               dict(stride=-1)]
-    for wrong in common + [dict(cu=None), dict(owners=None), dict(positions=None), dict(slots=None), dict(space=None, rows=5000), dict(space=some + 2), dict(slots=some + 4), dict(rows=-1)]:
+    for wrong in common + [dict(cu=None), dict(owners=None), dict(positions=None), dict(slots=None), dict(space=None, rows=9000),
+                           dict(space=some + 2), dict(slots=some + 4), dict(rows=-1)]:
         assert reserve(**wrong) == -1, wrong
     for wrong in common:
         assert release(**wrong) == -1, wrong
@@ -70,7 +71,7 @@ def test_tables_entry_points_refuse():
             assert call(**wrong) == -4, wrong
     assert reserve(rows=1 << 30) == -4
     size = lib.moba_paged_reserve_workspace_bytes
-    assert size(0, 5000) == size(7, 4096) == 0 and size(7, 4097) == 32
+    assert size(0, 9000) == size(7, 8192) == 0 and size(7, 8193) == 32
 
 
 def attention_args(**changes):
