@@ -169,14 +169,16 @@ __global__ __launch_bounds__(kTableThreads) void paged_reserve_kernel(const Tabl
 // the same for rows, and pages, that are many: each thread four of them (there are no more pages than rows)
 __global__ __launch_bounds__(256) void paged_rows_kernel(const TableParams p) {
   extern __shared__ int lds[];
-  int *const cu = lds, *const rank = lds + p.B + 1;
+  int *const cu = lds, *const rank = cu + p.B + 1, *const length = rank + p.B + 1;
+  const int left = *p.pool.free_count;
   for (int b = threadIdx.x; b <= p.B; b += 256) {
     cu[b] = p.cu_new[b];
     rank[b] = p.ranks[b];
+    if (b < p.B) length[b] = max(p.lengths[b], 0);
   }
   __syncthreads();
-  const int top = *p.pool.free_count + rank[p.B];
-  auto old = [&](int b) { return max(p.lengths[b], 0) - (cu[b + 1] - cu[b]); };
+  const int top = left + rank[p.B];
+  auto old = [&](int b) { return length[b] - (cu[b + 1] - cu[b]); };
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const int64_t t = (int64_t)blockIdx.x * 1024 + k * 256 + threadIdx.x;
@@ -300,11 +302,11 @@ extern "C" int moba_paged_reserve(int32_t* free_pages, int32_t* free_count, int3
   const int need = (3 * B + 2) * 4;
   static bool allowed[2][kMaxDevices];
   if (!allow_dynamic_lds((const void*)paged_reserve_kernel, (3 * kMostTableSequences + 2) * 4, allowed[0]) ||
-      !allow_dynamic_lds((const void*)paged_rows_kernel, (2 * kMostTableSequences + 2) * 4, allowed[1]))
+      !allow_dynamic_lds((const void*)paged_rows_kernel, (3 * kMostTableSequences + 2) * 4, allowed[1]))
     return MOBA_ERR_LAUNCH;
   hipLaunchKernelGGL(paged_reserve_kernel, dim3(1), dim3(kTableThreads), need, st, p);
   if (rows > kRowsAtOnce)
-    hipLaunchKernelGGL(paged_rows_kernel, dim3((unsigned)((rows + 1023) / 1024)), dim3(256), (2 * B + 2) * 4, st, p);
+    hipLaunchKernelGGL(paged_rows_kernel, dim3((unsigned)((rows + 1023) / 1024)), dim3(256), need, st, p);
   return launch_check.result();
 }
 
