@@ -482,7 +482,7 @@ int moba_paged_block_attention(const void* q, void* out, const void* k_pages, co
 
 /* Pages from a pool and back, on the device.  The pool is a stack: free_pages [num_pages] int32, of which the first free_count [1]
  * are free.  page_table [B, max_pages] int32 with rows of table_stride entries, lengths [B] int32.  B at most 8192, B * max_pages
- * below 2^31.
+ * below 2^31.  Calls that share a pool or a table have to run one after the other.
  *
  * moba_paged_reserve: new_tokens [B] int32 more tokens for every sequence.  One whose tokens do not fit its row of the table gets none; of
  *   the others one is served if its tokens and those asked for before it are at most `rows`, and the pages that it and those before

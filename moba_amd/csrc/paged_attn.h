@@ -209,7 +209,9 @@ template <int D, bool k8, class Table>
 constexpr int few_lds_bytes() { return few_list_at<D, k8>() + (kChooses<Table> ? kListBytes : 0); }
 
 // Position of new token j of a unit's rows, every lane its own (mine: the lane's sequence of find_unit()); the least of a wave's 32 rows'
-__device__ __forceinline__ int position_at(const PageTable&, const Unit& u, int j, const Sequence&) { return (int)u.seq.length - (u.seq.hi - u.seq.lo) + j; }
+__device__ __forceinline__ int position_at(const PageTable&, const Unit& u, int j, const Sequence&) {
+  return (int)u.seq.length - (u.seq.hi - u.seq.lo) + j;
+}
 __device__ __forceinline__ int least_position(const PageTable& t, const Unit& u, int first, int) { return position_at(t, u, first, u.seq); }
 // the last key that new tokens up to j of a unit's rows see
 __device__ __forceinline__ int last_seen(const PageTable& t, const Unit& u, int j) { return position_at(t, u, j, u.seq); }
@@ -1298,7 +1300,9 @@ __global__ __launch_bounds__(256) void paged_merge_many_kernel(const PagedParams
       const bool second = kSides > 1 && i >= parts[0].runs;
       return second ? parts[kSides - 1].first + (i - parts[0].runs) * parts[kSides - 1].step : parts[0].first + i * parts[0].step;
     };
-    auto side_of = [&](int i) __attribute__((always_inline)) -> const Parts& { return kSides > 1 && i >= parts[0].runs ? parts[kSides - 1] : parts[0]; };
+    auto side_of = [&](int i) __attribute__((always_inline)) -> const Parts& {
+      return kSides > 1 && i >= parts[0].runs ? parts[kSides - 1] : parts[0];
+    };
     float top = kNoMax, ll = 0.f, o[kPer] = {};
     for (int i0 = 0; __any(i0 < runs); i0 += kLse) {
       float lse[kLse], mm = top;

@@ -91,7 +91,8 @@ def paged_reserve(pool: PagePool, page_table: torch.Tensor, lengths: torch.Tenso
     A sequence gets all that it wants or nothing (its row of the table, its length and the pool stay as they are, and it has no
     rows): nothing if its tokens do not fit its row of the table; if they, with those that the others before it want (those that do
     not fit aside), are more than ``rows``; or if it needs more pages and they, with those that the others before it need, are more
-    than the pool has.  The index tensors stay on the device: a captured call follows them.  At most 8192 sequences.
+    than the pool has.  The index tensors stay on the device: a captured call follows them.  Calls that share a pool or a table have to
+    run one after the other (one stream, or streams that wait for each other).  At most 8192 sequences.
     """
     out = _lib.host().paged_reserve(pool.free_pages, pool.free_count, page_table, lengths, new_tokens, rows, pool.page_size)
     if out is not NotImplemented:

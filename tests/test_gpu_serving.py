@@ -154,10 +154,13 @@ def test_wrong_tensors_are_told_apart():
                         (lambda: m.paged_prefix_attention(q.float(), cache, *good, ints(0, 2), ints(192)), TypeError),
                         (lambda: m.paged_prefix_attention(q, cache, *good, ints(0, 2, 3), ints(192)), ValueError),
                         (lambda: m.paged_prefix_attention(q, cache, *good, ints(0, 2).cpu(), ints(192)), ValueError),
-                        (lambda: m.paged_key_sums(cache, sums[1:], *good, 9), ValueError), (lambda: m.paged_key_sums(cache, sums, *good, -1), ValueError),
+                        (lambda: m.paged_key_sums(cache, sums[1:], *good, 9), ValueError),
+                        (lambda: m.paged_key_sums(cache, sums, *good, -1), ValueError),
                         (lambda: m.paged_key_sums(cache, sums.double(), *good, 9), TypeError),
-                        (lambda: m.paged_select_blocks(q, sums, *good, 32, 48, 3), ValueError), (lambda: m.paged_select_blocks(q, sums, *good, 32, 64, 65), ValueError),
-                        (lambda: m.paged_select_blocks(q, sums, *good, 8, 64, 3), ValueError), (lambda: m.paged_select_blocks(q, sums, *good, 32, 64, 0), ValueError),
+                        (lambda: m.paged_select_blocks(q, sums, *good, 32, 48, 3), ValueError),
+                        (lambda: m.paged_select_blocks(q, sums, *good, 32, 64, 65), ValueError),
+                        (lambda: m.paged_select_blocks(q, sums, *good, 8, 64, 3), ValueError),
+                        (lambda: m.paged_select_blocks(q, sums, *good, 32, 64, 0), ValueError),
                         (lambda: m.paged_block_attention(q, cache, blocks[1:], *good, 64), ValueError),
                         (lambda: m.paged_block_attention(q, cache, blocks.long(), *good, 64), TypeError),
                         (lambda: m.paged_block_attention(q, cache, blocks, *good, 0), ValueError),
