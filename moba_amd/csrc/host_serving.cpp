@@ -19,6 +19,7 @@ decltype(&moba_paged_reserve_workspace_bytes) reserve_bytes = nullptr;
 decltype(&moba_paged_release) release_call = nullptr;
 
 constexpr int64_t kMostTokens = 1 << 24;   // fewer than these
+constexpr int64_t kMostBlocks = 16384;      // of a row of the table that the selection chooses from
 
 bool ints(const Tensor* t, int64_t dim, const at::Device& device) {
   return t && t->scalar_type() == at::kInt && t->dim() == dim && t->device() == device && t->is_contiguous();
@@ -163,7 +164,7 @@ PyObject* py_paged_select_blocks(PyObject*, PyObject* const* args, Py_ssize_t n)
   const int64_t page = number[0], block_size = number[1], topk = number[2], hkv = sums->size(1);
   int64_t strides[3];
   if (!query_fits(*query, hkv, strides) || page < 16 || page > 256 || (page & (page - 1)) || block_size < 1 || block_size > (1 << 24) ||
-      block_size % page || topk < 1 || topk > 64)
+      block_size % page || topk < 1 || topk > 64 || index.table->size(1) > kMostBlocks * (block_size / page))
     Py_RETURN_NOTIMPLEMENTED;
   strides[2] = index.table->stride(0);
   Tensor out;
