@@ -457,8 +457,8 @@ int moba_paged_prefix_attention(const void* q, void* out, const void* k_pages, c
  *   (T / page_size + 2 * B) * Hkv below 2^25.
  * moba_paged_select_blocks: blocks [T,H,topk] int32: of every row the topk - 1 blocks in front of its token's own whose products
  *   q . (sum of their pages' sums), in 64 bits, are largest (of equal ones the lowest; NaN as minus infinity), and its own, ascending;
- *   -1 behind the last.  topk at most 64; the table at most 16384 blocks wide.  q, sums 16-byte aligned; strides {q token, q head,
- *   page_table row}, the first two multiples of 8.  workspace (scores): 8-byte aligned.
+ *   -1 behind the last.  topk at most 64; the table at most 16384 blocks wide; T < 2^24, T * H < 2^31, B * Hkv below 2^23.  q, sums
+ *   16-byte aligned; strides {q token, q head, page_table row}, the first two multiples of 8.  workspace (scores): 8-byte aligned.
  * moba_paged_block_attention: softmax attention of every row over the keys of its blocks (any [T,H,topk] int32: an entry that is no
  *   block of the sequence up to the token's own is none, the same block twice is once) up to its token.  Up to 32 rows
  *   (tokens times heads) of a sequence and key/value head read the union of their blocks once.  Precision: that of few rows in

@@ -250,6 +250,7 @@ struct PickParams {
   SelectShape s;
   const double* scores;
   int32_t* out;         // [T, H, topk]
+  int64_t row0;         // of this launch, among the rows (tokens times heads) that have scores
 };
 
 // A row for kWaves waves, kPer scores to a lane: block i * 64 * kWaves + thread is register i of a thread
@@ -259,7 +260,7 @@ __global__ __launch_bounds__(kWaves == 1 ? 256 : 64 * kWaves) void paged_pick_ke
   __shared__ int counts[2][kWaves], places[kPer * kWaves];
   const SelectShape& s = p.s;
   const int lane = threadIdx.x & 63, wave = kWaves == 1 ? 0 : threadIdx.x >> 6, tid = kWaves == 1 ? lane : threadIdx.x;
-  const int64_t row = kWaves == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : (int64_t)blockIdx.x;
+  const int64_t row = p.row0 + (kWaves == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : (int64_t)blockIdx.x);
   if (row >= (int64_t)s.tokens * s.H) return;
   const int t = s.t0 + (int)(row / s.H);
   int32_t* const out = p.out + ((int64_t)s.t0 * s.H + row) * s.topk;
@@ -368,6 +369,7 @@ __global__ __launch_bounds__(kWaves == 1 ? 256 : 64 * kWaves) void paged_pick_ke
 }
 
 static constexpr int64_t kScoreBytes = 1LL << 29;   // of a launch's scores: more tokens are several launches
+constexpr int64_t kPickRows = 1LL << 21;            // of a launch: below 2^32 threads for up to sixteen waves to a row
 constexpr int kMostTopk = 64;
 
 static int blocks_of(int64_t max_pages, int each) { return (int)((max_pages + each - 1) / each); }
@@ -396,12 +398,15 @@ static int launch_select(SelectParams<E> p, int32_t* out, int64_t T, hipStream_t
     const int z = (int)(want < 1 ? 1 : want < chunks() ? want : chunks());
     hipLaunchKernelGGL((paged_score_kernel<E, D>), dim3((unsigned)units, s.Hkv, z), dim3(256), 0, st, p);
     const int64_t rows = (int64_t)s.tokens * s.H;
-    const PickParams pick = {s, p.scores, out};
-    const dim3 four((unsigned)((rows + 3) / 4));
-    if (s.blocks <= 64) hipLaunchKernelGGL((paged_pick_kernel<1, 1>), four, dim3(256), 0, st, pick);
-    else if (s.blocks <= 256) hipLaunchKernelGGL((paged_pick_kernel<1, 4>), four, dim3(256), 0, st, pick);
-    else if (s.blocks <= 1024) hipLaunchKernelGGL((paged_pick_kernel<1, 16>), four, dim3(256), 0, st, pick);
-    else hipLaunchKernelGGL((paged_pick_kernel<16, 16>), dim3((unsigned)rows), dim3(1024), 0, st, pick);
+    for (int64_t row0 = 0; row0 < rows; row0 += kPickRows) {
+      const PickParams pick = {s, p.scores, out, row0};
+      const int64_t here = rows - row0 < kPickRows ? rows - row0 : kPickRows;
+      const dim3 four((unsigned)((here + 3) / 4));
+      if (s.blocks <= 64) hipLaunchKernelGGL((paged_pick_kernel<1, 1>), four, dim3(256), 0, st, pick);
+      else if (s.blocks <= 256) hipLaunchKernelGGL((paged_pick_kernel<1, 4>), four, dim3(256), 0, st, pick);
+      else if (s.blocks <= 1024) hipLaunchKernelGGL((paged_pick_kernel<1, 16>), four, dim3(256), 0, st, pick);
+      else hipLaunchKernelGGL((paged_pick_kernel<16, 16>), dim3((unsigned)here), dim3(1024), 0, st, pick);
+    }
   }
   return launch_check.result();
 }
@@ -479,7 +484,7 @@ extern "C" int moba_paged_select_blocks(const void* q, const float* sums, int32_
   const SelectShape shape = {table_of(page_table, lengths, cu_new, strides[2], T, B, num_pages, max_pages, page_log2), H, Hkv, H / Hkv, each,
                              blocks_of(max_pages, each), topk, 0, 0};
   const int64_t step = tokens_at_once(T, H, shape.blocks), units = step * shape.rep / kScoreRows + B;
-  if (units * Hkv * 256 >= 1LL << 32 || step * H * (shape.blocks > 1024 ? 1024 : 64) >= 1LL << 32) return MOBA_ERR_LIMIT;
+  if (units * Hkv * 256 >= 1LL << 32) return MOBA_ERR_LIMIT;
   auto launch = [&](auto e) {
     typedef decltype(e) E;
     const SelectParams<E> p = {shape, (const typename E::elem*)q, strides[0], strides[1], sums, (double*)workspace, 0};

@@ -24,3 +24,15 @@ def test_wide_tables_of_the_selection():
             assert got.shape == (3, 2, 2) and got.max() == 99 // block
             with pytest.raises(ValueError, match="16384 blocks"):
                 paged_select_blocks(query, sums, table, ints(100), ints(0, 3), page, block, 2)
+
+
+def test_one_block_for_many_rows():
+    """2^26 rows and more of a table of one block (the query's tokens are one token's)."""
+    from moba_amd import paged_select_blocks
+    tokens, heads, page = (1 << 20) + 5, 64, 256
+    q = torch.ones((1, heads, 64), dtype=BF16, device="cuda").expand(tokens, -1, -1)
+    table, sums = torch.zeros((1, 4100), dtype=torch.int32, device="cuda"), torch.zeros((1, 1, 64), device="cuda")
+    for rows in (tokens, tokens - 9):      # (the last nine belong to no sequence)
+        got = paged_select_blocks(q, sums, table, ints(rows), ints(0, rows), page, 4100 * page, 2)
+        assert got.shape == (tokens, heads, 2)
+        assert (got[:rows, :, 0] == 0).all() and (got[:rows, :, 1] == -1).all() and (got[rows:] == -1).all()
