@@ -454,7 +454,7 @@ int moba_paged_prefix_attention(const void* q, void* out, const void* k_pages, c
  *
  * moba_paged_key_sums: sums [num_pages, Hkv, D] fp32 of the keys that a page holds, for the pages that have received the new tokens
  *   (of T packed rows); other pages' are left as they are.  k_pages 16-byte aligned.  table_stride: of the page table, in entries.
- *   (T / page_size + 2 * B) * Hkv below 2^25.
+ *   T < 2^30, B * Hkv below 2^24.
  * moba_paged_select_blocks: blocks [T,H,topk] int32: of every row the topk - 1 blocks in front of its token's own whose products
  *   q . (sum of their pages' sums), in 64 bits, are largest (of equal ones the lowest; NaN as minus infinity), and its own, ascending;
  *   -1 behind the last.  topk at most 64; the table at most 16384 blocks wide; T < 2^24, T * H < 2^31, B * Hkv below 2^23.  q, sums

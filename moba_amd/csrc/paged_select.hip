@@ -30,8 +30,10 @@ struct SumParams {
   const char* pages;
   const float* scales;   // 8-bit pages
   float* sums;           // [num_pages, Hkv, D]
-  int Hkv, items;        // waves
+  int64_t unit0;         // pages of the batch, numbered through, of this launch: the first,
+  int Hkv, items;        // and how many times heads (waves)
 };
+constexpr int64_t kSumItems = (1 << 25) - 1;   // of a launch: below 2^31 threads
 
 // One wave to a page and head: 64 / L tokens at a time, L lanes of 16 bytes to a token, kAhead such steps on their way together.  (Eight of
 // them: 22.4 us for 131072 tokens as above, 22.7 so, but 8192 on pages of 16 6.3 and 5.0.  Two heads to a wave: 23.6 and 4.9, and the next
@@ -43,7 +45,8 @@ __global__ __launch_bounds__(256) void paged_key_sums_kernel(const SumParams<E> 
   const int item = __builtin_amdgcn_readfirstlane((int)blockIdx.x * 4 + (threadIdx.x >> 6));
   if (item >= p.items) return;
   const PageTable& table = p.table;
-  const int u = item / p.Hkv, hkv = item - u * p.Hkv;
+  const int unit = item / p.Hkv, hkv = item - unit * p.Hkv;
+  const int64_t u = p.unit0 + unit;
   Sequence seq = {};
   auto start = [&](int b, int lo) { return (int64_t)(lo >> table.page_log2) + 2 * (int64_t)b; };
   const int b = last_up_to(table, u, lane, seq, start);
@@ -433,15 +436,18 @@ extern "C" int moba_paged_key_sums(const void* k_pages, const float* k_scales, f
   if ((D != 64 && D != 128) || page_log2 < 0 || (dtype != MOBA_DTYPE_BF16 && dtype != MOBA_DTYPE_F16)) return MOBA_ERR_UNSUPPORTED;
   if (((uintptr_t)k_pages & 15) || ((uintptr_t)sums & 3)) return MOBA_ERR_ARG;
   const int64_t units = (T >> page_log2) + 2 * (int64_t)B;   // (sequence b's pages are numbered from (its first row / page_size) + 2b on)
-  const int64_t items = units * Hkv;
-  if (T >= 1LL << 30 || num_pages >= 1LL << 31 || max_pages >= 1LL << 31 || items >= 1LL << 25) return MOBA_ERR_LIMIT;   // (2^31 threads)
+  if (T >= 1LL << 30 || num_pages >= 1LL << 31 || max_pages >= 1LL << 31 || (int64_t)B * Hkv >= 1LL << 24) return MOBA_ERR_LIMIT;
   LaunchCheck launch_check;
   auto launch = [&](auto e, auto d, auto c8) {
     typedef decltype(e) E;
-    const SumParams<E> p = {table_of(page_table, lengths, cu_new, table_stride, T, B, num_pages, max_pages, page_log2), (const char*)k_pages,
-                            k_scales, sums, Hkv, (int)items};
-    const dim3 grid((unsigned)((items + 3) / 4));
-    hipLaunchKernelGGL((paged_key_sums_kernel<E, d, c8>), grid, dim3(256), 0, (hipStream_t)stream, p);
+    SumParams<E> p = {table_of(page_table, lengths, cu_new, table_stride, T, B, num_pages, max_pages, page_log2), (const char*)k_pages,
+                      k_scales, sums, 0, Hkv, 0};
+    const int64_t step = kSumItems / Hkv;
+    for (; p.unit0 < units; p.unit0 += step) {
+      p.items = (int)(units - p.unit0 < step ? units - p.unit0 : step) * Hkv;
+      const dim3 grid((unsigned)((p.items + 3) / 4));
+      hipLaunchKernelGGL((paged_key_sums_kernel<E, d, c8>), grid, dim3(256), 0, (hipStream_t)stream, p);
+    }
   };
   constexpr std::integral_constant<int, 64> d64;
   constexpr std::integral_constant<int, 128> d128;

@@ -36,3 +36,20 @@ def test_one_block_for_many_rows():
         got = paged_select_blocks(q, sums, table, ints(rows), ints(0, rows), page, 4100 * page, 2)
         assert got.shape == (tokens, heads, 2)
         assert (got[:rows, :, 0] == 0).all() and (got[:rows, :, 1] == -1).all() and (got[rows:] == -1).all()
+
+
+def test_key_sums_of_many_rows():
+    """Rows beyond 2^25 waves' pages: a sequence of 2^26 new tokens, most of whose pages the table names wrongly, and a short one."""
+    from moba_amd import PagedKVCache, paged_key_sums
+    page, heads, long = 16, 8, 1 << 26
+    g = torch.Generator().manual_seed(1)
+    k = torch.randn((6, heads, page, 64), generator=g).to(BF16).cuda()
+    cache = PagedKVCache(k, torch.zeros_like(k))
+    table = torch.full((2, long // page), -1, dtype=torch.int32, device="cuda")
+    table[0, 0], table[0, 12345], table[0, -1], table[1, 0], table[1, 1] = 4, 2, 0, 3, 1
+    sums = torch.full((6, heads, 64), 7.5, device="cuda")
+    paged_key_sums(cache, sums, table, ints(long, 21), ints(0, long, long + 21), long + 21)
+    for id, held in ((4, 16), (2, 16), (0, 16), (3, 16), (1, 5)):
+        part = k[id, :, :held].double()
+        assert ((sums[id].double() - part.sum(1)).abs() <= 18 * 2.0 ** -24 * part.abs().sum(1)).all(), id
+    assert (sums[5] == 7.5).all()
