@@ -203,9 +203,9 @@ struct Tables {
     for (const Tensor* t : {&free_pages, &free_count, &lengths, &asked})
       if (t->dim() != 1 || !t->is_contiguous() || t->device() != device) return false;
     const int64_t b = lengths.size(0);
-    return table.device() == device && free_count.size(0) == 1 && free_pages.size(0) > 0 && b > 0 && b <= 8192 && asked.size(0) == b &&
-           table.dim() == 2 && table.size(0) == b && table.size(1) > 0 && (b == 1 || table.stride(0) >= table.size(1)) &&
-           (table.size(1) == 1 || table.stride(1) == 1) && page >= 16 && page <= 256 && !(page & (page - 1));
+    return table.device() == device && free_count.size(0) == 1 && free_pages.size(0) > 0 && free_pages.size(0) <= INT32_MAX && b > 0 &&
+           b <= 8192 && asked.size(0) == b && table.dim() == 2 && table.size(0) == b && table.size(1) > 0 && table.numel() <= INT32_MAX &&
+           (b == 1 || table.stride(0) >= table.size(1)) && (table.size(1) == 1 || table.stride(1) == 1) && page >= 16 && page <= 256 && !(page & (page - 1));
   }
   int32_t* of(const Tensor& t) const { return (int32_t*)t.mutable_data_ptr(); }
 };

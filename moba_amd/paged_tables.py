@@ -14,6 +14,7 @@ from .paged import PAGE_SIZES, _plain, _table, _taken
 
 MAX_SEQUENCES = 8192   # of a call
 MAX_ROWS = (1 << 30) - 1
+MAX_ENTRIES = (1 << 31) - 1   # of a page table, or a pool
 
 
 @dataclass(frozen=True, eq=False)
@@ -38,6 +39,8 @@ class PagePool:
                 raise ValueError(f"{name} must be contiguous, of one dimension")
         if not self.free_pages.numel() or self.free_count.numel() != 1:
             raise ValueError("there must be pages, and one free_count")
+        if self.free_pages.numel() > MAX_ENTRIES:
+            raise ValueError("fewer than 2^31 pages")
         if self.free_count.device != self.free_pages.device:
             raise ValueError("all tensors of a pool must be on one device")
         if self.page_size not in PAGE_SIZES:
@@ -66,6 +69,8 @@ def _check(pool, page_table, lengths, name, asked):
         raise ValueError(f"page_table must be [sequences, pages], lengths and {name} [sequences]")
     if b > MAX_SEQUENCES:
         raise ValueError(f"at most {MAX_SEQUENCES} sequences")
+    if page_table.numel() > MAX_ENTRIES:
+        raise ValueError("page_table must have fewer than 2^31 entries")
     # (they are written)
     if not lengths.is_contiguous() or _table(page_table) is not page_table or (b > 1 and page_table.stride(0) < page_table.shape[1]):
         raise ValueError("lengths and the rows of page_table must be contiguous and apart from each other")
@@ -92,7 +97,8 @@ def paged_reserve(pool: PagePool, page_table: torch.Tensor, lengths: torch.Tenso
     rows): nothing if its tokens do not fit its row of the table; if they, with those that the others before it want (those that do
     not fit aside), are more than ``rows``; or if it needs more pages and they, with those that the others before it need, are more
     than the pool has.  The index tensors stay on the device: a captured call follows them.  Calls that share a pool or a table have to
-    run one after the other (one stream, or streams that wait for each other).  At most 8192 sequences.
+    run one after the other (one stream, or streams that wait for each other).  At most 8192 sequences, and fewer than 2^31 entries of the
+    table.
     """
     out = _lib.host().paged_reserve(pool.free_pages, pool.free_count, page_table, lengths, new_tokens, rows, pool.page_size)
     if out is not NotImplemented:
@@ -120,7 +126,7 @@ def paged_release(pool: PagePool, page_table: torch.Tensor, lengths: torch.Tenso
 
     Undoes ``paged_reserve``: the pages go back so that they come out again in the order in which they came.  Entries that name no
     page of the pool do not go back.  A page that several sequences share would go back with each of them: keep the tokens that
-    are shared, and release their pages once, with the sequence that they belong to.
+    are shared, and release their pages once, with the sequence that they belong to.  Limits are those of ``paged_reserve``.
     """
     if _lib.host().paged_release(pool.free_pages, pool.free_count, page_table, lengths, keep, pool.page_size) is not NotImplemented:
         return

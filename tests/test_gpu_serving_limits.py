@@ -53,3 +53,13 @@ def test_key_sums_of_many_rows():
         part = k[id, :, :held].double()
         assert ((sums[id].double() - part.sum(1)).abs() <= 18 * 2.0 ** -24 * part.abs().sum(1)).all(), id
     assert (sums[5] == 7.5).all()
+
+
+def test_large_tables():
+    """2^31 entries and more are no table of a pool's."""
+    from moba_amd import PagePool, paged_release, paged_reserve
+    pool = PagePool.full(4, 16)
+    table, lengths = torch.empty((8192, 1 << 18), dtype=torch.int32, device="cuda"), torch.zeros(8192, dtype=torch.int32, device="cuda")
+    for call in (lambda: paged_reserve(pool, table, lengths, lengths, 4), lambda: paged_release(pool, table, lengths, lengths)):
+        with pytest.raises(ValueError, match="2\\^31"):
+            call()
