@@ -108,7 +108,7 @@ struct Index {
       if (t->scalar_type() != at::kInt || t->device() != device) return false;
     if (table->dim() != 2 || lengths->dim() != 1 || cu->dim() != 1 || !lengths->is_contiguous() || !cu->is_contiguous()) return false;
     const int64_t b = table->size(0);
-    return b > 0 && b < INT32_MAX && table->size(1) > 0 && (table->stride(1) == 1 || table->size(1) == 1) && lengths->size(0) == b &&
+    return b > 0 && b < INT32_MAX && table->size(1) > 0 && table->size(1) <= INT32_MAX && (table->stride(1) == 1 || table->size(1) == 1) && lengths->size(0) == b &&
            cu->size(0) == b + 1;
   }
 };

@@ -95,6 +95,8 @@ def _check_table(cache, page_table, lengths, cu_new, device):
     b = page_table.shape[0]
     if lengths.shape[0] != b or cu_new.shape[0] != b + 1 or (b and not page_table.shape[1]):
         raise ValueError("page_table must be [sequences, pages], lengths [sequences], cu_new [sequences + 1]")
+    if page_table.shape[1] >= 1 << 31:
+        raise ValueError("page_table must have fewer than 2^31 pages in a row")
     if cache.k_pages.device != device:
         raise ValueError("all tensors must be on one device")
 

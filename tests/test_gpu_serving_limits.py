@@ -63,3 +63,17 @@ def test_large_tables():
     for call in (lambda: paged_reserve(pool, table, lengths, lengths, 4), lambda: paged_release(pool, table, lengths, lengths)):
         with pytest.raises(ValueError, match="2\\^31"):
             call()
+
+
+def test_wide_tables():
+    """Rows of 2^31 pages and more are refused by every operator on the cache."""
+    import moba_amd as m
+    cache = m.PagedKVCache.empty(3, 2, 64, 16, dtype=BF16)
+    q, kv, sums = torch.zeros((5, 4, 64), dtype=BF16, device="cuda"), torch.zeros((5, 2, 64), dtype=BF16, device="cuda"), cache.key_sums()
+    blocks = torch.zeros((5, 4, 3), dtype=torch.int32, device="cuda")
+    index = (torch.empty((1, 1 << 31), dtype=torch.int32, device="cuda"), ints(5), ints(0, 5))
+    for call in (lambda: m.paged_append(cache, kv, kv, *index), lambda: m.paged_attention(q, cache, *index),
+                 lambda: m.paged_prefix_attention(q, cache, *index, ints(0, 1), ints(0)), lambda: m.paged_key_sums(cache, sums, *index, 5),
+                 lambda: m.paged_select_blocks(q, sums, *index, 16, 1 << 24, 3), lambda: m.paged_block_attention(q, cache, blocks, *index, 32)):
+        with pytest.raises(ValueError, match="2\\^31"):
+            call()

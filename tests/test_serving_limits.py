@@ -23,3 +23,20 @@ def test_large_tables_are_refused():
                 call(pool, meta(sequences, wide), meta(sequences), meta(sequences), *rows)
             with pytest.raises(RuntimeError, match="AMD GPU"):
                 call(pool, meta(sequences, wide - 1), meta(sequences), meta(sequences), *rows)
+
+
+def test_wide_tables_are_refused():
+    """Rows of 2^31 pages and more, by every operator on the cache."""
+    from moba_amd import (PagedKVCache, paged_append, paged_attention, paged_block_attention, paged_key_sums, paged_prefix_attention,
+                          paged_select_blocks)
+    cache = PagedKVCache.empty(3, 2, 64, 16, dtype=torch.bfloat16, device="meta")
+    q, kv, sums = (torch.empty(s, device="meta").to(d) for s, d in (((5, 4, 64), torch.bfloat16), ((5, 2, 64), torch.bfloat16),
+                                                                    ((3, 2, 64), torch.float32)))
+    calls = (lambda *i: paged_append(cache, kv, kv, *i), lambda *i: paged_attention(q, cache, *i),
+             lambda *i: paged_prefix_attention(q, cache, *i, meta(2), meta(1)), lambda *i: paged_key_sums(cache, sums, *i, 5),
+             lambda *i: paged_select_blocks(q, sums, *i, 16, 1 << 24, 3), lambda *i: paged_block_attention(q, cache, meta(5, 4, 3), *i, 32))
+    for call in calls:
+        with pytest.raises(ValueError, match="2\\^31"):
+            call(meta(1, 1 << 31), meta(1), meta(2))
+        with pytest.raises(RuntimeError, match="AMD GPU"):
+            call(meta(1, 9), meta(1), meta(2))
