@@ -462,8 +462,8 @@ int moba_paged_prefix_attention(const void* q, void* out, const void* k_pages, c
  * moba_paged_block_attention: softmax attention of every row over the keys of its blocks (any [T,H,topk] int32: an entry that is no
  *   block of the sequence up to the token's own is none, the same block twice is once) up to its token.  Up to 32 rows
  *   (tokens times heads) of a sequence and key/value head read the union of their blocks once.  Precision: that of few rows in
- *   moba_paged_attention.  Rows without a key are zeros.  topk at most 64, block_size at most 2^24;
- *   (T * H / Hkv / 32 + B) * Hkv below 2^24.  The rest as for moba_paged_attention. */
+ *   moba_paged_attention.  Rows without a key are zeros.  topk at most 64, block_size at most 2^24; T < 2^24, T * H < 2^31, B * Hkv
+ *   below 2^24.  The rest as for moba_paged_attention. */
 int moba_paged_key_sums(const void* k_pages, const float* k_scales, float* sums, const int32_t* page_table, const int32_t* lengths,
                         const int32_t* cu_new, int64_t T, int B, int Hkv, int D, int page_size, int64_t num_pages,
                         int64_t max_pages, int64_t table_stride, int cache8, int dtype, void* stream);

@@ -32,6 +32,7 @@
 #pragma once
 #include "attn_common.h"
 #include "paged_cut.h"
+#include <algorithm>
 #include <type_traits>
 
 namespace moba {
@@ -635,7 +636,7 @@ __global__ __launch_bounds__(64 * kFewWaves, kSets > 1 && D == 128 ? 1 : 2) void
         const int64_t orow = (int64_t)(seq.lo + jj) * shape.H + hkv * shape.rep + gg;
         *reinterpret_cast<u32x2*>(p.out + orow * D + d) = u32x2{pack2<E>(oo[0] * inv, oo[1] * inv), pack2<E>(oo[2] * inv, oo[3] * inv)};
       } else {
-        const int64_t prow = ((int64_t)blockIdx.x * kSets + q) * kFewRows + rr;
+        const int64_t number = blockIdx.x + (int64_t)first_unit(table) * shape.Hkv, prow = (number * kSets + q) * kFewRows + rr;
         *reinterpret_cast<f32x4*>(p.few_o + prow * D + d) = f32x4{oo[0] * inv, oo[1] * inv, oo[2] * inv, oo[3] * inv};
         if (d == 0) p.few_lse[prow] = ll == 0.f ? -INFINITY : mm - ProbShift<V>::value + fast_log2(ll);
       }
@@ -1422,7 +1423,7 @@ static int check_paged(PageTable& table, const void* q, const void* out, const v
   return MOBA_OK;
 }
 
-// Of a call whose batch counts as `sequences`: false where a launch would have more threads than 32 bits number
+// Of a call whose batch counts as `sequences`: false where a launch would have more threads than 32 bits number (kChooses: several launches)
 template <class E, class Table>
 static bool set_params(PagedParams<E, Table>& p, const Cuts& cuts, const void* q, void* out, const void* k_pages, const void* v_pages,
                        const float* k_scales, const float* v_scales, char* workspace, int sequences, int D, const int64_t* strides,
@@ -1432,7 +1433,8 @@ static bool set_params(PagedParams<E, Table>& p, const Cuts& cuts, const void* q
   const int64_t many_threads = 64 * (D == 128 && cache8 ? kManyWaves<128, true> : kManyWaves<64, false>);
   p.few = cuts.few;
   p.many = cuts.many;
-  if ((int64_t)p.few.most * Hkv * 64 * kFewWaves >= 1LL << 32 || (int64_t)p.many.most * Hkv * many_threads >= 1LL << 32) return false;
+  if ((!kChooses<Table> && (int64_t)p.few.most * Hkv * 64 * kFewWaves >= 1LL << 32) || (int64_t)p.many.most * Hkv * many_threads >= 1LL << 32)
+    return false;
   p.q = (const elem*)q; p.out = (elem*)out;
   p.pages[0] = (const char*)k_pages; p.pages[1] = (const char*)v_pages;
   p.scales[0] = k_scales; p.scales[1] = v_scales;
@@ -1477,8 +1479,15 @@ static int launch_paged(const PagedParams<E, Table>& p, hipStream_t st) {
   static bool allowed[2][kMaxDevices];
   const auto few = paged_few_kernel<E, D, k8, Table, few_sets<Table>(D)>;
   if (!allow_dynamic_lds((const void*)few, few_lds_bytes<D, k8, Table>(), allowed[0])) return MOBA_ERR_LAUNCH;
-  hipLaunchKernelGGL(few, dim3((unsigned)p.few.most * p.shape.Hkv), dim3(64 * kFewWaves), (few_lds_bytes<D, k8, Table>()), st, p);
-  if constexpr (!kChooses<Table>) {
+  auto launch_few = [&](const PagedParams<E, Table>& now, int units) {
+    hipLaunchKernelGGL(few, dim3((unsigned)units * now.shape.Hkv), dim3(64 * kFewWaves), (few_lds_bytes<D, k8, Table>()), st, now);
+  };
+  if constexpr (kChooses<Table>) {   // (a launch's lists lie where those of the one before it have been)
+    PagedParams<E, Table> now = p;
+    const int step = now.shape.table.units;
+    for (int& unit0 = now.shape.table.unit0; unit0 < p.few.most; unit0 += step) launch_few(now, std::min(step, p.few.most - unit0));
+  } else {
+    launch_few(p, p.few.most);
     if (p.many.most > 0) {
       const auto many = paged_many_kernel<E, D, k8, Table>;
       if (!allow_dynamic_lds((const void*)many, many_lds_bytes<D>(), allowed[1])) return MOBA_ERR_LAUNCH;

@@ -7,6 +7,7 @@
 namespace moba {
 
 constexpr int kMostTopk = 64;
+constexpr int64_t kListsAtOnce = 1LL << 29;   // bytes of a launch's lists in memory: more units are several launches
 static_assert(64 * kFewWaves == kListThreads && kLdsEntries * sizeof(Chosen) == kListBytes);
 static_assert(few_list_at<64, true>() >= 4 * kWindow + 64);
 
@@ -14,6 +15,7 @@ static_assert(few_list_at<64, true>() >= 4 * kWindow + 64);
 struct ChosenSizes {
   Cuts cuts;
   int room_of_list;     // 0: in LDS
+  int units;            // of a launch
   int64_t lists_at, bytes;
 };
 static ChosenSizes chosen_sizes(int64_t T, int B, int rep, int Hkv, int D, int64_t max_pages, int each, int topk, bool cache8) {
@@ -23,7 +25,11 @@ static ChosenSizes chosen_sizes(int64_t T, int B, int rep, int Hkv, int D, int64
   const int64_t room = rows * topk < blocks ? rows * topk : blocks;
   s.room_of_list = room > kLdsEntries ? (int)room : 0;
   s.lists_at = ((int64_t)paged_workspace_bytes(s.cuts, B, Hkv, D) + 15) / 16 * 16;
-  s.bytes = s.lists_at + (int64_t)s.cuts.few.most * Hkv * s.room_of_list * (int64_t)sizeof(Chosen);
+  const int64_t list = s.room_of_list * (int64_t)sizeof(Chosen);
+  int64_t units = ((1 << 24) - 1) / Hkv;   // (2^32 threads)
+  if (list && units > kListsAtOnce / (list * Hkv)) units = std::max(kListsAtOnce / (list * Hkv), (int64_t)1);
+  s.units = (int)std::min(units, (int64_t)s.cuts.few.most);
+  s.bytes = s.lists_at + s.units * Hkv * list;
   return s;
 }
 
@@ -42,7 +48,9 @@ static int block_attention(const ChosenTable& table, const ChosenSizes& s, const
 static int check_blocks(int64_t T, int B, int H, int Hkv, int page_size, int64_t max_pages, int block_size, int topk) {
   if (!paged_sizes_ok(T, B, H, Hkv) || max_pages <= 0 || topk <= 0) return MOBA_ERR_ARG;
   if (page_log2_of(page_size) < 0 || block_size <= 0 || block_size % page_size) return MOBA_ERR_UNSUPPORTED;
-  if (T >= 1LL << 24 || T * H >= 1LL << 31 || max_pages >= 1LL << 31 || topk > kMostTopk || block_size > 1 << 24) return MOBA_ERR_LIMIT;
+  if (T >= 1LL << 24 || T * H >= 1LL << 31 || max_pages >= 1LL << 31 || topk > kMostTopk || block_size > 1 << 24 ||
+      (int64_t)B * Hkv >= 1LL << 24)
+    return MOBA_ERR_LIMIT;
   return MOBA_OK;
 }
 
@@ -72,7 +80,7 @@ extern "C" int moba_paged_block_attention(const void* q, void* out, const void* 
   const ChosenSizes s = chosen_sizes(T, B, H / Hkv, Hkv, D, max_pages, each, topk, cache8 != 0);
   char* const space = (char*)workspace;
   const ChosenTable chosen = {table, blocks, s.room_of_list ? (Chosen*)(space + s.lists_at) : nullptr, topk, each, divisor_or_one(each),
-                              s.room_of_list};
+                              s.room_of_list, 0, s.units};
   hipStream_t st = (hipStream_t)stream;
   return dtype == MOBA_DTYPE_F16
              ? block_attention<F16>(chosen, s, q, out, k_pages, v_pages, k_scales, v_scales, space, H, Hkv, D, strides, cache8, scale, st)

@@ -28,14 +28,16 @@ struct Chosen {
 };
 struct ChosenTable : PageTable {
   const int32_t* blocks;  // [T, H, K], as they were given: any numbers
-  Chosen* lists;          // [workgroups, room_of_list] for lists that may be longer than kLdsEntries, or null
+  Chosen* lists;          // [workgroups of a launch, room_of_list] for lists that may be longer than kLdsEntries, or null
   int K, each;            // entries of a row; pages of a block
   Divisor by_each;
   int room_of_list;
+  int unit0, units;       // the first of this launch; of a launch
 };
 template <>
 constexpr bool kChooses<ChosenTable> = true;
 
+__device__ __forceinline__ int first_unit(const ChosenTable& t) { return t.unit0; }
 __device__ __forceinline__ int block_keys(const ChosenTable& t) { return t.each << t.page_log2; }
 
 __device__ __forceinline__ Chosen* list_of(const ChosenTable& t, char* lds) {

@@ -29,13 +29,14 @@ constexpr int kWholeRun = 0x3fffffff;  // tiles
 // long one among them: one token each for 255 sequences, 131072 keys and 254 of 513, 8 heads, 8 bits: 120 us; one more of these: 1135.
 constexpr int kWholeAt = 4;
 
-// Table: PageTable, or another that has its own count_of(), sequence_of() and share_at(), and kShares or kChooses
+// Table: PageTable, or another that has its own of the functions below, and kShares or kChooses
 template <class Table>
 struct Shape {
   Table table;
   int H, Hkv, rep;
 };
 __device__ __forceinline__ int count_of(const PageTable& t) { return t.B; }                // sequences
+__device__ __forceinline__ int first_unit(const PageTable&) { return 0; }                  // of a launch
 template <class Table>
 constexpr bool kShares = false;   // whether a token attends keys of more than one sequence
 template <class Table>
@@ -206,8 +207,8 @@ __device__ __forceinline__ Unit unit_at(const Shape<Table>& p, const Cut& c, int
 // are numbered by unit and head.  first: share_at() of the lanes.
 template <class Table>
 __device__ __forceinline__ bool find_unit(const Shape<Table>& p, const Cut& c, int lane, Unit& unit, int& hkv, int& item, Share& first) {
-  const int u = (int)blockIdx.x / p.Hkv;
-  hkv = (int)blockIdx.x - u * p.Hkv;
+  const int at = (int)blockIdx.x / p.Hkv, u = first_unit(p.table) + at;
+  hkv = (int)blockIdx.x - at * p.Hkv;
   first = share_at(p, c, lane);
   const int run = run_tiles(p, c, lane, first);
   if (run == 0) return false;   // (no work at all)

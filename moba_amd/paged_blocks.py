@@ -129,7 +129,8 @@ def paged_block_attention(query: torch.Tensor, cache: PagedKVCache, blocks: torc
     Up to 32 rows (new tokens times heads on a key/value head) of a sequence read the union of their blocks once.  Made for one or some
     new tokens of each sequence; a long piece of a prompt is cut into groups of 32 rows, each of which reads its own union.
     Scores, softmax statistics and sums are 32 bits, a probability the sum of two 16-bit elements, as in ``paged_attention`` for few
-    rows.
+    rows.  The workspace holds parts of the rows in 32 bits and, where 32 rows may choose more than 1024 of a table's blocks, the lists of these,
+    up to 512 MiB.  At most 2^24 - 1 tokens, fewer than 2^31 tokens times heads, and some million sequences times key/value heads.
     """
     out = _lib.host().paged_block_attention(cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales, query, page_table, lengths, cu_new,
                                             blocks, block_size, scaling)

@@ -77,3 +77,37 @@ def test_wide_tables():
                  lambda: m.paged_select_blocks(q, sums, *index, 16, 1 << 24, 3), lambda: m.paged_block_attention(q, cache, blocks, *index, 32)):
         with pytest.raises(ValueError, match="2\\^31"):
             call()
+
+
+@pytest.mark.parametrize("quantized", [True, False])
+def test_block_attention_in_several_launches(quantized):
+    """More lists of blocks than a launch's workspace takes: the same as pieces of the tokens, each in one launch."""
+    from moba_amd import PagedKVCache, _lib, paged_block_attention
+    heads, kv_heads, page, d = 64, 8, 16, 64
+    old, new, pages = (20000, 300), (13000, 5000), 2400
+    g = torch.Generator(device="cuda").manual_seed(2)
+    k, v = (torch.randn((pages + 400, kv_heads, page, d), generator=g, device="cuda") for _ in range(2))
+    if quantized:
+        cache = PagedKVCache(*(x.to(torch.float8_e4m3fn) for x in (k, v)), *(torch.rand((pages + 400, kv_heads), generator=g, device="cuda") for _ in range(2)))
+    else:
+        cache = PagedKVCache(k.to(BF16), v.to(BF16))
+    table = torch.full((2, pages), -1, dtype=torch.int32, device="cuda")
+    ids = torch.randperm(pages + 400, generator=g, device="cuda").int()
+    table[0], table[1, :400] = ids[:pages], ids[pages:]
+    tokens = sum(new)
+    q = torch.randn((tokens, heads, d), generator=g, device="cuda").to(BF16)
+    at = torch.cat([torch.arange(o, o + n, device="cuda") for o, n in zip(old, new)]) // page
+    blocks = torch.full((tokens, heads, 64), -1, dtype=torch.int32, device="cuda")
+    for i in (0, 17, 63):
+        blocks[..., i] = (torch.rand((tokens, heads), generator=g, device="cuda") * (at + 1)[:, None]).int()
+    size = _lib.load().moba_paged_block_attention_workspace_bytes
+    assert size(tokens, 2, heads, kv_heads, d, page, pages, page, 64, quantized) < 1 << 30
+    got = paged_block_attention(q, cache, blocks, table, ints(old[0] + new[0], old[1] + new[1]), ints(0, new[0], tokens), page)
+    row = 0
+    for b in range(2):
+        for first in range(0, new[b], 4000):
+            n = min(4000, new[b] - first)
+            part = paged_block_attention(q[row:row + n], cache, blocks[row:row + n], table[b:b + 1], ints(old[b] + first + n), ints(0, n), page)
+            assert torch.equal(got[row:row + n], part), (b, first)
+            row += n
+    assert row == tokens

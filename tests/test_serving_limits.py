@@ -40,3 +40,14 @@ def test_wide_tables_are_refused():
             call(meta(1, 1 << 31), meta(1), meta(2))
         with pytest.raises(RuntimeError, match="AMD GPU"):
             call(meta(1, 9), meta(1), meta(2))
+
+
+def test_the_lists_of_long_pieces_are_bounded():
+    """The workspace of the attention over chosen blocks: lists of up to 512 MiB beside the rows' parts, however many rows there are."""
+    from moba_amd import _lib
+    size = _lib.load().moba_paged_block_attention_workspace_bytes
+    for tokens in (1 << 17, 1 << 20, (1 << 24) - 1):
+        for d, cache8 in ((64, 1), (128, 0)):
+            short, long = (size(tokens, 1, 32, 8, d, 64, pages, 64, 64, cache8) for pages in (1024, 4096))
+            assert 0 < short < 1 << 29 and 0 < long - short <= 1 << 29, (tokens, d, short, long)
+    assert size((1 << 24) - 1, 1, 128, 1, 64, 64, 4096, 64, 64, 1) > 0     # (2^26 units)
