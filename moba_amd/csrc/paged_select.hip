@@ -5,9 +5,9 @@
 //   score[t, h, j]    = q[t, h, :] . sum over block j's pages of sum[page, h / rep, :], 64 bits
 //   blocks[t, h, :]   = the topk - 1 blocks before the token's own with the largest scores (of equal ones the lowest), and its own;
 //                       ascending, -1 behind the last
-// Blocks before a token's own are whole, so that the order of the sums is that of the means.  64 bits, because which blocks are in
-// should not depend on the order in which a sum is formed: products of 24 and 11 bits are exact, and blocks of equal sums have equal
-// scores.
+// Blocks before a token's own are whole, so that the order of the sums is that of the means.  In 64 bits a score is off by some 2^-53 of
+// the sum of its terms' magnitudes for each of its additions; of scores nearer than that rounding decides, and always alike: a score is
+// the result of the same operations in the same order whatever else is in the batch, and blocks of the same pages have equal scores.
 //
 // All three kernels are bound by memory or latency.
 //   Sums       the keys of the pages that have received tokens, once: 131072 tokens, 8 heads, 8 bits: 143 MB in 22.7 us where they are in
@@ -181,13 +181,12 @@ __global__ __launch_bounds__(256) void paged_score_kernel(const SelectParams<E> 
   }
   const int quad = tid % kQuads;
   for (int j0 = blockIdx.z * at_once; j0 < history; j0 += gridDim.z * at_once) {
-    // sum number i: of block i % at_once, its pages i / at_once, .. + split, ..
-    double acc[kRounds][4];
-#pragma unroll
-    for (int k = 0; k < kRounds; ++k)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[k][e] = 0.;
-    for (int i0 = 0; i0 < s.each; i0 += split * kAhead) {
+    // Sum number i: of block i % at_once, its pages i / at_once, .. + split, ..  Whatever the split, pages that are half as many apart as
+    // the block has places for (its pages, rounded up to a power of two) are added first, then sums that are a quarter apart, and so on
+    // (of blocks of more than 64 pages, which are always split alike, those 64 apart first): a thread's sums by their distance,
+    // then those of the threads.
+    double acc[kRounds][kAhead][4];
+    auto add_pages = [&](int i0, auto first) __attribute__((always_inline)) {
       f32x4 x[kRounds][kAhead];
 #pragma unroll
       for (int k = 0; k < kRounds; ++k) {
@@ -205,21 +204,36 @@ __global__ __launch_bounds__(256) void paged_score_kernel(const SelectParams<E> 
 #pragma unroll
         for (int a = 0; a < kAhead; ++a)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[k][e] += (double)x[k][a][e];
-    }
+          for (int e = 0; e < 4; ++e) acc[k][a][e] = first ? (double)x[k][a][e] : acc[k][a][e] + (double)x[k][a][e];
+    };
+    add_pages(0, std::true_type{});
+    for (int i0 = split * kAhead; i0 < s.each; i0 += split * kAhead) add_pages(i0, std::false_type{});
+    static_assert(kAhead == 4);
 #pragma unroll
     for (int k = 0; k < kRounds; ++k)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) part[tid / kQuads + k * kThreads][4 * quad + e] = acc[k][e];
+      for (int e = 0; e < 4; ++e)
+        part[tid / kQuads + k * kThreads][4 * quad + e] = (acc[k][0][e] + acc[k][2][e]) + (acc[k][1][e] + acc[k][3][e]);
     __syncthreads();
-    if (split > 1) {
-      for (int i = tid; i < at_once * D; i += 256) {
-        double x = part[i / D][i % D];
-        for (int k = 1; k < split; ++k) x += part[k * at_once + i / D][i % D];
-        part[i / D][i % D] = x;
+    auto join = [&](auto log2) __attribute__((always_inline)) {
+      constexpr int kSplit = 1 << log2, kBlocks = kScoreSums / kSplit;
+      for (int i = tid; i < kBlocks * D; i += 256) {
+        double x[kSplit];
+#pragma unroll
+        for (int k = 0; k < kSplit; ++k) x[k] = part[k * kBlocks + i / D][i % D];
+#pragma unroll
+        for (int h = kSplit / 2; h >= 1; h /= 2)
+#pragma unroll
+          for (int k = 0; k < h; ++k) x[k] += x[k + h];
+        part[i / D][i % D] = x[0];
       }
       __syncthreads();
-    }
+    };
+    static_assert(kScoreSumsLog2 == 4);
+    if (p.split_log2 == 1) join(std::integral_constant<int, 1>{});
+    else if (p.split_log2 == 2) join(std::integral_constant<int, 2>{});
+    else if (p.split_log2 == 3) join(std::integral_constant<int, 3>{});
+    else if (p.split_log2 == 4) join(std::integral_constant<int, 4>{});
     // (rows and blocks that are none have columns and rows of their own)
     for (int r0 = 0; r0 < rows_here; r0 += 16) {
       f64x4 c = {0., 0., 0., 0.};

@@ -76,8 +76,8 @@ def paged_select_blocks(query: torch.Tensor, sums: torch.Tensor, page_table: tor
         [tokens, heads, topk] int32: numbers of blocks in the sequence, ascending; -1 behind the last where there are fewer, and
         throughout where a row belongs to no sequence.
 
-    The products are with the sums of a block's pages, in 64 bits (all blocks before a token's own are whole); of equal ones the
-    lowest block counts as larger, NaN as minus infinity.  A page that the table names wrongly adds nothing.  Tables of at most 16384
+    The products are with the sums of a block's pages, in 64 bits (all blocks before a token's own are whole), and do not depend on what
+    else is in the batch; of equal ones the lowest block counts as larger, NaN as minus infinity.  A page that the table names wrongly adds nothing.  Tables of at most 16384
     blocks; at most 2^24 - 1 tokens, fewer than 2^31 tokens times heads, and some million sequences times key/value heads.  The workspace
     holds the scores, up to 512 MiB (one token's at least).
     (``moba_attn_varlen`` rounds the blocks' means to the keys' type first, which can decide between blocks of nearly equal
