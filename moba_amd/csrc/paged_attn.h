@@ -222,7 +222,7 @@ __device__ __forceinline__ int list_of(const PageTable&, char*) { return 0; }
 
 // kSets: sets of 32 rows to a workgroup, which read, and for 8-bit pages convert, K and V once for all of them
 template <class E, int D, bool k8, class Table, int kSets>
-__global__ __launch_bounds__(64 * kFewWaves, kSets > 1 && D == 128 ? 1 : 2) void paged_few_kernel(const PagedParams<E, Table> p) {
+__global__ __launch_bounds__(64 * kFewWaves, 2) void paged_few_kernel(const PagedParams<E, Table> p) {
   static_assert(kSets == 1 || !kChooses<Table>);
   MOBA_ELEM_TYPES(E)
   using V = std::conditional_t<k8, Bf16, E>;       // type of the second product
@@ -1281,29 +1281,25 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams<E, T
 // tokens of 32 heads, three runs and more of each, 16 us, and 23.6 with a head to a wave.
 template <class E, int D, class Table>
 __global__ __launch_bounds__(256) void paged_merge_many_kernel(const PagedParams<E, Table> p, int heads) {
+  static_assert(kShares<Table>);
   constexpr int kPer = D / 16, kHeads = 4, kLse = 16, kRowsAhead = 4;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const auto& shape = p.shape;
   const int per_token = (shape.H + heads - 1) / heads, item = (int)blockIdx.x * 4 + wave;
   const int t = item / per_token, h0 = (item - t * per_token) * heads;
   if (t >= shape.table.T) return;
-  constexpr int kSides = kShares<Table> ? 2 : 1;
   const MergeToken<E, Table> token(p, t, lane);
-  if (token.done()) return;
   const int d0 = (lane & 15) * kPer, end = min(h0 + heads, shape.H);
   for (int h1 = h0; h1 < end; h1 += kHeads) {
     const int head = h1 + (lane >> 4), h = min(head, end - 1), hkv = h / shape.rep;   // (heads behind the last are it again)
-    Parts parts[kSides];
+    Parts parts[2];   // (one side's runs after the other's)
 #pragma unroll
-    for (int s = 0; s < kSides; ++s) parts[s] = token.parts(p, hkv, h - hkv * shape.rep, s);
-    const int runs = parts[0].runs + (kSides > 1 ? parts[kSides - 1].runs : 0);
+    for (int s = 0; s < 2; ++s) parts[s] = token.parts(p, hkv, h - hkv * shape.rep, s);
+    const int runs = parts[0].runs + parts[1].runs;
     auto row_of = [&](int i) __attribute__((always_inline)) {
-      const bool second = kSides > 1 && i >= parts[0].runs;
-      return second ? parts[kSides - 1].first + (i - parts[0].runs) * parts[kSides - 1].step : parts[0].first + i * parts[0].step;
+      return i >= parts[0].runs ? parts[1].first + (i - parts[0].runs) * parts[1].step : parts[0].first + i * parts[0].step;
     };
-    auto side_of = [&](int i) __attribute__((always_inline)) -> const Parts& {
-      return kSides > 1 && i >= parts[0].runs ? parts[kSides - 1] : parts[0];
-    };
+    auto side_of = [&](int i) __attribute__((always_inline)) -> const Parts& { return i >= parts[0].runs ? parts[1] : parts[0]; };
     float top = kNoMax, ll = 0.f, o[kPer] = {};
     for (int i0 = 0; __any(i0 < runs); i0 += kLse) {
       float lse[kLse], mm = top;
