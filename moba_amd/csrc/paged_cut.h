@@ -22,7 +22,7 @@ struct Cut {
   int target;      // units per key/value head that fill the chip
   int most;        // no more units per key/value head than this, whatever the batch
   int parts;       // no more than this of them where there is a sequence of several runs
-  bool even;       // runs by even_run()
+  bool even;       // kShares: runs by even_run()
 };
 constexpr int kWholeRun = 0x3fffffff;  // tiles
 // With this many times `target` groups and more, a sequence's keys are one run.  That is right for sequences of like lengths, and slow for one
@@ -145,7 +145,9 @@ __device__ __forceinline__ int run_tiles(const Shape<Table>& p, const Cut& c, in
     return a < 1LL << 31 ? (int)(((uint32_t)a + (uint32_t)b - 1) / (uint32_t)b) : (int)min((a + b - 1) / b, (int64_t)kWholeRun);
   };
   const int safe = max(ceil_div(work, max(max((int64_t)c.target - groups, (int64_t)c.target / 2), (int64_t)1)), work > 0 ? c.least_tiles : 0);
-  if (c.even && groups > 0 && count_of(p.table) <= 64 && work < 1LL << 24) return even_run(c, lane, first, count_of(p.table), work, safe);
+  if constexpr (kShares<Table>) {
+    if (c.even && groups > 0 && count_of(p.table) <= 64 && work < 1LL << 24) return even_run(c, lane, first, count_of(p.table), work, safe);
+  }
   if (count_of(p.table) <= 64 && groups <= c.target)
     for (int run = max(ceil_div(work, c.target), c.least_tiles); run < safe; run += run / 16 + 1)
       if (wave_sum(first.groups ? first.groups * runs_of(first.tiles, run) : 0) <= (uint32_t)c.target) return run;
