@@ -8,9 +8,10 @@
 // sequence's last) and cut into as many runs as the batch's cut says, which knows only how many blocks the rows may have: about as many
 // as if each had chosen its number at random.
 //
-// One token of 32 heads on 8, twelve blocks of 4096 behind 131072, 8 bits: 41.9 us, some 181 MB; sixteen users' tokens, sixteen blocks of
-// 512, fp16: 47.8.  A kernel before that makes the lists, and a cut by their lengths: 46.2 and 53.3; a cut half way between rows that
-// choose alike and at random: 41.9 and 50.6; more workgroups than fill the chip once: 50 and 54 and more.
+// One token of 32 heads on 8, twelve blocks of 4096 behind 131072, 8 bits: 39 us and 4.8 for the merge, some 181 MB; sixteen users' tokens,
+// sixteen blocks of 512, fp16: 47 and 4.6.  On one state, whose keys are partly in the last-level cache, the calls are 41.9 and 47.8; with a
+// kernel before that makes the lists, and a cut by their lengths, 46.2 and 53.3; with a cut half way between rows that choose alike and
+// at random 41.9 and 50.6; with more workgroups than fill the chip once 50 and 54 and more.
 #pragma once
 #include "attn_common.h"
 #include "paged_cut.h"

@@ -1,8 +1,8 @@
 // Attention of new tokens over the paged cache where sequences begin with the same pages: what they share is read once for all of
 // them, by the kernels of paged_attn.h over the batch as paged_shared.h cuts it.  Sixteen users' tokens, 32 heads on 8, 8 bits, behind
-// 32768 shared tokens and up to 8000 of their own: 133 MB in 38.0 us, of which the shared keys pass twice (64 rows of a key/value head,
-// 32 to a workgroup), and the merge in 6.0; 33 us of the 38 are as many steps as the longest run has.  898 tokens of prompts behind
-// 12288 and 69 of other users: products, 190 Gflop, 241 to 254 us, 25.8 for the few rows, 15.5 for the merge.
+// 32768 shared tokens and up to 8000 of their own: 133 MB in 39 us, of which the shared keys pass twice (64 rows of a key/value head,
+// 32 to a workgroup), and the merge in 6.2; 33 us of the 39 are as many steps as the longest run has.  898 tokens of prompts behind
+// 12288 and 69 of other users: products, 185 Gflop, 225 us (219 to 255 by the box), 24.6 for the few rows, 15.6 for the merge.
 #include "paged_attn.h"
 #include "paged_shared.h"
 

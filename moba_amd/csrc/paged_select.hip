@@ -10,14 +10,14 @@
 // the result of the same operations in the same order whatever else is in the batch, and blocks of the same pages have equal scores.
 //
 // All three kernels are bound by memory or latency.
-//   Sums       the keys of the pages that have received tokens, once: 131072 tokens, 8 heads, 8 bits: 143 MB in 22.7 us where they are in
-//              the last-level cache, 30 where they are not; the next token of 16 sequences 3.8.
+//   Sums       the keys of the pages that have received tokens, once: 131072 tokens, 8 heads, 8 bits: 143 MB in 30.4 us, 22.7 where they
+//              are in the last-level cache; the next token of 16 sequences 3.6.
 //   Scores     the sums of the history's pages once for up to 32 rows (tokens times heads) of a key/value head; a workgroup's threads
 //              take 16 bytes of a page each, so that a whole block of many pages is on its way at once.  32 heads on 8, blocks of 4096
-//              behind 131072: 6.4 us; 16 sequences of five tokens, blocks of 512, 15 MB: 12.9.
+//              behind 131072: 8.0 us, 6.2 where the sums are in a cache; 16 sequences of five tokens, blocks of 512, 15 MB: 15.4 and 12.7.
 //   Selection  the scores of a row stay in registers, as whole numbers in the same order, of which the (topk - 1)-th largest is found
 //              bit by bit: a comparison and a count for each of a lane's scores and bit, until the count is right (some 20 bits).
-//              3.9 and 5.8 us of these.
+//              3.8 and 5.4 us of these.
 #include "attn_common.h"
 #include "paged_cut.h"
 
@@ -184,7 +184,7 @@ __global__ __launch_bounds__(256) void paged_score_kernel(const SelectParams<E> 
     // Sum number i: of block i % at_once, its pages i / at_once, .. + split, ..  Whatever the split, pages that are half as many apart as
     // the block has places for (its pages, rounded up to a power of two) are added first, then sums that are a quarter apart, and so on
     // (of blocks of more than 64 pages, which are always split alike, those 64 apart first): a thread's sums by their distance,
-    // then those of the threads.
+    // then those of the threads.  (Sums whose order the split decides: single tokens of 256 sequences, 8 pages to a block, 43.2 us, 44.3 so.)
     double acc[kRounds][kAhead][4];
     auto add_pages = [&](int i0, auto first) __attribute__((always_inline)) {
       f32x4 x[kRounds][kAhead];
@@ -405,7 +405,9 @@ static int launch_select(SelectParams<E> p, int32_t* out, int64_t T, hipStream_t
     s.tokens = (int)(T - t0 < step ? T - t0 : step);
     const int64_t units = (int64_t)s.tokens * s.rep / kScoreRows + s.table.B;
     // (a thread has up to eight pages of a block on its way; fewer where there are not enough blocks for the chip.  Blocks of 64 pages behind
-    // 131072 tokens 6.2 us, 7.5 without the latter, 30 with a thread to a block; of 8 pages behind 20000 5.0 and 7.2)
+    // 131072 tokens 6.2 us, 7.5 without the latter, 30 with a thread to a block; of 8 pages behind 20000 5.0 and 7.2.  Up to four, two and one
+    // page to a thread wherever a block has several, the whole call: 16 sequences of five tokens, 8 pages to a block, 19, 22 and 32 us, 16.5
+    // so; 2048 tokens behind 131072, 64 pages, 588, 455 so)
     auto chunks = [&]() { return (s.blocks - 1) / (kScoreSums >> p.split_log2) + 1; };
     p.split_log2 = 0;
     while (p.split_log2 < kScoreSumsLog2 &&

@@ -38,9 +38,9 @@ def paged_prefix_attention(query: torch.Tensor, cache: PagedKVCache, page_table:
         also where ``shared`` says more than a sequence has.  Rows that see nothing are zeros.
 
     Precision is that of ``paged_attention`` for few rows where a group (for what it shares), or a sequence (for the rest), has up to
-    256 rows, new tokens times heads on a key/value head; 128 with 16-bit pages and heads of 128.  Otherwise it is that for many.  The
-    index tensors stay on the device: a captured call follows them.  The workspace holds every row's parts in 32 bits, two or three of
-    them with many tokens.  No gradients.
+    256 rows, new tokens times heads on a key/value head; 128 with 16-bit pages and heads of 128.  Otherwise it is that for many, for
+    the shared keys of a large group also where its sequences have few rows each.  The index tensors stay on the device: a captured call
+    follows them.  The workspace holds every row's parts in 32 bits, two or three of them with many tokens.  No gradients.
     """
     out = _lib.host().paged_prefix_attention(cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales, query, page_table, lengths, cu_new,
                                              cu_groups, shared, scaling)
