@@ -28,7 +28,7 @@ def paged_key_sums(cache: PagedKVCache, sums: torch.Tensor, page_table: torch.Te
         cache, page_table, lengths, cu_new: as ``paged_append`` has had them
         sums: [num_pages, kv_heads, head_dim] float32, to be kept with the cache: ``sums[page, head]`` becomes the sum, in 32 bits,
             of the keys of the tokens that the page holds up to its sequence's last.  Other pages' sums are left as they are.
-        rows: the packed rows that cu_new counts in (its last number or more); at most 2^30 - 1
+        rows: the packed rows that cu_new counts in (its last number or more, for which time is spent); at most 2^30 - 1
 
     At most some million sequences times key/value heads.
     """
